@@ -226,7 +226,9 @@ def _plain_sample(s):
     last = classes - 1 - torch.argmax(kept.flip(1).int(), 1)
     index = torch.minimum((mass <= s["uniform"][:, None] * mass[:, -1:]).sum(1), last)
     logprob = ((x.gather(1, index[:, None]) - m) / t)[:, 0] - torch.log(w.sum(1))
-    return {"index": index.int(), "logprob": torch.where(greedy.expand(x.shape[0], 1)[:, 0], 0.0, logprob).float()}
+    logprob = torch.where(greedy.expand(x.shape[0], 1)[:, 0], 0.0, logprob)
+    empty = m[:, 0] == float("-inf")   # a row that may answer nothing
+    return {"index": torch.where(empty, -1, index).int(), "logprob": torch.where(empty, float("-inf"), logprob).float()}
 
 
 def run(state):
@@ -328,7 +330,8 @@ def _exact_sample(s, a, b):
         found[:, -1] |= ~found.any(1)
         at = found.argmax(1)
         logprob = np.take_along_axis(z, at[:, None], 1)[:, 0] - np.log(w.sum(1))
-    return {"index": None, "logprob": torch.from_numpy(np.where(t[:, 0] <= 0, 0.0, logprob))}
+    logprob = np.where(best[:, 0] == -np.inf, -np.inf, np.where(t[:, 0] <= 0, 0.0, logprob))
+    return {"index": None, "logprob": torch.from_numpy(logprob)}
 
 
 def exact(case, seed):
