@@ -10,6 +10,9 @@ thin ctypes front-end used by the tests and ``bench.py``:
 * :class:`Trainer` drives the boosting loop exactly like cb-train's device branch
   (crates/cb-train/src/boosting.rs:6532-7300) through ``cbt_*``.
 
+The operators on class scores (:func:`top_classes`, :func:`distill_gradients`,
+:func:`sample_classes`) take torch tensors on the GPU.
+
 There is no CPU fallback: if the library is missing or no GPU is present, calls raise.
 """
 from __future__ import annotations
@@ -128,7 +131,9 @@ EXPORTS = ["cbh_session_begin", "cbh_session_begin_u8", "cbh_session_grow",
            "cbt_read_approx", "cbt_stats", "cbt_reset_stats", "cbt_bias", "cbt_close", "cbh_session_set_profile",
            "cbt_set_profile", "cbh_session_set_ctr", "cbt_set_ctr", "cbh_session_read_ctr_bins",
            "cbt_open_ctr", "cbh_hist_build_noalloc", "cbh_session_capture_hists", "cbh_session_level_hist",
-           "cbh_columns_from_rows", "cbh_session_fill_tile", "cbt_fill_tile"]
+           "cbh_columns_from_rows", "cbh_session_fill_tile", "cbt_fill_tile", "cbh_top_classes",
+           "cbh_top_classes_workspace", "cbh_distill_gradients", "cbh_distill_gradients_workspace",
+           "cbh_sample_classes", "cbh_sample_classes_workspace"]
 
 _lib = None
 
@@ -191,6 +196,15 @@ def load(path: str = LIB_PATH):
     L.cbh_session_read_ctr_bins.argtypes = [P, C.c_int32, P, C.c_uint64]
     L.cbt_open_ctr.argtypes = [C.POINTER(TrainParams), P, C.c_uint64, C.c_uint32, C.c_uint32, P, P,
                                C.POINTER(DeviceCtrConfig), P, P, C.POINTER(P)]
+    U64, U32, I64, I32, F64 = C.c_uint64, C.c_uint32, C.c_int64, C.c_int32, C.c_double
+    scores = [P, I32, U64, U32, I64, I64]
+    L.cbh_top_classes.argtypes = scores + [U32, F64, P, P, P, P, U64, P]
+    L.cbh_distill_gradients.argtypes = scores + [P, P, U32, P, F64, P, P, P, I64, I64, P, U64, P]
+    L.cbh_sample_classes.argtypes = scores + [P, F64, P, U32, P, F64, P, F64, P, P, I64, P, P, P, U64, P]
+    L.cbh_top_classes_workspace.argtypes = [U64, U32, U32]
+    L.cbh_distill_gradients_workspace.argtypes = L.cbh_sample_classes_workspace.argtypes = [U64, U32]
+    for fn in (L.cbh_top_classes_workspace, L.cbh_distill_gradients_workspace, L.cbh_sample_classes_workspace):
+        fn.restype = U64
     L.cbt_close.argtypes = [P]
     L.cbt_close.restype = None
     _lib = L
@@ -205,6 +219,9 @@ def _check(rc: int):
 def _ptr(a):
     return None if a is None else a.ctypes.data_as(C.c_void_p)
 
+
+# operators on class scores that live on the GPU (torch tensors; torch is imported at the first call)
+from .class_scores import distill_gradients, sample_classes, top_classes  # noqa: E402
 
 # ---------------------------------------------------------------------------------------
 # kernel-level entry points

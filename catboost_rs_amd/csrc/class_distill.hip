@@ -1,0 +1,400 @@
+// Distillation from a teacher's top classes: the loss and the gradient of a student's scores.
+//
+// With p = softmax(x / t), the teacher's probabilities q of its listed classes and `rest` what they
+// leave to the others (one bucket):
+//   loss = w t^2 [ sum_l q_l (log q_l - log p_l) + rest (log rest - log sum_others p) ]
+//   grad = w t [ p_j H - q_j ] (listed),  w t p_j (H - rest / sum_others p) (others),  H = sum q + rest
+// The others' softmax mass is summed over the others themselves (the listed classes are marked in
+// an LDS bit mask and read as -inf), never as the difference 1 - listed: a student that is
+// sure of its answer leaves the others a mass that such a difference would lose.  What belongs to the
+// listed classes is f64: their gradient is a difference of nearly equal probabilities.
+#include "class_scores.hpp"
+
+namespace {
+using namespace cbh::cls;
+
+constexpr uint32_t kMaxList = 1024;
+constexpr int kUnroll = 4;
+constexpr uint32_t kMaxSeg = 1u << 18;   // classes a workgroup takes: their marks are 32 KB of LDS
+
+struct Lists {   // the teacher's, and what weighs the rows
+    const float* scores;     // [rows][k]
+    const int32_t* index;
+    const float* lse;        // nullable
+    const float* weight;     // nullable
+    uint32_t k;
+};
+template <class T>
+struct Grad {
+    T* data;   // nullable
+    int64_t rs, cs;
+};
+
+// Sums over a row's list, and the factors of its outputs.
+struct RowSums {
+    double held, entropy;   // sum q, sum q log q
+    uint32_t listed;        // valid entries
+    double base, base_log;  // log q = (u / t - base) - base_log
+};
+struct Outcome {
+    double loss;
+    float M, others;   // gradient of an other class: 2^((x - M) c) * others
+    double whole, inv_s;   // of a listed one: wt (2^((x - M) c) * inv_s * whole - q)
+};
+
+// (M, S_o): running maximum and sum of the others; S_l the listed classes' sum at the same M; lin = sum q
+// log p_l.  t, w as in the loss.
+__device__ __forceinline__ double row_rest(const RowSums& r, bool has_lse, uint32_t n) {
+    return has_lse && r.listed < n ? fmax(0.0, 1.0 - r.held) : 0.0;
+}
+__device__ __forceinline__ Outcome outcome(const RowSums& r, double rest, double M, double s_others, double s_listed,
+                                           double lin, double t, double w) {
+    Outcome o;
+    const double S = s_others + s_listed;
+    o.M = (float)M;
+    o.whole = r.held + rest;
+    o.inv_s = S > 0.0 ? 1.0 / S : S == 0.0 ? 0.0 : S;   // (NaN stays)
+    // share of the others in the gradient: whole / S - rest / s_others
+    o.others = (float)(w * t * (o.whole * o.inv_s - (s_others > 0.0 ? rest / s_others : 0.0)));
+    double loss = r.entropy - lin;
+    if (rest > 0.0) loss += rest * (log(rest) - log(s_others * o.inv_s));
+    o.loss = w * t * t * loss;
+    return o;
+}
+// (the list's own log-sum-exp stays in two parts: next to the lowest f32 one number would lose the logarithm)
+__device__ __forceinline__ double log_q(float u, double it, const RowSums& r) { return ((double)u * it - r.base) - r.base_log; }
+// q log q and q log p, 0 where q is
+__device__ __forceinline__ double times_log(double q, double l) { return q == 0.0 ? 0.0 : q * l; }
+
+// A workgroup takes a row (kPhase 0), or a segment of one (few rows of many classes): phase 1 leaves the
+// segment's (m, s) of its others, phase 2 reads all of the row's and writes its part of the gradient.
+template <class T, bool kUnit, int THREADS, int kPhase>
+__global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, float c, double it, double t,
+                                                          uint32_t parts, uint32_t seg, float* __restrict__ loss,
+                                                          Grad<T> G, float2* __restrict__ part_ms) {
+    constexpr int V = Pack<T>::V, W = THREADS / 64;
+    constexpr uint32_t kTile = THREADS * V * kUnroll;
+    extern __shared__ uint32_t mark[];   // a bit a class of the segment
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    __shared__ uint32_t tmp_u[W];
+    const uint32_t words = (min(seg, X.classes) + 31) / 32;
+
+    for (uint64_t job = blockIdx.x; job < X.rows * parts; job += gridDim.x) {
+        const uint64_t row = job / parts;
+        const uint32_t first = (uint32_t)(job % parts) * seg, n = min(X.classes - first, seg);
+        const T* x0 = X.data + (int64_t)row * X.rs + (int64_t)first * X.cs;
+        T* g0 = G.data ? G.data + (int64_t)row * G.rs + (int64_t)first * G.cs : nullptr;
+        const float* u = L.scores + row * L.k;
+        const int32_t* ix = L.index + row * L.k;
+        const double w = L.weight ? (double)L.weight[row] : 1.0;
+        if (w == 0.0) {   // (uniform: the whole workgroup)
+            if (kPhase != 1) {
+                if (loss && first == 0 && threadIdx.x == 0) loss[row] = 0.0f;
+                if (g0) {
+                    float z[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) z[v] = 0.0f;
+                    for (uint32_t i = threadIdx.x * V; i < n; i += THREADS * V) store_pack<T, kUnit>(g0, G.cs, i, n, z);
+                }
+            }
+            continue;
+        }
+        Running run;
+        if (kPhase != 2) {
+            for (uint32_t i = threadIdx.x; i < words; i += THREADS) mark[i] = 0;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
+                const uint32_t j = (uint32_t)ix[i] - first;
+                if (j < n) atomicOr(&mark[j >> 5], 1u << (j & 31));
+            }
+            __syncthreads();
+            for (uint32_t base = 0; base < n; base += kTile) {
+                float x[kUnroll][V], tm = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q)
+                    load_pack<T, kUnit>(x0, X.cs, base + (q * THREADS + threadIdx.x) * V, n, -INFINITY, x[q]);
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q) {
+                    const uint32_t i = base + (q * THREADS + threadIdx.x) * V;
+                    const uint32_t bits = i < n ? mark[i >> 5] >> (i & 31) : 0;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        x[q][v] = bits >> v & 1 ? -INFINITY : x[q][v];
+                        tm = fmaxf(tm, x[q][v]);
+                    }
+                }
+                run.raise(tm, c);
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) run.add(x[q][v], c);
+            }
+        } else {
+            for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
+                const float2 ms = part_ms[row * parts + p];
+                run.raise(ms.x, c);
+                run.s += ms.y * exp2_fast((ms.x - run.m) * c);
+            }
+        }
+        float mo;
+        double so;
+        block_running<THREADS>(run, c, mo, so, tmp_f, tmp_d);
+        if (kPhase == 1) {
+            if (threadIdx.x == 0) part_ms[job] = float2{mo, (float)so};
+            continue;
+        }
+        // the list: the teacher's sums, the student's largest listed score
+        RowSums r{};
+        float lmax = kLowest;
+        double umax = -INFINITY;
+        const T* xr = X.data + (int64_t)row * X.rs;
+        uint32_t listed = 0;
+        for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
+            const uint32_t j = (uint32_t)ix[i];
+            if (j >= X.classes) continue;
+            ++listed;
+            umax = fmax(umax, (double)u[i] * it);
+            lmax = fmaxf(lmax, to_f32(xr[(int64_t)j * X.cs]));
+        }
+        r.listed = block_reduce<THREADS>(listed, Add(), tmp_u);
+        const float M = fmaxf(mo, block_reduce<THREADS>(lmax, MaxF(), tmp_f));
+        if (L.lse) {
+            r.base = (double)L.lse[row];
+        } else {
+            umax = block_reduce<THREADS>(umax, MaxF(), tmp_d);
+            double s = 0.0;
+            for (uint32_t i = threadIdx.x; i < L.k; i += THREADS)
+                if ((uint32_t)ix[i] < X.classes) s += exp((double)u[i] * it - umax);
+            r.base = umax;
+            r.base_log = log(block_reduce<THREADS>(s, Add(), tmp_d));
+        }
+        double held = 0.0, entropy = 0.0, sl = 0.0;
+        for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
+            const uint32_t j = (uint32_t)ix[i];
+            if (j >= X.classes) continue;
+            const double lq = log_q(u[i], it, r), q = exp(lq);
+            held += q;
+            entropy += times_log(q, lq);
+            sl += exp(((double)to_f32(xr[(int64_t)j * X.cs]) - (double)M) * it);
+        }
+        r.held = block_reduce<THREADS>(held, Add(), tmp_d);
+        r.entropy = block_reduce<THREADS>(entropy, Add(), tmp_d);
+        sl = block_reduce<THREADS>(sl, Add(), tmp_d);
+        so = so == 0.0 ? 0.0 : so * exp(((double)mo - (double)M) * it);   // (in f64: far below M it must not vanish)
+        const double log_s = log(so + sl);
+        double lin = 0.0;
+        for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
+            const uint32_t j = (uint32_t)ix[i];
+            if (j >= X.classes) continue;
+            const float x = to_f32(xr[(int64_t)j * X.cs]);
+            const double q = exp(log_q(u[i], it, r));
+            lin += times_log(q, x == -INFINITY ? -(double)INFINITY : ((double)x - (double)M) * it - log_s);
+        }
+        lin = block_reduce<THREADS>(lin, Add(), tmp_d);
+        const double rest = row_rest(r, L.lse != nullptr, X.classes);
+        const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
+        if (loss && first == 0 && threadIdx.x == 0) loss[row] = (float)o.loss;
+        if (g0) {
+            for (uint32_t base = 0; base < n; base += kTile) {
+                float x[kUnroll][V];
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q)
+                    load_pack<T, kUnit>(x0, X.cs, base + (q * THREADS + threadIdx.x) * V, n, -INFINITY, x[q]);
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q) {
+                    const uint32_t i = base + (q * THREADS + threadIdx.x) * V;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[q][v] = exp2_fast((x[q][v] - o.M) * c) * o.others;
+                    if (i < n) store_pack<T, kUnit>(g0, G.cs, i, n, x[q]);
+                }
+            }
+            __syncthreads();   // the listed classes are written over
+            for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
+                const uint32_t j = (uint32_t)ix[i];
+                if (j - first >= n) continue;
+                const double p = exp(((double)to_f32(xr[(int64_t)j * X.cs]) - (double)M) * it) * o.inv_s;
+                g0[(int64_t)(j - first) * G.cs] = from_f32<T>((float)(w * t * (p * o.whole - exp(log_q(u[i], it, r)))));
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Few classes: a row a thread, its scores in registers, the listed classes a bit mask.
+template <class T, int NMAX>
+__global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, float c, double it, double t,
+                                                          float* __restrict__ loss, Grad<T> G) {
+    const uint32_t n = X.classes;
+    for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
+        const T* x0 = X.data + (int64_t)row * X.rs;
+        T* g0 = G.data ? G.data + (int64_t)row * G.rs : nullptr;
+        const double w = L.weight ? (double)L.weight[row] : 1.0;
+        if (w == 0.0) {
+            if (loss) loss[row] = 0.0f;
+            if (g0)
+                for (uint32_t j = 0; j < n; ++j) g0[(int64_t)j * G.cs] = from_f32<T>(0.0f);
+            continue;
+        }
+        float x[NMAX], M = kLowest, mo = kLowest;
+#pragma unroll
+        for (int j = 0; j < NMAX; ++j) x[j] = (uint32_t)j < n ? to_f32(x0[(int64_t)j * X.cs]) : -INFINITY;
+        const float* u = L.scores + row * L.k;
+        const int32_t* ix = L.index + row * L.k;
+        uint32_t mask = 0;
+        double umax = -INFINITY;
+        for (uint32_t i = 0; i < L.k; ++i)
+            if ((uint32_t)ix[i] < n) {
+                mask |= 1u << ix[i];
+                umax = fmax(umax, (double)u[i] * it);
+            }
+        RowSums r{};
+        r.listed = (uint32_t)__popc(mask);
+        if (L.lse) {
+            r.base = (double)L.lse[row];
+        } else {
+            double s = 0.0;
+            for (uint32_t i = 0; i < L.k; ++i)
+                if ((uint32_t)ix[i] < n) s += exp((double)u[i] * it - umax);
+            r.base = umax;
+            r.base_log = log(s);
+        }
+#pragma unroll
+        for (int j = 0; j < NMAX; ++j) {
+            M = fmaxf(M, x[j]);
+            mo = fmaxf(mo, mask >> j & 1 ? -INFINITY : x[j]);
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NMAX; ++j) {
+            const float e = exp2_fast((x[j] - mo) * c);
+            s += mask >> j & 1 ? 0.0f : e;
+        }
+        const double so = s == 0.0f ? 0.0 : (double)s * exp(((double)mo - (double)M) * it);
+        double sl = 0.0;
+        for (uint32_t i = 0; i < L.k; ++i)
+            if ((uint32_t)ix[i] < n) sl += exp(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it);
+        const double log_s = log(so + sl);
+        double lin = 0.0;
+        for (uint32_t i = 0; i < L.k; ++i)
+            if ((uint32_t)ix[i] < n) {
+                const double lq = log_q(u[i], it, r), q = exp(lq);
+                const float xl = to_f32(x0[(int64_t)ix[i] * X.cs]);
+                r.held += q;
+                r.entropy += times_log(q, lq);
+                lin += times_log(q, xl == -INFINITY ? -(double)INFINITY : ((double)xl - (double)M) * it - log_s);
+            }
+        const double rest = row_rest(r, L.lse != nullptr, n);
+        const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
+        if (loss) loss[row] = (float)o.loss;
+        if (g0) {
+#pragma unroll
+            for (int j = 0; j < NMAX; ++j)
+                if ((uint32_t)j < n && !(mask >> j & 1))
+                    g0[(int64_t)j * G.cs] = from_f32<T>(exp2_fast((x[j] - o.M) * c) * o.others);
+            for (uint32_t i = 0; i < L.k; ++i)
+                if ((uint32_t)ix[i] < n) {
+                    const double p = exp(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it) * o.inv_s;
+                    g0[(int64_t)ix[i] * G.cs] = from_f32<T>((float)(w * t * (p * o.whole - exp(log_q(u[i], it, r)))));
+                }
+        }
+    }
+}
+
+constexpr uint32_t kMinSeg = 16384;
+uint32_t plan_parts(uint64_t rows, uint32_t classes) {
+    uint32_t parts = (classes + kMaxSeg - 1) / kMaxSeg;
+    if (rows > 0 && rows < 512 && classes >= 2 * kMinSeg)
+        parts = std::max(parts, (uint32_t)std::min<uint64_t>((512 + rows - 1) / rows, classes / kMinSeg));
+    return parts;
+}
+// Segments start at a multiple of 32 classes: a vector's marks lie in one word.
+uint32_t segment(uint32_t classes, uint32_t parts) { return ((classes + parts - 1) / parts + 31) / 32 * 32; }
+
+template <class T, bool kUnit, int THREADS>
+int launch_rows(const Rows<T>& X, const Lists& L, float c, double t, uint32_t parts, float* loss, const Grad<T>& G,
+                void* workspace, hipStream_t st) {
+    const uint32_t seg = segment(X.classes, parts);
+    const unsigned grid = row_grid(X.rows * parts);
+    const size_t lds = 4 * (size_t)((std::min(seg, X.classes) + 31) / 32);
+    float2* ms = (float2*)workspace;
+    const double it = 1.0 / t;
+    if (parts == 1) {
+        distill_kernel<T, kUnit, THREADS, 0><<<grid, THREADS, lds, st>>>(X, L, c, it, t, 1, seg, loss, G, ms);
+    } else {
+        distill_kernel<T, kUnit, THREADS, 1><<<grid, THREADS, lds, st>>>(X, L, c, it, t, parts, seg, loss, G, ms);
+        CLS_TRY(hipGetLastError());
+        distill_kernel<T, kUnit, THREADS, 2><<<grid, THREADS, 0, st>>>(X, L, c, it, t, parts, seg, loss, G, ms);
+    }
+    CLS_TRY(hipGetLastError());
+    return CBH_OK;
+}
+
+template <class T>
+int run_distill(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t cs, const Lists& L, double t,
+                uint32_t parts, float* loss, void* grad, int64_t grs, int64_t gcs, void* workspace, hipStream_t st) {
+    const Rows<T> X{(const T*)scores, rows, n, rs, cs};
+    const Grad<T> G{(T*)grad, grs, gcs};
+    const float c = (float)(1.4426950408889634 / t);
+    if (n <= 32) {
+        const unsigned grid = row_grid((rows + 255) / 256);
+        const double it = 1.0 / t;
+        if (n <= 8) distill_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+        else if (n <= 16) distill_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+        else distill_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+        CLS_TRY(hipGetLastError());
+        return CBH_OK;
+    }
+    const bool unit = cs == 1 && (!grad || gcs == 1);
+    if (n <= 2048)
+        return unit ? launch_rows<T, true, 64>(X, L, c, t, parts, loss, G, workspace, st)
+                    : launch_rows<T, false, 64>(X, L, c, t, parts, loss, G, workspace, st);
+    return unit ? launch_rows<T, true, 256>(X, L, c, t, parts, loss, G, workspace, st)
+                : launch_rows<T, false, 256>(X, L, c, t, parts, loss, G, workspace, st);
+}
+
+}  // namespace
+
+extern "C" uint64_t cbh_distill_gradients_workspace(uint64_t rows, uint32_t classes) {
+    const uint32_t parts = plan_parts(rows, classes);
+    return parts <= 1 ? 0 : rows * parts * 8;
+}
+
+extern "C" int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes,
+                                     int64_t row_stride, int64_t class_stride, const float* top_scores,
+                                     const int32_t* top_index, uint32_t k, const float* top_lse, double temperature,
+                                     const float* weight, float* loss, void* grad, int64_t grad_row_stride,
+                                     int64_t grad_class_stride, void* workspace, uint64_t workspace_bytes,
+                                     void* stream) {
+    try {
+        int rc = check_scores(scores, type, rows, classes, row_stride, class_stride);
+        if (rc != CBH_OK) return rc;
+        if (k < 1 || k > kMaxList) return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "k must be in 1 .. 1024");
+        if (!good_temperature(temperature))
+            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "temperature must be positive and finite");
+        if (rows == 0) return CBH_OK;
+        if (!top_scores || !top_index) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "the teacher's lists are null");
+        if (!loss && !grad) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "loss and grad are both null");
+        if (grad) {
+            rc = check_scores(grad, type, rows, classes, grad_row_stride, grad_class_stride);
+            if (rc != CBH_OK) return rc;
+        }
+        const uint64_t need = cbh_distill_gradients_workspace(rows, classes);
+        if (need > workspace_bytes || (need && (!workspace || (uintptr_t)workspace % 8)))
+            return cbh_internal_fail(CBH_ERR_LENGTH_MISMATCH, "the workspace needs " + std::to_string(need) +
+                                                                  " bytes, aligned to 8");
+        const uint32_t parts = plan_parts(rows, classes);
+        const Lists L{top_scores, top_index, top_lse, weight, k};
+        hipStream_t st = (hipStream_t)stream;
+#define RUN(T) run_distill<T>(scores, rows, classes, row_stride, class_stride, L, temperature, parts, loss, grad, \
+                              grad_row_stride, grad_class_stride, workspace, st)
+        switch (type) {
+            case CBH_TYPE_F32: return RUN(float);
+            case CBH_TYPE_F16: return RUN(_Float16);
+            default: return RUN(bf16_t);
+        }
+#undef RUN
+    } catch (const std::exception& e) {
+        return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
+    }
+}

@@ -1,0 +1,239 @@
+// Shared parts of the operators on class scores (class_top.hip, class_distill.hip,
+// class_sample.hip): reading rows of scores in any of the three types and any strides, keys
+// that order scores, and sums over a wave or a workgroup.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "../../include/cbhip.h"
+
+int cbh_internal_fail(int code, const std::string& msg);  // session.hip
+
+namespace cbh {
+namespace cls {
+
+typedef unsigned long long u64;
+
+constexpr float kLowest = -3.402823466e38f;   // the lowest finite f32
+constexpr uint32_t kMaxClasses = 1u << 24;
+
+// ---- element types: f32, IEEE half, bfloat16 ------------------------------------------------
+struct bf16_t {
+    uint16_t bits;
+};
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float to_f32(bf16_t x) { return __builtin_bit_cast(float, (uint32_t)x.bits << 16); }
+template <class T>
+__device__ __forceinline__ T from_f32(float x);   // round to nearest even
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ _Float16 from_f32<_Float16>(float x) { return (_Float16)x; }
+template <>
+__device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) {
+    return __builtin_bit_cast(bf16_t, (__bf16)x);
+}
+
+// One vector load or store moves 16 bytes; the address needs the element's alignment only (rows of odd
+// length start anywhere).
+template <class T>
+struct Pack {
+    static constexpr int V = 16 / (int)sizeof(T);
+    T v[V];
+};
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    Pack<T> p;
+};
+
+// Scores as the kernels take them.
+template <class T>
+struct Rows {
+    const T* data;
+    uint64_t rows;
+    uint32_t classes;
+    int64_t rs, cs;   // strides in elements
+};
+
+// The V scores from class i on, as f32; classes at n and beyond read as `fill`.
+template <class T, bool kUnit>
+__device__ __forceinline__ void load_pack(const T* row, int64_t cs, uint32_t i, uint32_t n, float fill,
+                                          float (&x)[Pack<T>::V]) {
+    constexpr int V = Pack<T>::V;
+    if (kUnit && i + V <= n) {
+        const Pack<T> p = ((const Loose<T>*)(row + i))->p;
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = to_f32(p.v[v]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            x[v] = i + (uint32_t)v < n ? to_f32(row[kUnit ? (int64_t)(i + v) : (int64_t)(i + v) * cs]) : fill;
+    }
+}
+template <class T, bool kUnit>
+__device__ __forceinline__ void store_pack(T* row, int64_t cs, uint32_t i, uint32_t n, const float (&x)[Pack<T>::V]) {
+    constexpr int V = Pack<T>::V;
+    if (kUnit && i + V <= n) {
+        Pack<T> p;
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.v[v] = from_f32<T>(x[v]);
+        ((Loose<T>*)(row + i))->p = p;
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (i + (uint32_t)v < n) row[kUnit ? (int64_t)(i + v) : (int64_t)(i + v) * cs] = from_f32<T>(x[v]);
+    }
+}
+
+// ---- order of scores ------------------------------------------------------------------------
+// A u32 that orders as the score does: -0 and +0 alike, NaN (of either sign) above +inf.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    x = x + 0.0f;   // -0 -> +0
+    uint32_t u = __builtin_bit_cast(uint32_t, x);
+    u = x != x ? 0x7FC00000u : u;
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+    return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// Larger for the larger score, and for the lower class among equal ones; never 0.
+__device__ __forceinline__ u64 rank_key(float x, uint32_t cls) { return ((u64)order_key(x) << 32) | (uint32_t)~cls; }
+
+// ---- waves and workgroups -------------------------------------------------------------------
+__device__ __forceinline__ uint32_t lane_id() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
+// What the lanes of a wave have written to LDS is seen by its other lanes.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <class V, class Op>
+__device__ __forceinline__ V wave_reduce(V v, Op op) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
+    return v;
+}
+// Reduction over a workgroup, in a fixed order; every thread gets it.  `tmp` holds a value a wave; the
+// call ends with a barrier after which tmp may be used again.
+template <int THREADS, class V, class Op>
+__device__ __forceinline__ V block_reduce(V v, Op op, V* tmp) {
+    v = wave_reduce(v, op);
+    if (THREADS == 64) return v;
+    if (lane_id() == 0) tmp[threadIdx.x / 64] = v;
+    __syncthreads();
+    V r = tmp[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) r = op(r, tmp[w]);
+    __syncthreads();
+    return r;
+}
+struct Add {
+    template <class V>
+    __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct MaxF {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
+};
+
+// Where a sum over 256 bins in LDS, taken from bin 255 down, reaches `want`: the bin, what lies above it
+// and what it holds (the lowest non-zero place if the sum stays below).  Every wave finds it by itself: lane l
+// holds bins 255 - 4 l .. 252 - 4 l.  (Walked bin by bin with wave-uniform 64-bit sums, hipcc 7.2 selected
+// the next sum by a stale condition code.)
+template <class V>
+struct Found {
+    uint32_t bin;
+    V above, inside;
+};
+template <class V>
+__device__ __forceinline__ Found<V> find_bin(const V* hist, V want) {
+    const uint32_t l = lane_id();
+    V c[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        c[j] = hist[255 - 4 * l - j];
+        sum += c[j];
+    }
+    V upto = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const V v = __shfl_up(upto, o);
+        if (l >= (uint32_t)o) upto += v;
+    }
+    V above = upto - sum, inside = c[0];
+    uint32_t b = 255 - 4 * l;
+    const u64 cross = __ballot(upto >= want);
+    const int at = cross ? __builtin_ctzll(cross) : 63;
+#pragma unroll
+    for (int j = 1; j < 4; ++j)
+        if (above + inside < want) {
+            above += inside;
+            inside = c[j];
+            --b;
+        }
+    return Found<V>{(uint32_t)__shfl(b, at), __shfl(above, at), __shfl(inside, at)};
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A running softmax denominator: sum over the scores seen of 2^((x - m) c), c = log2(e) / temperature.
+// m starts at the lowest finite value, so that a score of -inf adds 0 and a row of nothing else
+// keeps s = 0; a NaN, or a score of +inf (inf - inf), leaves NaN in s.  The difference is taken before
+// the product: the product's rounding then counts against x - m, which is small for the scores
+// that matter, and not against x.
+struct Running {
+    float m = kLowest, s = 0.0f;
+    __device__ __forceinline__ void raise(float to, float c) {
+        if (to > m) {
+            s *= exp2_fast((m - to) * c);
+            m = to;
+        }
+    }
+    __device__ __forceinline__ void add(float x, float c) { s += exp2_fast((x - m) * c); }
+};
+// (m, s) pairs of several threads together: the largest m, and the sums in f64.
+template <int THREADS>
+__device__ __forceinline__ void block_running(Running r, float c, float& m, double& s, float* tmp_f, double* tmp_d) {
+    m = block_reduce<THREADS>(r.m, MaxF(), tmp_f);
+    s = block_reduce<THREADS>((double)(r.s * exp2_fast((r.m - m) * c)), Add(), tmp_d);
+}
+
+// ---- host -----------------------------------------------------------------------------------
+#define CLS_TRY(expr)                                                                            \
+    do {                                                                                         \
+        hipError_t e_ = (expr);                                                                  \
+        if (e_ != hipSuccess)                                                                    \
+            return cbh_internal_fail(CBH_ERR_DEVICE, std::string(#expr ": ") + hipGetErrorString(e_)); \
+    } while (0)
+
+inline size_t type_bytes(int32_t type) { return type == CBH_TYPE_F32 ? 4 : 2; }
+
+// What every operator asks of its scores.
+inline int check_scores(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                        int64_t class_stride) {
+    if (type != CBH_TYPE_F32 && type != CBH_TYPE_F16 && type != CBH_TYPE_BF16)
+        return cbh_internal_fail(CBH_ERR_UNSUPPORTED, "scores are f32, f16 or bf16");
+    if (rows > 0x7FFFFFFFull) return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "more than 2^31 - 1 rows");
+    if (classes == 0 || classes > kMaxClasses)
+        return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "classes must be in 1 .. 2^24");
+    if (rows && !scores) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "scores are null");
+    if ((uintptr_t)scores % type_bytes(type))
+        return cbh_internal_fail(CBH_ERR_INVALID_ARG, "scores are not aligned to their type");
+    const double lim = 4.0e18 / (double)type_bytes(type);
+    if (std::abs((double)row_stride) * (double)rows + std::abs((double)class_stride) * (double)classes > lim)
+        return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "strides pass the address range");
+    return CBH_OK;
+}
+inline bool good_temperature(double t) { return t > 0.0 && std::isfinite(t) && std::isfinite(1.0 / t); }
+
+// The grid of a kernel whose workgroups walk over the rows: a launch holds fewer than 2^32 threads.
+inline unsigned row_grid(uint64_t blocks) { return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(blocks, 1u << 20)); }
+
+}  // namespace cls
+}  // namespace cbh

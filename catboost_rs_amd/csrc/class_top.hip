@@ -1,0 +1,400 @@
+// Top classes: the k largest scores of a row, ties to the lowest class, and the row's
+// log-sum-exp at a temperature, in one pass over the scores.
+//
+//   values[r][i], index[r][i]   the i-th largest score of row r and its class
+//   lse[r] = log sum_j exp(x_rj / temperature)
+//
+// What has to be read is the scores; a row's candidates live in LDS.  A wave keeps those of its
+// scores that can still be among the k largest (`Candidates`); a score is compared with the bound as an
+// f32 in a register, so that most scores cost one comparison beside the log-sum-exp's
+// subtraction, exponential and sum.
+#include "class_scores.hpp"
+
+namespace {
+using namespace cbh::cls;
+
+constexpr uint32_t kMaxTop = 1024;
+constexpr int kUnroll = 4;   // 16-byte loads a thread has in flight
+
+// The k-th largest of the keys get(0 .. n - 1) (0: no key; at least k are not 0), or any bound that
+// exactly k keys reach, by bytes from the top; `stop`: the lowest bit looked at.  All threads call it and get
+// the same value.  hist: 256 words of LDS.
+template <int THREADS, class Get>
+__device__ u64 block_kth(Get get, uint32_t n, uint32_t k, int stop, uint32_t* hist) {
+    u64 prefix = 0;
+    uint32_t need = k;
+    for (int shift = 56; shift >= stop; shift -= 8) {
+        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) hist[b] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+            const u64 key = get(i);
+            if (key != 0 && (shift == 56 || (key >> (shift + 8)) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        const Found<uint32_t> f = find_bin(hist, need);
+        prefix = (prefix << 8) | f.bin;
+        need -= f.above;
+        __syncthreads();
+        if (f.inside == need) return prefix << shift;
+    }
+    return prefix << (stop < 0 ? 0 : stop);
+}
+
+// One wave's candidates, CAP of them in LDS: the keys above `bound` that it has met.  Full, the wave
+// keeps the k largest and raises the bound to the smallest of them.
+template <int CAP>
+struct Candidates {
+    u64* keys;
+    uint32_t count;   // wave-uniform
+    u64 bound;        // keys at or below it are not among the k largest
+    float fbound;     // no score below it passes (NaN: all pass)
+    __device__ __forceinline__ void set_bound(u64 b) {
+        if (b > bound) {
+            bound = b;
+            fbound = key_score((uint32_t)(b >> 32));
+        }
+    }
+    __device__ __forceinline__ void compact(uint32_t k) {
+        constexpr int R = CAP / 64;
+        wave_fence();
+        const uint32_t l = lane_id();
+        u64 key[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint32_t i = r * 64 + l;
+            key[r] = i < count ? keys[i] : 0;
+        }
+        u64 kth = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const u64 t = kth | (1ull << bit);
+            uint32_t c = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) c += (uint32_t)__popcll(__ballot(key[r] >= t));
+            if (c >= k) kth = t;
+            if (c == k) break;
+        }
+        uint32_t kept = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const u64 b = __ballot(key[r] >= kth);
+            if (key[r] >= kth) keys[kept + (uint32_t)__popcll(b & ((1ull << l) - 1))] = key[r];
+            kept += (uint32_t)__popcll(b);
+        }
+        count = kept;
+        wave_fence();
+        set_bound(kth - 1);   // (the smallest kept key is in; a key equal to it does not come again)
+    }
+    // x: this lane's score of class cls, or no score
+    __device__ __forceinline__ void offer(float x, uint32_t cls, bool have, uint32_t k) {
+        const u64 key = rank_key(x, cls);
+        bool in = have && key > bound;
+        u64 b = __ballot(in);
+        if (!b) return;
+        if (count + (uint32_t)__popcll(b) > (uint32_t)CAP) {
+            compact(k);
+            in = in && key > bound;
+            b = __ballot(in);
+        }
+        if (in) keys[count + (uint32_t)__popcll(b & ((1ull << lane_id()) - 1))] = key;
+        count += (uint32_t)__popcll(b);
+    }
+};
+
+// A workgroup takes a row, or one of the `parts` segments of `seg` classes of a row (few rows of many
+// classes), whose k largest keys and (m, s) go to the workspace for merge_kernel.
+template <class T, bool kUnit, int THREADS, int CAP>
+__global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, float c, double inv_t, uint32_t parts,
+                                                      uint32_t seg, float* __restrict__ values,
+                                                      int32_t* __restrict__ index, float* __restrict__ lse,
+                                                      u64* __restrict__ part_keys, float2* __restrict__ part_ms) {
+    constexpr int V = Pack<T>::V, W = THREADS / 64, KMAX = CAP / 2;
+    constexpr uint32_t kTile = THREADS * V * kUnroll;
+    __shared__ u64 cand[W][CAP];
+    __shared__ u64 best[KMAX];
+    __shared__ uint32_t vmax[THREADS * kUnroll];
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t counts[W], nbest;
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    auto cand_at = [&](uint32_t i) -> u64 { return i % CAP < counts[i / CAP] ? cand[i / CAP][i % CAP] : 0; };
+
+    for (uint64_t job = blockIdx.x; job < X.rows * parts; job += gridDim.x) {
+        const uint64_t row = job / parts;
+        const uint32_t first = (uint32_t)(job % parts) * seg, n = min(X.classes - first, seg);
+        const T* x0 = X.data + (int64_t)row * X.rs + (int64_t)first * X.cs;
+        Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
+        Running run;
+        for (uint32_t base = 0; base < n; base += kTile) {
+            float x[kUnroll][V];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                load_pack<T, kUnit>(x0, X.cs, base + (u * THREADS + threadIdx.x) * V, n, -INFINITY, x[u]);
+            float vm[kUnroll], tm = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                vm[u] = x[u][0];
+#pragma unroll
+                for (int v = 1; v < V; ++v) vm[u] = fmaxf(vm[u], x[u][v]);
+                tm = fmaxf(tm, vm[u]);
+            }
+            run.raise(tm, c);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) run.add(x[u][v], c);
+            if (base == 0) {
+                // the first bound: k of the tile's vectors hold a score that reaches the k-th largest of
+                // their maxima
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    const uint32_t i = (u * THREADS + threadIdx.x);
+                    vmax[i] = i * V < n ? order_key(vm[u]) : 0;
+                }
+                __syncthreads();
+                const uint32_t vecs = min((uint32_t)(THREADS * kUnroll), (n + V - 1) / V);
+                if (k <= vecs)
+                    C.set_bound(block_kth<THREADS>([&](uint32_t i) { return (u64)vmax[i] << 32; }, vecs, k, 32, hist));
+            } else if (base == kTile || base == 3 * kTile) {
+                // the candidates of the first tiles give a better one
+                if ((threadIdx.x & 63) == 0) counts[wave] = C.count;
+                __syncthreads();
+                uint32_t total = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) total += counts[w];
+                if (total >= k) {
+                    const u64 kth = block_kth<THREADS>(cand_at, W * CAP, k, 0, hist);
+                    C.set_bound(kth - 1);
+                }
+                __syncthreads();
+            }
+            // vectors that hold a score at the bound or above (NaN: somewhere in this thread's scores) are
+            // read again, score by score
+            uint32_t vecs = 0;
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) vecs |= (uint32_t)!(vm[u] < C.fbound) << u;
+            if (run.s != run.s) vecs = (1u << kUnroll) - 1;
+            while (__any(vecs != 0)) {
+                const uint32_t u = vecs ? (uint32_t)__builtin_ctz(vecs) : 0;
+                const uint32_t i0 = base + (u * THREADS + threadIdx.x) * V;
+                float y[V];
+                load_pack<T, kUnit>(x0, X.cs, i0, vecs ? n : 0, -INFINITY, y);
+                uint32_t hits = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) hits |= (uint32_t)(i0 + v < n && !(y[v] < C.fbound)) << v;
+                if (!vecs) hits = 0;
+                while (__any(hits != 0)) {
+                    const uint32_t v = hits ? (uint32_t)__builtin_ctz(hits) : 0;
+                    float z = y[0];
+#pragma unroll
+                    for (int q = 1; q < V; ++q) z = v == (uint32_t)q ? y[q] : z;
+                    C.offer(z, first + i0 + v, hits != 0, k);
+                    hits &= hits - 1;
+                }
+                vecs &= vecs - 1;
+            }
+        }
+        if ((threadIdx.x & 63) == 0) counts[wave] = C.count;
+        if (threadIdx.x == 0) nbest = 0;
+        float m;
+        double s;
+        __syncthreads();
+        block_running<THREADS>(run, c, m, s, tmp_f, tmp_d);
+        uint32_t total = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) total += counts[w];
+        u64 kth = 1;
+        if (total > k) kth = block_kth<THREADS>(cand_at, W * CAP, k, 0, hist);
+        for (uint32_t i = threadIdx.x; i < W * CAP; i += THREADS) {
+            const u64 key = cand_at(i);
+            if (key >= kth) best[atomicAdd(&nbest, 1u)] = key;
+        }
+        __syncthreads();
+        const uint32_t got = nbest;   // k, or all of a segment of fewer
+        if (parts == 1) {
+            for (uint32_t i = threadIdx.x; i < got; i += THREADS) {
+                const u64 key = best[i];
+                uint32_t rank = 0;
+                for (uint32_t j = 0; j < got; ++j) rank += best[j] > key;
+                values[row * k + rank] = key_score((uint32_t)(key >> 32));
+                index[row * k + rank] = (int32_t)~(uint32_t)key;
+            }
+            if (threadIdx.x == 0) lse[row] = m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(s));
+        } else {
+            for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = i < got ? best[i] : 0;
+            if (threadIdx.x == 0) part_ms[job] = float2{m, (float)s};
+        }
+        __syncthreads();
+    }
+}
+
+// The segments of a row together.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ part_keys,
+                                                        const float2* __restrict__ part_ms, uint32_t parts, uint32_t k,
+                                                        float c, double inv_t, float* __restrict__ values,
+                                                        int32_t* __restrict__ index, float* __restrict__ lse) {
+    __shared__ u64 best[kMaxTop];
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t nbest;
+    __shared__ float tmp_f[THREADS / 64];
+    __shared__ double tmp_d[THREADS / 64];
+    const uint64_t row = blockIdx.x;
+    const u64* keys = part_keys + row * parts * k;
+    if (threadIdx.x == 0) nbest = 0;
+    Running run;
+    for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
+        const float2 ms = part_ms[row * parts + p];
+        run.raise(ms.x, c);
+        run.s += ms.y * exp2_fast((ms.x - run.m) * c);
+    }
+    float m;
+    double s;
+    __syncthreads();
+    block_running<THREADS>(run, c, m, s, tmp_f, tmp_d);
+    const u64 kth = block_kth<THREADS>([&](uint32_t i) { return keys[i]; }, parts * k, k, 0, hist);
+    for (uint32_t i = threadIdx.x; i < parts * k; i += THREADS) {
+        const u64 key = keys[i];
+        if (key != 0 && key >= kth) best[atomicAdd(&nbest, 1u)] = key;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
+        const u64 key = best[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < k; ++j) rank += best[j] > key;
+        values[row * k + rank] = key_score((uint32_t)(key >> 32));
+        index[row * k + rank] = (int32_t)~(uint32_t)key;
+    }
+    if (threadIdx.x == 0) lse[row] = m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(s));
+}
+
+// Few classes: a row a thread, its scores in registers; a score's place is the count of those ahead.
+template <class T, int NMAX>
+__global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, float c, double inv_t,
+                                                      float* __restrict__ values, int32_t* __restrict__ index,
+                                                      float* __restrict__ lse) {
+    const uint32_t n = X.classes;
+    for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
+        const T* x0 = X.data + (int64_t)row * X.rs;
+        float x[NMAX];
+        uint32_t key[NMAX], rank[NMAX];
+        Running run;
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) {
+            x[i] = (uint32_t)i < n ? to_f32(x0[(int64_t)i * X.cs]) : -INFINITY;
+            key[i] = (uint32_t)i < n ? order_key(x[i]) : 0;
+            rank[i] = 0;
+            run.m = fmaxf(run.m, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) {
+            run.add(x[i], c);
+#pragma unroll
+            for (int j = 0; j < i; ++j) {
+                const bool ahead = key[j] >= key[i];
+                rank[i] += ahead;
+                rank[j] += !ahead;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i)
+            if ((uint32_t)i < n && rank[i] < k) {
+                values[row * k + rank[i]] = key_score(key[i]);
+                index[row * k + rank[i]] = i;
+            }
+        lse[row] = run.m == INFINITY ? INFINITY : (float)((double)run.m * inv_t + log((double)run.s));
+    }
+}
+
+// Segments of a row: one, unless the rows alone leave CUs idle and a row is long.
+constexpr uint32_t kMinSeg = 16384;
+uint32_t plan_parts(uint64_t rows, uint32_t classes) {
+    if (rows == 0 || rows >= 512 || classes < 2 * kMinSeg) return 1;
+    return (uint32_t)std::min<uint64_t>((512 + rows - 1) / rows, classes / kMinSeg);
+}
+
+template <class T, bool kUnit>
+int launch_top(const Rows<T>& X, uint32_t k, double t, float* values, int32_t* index, float* lse, uint32_t parts,
+               void* workspace, hipStream_t st) {
+    const float c = (float)(1.4426950408889634 / t);
+    const double it = 1.0 / t;
+    const uint32_t n = X.classes;
+    if (n <= 32) {
+        const unsigned grid = row_grid((X.rows + 255) / 256);
+        if (n <= 8) top_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, k, c, it, values, index, lse);
+        else if (n <= 16) top_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, k, c, it, values, index, lse);
+        else top_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, k, c, it, values, index, lse);
+        CLS_TRY(hipGetLastError());
+        return CBH_OK;
+    }
+    const uint32_t seg = (n + parts - 1) / parts;
+    u64* pk = (u64*)workspace;
+    float2* pm = parts > 1 ? (float2*)(pk + X.rows * parts * k) : nullptr;
+    const unsigned grid = row_grid(X.rows * parts);
+#define TOP(TH, CAP) top_kernel<T, kUnit, TH, CAP><<<grid, TH, 0, st>>>(X, k, c, it, parts, seg, values, index, lse, pk, pm)
+    if (n <= 2048) {
+        if (k <= 128) TOP(64, 256);
+        else if (k <= 256) TOP(64, 512);
+        else TOP(64, 2048);
+    } else {
+        if (k <= 128) TOP(256, 256);
+        else if (k <= 256) TOP(256, 512);
+        else TOP(256, 2048);
+    }
+#undef TOP
+    CLS_TRY(hipGetLastError());
+    if (parts > 1) {
+        merge_kernel<256><<<(unsigned)X.rows, 256, 0, st>>>(pk, pm, parts, k, c, it, values, index, lse);
+        CLS_TRY(hipGetLastError());
+    }
+    return CBH_OK;
+}
+
+template <class T>
+int run_top(const void* scores, uint64_t rows, uint32_t classes, int64_t rs, int64_t cs, uint32_t k, double t,
+            float* values, int32_t* index, float* lse, uint32_t parts, void* workspace, hipStream_t st) {
+    const Rows<T> X{(const T*)scores, rows, classes, rs, cs};
+    return cs == 1 ? launch_top<T, true>(X, k, t, values, index, lse, parts, workspace, st)
+                   : launch_top<T, false>(X, k, t, values, index, lse, parts, workspace, st);
+}
+
+}  // namespace
+
+extern "C" uint64_t cbh_top_classes_workspace(uint64_t rows, uint32_t classes, uint32_t k) {
+    const uint32_t parts = plan_parts(rows, classes);
+    return parts == 1 ? 0 : rows * parts * (8 * (uint64_t)k + 8);
+}
+
+extern "C" int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                               int64_t class_stride, uint32_t k, double temperature, float* values, int32_t* index,
+                               float* lse, void* workspace, uint64_t workspace_bytes, void* stream) {
+    try {
+        const int rc = check_scores(scores, type, rows, classes, row_stride, class_stride);
+        if (rc != CBH_OK) return rc;
+        if (k < 1 || k > classes || k > kMaxTop)
+            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "k must be in 1 .. min(classes, 1024)");
+        if (!good_temperature(temperature))
+            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "temperature must be positive and finite");
+        if (rows == 0) return CBH_OK;
+        if (!values || !index || !lse) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "outputs are null");
+        const uint64_t need = cbh_top_classes_workspace(rows, classes, k);
+        if (need > workspace_bytes || (need && (!workspace || (uintptr_t)workspace % 8)))
+            return cbh_internal_fail(CBH_ERR_LENGTH_MISMATCH, "the workspace needs " + std::to_string(need) +
+                                                                  " bytes, aligned to 8");
+        const uint32_t parts = plan_parts(rows, classes);
+        hipStream_t st = (hipStream_t)stream;
+        switch (type) {
+            case CBH_TYPE_F32:
+                return run_top<float>(scores, rows, classes, row_stride, class_stride, k, temperature, values, index,
+                                      lse, parts, workspace, st);
+            case CBH_TYPE_F16:
+                return run_top<_Float16>(scores, rows, classes, row_stride, class_stride, k, temperature, values,
+                                         index, lse, parts, workspace, st);
+            default:
+                return run_top<bf16_t>(scores, rows, classes, row_stride, class_stride, k, temperature, values, index,
+                                       lse, parts, workspace, st);
+        }
+    } catch (const std::exception& e) {
+        return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
+    }
+}

@@ -471,6 +471,78 @@ int cbh_ctr_columns(const uint32_t* buckets, uint32_t n_buckets, uint64_t n, con
                     uint32_t border_count, uint8_t* bins_out, double* values_out,
                     uint32_t* class_counts_out);
 
+/* ---- class scores: top classes, distillation, drawn classes (no counterpart in the reference) ----
+ *
+ * Operators on a matrix of class scores (the raw approximant of a MultiClass model, or any other
+ * classifier's logits).  All pointers are DEVICE pointers; the work is enqueued on `stream` (a
+ * hipStream_t, NULL = the default stream) and not waited for; nothing is allocated, so the calls may be
+ * captured into a graph.
+ *   scores         score of row r, class j at scores[r * row_stride + j * class_stride], of `type`; strides
+ *                  in elements (class_stride 1: a row's classes next to each other; row_stride 1: the
+ *                  [classes][rows] layout of cbh_session_read_approx and cbh_apply_oblivious)
+ *   rows, classes  0 <= rows < 2^31 (no rows: nothing is done), 1 <= classes <= 2^24
+ *   workspace      device memory of at least cbh_*_workspace() bytes, aligned to 8; its content is not
+ *                  kept.  NULL where that is 0.
+ * Arithmetic is f32 or wider whatever the type; results do not depend on the order of execution. */
+enum { CBH_TYPE_F32 = 0, CBH_TYPE_F16 = 1, CBH_TYPE_BF16 = 2 };
+
+/* The k largest scores of every row, largest first, the lowest class first among equal ones, and the row's
+ * log-sum-exp of scores / temperature (temperature > 0):
+ *   values [rows][k] f32, index [rows][k], lse [rows] f32;  1 <= k <= min(classes, 1024)
+ * -0 and +0 are equal (and come back as 0); NaN counts as larger than +inf and makes the row's lse NaN; a
+ * row of -inf alone has lse = -inf. */
+uint64_t cbh_top_classes_workspace(uint64_t rows, uint32_t classes, uint32_t k);
+int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                    int64_t class_stride, uint32_t k, double temperature, float* values, int32_t* index,
+                    float* lse, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Distillation of a student's scores x from a teacher's top classes: loss and its gradient in one call.
+ * With t = temperature, p = softmax(x / t), u_i = top_scores[r][i] the teacher's score of class
+ * top_index[r][i], and q_i = exp(u_i / t - top_lse[r]) (the teacher's probability, top_lse its log-sum-exp
+ * at t; NULL: over the listed classes alone, which then hold the whole mass):
+ *   rest  = max(0, 1 - sum q) when top_lse is given and a class is not listed, else 0
+ *   loss  = weight t^2 (sum_i q_i (log q_i - log p_i) + rest (log rest - log(sum of the other p)))
+ *   grad  = d loss / d x, of the scores' type:
+ *             weight t (p_j (sum q + rest) - q_j)                          listed j
+ *             weight t p_j (sum q + rest - rest / (sum of the other p))    other j
+ *   top_scores, top_index  [rows][k], 1 <= k <= 1024.  An index outside [0, classes) is no entry (a list
+ *                  shorter than k); a class listed twice in a row gives an undefined result for that row.
+ *   weight         nullable [rows]; a row of weight 0 gives 0 whatever its scores hold
+ *   loss           nullable [rows] f32; grad nullable, with strides of its own (not both null)
+ * A teacher's entry of -inf has q = 0.  A student's row of -inf alone has p = 0 everywhere and an
+ * infinite loss; NaN or +inf in a student's row makes that row's loss and gradient NaN. */
+uint64_t cbh_distill_gradients_workspace(uint64_t rows, uint32_t classes);
+int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                          int64_t class_stride, const float* top_scores, const int32_t* top_index, uint32_t k,
+                          const float* top_lse, double temperature, const float* weight, float* loss, void* grad,
+                          int64_t grad_row_stride, int64_t grad_class_stride, void* workspace,
+                          uint64_t workspace_bytes, void* stream);
+
+/* One class drawn from every row, from a given uniform number.  With w_j = exp((x_j - max x) / temperature)
+ * over the allowed classes, ordered by score (largest first, the lowest class first among equal ones):
+ *   top_k   > 0: the first top_k classes stay (0, or classes and more: all)
+ *   top_p   < 1: of those, a class stays while the mass ahead of it is below top_p of their mass
+ *   min_p      : of those, the classes with w >= min_p stay
+ * The first class always stays; classes of -inf, NaN, or a bit that is 0 are never drawn.  index[r] is the
+ * first class, in the order of the classes, whose running kept mass exceeds uniform[r] times the whole kept
+ * mass; logprob[r] its log probability before the cuts, (x - max x) / temperature - log sum w.  With
+ * temperature <= 0 the first class is drawn, with logprob 0.  A row that allows no class has index -1 and
+ * logprob -inf.
+ * Masses are integers in units of 2^-51 of the row's largest weight (2^-(62 - b) beyond 2^b = 2^11
+ * classes), so that sums are exact and the same for every launch shape.
+ *   uniform        [rows] f64 in [0, 1)
+ *   temperature, top_k, top_p, min_p   values for every row; *_rows: nullable [rows], used in their place
+ *   allowed        nullable; bit j & 31 of word allowed[r * allowed_stride + (j >> 5)] allows class j of row r
+ *                  (allowed_stride 0: one list for all rows)
+ *   index [rows] i32, logprob nullable [rows] f32 */
+uint64_t cbh_sample_classes_workspace(uint64_t rows, uint32_t classes);
+int cbh_sample_classes(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                       int64_t class_stride, const double* uniform, double temperature,
+                       const float* temperature_rows, uint32_t top_k, const int32_t* top_k_rows, double top_p,
+                       const float* top_p_rows, double min_p, const float* min_p_rows, const uint32_t* allowed,
+                       int64_t allowed_stride, int32_t* index, float* logprob, void* workspace,
+                       uint64_t workspace_bytes, void* stream);
+
 /* Version / build information. */
 const char* cbh_version(void);
 const char* cbh_last_error(void);
