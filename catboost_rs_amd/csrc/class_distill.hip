@@ -125,16 +125,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
                     }
                 }
                 run.raise(tm, c);
-#pragma unroll
-                for (int q = 0; q < kUnroll; ++q)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) run.add(x[q][v], c);
+                run.add(x, c);
             }
         } else {
             for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
                 const float2 ms = part_ms[row * parts + p];
-                run.raise(ms.x, c);
-                run.s += ms.y * exp2_fast((ms.x - run.m) * c);
+                run.join(ms.x, ms.y, c);
             }
         }
         float mo;

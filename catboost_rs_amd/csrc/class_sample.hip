@@ -44,14 +44,34 @@ __device__ __forceinline__ Row settings(const Settings& S, uint64_t row, uint32_
 __device__ __forceinline__ uint32_t class_key(float x, bool allowed) {
     return allowed && x > -INFINITY ? order_key(x) : 0;
 }
-// The weight of a score in [0, 1], and its mass in units of 2^-S: S <= 51, the product with 2^S is
-// rounded to an integer by the addition of 2^52.
-__device__ __forceinline__ double weight_of(float x, float m, double rt) {
-    return x == m ? 1.0 : exp(((double)x - (double)m) * rt);
+// 2^f for |f| <= 1/2: the terms (f ln 2)^i / i! up to i = 11 (what is left out is below 2^-47).
+__device__ __forceinline__ double exp2_part(double f) {
+    double p = 4.4455382718708116e-10;
+    p = __builtin_fma(p, f, 7.0549116208011235e-09);
+    p = __builtin_fma(p, f, 1.0178086009239699e-07);
+    p = __builtin_fma(p, f, 1.3215486790144307e-06);
+    p = __builtin_fma(p, f, 1.5252733804059841e-05);
+    p = __builtin_fma(p, f, 1.5403530393381609e-04);
+    p = __builtin_fma(p, f, 1.3333558146428443e-03);
+    p = __builtin_fma(p, f, 9.6181291076284772e-03);
+    p = __builtin_fma(p, f, 5.5504108664821580e-02);
+    p = __builtin_fma(p, f, 2.4022650695910071e-01);
+    p = __builtin_fma(p, f, 6.9314718055994531e-01);
+    return __builtin_fma(p, f, 1.0);
 }
-__device__ __forceinline__ u64 mass_of(double w, double unit) {
-    return __builtin_bit_cast(u64, __builtin_fma(w, unit, 4503599627370496.0)) - 0x4330000000000000ull;
-}
+// The mass of a score: 2^((x - m) c) in units of 2^-S, rounded to an integer by the addition of 2^52
+// (S <= 51).  -inf and NaN have none (the maximum with a number drops NaN).  m is finite.
+struct Masses {
+    double m, c;   // largest score, log2(e) / temperature
+    int S;
+    __device__ __forceinline__ u64 raw(float x) const {   // the mass plus kRaw
+        const double y = fmax(((double)x - m) * c, -1100.0);
+        const double k = rint(y);
+        return __builtin_bit_cast(u64, ldexp(exp2_part(y - k), (int)k + S) + 4503599627370496.0);
+    }
+    static constexpr u64 kRaw = 0x4330000000000000ull;
+    __device__ __forceinline__ u64 operator()(float x) const { return raw(x) - kRaw; }
+};
 // floor(u total), below total
 __device__ __forceinline__ u64 target_of(double u, u64 total) {
     const double d = u * (double)total;
@@ -64,198 +84,777 @@ __device__ __forceinline__ u64 nucleus_of(double p, u64 total) {
     const u64 v = d > 0.0 ? (u64)d : 0;
     return v < 1 ? 1 : v > total ? total : v;
 }
+// the mass of a weight of min_p (0 and NaN: none)
+__device__ __forceinline__ u64 least_mass(double min_p, int S) {
+    return min_p > 0.0 ? (u64)ceil(ldexp(min_p, S)) : 0;
+}
 
-struct Cut {   // kept: classes with a larger key, and the first `ties` with this one
-    uint32_t key, ties;
-    u64 mass;   // kept mass
+
+// ---- selection among entries in registers -----------------------------------------------------
+struct SelectLds {
+    u64 mass[256];
+    uint32_t count[256];
+};
+struct Crossing {
+    u64 prefix;   // the crossing entry's rank without its low `shift` bits
+    int shift;
 };
 
-// A workgroup a row.
-template <class T, int THREADS>
-struct Walk {
-    static constexpr int W = THREADS / 64;
-    const T* x0;
-    int64_t cs;
-    uint32_t n;
-    Row r;
-    float m;
-    double unit;
-    __device__ __forceinline__ float score(uint32_t i) const { return to_f32(x0[(int64_t)i * cs]); }
-    __device__ __forceinline__ uint32_t key(uint32_t i, float x) const {
-        return class_key(x, !r.allowed || (r.allowed[i >> 5] >> (i & 31) & 1));
-    }
-    __device__ __forceinline__ u64 mass(float x) const { return mass_of(weight_of(x, m, r.rt), unit); }
-
-    // The shortest prefix of the order that holds `count` classes (by_mass false) or a mass of `want`;
-    // keys below `floor` are no candidates.  By bytes of the key from the top.
-    __device__ Cut select(bool by_mass, u64 want, uint32_t floor, uint32_t* hist, u64* hist_mass) const {
-        uint32_t prefix = 0;
-        u64 above = 0, above_mass = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (uint32_t b = threadIdx.x; b < 256; b += THREADS) {
-                hist[b] = 0;
-                hist_mass[b] = 0;
-            }
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const float x = score(i);
-                const uint32_t q = key(i, x);
-                if (q == 0 || q < floor || (shift < 24 && (q >> (shift + 8)) != prefix)) continue;
-                atomicAdd(&hist[q >> shift & 255], 1u);
-                atomicAdd(&hist_mass[q >> shift & 255], mass(x));
-            }
-            __syncthreads();
-            uint32_t bin;
-            if (by_mass) {
-                const Found<u64> f = find_bin(hist_mass, want - above_mass);
-                bin = f.bin;
-                above_mass += f.above;
-            } else {
-                const Found<uint32_t> f = find_bin(hist, (uint32_t)(want - above));
-                bin = f.bin;
-                above += f.above;
-                u64 m = 0;
-                for (uint32_t b = lane_id(); b < 256; b += 64) m += b > bin ? hist_mass[b] : 0;
-                above_mass += wave_reduce(m, Add());
-            }
-            prefix = prefix << 8 | bin;
-            if (shift == 0) {
-                const uint32_t ties = hist[bin];
-                const u64 each = ties ? hist_mass[bin] / ties : 0;
-                u64 need = want - (by_mass ? above_mass : above);
-                if (by_mass) need = each ? (need + each - 1) / each : ties;
-                Cut c;
-                c.key = prefix;
-                c.ties = (uint32_t)(need < ties ? need : ties);
-                c.mass = above_mass + (u64)c.ties * each;
-                __syncthreads();
-                return c;
-            }
-            __syncthreads();
+// Entries have ranks (64 bits, their bits at top_shift + 8 and above all equal) and weights: 1, or their mass.
+// Taken from the largest rank down, where do the weights reach `want` (at most their sum)?  By bytes of
+// the rank; done as soon as one entry is left, or (kWhole) the ones left are all needed.
+template <int THREADS, bool kMass, bool kWhole, class ForEach>
+__device__ Crossing select(ForEach for_each, u64 want, int top_shift, SelectLds* lds) {
+    u64 prefix = 0;
+    for (int shift = top_shift; ; shift -= 8) {
+        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) {
+            lds->count[b] = 0;
+            if (kMass) lds->mass[b] = 0;
         }
-        return Cut{};
+        __syncthreads();
+        for_each([&](u64 rank, u64 mass) {
+            if (shift != top_shift && (rank >> shift >> 8) != prefix) return;
+            atomicAdd(&lds->count[rank >> shift & 255], 1u);
+            if (kMass) atomicAdd(&lds->mass[rank >> shift & 255], mass);
+        });
+        __syncthreads();
+        bool done;
+        if (kMass) {
+            const Found<u64> f = find_bin(lds->mass, want);
+            prefix = shift == top_shift ? f.bin : prefix << 8 | f.bin;
+            want -= f.above;
+            done = lds->count[f.bin] <= 1 || (kWhole && f.inside == want);
+        } else {
+            const Found<uint32_t> f = find_bin(lds->count, (uint32_t)want);
+            prefix = shift == top_shift ? f.bin : prefix << 8 | f.bin;
+            want -= f.above;
+            done = f.inside <= 1 || (kWhole && f.inside == want);
+        }
+        done = __builtin_amdgcn_readfirstlane((uint32_t)done) != 0 || shift == 0;
+        __syncthreads();
+        if (done) return Crossing{prefix, shift};
+    }
+}
+
+// Exclusive prefix sum over the workgroup, in thread order, and the sum of all.
+template <int THREADS>
+__device__ __forceinline__ u64 block_scan(u64 v, u64& all, u64* tmp) {
+    const uint32_t lane = lane_id(), wave = threadIdx.x / 64;
+    u64 upto = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 t = __shfl_up(upto, o);
+        if (lane >= (uint32_t)o) upto += t;
+    }
+    if (THREADS == 64) {
+        all = __shfl(upto, 63);
+        return upto - v;
+    }
+    if (lane == 63) tmp[wave] = upto;
+    __syncthreads();
+    u64 before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        before += (uint32_t)w < wave ? tmp[w] : 0;
+        sum += tmp[w];
+    }
+    __syncthreads();
+    all = sum;
+    return before + upto - v;
+}
+
+// What a row's answer is written through.
+struct Out {
+    int32_t* index;
+    float* logprob;
+    __device__ __forceinline__ void put(uint64_t row, uint32_t cls, double lp) const {
+        index[row] = (int32_t)cls;
+        if (logprob) logprob[row] = (float)lp;
+    }
+    __device__ __forceinline__ void empty(uint64_t row) const {
+        index[row] = -1;
+        if (logprob) logprob[row] = -INFINITY;
     }
 };
 
-template <class T, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_kernel(Rows<T> X, Settings S, double unit,
-                                                         int32_t* __restrict__ index, float* __restrict__ logprob) {
-    constexpr int W = THREADS / 64;
-    __shared__ uint32_t hist[256];
-    __shared__ u64 hist_mass[256];
-    __shared__ u64 tmp_u[W], wave_mass[W];
-    __shared__ uint32_t wave_ties[W];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
-    const uint32_t n = X.classes;
+// Entries of a row in registers: cut them, and draw.  Entry e of a thread has order key key[e] (0: none) and
+// class idx[e].
+template <int THREADS, int E>
+struct Entries {
+    uint32_t key[E], idx[E];
+    u64 mass[E];
+    __device__ __forceinline__ u64 rank(int e) const { return ((u64)key[e] << 32) | (uint32_t)~idx[e]; }
+    __device__ __forceinline__ void keep_from(Crossing c) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if ((rank(e) >> c.shift) < c.prefix) key[e] = 0;
+    }
+    __device__ void cut_count(uint32_t k, SelectLds* lds, u64* tmp) {
+        uint32_t have = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) have += key[e] != 0;
+        if (block_reduce<THREADS>((u64)have, Add(), tmp) <= k) return;
+        keep_from(select<THREADS, false, true>(
+            [&](auto f) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (key[e]) f(rank(e), 0);
+            },
+            k, 56, lds));
+    }
+    __device__ __forceinline__ void weigh(const Masses& M) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) mass[e] = key[e] ? M(key_score(key[e])) : 0;
+    }
+    __device__ __forceinline__ u64 sum(u64* tmp) const {
+        u64 s = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += key[e] ? mass[e] : 0;
+        return block_reduce<THREADS>(s, Add(), tmp);
+    }
+    // the shortest prefix of the order with a mass of `want` stays
+    __device__ void cut_mass(u64 want, SelectLds* lds) {
+        keep_from(select<THREADS, true, true>(
+            [&](auto f) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (key[e] && mass[e]) f(rank(e), mass[e]);
+            },
+            want, 56, lds));
+    }
+    __device__ __forceinline__ void drop_below(u64 least) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (mass[e] < least) key[e] = 0;
+    }
+};
+
+// ---- rows that fit the registers of a workgroup -----------------------------------------------
+// Thread t holds classes [t E, (t + 1) E).
+template <class T, bool kUnit, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settings S, int shift, Out out) {
+    constexpr int E = 8, V = Pack<T>::V, W = THREADS / 64;
+    __shared__ SelectLds lds;
+    __shared__ u64 tmp[W];
+    const uint32_t n = X.classes, i0 = threadIdx.x * E;
     for (uint64_t row = blockIdx.x; row < X.rows; row += gridDim.x) {
-        Walk<T, THREADS> K{X.data + (int64_t)row * X.rs, X.cs, n, settings(S, row, n), 0.0f, unit};
+        const Row r = settings(S, row, n);
+        const T* x0 = X.data + (int64_t)row * X.rs;
+        float x[E];
+#pragma unroll
+        for (int q = 0; q < E / V; ++q)
+            load_pack<T, kUnit>(x0, X.cs, i0 + q * V, n, -INFINITY, *(float(*)[V])&x[q * V]);
+        const uint32_t bits = r.allowed && i0 < n ? r.allowed[i0 >> 5] >> (i0 & 31) : ~0u;
+        Entries<THREADS, E> L;
         u64 top = 0;
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-            const uint32_t q = K.key(i, K.score(i));
-            const u64 key = q ? ((u64)q << 32) | (uint32_t)~i : 0;
-            top = key > top ? key : top;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            L.idx[e] = i0 + e;
+            L.key[e] = class_key(x[e], bits >> e & 1);
+            const u64 k = L.key[e] ? L.rank(e) : 0;
+            top = k > top ? k : top;
         }
-        top = block_reduce<THREADS>(top, [](u64 a, u64 b) { return a > b ? a : b; }, tmp_u);
-        if (top == 0 || K.r.greedy) {
-            if (threadIdx.x == 0) {
-                index[row] = top ? (int32_t)~(uint32_t)top : -1;
-                if (logprob) logprob[row] = top ? 0.0f : -INFINITY;
-            }
+        top = block_reduce<THREADS>(top, [](u64 a, u64 b) { return a > b ? a : b; }, tmp);
+        if (top == 0) {
+            if (threadIdx.x == 0) out.empty(row);
             continue;
         }
-        K.m = key_score((uint32_t)(top >> 32));
-        u64 total = 0;
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-            const float x = K.score(i);
-            if (K.key(i, x)) total += K.mass(x);
+        const uint32_t first = ~(uint32_t)top;
+        const float m = key_score((uint32_t)(top >> 32));
+        if (r.greedy) {
+            if (threadIdx.x == 0) out.put(row, first, 0.0);
+            continue;
         }
-        total = block_reduce<THREADS>(total, Add(), tmp_u);
-        Cut cut{0, 0, total};
-        if (K.r.min_p > 1.0) {
-            cut = Cut{(uint32_t)(top >> 32), 1, mass_of(1.0, unit)};
-        } else {
-            if (K.r.k) cut = K.select(false, K.r.k, 0, hist, hist_mass);
-            if (K.r.p < 1.0) cut = K.select(true, nucleus_of(K.r.p, cut.mass), cut.key, hist, hist_mass);
-        }
-        // wave w holds the classes [w per, (w + 1) per), lanes side by side
-        const uint32_t per = ((n + W - 1) / W + 63) / 64 * 64;
-        const uint32_t a = wave * per, b = min(n, a + per);
-        uint32_t ties = 0;
-        for (uint32_t i = a + lane; i < b; i += 64) {
-            const uint32_t q = K.key(i, K.score(i));
-            ties += q != 0 && q == cut.key;
-        }
-        ties = wave_reduce(ties, Add());
-        if (lane == 0) wave_ties[wave] = ties;
-        __syncthreads();
-        uint32_t ties_before = 0;
-        for (uint32_t v = 0; v < wave; ++v) ties_before += wave_ties[v];
-        // the kept mass of class i (no class at b and beyond); `seen` counts the ties passed
-        auto kept = [&](uint32_t i, uint32_t& seen) -> u64 {
-            const float x = i < b ? K.score(i) : 0.0f;
-            const uint32_t q = i < b ? K.key(i, x) : 0;
-            const bool tie = q != 0 && q == cut.key;
-            const u64 t = __ballot(tie);
-            bool in = q > cut.key || (tie && seen + (uint32_t)__popcll(t & ((1ull << lane) - 1)) < cut.ties);
-            seen += (uint32_t)__popcll(t);
-            if (!in) return 0;
-            const double w = weight_of(x, K.m, K.r.rt);
-            return !(w < K.r.min_p) || K.r.min_p > 1.0 ? mass_of(w, unit) : 0;
-        };
-        u64 mine = 0;
-        uint32_t seen = ties_before;
-        for (uint32_t i = a; i < b; i += 64) mine += kept(i + lane, seen);
-        mine = wave_reduce(mine, Add());
-        if (lane == 0) wave_mass[wave] = mine;
-        __syncthreads();
-        u64 sum = 0, before = 0;
-        for (uint32_t v = 0; v < W; ++v) {
-            if (v == wave) before = sum;
-            sum += wave_mass[v];
-        }
-        const u64 target = target_of(K.r.u, sum);
-        if (target >= before && target < before + mine) {
-            seen = ties_before;
-            for (uint32_t i = a; i < b; i += 64) {
-                u64 c = kept(i + lane, seen);
+        // (beside +inf nothing has mass: the classes of +inf become 0, the others -inf)
+        const bool inf = m == INFINITY;
+        const Masses M{inf ? 0.0 : (double)m, r.rt * 1.4426950408889634, shift};
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const u64 v = __shfl_up(c, o);
-                    if (lane >= (uint32_t)o) c += v;
+        for (int e = 0; e < E; ++e) {
+            const float y = !inf ? key_score(L.key[e]) : L.key[e] == (uint32_t)(top >> 32) ? 0.0f : -INFINITY;
+            L.mass[e] = L.key[e] ? M(y) : 0;
+        }
+        const u64 total = L.sum(tmp);
+        if (r.min_p > 1.0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (L.idx[e] != first) L.key[e] = 0;
+        } else {
+            if (r.k) L.cut_count(r.k, &lds, tmp);
+            if (r.p < 1.0) L.cut_mass(nucleus_of(r.p, r.k ? L.sum(tmp) : total), &lds);
+            L.drop_below(least_mass(r.min_p, shift));
+        }
+        u64 mine = 0, all;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine += L.key[e] ? L.mass[e] : 0;
+        u64 before = block_scan<THREADS>(mine, all, tmp);
+        const u64 target = target_of(r.u, all);
+        if (target >= before && target - before < mine) {
+            uint32_t cls = first;
+            float xs = m;
+            bool found = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const u64 w = L.key[e] ? L.mass[e] : 0;
+                if (!found && target - before < w) {
+                    found = true;
+                    cls = L.idx[e];
+                    xs = key_score(L.key[e]);
                 }
-                const u64 hit = __ballot(before + c > target);
-                if (hit) {
-                    const uint32_t j = i + (uint32_t)__builtin_ctzll(hit);
-                    if (lane == 0) {
-                        index[row] = (int32_t)j;
-                        if (logprob)
-                            logprob[row] = (float)(((double)K.score(j) - (double)K.m) * K.r.rt - log((double)total / unit));
-                    }
-                    break;
-                }
-                before += __shfl(c, 63);
+                before += w;
             }
+            out.put(row, cls, (inf ? 0.0 : ((double)xs - (double)m) * r.rt) - log(ldexp((double)total, -shift)));
         }
         __syncthreads();
     }
 }
 
-// Masses are sums of at most n weights of 1.
-double unit_of(uint32_t n) {
+// ---- long rows --------------------------------------------------------------------------------
+// A wave takes 2048 classes at a time (a segment), a lane 32 of them (a group): 16-byte vectors, lanes side by
+// side.  Which classes can be kept is found from the maxima of the groups (few of many: top_k), or from a
+// histogram of counts or masses over the distance from the largest score; those, or those of the one
+// bin in which the cut lies, are listed, and the list cut exactly in registers.  Kept masses of the
+// bins above a nucleus's last are summed by segments, and the draw looks through one of them.
+constexpr uint32_t kSeg = 2048, kGroup = 32, kGroupSegs = 128;
+constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
+constexpr float kBinsPerNat = 32.0f;
+__device__ __forceinline__ uint32_t bin_at(uint32_t b) { return b + (b >> 4); }   // (its place in LDS)
+
+enum Mode : uint32_t { kGreedy, kWhole, kList, kNucleus, kSlow };
+
+template <class T, bool kUnit, int THREADS>
+struct Long {
+    static constexpr int V = Pack<T>::V, U = kGroup / V, W = THREADS / 64, CAP = THREADS * 8;
+    const T* x0;
+    int64_t cs;
+    uint32_t n;
+    Row r;
+    int S;
+    uint32_t lane, wave;
+
+    __device__ __forceinline__ Long(const Rows<T>& X, const Settings& St, uint64_t row, int shift)
+        : x0(X.data + (int64_t)row * X.rs), cs(X.cs), n(X.classes), r(settings(St, row, X.classes)), S(shift),
+          lane(lane_id()), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)) {}
+
+    __device__ __forceinline__ uint32_t at(uint32_t seg, int u, uint32_t ln) const { return seg * kSeg + (u * 64 + ln) * V; }
+    // classes that are not allowed read as -inf
+    __device__ __forceinline__ void load(uint32_t i, float (&x)[V]) const {
+        load_pack<T, kUnit>(x0, cs, i, n, -INFINITY, x);
+        if (r.allowed && i < n) {
+            const uint32_t bits = r.allowed[i >> 5] >> (i & 31);
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = bits >> v & 1 ? x[v] : -INFINITY;
+        }
+    }
+    __device__ __forceinline__ float score(uint32_t i) const {
+        if (i >= n || (r.allowed && !(r.allowed[i >> 5] >> (i & 31) & 1))) return -INFINITY;
+        return to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * cs]);
+    }
+    __device__ __forceinline__ Mode mode() const {
+        return r.greedy || r.min_p > 1.0 ? kGreedy : r.k ? kList : r.p < 1.0 ? kNucleus : kWhole;
+    }
+    // top_k from the groups' maxes: a quarter of them at most, so that few classes beside the k largest reach
+    // the k-th of the maxima; 2^18 classes at most (32 KB of maxima)
+    __device__ __forceinline__ bool by_groups(uint32_t segs) const {
+        return segs <= kGroupSegs && r.k <= segs * 16 && r.k * 4 <= (uint32_t)CAP;
+    }
+
+    // Largest score of the segments [s0, s1) and the segment it was first met in, per thread; into `groups`
+    // (nullable) every group's largest as an order key (0: nothing to draw); with `sums` the running softmax
+    // denominator.
+    __device__ __forceinline__ void scan(uint32_t s0, uint32_t s1, uint32_t* groups, bool sums, float c,
+                                         float& best, uint32_t& best_seg, Running& run) const {
+        best = -INFINITY;
+        best_seg = s0;
+        for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
+            float x[U][V], gm = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(at(seg, u, lane), x[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) gm = fmaxf(gm, x[u][v]);
+            if (gm > best) {
+                best = gm;
+                best_seg = seg;
+            }
+            if (groups) groups[(seg - s0) * 64 + lane] = gm > -INFINITY ? order_key(gm) : 0;
+            if (sums) {
+                run.raise(gm, c);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[u][v] = x[u][v] == x[u][v] ? x[u][v] : -INFINITY;   // (NaN is no class)
+                run.add(x, c);
+            }
+        }
+    }
+    // The first class at the score m, of the threads that have met it in best_seg; n if there is none.
+    __device__ __forceinline__ uint32_t first_at(float m, float best, uint32_t best_seg) const {
+        if (!(best == m) || m == -INFINITY) return 0xFFFFFFFFu;
+        uint32_t first = 0xFFFFFFFFu;
+#pragma unroll 1
+        for (int u = U - 1; u >= 0; --u) {
+            float x[V];
+            const uint32_t i = at(best_seg, u, lane);
+            load(i, x);
+#pragma unroll
+            for (int v = V - 1; v >= 0; --v) first = x[v] == m ? i + v : first;
+        }
+        return first;
+    }
+
+    // ---- bins: monotone in the score, the largest in bin 0 ----
+    float bm, bscale;
+    __device__ __forceinline__ void set_bins(float m) {
+        bm = m;
+        bscale = (float)(r.rt * kBinsPerNat);
+    }
+    __device__ __forceinline__ uint32_t bin(float x) const {
+        const float z = (bm - x) * bscale;
+        return z < (float)(kBins - 1) ? (uint32_t)z : kBins - 1;   // (NaN: the last)
+    }
+    // Histogram of the segments' counts or masses, added into `hist` in LDS (padded).
+    template <bool kMass>
+    __device__ __forceinline__ void histogram(uint32_t s0, uint32_t s1, const Masses& M, u64* hist) const {
+        for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
+#pragma unroll 2
+            for (int u = 0; u < U; ++u) {
+                float x[V];
+                load(at(seg, u, lane), x);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (kMass) {
+                        const u64 w = M(x[v]);
+                        if (w) atomicAdd(&hist[bin_at(bin(x[v]))], w);
+                    } else if (x[v] > -INFINITY) {
+                        atomicAdd((uint32_t*)&hist[bin_at(bin(x[v]))], 1u);
+                    }
+                }
+            }
+        }
+    }
+    // Kept masses of the segments: of all classes of at least `least` (cut = kBins), or of those in the bins
+    // before `cut`; the classes in bin `cut`, and with `all` those before, go to the list.
+    template <bool kSum>
+    __device__ __forceinline__ void collect(uint32_t s0, uint32_t s1, const Masses& M, uint32_t cut, bool all, u64 least,
+                                            u64* segs, u64* list, uint32_t* count) const {
+        for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
+            u64 sum = 0;
+#pragma unroll 2
+            for (int u = 0; u < U; ++u) {
+                float x[V];
+                const uint32_t i = at(seg, u, lane);
+                load(i, x);
+                uint32_t hits = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const uint32_t b = cut < kBins ? bin(x[v]) : 0;
+                    if (kSum && (cut == kBins || b < cut)) {
+                        const u64 w = M(x[v]);
+                        sum += w >= least ? w : 0;
+                    }
+                    if (cut < kBins && x[v] > -INFINITY && (b == cut || (all && b < cut))) hits |= 1u << v;
+                }
+                while (__any(hits != 0)) {
+                    const bool in = hits != 0;
+                    const uint32_t v = in ? (uint32_t)__builtin_ctz(hits) : 0;
+                    float z = x[0];
+#pragma unroll
+                    for (int q = 1; q < V; ++q) z = v == (uint32_t)q ? x[q] : z;
+                    const u64 b = __ballot(in);
+                    uint32_t base = 0;
+                    if (lane == 0) base = atomicAdd(count, (uint32_t)__popcll(b));
+                    base = __builtin_amdgcn_readfirstlane(base) + (uint32_t)__popcll(b & ((1ull << lane) - 1));
+                    if (in && base < (uint32_t)CAP) list[base] = rank_key(z, i + v);
+                    hits &= hits - 1;
+                }
+            }
+            if (kSum) {
+                sum = wave_reduce(sum, Add());
+                if (lane == 0) segs[seg] = sum;
+            }
+        }
+    }
+    // Classes of the groups whose largest reaches the bound go to the list.
+    __device__ __forceinline__ void gather(uint32_t segs, const uint32_t* groups, uint32_t bound, u64* list,
+                                           uint32_t* count) const {
+        for (uint32_t g0 = wave * 64; g0 < segs * 64; g0 += THREADS) {
+            u64 hit = __ballot(groups[g0 + lane] >= bound && groups[g0 + lane] != 0);
+            // a group at a time: lane l reads its class l
+            while (hit) {
+                const uint32_t ln = (uint32_t)__builtin_ctzll(hit);
+                hit &= hit - 1;
+                const uint32_t i = at(g0 / 64, (int)(lane % kGroup) / V, ln) + lane % V;
+                const float x = lane < kGroup ? score(i) : -INFINITY;
+                const bool in = x > -INFINITY && order_key(x) >= bound;
+                const u64 b = __ballot(in);
+                uint32_t base = 0;
+                if (lane == 0) base = atomicAdd(count, (uint32_t)__popcll(b));
+                base = __builtin_amdgcn_readfirstlane(base) + (uint32_t)__popcll(b & ((1ull << lane) - 1));
+                if (in && base < (uint32_t)CAP) list[base] = rank_key(x, i);
+            }
+        }
+    }
+    __device__ __forceinline__ void read_list(Entries<THREADS, 8>& L, const u64* list, uint32_t count) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t i = e * THREADS + threadIdx.x;
+            const u64 k = i < count ? list[i] : 0;
+            L.key[e] = (uint32_t)(k >> 32);
+            L.idx[e] = ~(uint32_t)k;
+        }
+    }
+
+    // ---- the last steps ----
+    // A list that holds every class that may be kept: top_k, top_p, min_p, and the draw.
+    __device__ void finish_list(const u64* list, uint32_t count, const Masses& M, double log_z, uint64_t row, SelectLds* lds,
+                                u64* tmp, const Out& out) const {
+        Entries<THREADS, 8> L;
+        read_list(L, list, count);
+        L.cut_count(r.k, lds, tmp);
+        L.weigh(M);
+        if (r.p < 1.0) L.cut_mass(nucleus_of(r.p, L.sum(tmp)), lds);
+        L.drop_below(least_mass(r.min_p, S));
+        const u64 want = target_of(r.u, L.sum(tmp)) + 1;
+        const Crossing c = select<THREADS, true, false>(
+            [&](auto f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (L.key[e] && L.mass[e]) f((uint32_t)~L.idx[e], L.mass[e]);
+            },
+            want, 24, lds);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (L.key[e] && L.mass[e] && ((u64)(uint32_t)~L.idx[e] >> c.shift) == c.prefix)
+                out.put(row, L.idx[e], ((double)key_score(L.key[e]) - M.m) * r.rt - log_z);
+    }
+    // Segments' kept masses (and a nucleus's cut): the segment of the draw, then its class.
+    __device__ void finish_segments(const u64* segs, uint32_t n_segs, const Masses& M, uint32_t cut, u64 from, u64 least,
+                                    u64 total, uint64_t row, u64* tmp, u64* pick, const Out& out) const {
+        const uint32_t per = (n_segs + THREADS - 1) / THREADS, a = min(n_segs, threadIdx.x * per), b = min(n_segs, a + per);
+        u64 mine = 0, all;
+        for (uint32_t s = a; s < b; ++s) mine += segs[s];
+        u64 before = block_scan<THREADS>(mine, all, tmp);
+        const u64 target = target_of(r.u, all);
+        if (target >= before && target - before < mine) {
+            uint32_t s = a;
+            while (target - before >= segs[s]) before += segs[s++];
+            pick[0] = s;
+            pick[1] = before;
+        }
+        __syncthreads();
+        const uint32_t seg = (uint32_t)pick[0];
+        const u64 base = pick[1];
+        constexpr int Q = kSeg / THREADS;
+        u64 w[Q];
+        mine = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const uint32_t i = seg * kSeg + threadIdx.x * Q + q;
+            const float x = score(i);
+            bool in = x > -INFINITY;
+            if (cut < kBins) {
+                const uint32_t bi = bin(x);
+                in = in && (bi < cut || (bi == cut && rank_key(x, i) >= from));
+            }
+            w[q] = in ? M(x) : 0;
+            w[q] = w[q] >= least ? w[q] : 0;
+            mine += w[q];
+        }
+        before = base + block_scan<THREADS>(mine, all, tmp);
+        if (target >= before && target - before < mine) {
+            bool found = false;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                if (!found && target - before < w[q]) {
+                    found = true;
+                    const uint32_t i = seg * kSeg + threadIdx.x * Q + q;
+                    out.put(row, i, ((double)score(i) - M.m) * r.rt - log(ldexp((double)total, -S)));
+                }
+                before += w[q];
+            }
+        }
+    }
+    // Any row, by selection over the whole of it: rows of +inf, and those whose cut lies among more classes than
+    // a list holds (equal scores).
+    __device__ void slow(uint32_t top_key, uint32_t first, uint64_t row, SelectLds* lds, u64* tmp, u64* pick, const Out& out) const {
+        const float m = key_score(top_key);
+        const bool inf = m == INFINITY;
+        const Masses M{inf ? 0.0 : (double)m, r.rt * 1.4426950408889634, S};
+        auto mass = [&](float x) -> u64 { return M(!inf ? x : x == m ? 0.0f : -INFINITY); };
+        auto key_at = [&](uint32_t i) { return class_key(score(i), true); };
+        u64 total = 0;
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS)
+            if (key_at(i)) total += mass(score(i));
+        total = block_reduce<THREADS>(total, Add(), tmp);
+        u64 from = 0;   // ranks below it are cut
+        u64 have = 0, kept = total;
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) have += key_at(i) != 0;
+        have = block_reduce<THREADS>(have, Add(), tmp);
+        if (r.k && have > r.k) {
+            const Crossing c = select<THREADS, false, true>(
+                [&](auto f) {
+                    for (uint32_t i = threadIdx.x; i < n; i += THREADS)
+                        if (key_at(i)) f(rank_key(score(i), i), 0);
+                },
+                r.k, 56, lds);
+            from = c.prefix << c.shift;
+            kept = 0;
+            for (uint32_t i = threadIdx.x; i < n; i += THREADS)
+                if (key_at(i) && rank_key(score(i), i) >= from) kept += mass(score(i));
+            kept = block_reduce<THREADS>(kept, Add(), tmp);
+        }
+        if (r.p < 1.0) {
+            const Crossing c = select<THREADS, true, true>(
+                [&](auto f) {
+                    for (uint32_t i = threadIdx.x; i < n; i += THREADS)
+                        if (key_at(i) && rank_key(score(i), i) >= from) {
+                            const u64 w = mass(score(i));
+                            if (w) f(rank_key(score(i), i), w);
+                        }
+                },
+                nucleus_of(r.p, kept), 56, lds);
+            const u64 f = c.prefix << c.shift;
+            from = f > from ? f : from;
+        }
+        const u64 least = least_mass(r.min_p, S);
+        // thread t holds the classes [t per, (t + 1) per)
+        const uint32_t per = (n + THREADS - 1) / THREADS, a = min(n, threadIdx.x * per), b = min(n, a + per);
+        auto weight = [&](uint32_t i) -> u64 {
+            const float x = score(i);
+            if (!class_key(x, true) || rank_key(x, i) < from) return 0;
+            const u64 w = mass(x);
+            return w >= least ? w : 0;
+        };
+        u64 mine = 0, all;
+        for (uint32_t i = a; i < b; ++i) mine += weight(i);
+        u64 before = block_scan<THREADS>(mine, all, tmp);
+        const u64 target = target_of(r.u, all);
+        if (target >= before && target - before < mine) {
+            uint32_t i = a;
+            for (u64 w; target - before >= (w = weight(i)); ++i) before += w;
+            out.put(row, i, (inf ? 0.0 : ((double)score(i) - (double)m) * r.rt) - log(ldexp((double)total, -S)));
+        }
+        __syncthreads();
+    }
+};
+
+// Where the weights of the bins, from bin 0 on, reach `want`; every wave by itself.
+template <class Get>
+__device__ __forceinline__ Found<u64> find_cut(Get get, u64 want) {
+    const uint32_t l = lane_id();
+    u64 sum = 0;
+    for (uint32_t j = 0; j < kBins / 64; ++j) sum += get(l * (kBins / 64) + j);
+    u64 upto = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 v = __shfl_up(upto, o);
+        if (l >= (uint32_t)o) upto += v;
+    }
+    u64 above = upto - sum, inside = 0;
+    uint32_t b = l * (kBins / 64);
+    const u64 cross = __ballot(upto >= want);
+    const int at = cross ? __builtin_ctzll(cross) : 63;
+    bool open = true;
+    for (uint32_t j = 0; j < kBins / 64; ++j) {
+        const u64 c = get(l * (kBins / 64) + j);
+        if (open) {
+            b = l * (kBins / 64) + j;
+            inside = c;
+            if (above + c >= want) open = false;
+            else if (j + 1 < kBins / 64) above += c;
+        }
+    }
+    return Found<u64>{(uint32_t)__shfl(b, at), __shfl(above, at), __shfl(inside, at)};
+}
+
+// A workgroup a row, all steps in one launch.
+template <class T, bool kUnit, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Settings S, int shift, Out out) {
+    typedef Long<T, kUnit, THREADS> L;
+    constexpr int W = THREADS / 64;
+    extern __shared__ u64 pool[];   // list, or segments' masses behind it; groups
+    __shared__ u64 hist[kBinsPad];
+    __shared__ SelectLds lds;
+    __shared__ u64 tmp[W], pick[2];
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    __shared__ uint32_t count, khist[256];
+    const uint32_t n_segs = (X.classes + kSeg - 1) / kSeg;
+    u64* list = pool;
+    u64* segs = pool + L::CAP;
+    uint32_t* groups = (uint32_t*)(segs + n_segs);
+    for (uint64_t row = blockIdx.x; row < X.rows; row += gridDim.x) {
+        L R(X, S, row, shift);
+        const Mode mode = R.mode();
+        const float c = (float)(R.r.rt * 1.4426950408889634);
+        const bool by_groups = mode == kList && R.by_groups(n_segs);
+        float best;
+        uint32_t best_seg;
+        Running run;
+        R.scan(0, n_segs, by_groups ? groups : nullptr, mode == kList, c, best, best_seg, run);
+        for (uint32_t b = threadIdx.x; b < kBinsPad; b += THREADS) hist[b] = 0;
+        if (threadIdx.x == 0) count = 0;
+        const float m = block_reduce<THREADS>(best, MaxF(), tmp_f);
+        __syncthreads();
+        if (m == -INFINITY) {
+            if (threadIdx.x == 0) out.empty(row);
+            continue;
+        }
+        const bool slow_only = m == INFINITY;
+        uint32_t first = 0;
+        if (mode == kGreedy) {
+            const uint32_t f = R.first_at(m, best, best_seg);
+            u64 lo = block_reduce<THREADS>((u64)f, [](u64 a, u64 b) { return a < b ? a : b; }, tmp);
+            first = (uint32_t)lo;
+            if (R.r.greedy) {
+                if (threadIdx.x == 0) out.put(row, first, 0.0);
+                continue;
+            }
+        }
+        const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+        R.set_bins(m);
+        bool slow = slow_only;
+        if (!slow && mode == kGreedy) {   // (a least weight above 1: the first class, with its log probability)
+            u64 z = 0;
+            for (uint32_t seg = R.wave; seg < n_segs; seg += W)
+                for (int u = 0; u < L::U; ++u) {
+                    float x[L::V];
+                    R.load(R.at(seg, u, R.lane), x);
+#pragma unroll
+                    for (int v = 0; v < L::V; ++v) z += M(x[v]);
+                }
+            z = block_reduce<THREADS>(z, Add(), tmp);
+            if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)z, -shift)));
+            continue;
+        }
+        if (slow && mode == kGreedy) {
+            u64 z = 0;
+            for (uint32_t i = threadIdx.x; i < R.n; i += THREADS) z += R.score(i) == INFINITY;
+            z = block_reduce<THREADS>(z, Add(), tmp);
+            if (threadIdx.x == 0) out.put(row, first, -log((double)z));
+            continue;
+        }
+        if (!slow && mode == kWhole) {
+            const u64 least = least_mass(R.r.min_p, shift);
+            R.template collect<true>(0, n_segs, M, kBins, false, 0, segs, list, &count);
+            __syncthreads();
+            u64 z = 0;
+            for (uint32_t s = threadIdx.x; s < n_segs; s += THREADS) z += segs[s];
+            z = block_reduce<THREADS>(z, Add(), tmp);
+            if (least > 0) {
+                R.template collect<true>(0, n_segs, M, kBins, false, least, segs, list, &count);
+                __syncthreads();
+            }
+            R.finish_segments(segs, n_segs, M, kBins, 0, least, z, row, tmp, pick, out);
+        } else if (!slow && mode == kNucleus) {
+            R.template histogram<true>(0, n_segs, M, hist);
+            __syncthreads();
+            u64 z = 0;
+            for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) z += hist[bin_at(b)];
+            z = block_reduce<THREADS>(z, Add(), tmp);
+            const u64 want = nucleus_of(R.r.p, z), least = least_mass(R.r.min_p, shift);
+            const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
+            R.template collect<true>(0, n_segs, M, f.bin, false, least, segs, list, &count);
+            __syncthreads();
+            if (count > (uint32_t)L::CAP) {
+                slow = true;
+            } else {
+                Entries<THREADS, 8> E;
+                R.read_list(E, list, count);
+                E.weigh(M);
+                const Crossing x = select<THREADS, true, true>(
+                    [&](auto g) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (E.key[e] && E.mass[e]) g(E.rank(e), E.mass[e]);
+                    },
+                    want - f.above, 56, &lds);
+                E.keep_from(x);
+                E.drop_below(least);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (E.key[e] && E.mass[e]) atomicAdd(&segs[E.idx[e] / kSeg], E.mass[e]);
+                __syncthreads();
+                R.finish_segments(segs, n_segs, M, f.bin, x.prefix << x.shift, least, z, row, tmp, pick, out);
+            }
+        } else if (!slow) {
+            float mr;
+            double sr;
+            block_running<THREADS>(run, c, mr, sr, tmp_f, tmp_d);
+            const double log_z = log(sr);
+            bool listed = false;
+            if (by_groups) {
+                u64 have = 0;
+                for (uint32_t g = threadIdx.x; g < n_segs * 64; g += THREADS) have += groups[g] != 0;
+                have = block_reduce<THREADS>(have, Add(), tmp);
+                if (have >= R.r.k) {
+                    const u64 kth = block_kth<THREADS>([&](uint32_t i) { return (u64)groups[i] << 32; }, n_segs * 64, R.r.k, 32, khist);
+                    R.gather(n_segs, groups, (uint32_t)(kth >> 32), list, &count);
+                    __syncthreads();
+                    listed = count <= (uint32_t)L::CAP;
+                    __syncthreads();
+                }
+            }
+            if (!listed) {
+                if (threadIdx.x == 0) count = 0;
+                R.template histogram<false>(0, n_segs, M, hist);
+                __syncthreads();
+                u64 have = 0;
+                for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) have += hist[bin_at(b)];
+                have = block_reduce<THREADS>(have, Add(), tmp);
+                const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, have < R.r.k ? have : (u64)R.r.k);
+                if (f.above + f.inside > (u64)L::CAP) {
+                    slow = true;
+                } else {
+                    R.template collect<false>(0, n_segs, M, f.bin, true, 0, segs, list, &count);
+                    __syncthreads();
+                }
+            }
+            if (!slow) R.finish_list(list, count, M, log_z, row, &lds, tmp, out);
+        }
+        if (slow) R.slow(order_key(m), first, row, &lds, tmp, pick, out);
+        __syncthreads();
+    }
+}
+
+// Masses are sums of at most n weights of 1: they stay below 2^63.
+int shift_of(uint32_t n) {
     int b = 0;
     while ((1ull << b) < n) ++b;
-    return std::ldexp(1.0, std::min(51, 62 - b));
+    return std::min(51, 62 - b);
+}
+
+template <class T, bool kUnit, int THREADS>
+int launch_long(const Rows<T>& X, const Settings& S, int shift, const Out& out, hipStream_t st) {
+    typedef Long<T, kUnit, THREADS> L;
+    const size_t n_segs = (X.classes + kSeg - 1) / kSeg;
+    const size_t lds = sizeof(u64) * (L::CAP + n_segs) + (n_segs <= kGroupSegs ? sizeof(uint32_t) * 64 * n_segs : 0);
+    CLS_TRY(hipFuncSetAttribute((const void*)sample_long_kernel<T, kUnit, THREADS>,
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    sample_long_kernel<T, kUnit, THREADS><<<row_grid(X.rows), THREADS, lds, st>>>(X, S, shift, out);
+    CLS_TRY(hipGetLastError());
+    return CBH_OK;
+}
+
+template <class T, bool kUnit>
+int launch_sample(const Rows<T>& X, const Settings& S, const Out& out, hipStream_t st) {
+    const uint32_t n = X.classes;
+    const int shift = shift_of(n);
+    if (n <= 512) sample_short_kernel<T, kUnit, 64><<<row_grid(X.rows), 64, 0, st>>>(X, S, shift, out);
+    else if (n <= 2048) sample_short_kernel<T, kUnit, 256><<<row_grid(X.rows), 256, 0, st>>>(X, S, shift, out);
+    else if (n <= 8192) return launch_long<T, kUnit, 256>(X, S, shift, out, st);
+    else return launch_long<T, kUnit, 1024>(X, S, shift, out, st);
+    CLS_TRY(hipGetLastError());
+    return CBH_OK;
 }
 
 template <class T>
 int run_sample(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t cs, const Settings& S, int32_t* index,
                float* logprob, hipStream_t st) {
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
-    const double unit = unit_of(n);
-    if (n <= 2048) sample_kernel<T, 64><<<row_grid(rows), 64, 0, st>>>(X, S, unit, index, logprob);
-    else sample_kernel<T, 1024><<<row_grid(rows), 1024, 0, st>>>(X, S, unit, index, logprob);
-    CLS_TRY(hipGetLastError());
-    return CBH_OK;
+    const Out out{index, logprob};
+    return cs == 1 ? launch_sample<T, true>(X, S, out, st) : launch_sample<T, false>(X, S, out, st);
 }
 
 }  // namespace

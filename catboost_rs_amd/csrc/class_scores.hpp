@@ -180,6 +180,30 @@ __device__ __forceinline__ Found<V> find_bin(const V* hist, V want) {
     return Found<V>{(uint32_t)__shfl(b, at), __shfl(above, at), __shfl(inside, at)};
 }
 
+// The k-th largest of the keys get(0 .. n - 1) (0: no key; at least k are not 0), or any bound that
+// exactly k keys reach, by bytes from the top; `stop`: the lowest bit looked at.  All threads call it and get
+// the same value.  hist: 256 words of LDS.
+template <int THREADS, class Get>
+__device__ u64 block_kth(Get get, uint32_t n, uint32_t k, int stop, uint32_t* hist) {
+    u64 prefix = 0;
+    uint32_t need = k;
+    for (int shift = 56; shift >= stop; shift -= 8) {
+        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) hist[b] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+            const u64 key = get(i);
+            if (key != 0 && (shift == 56 || (key >> (shift + 8)) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        const Found<uint32_t> f = find_bin(hist, need);
+        prefix = (prefix << 8) | f.bin;
+        need -= f.above;
+        __syncthreads();
+        if (f.inside == need) return prefix << shift;
+    }
+    return prefix << (stop < 0 ? 0 : stop);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A running softmax denominator: sum over the scores seen of 2^((x - m) c), c = log2(e) / temperature.
@@ -187,21 +211,43 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // keeps s = 0; a NaN, or a score of +inf (inf - inf), leaves NaN in s.  The difference is taken before
 // the product: the product's rounding then counts against x - m, which is small for the scores
 // that matter, and not against x.
+// Sums of a tile's scores are taken side by side and then together, and added up in f64: beside a largest
+// weight of 1, each f32 addition in a row of many would lose up to 2^-25.
 struct Running {
-    float m = kLowest, s = 0.0f;
+    float m = kLowest;
+    double s = 0.0;
     __device__ __forceinline__ void raise(float to, float c) {
         if (to > m) {
-            s *= exp2_fast((m - to) * c);
+            s *= (double)exp2_fast((m - to) * c);
             m = to;
         }
     }
-    __device__ __forceinline__ void add(float x, float c) { s += exp2_fast((x - m) * c); }
+    template <int U, int V>
+    __device__ __forceinline__ void add(const float (&x)[U][V], float c) {
+        float e[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) e[v] = exp2_fast((x[0][v] - m) * c);
+#pragma unroll
+        for (int u = 1; u < U; ++u)
+#pragma unroll
+            for (int v = 0; v < V; ++v) e[v] += exp2_fast((x[u][v] - m) * c);
+#pragma unroll
+        for (int o = V / 2; o > 0; o /= 2)
+#pragma unroll
+            for (int v = 0; v < o; ++v) e[v] += e[v + o];
+        s += (double)e[0];
+    }
+    __device__ __forceinline__ void add_one(float x, float c) { s += (double)exp2_fast((x - m) * c); }
+    __device__ __forceinline__ void join(float m2, double s2, float c) {
+        raise(m2, c);
+        s += s2 * (double)exp2_fast((m2 - m) * c);
+    }
 };
 // (m, s) pairs of several threads together: the largest m, and the sums in f64.
 template <int THREADS>
 __device__ __forceinline__ void block_running(Running r, float c, float& m, double& s, float* tmp_f, double* tmp_d) {
     m = block_reduce<THREADS>(r.m, MaxF(), tmp_f);
-    s = block_reduce<THREADS>((double)(r.s * exp2_fast((r.m - m) * c)), Add(), tmp_d);
+    s = block_reduce<THREADS>(r.s * (double)exp2_fast((r.m - m) * c), Add(), tmp_d);
 }
 
 // ---- host -----------------------------------------------------------------------------------

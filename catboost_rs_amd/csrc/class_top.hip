@@ -16,30 +16,6 @@ using namespace cbh::cls;
 constexpr uint32_t kMaxTop = 1024;
 constexpr int kUnroll = 4;   // 16-byte loads a thread has in flight
 
-// The k-th largest of the keys get(0 .. n - 1) (0: no key; at least k are not 0), or any bound that
-// exactly k keys reach, by bytes from the top; `stop`: the lowest bit looked at.  All threads call it and get
-// the same value.  hist: 256 words of LDS.
-template <int THREADS, class Get>
-__device__ u64 block_kth(Get get, uint32_t n, uint32_t k, int stop, uint32_t* hist) {
-    u64 prefix = 0;
-    uint32_t need = k;
-    for (int shift = 56; shift >= stop; shift -= 8) {
-        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) hist[b] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-            const u64 key = get(i);
-            if (key != 0 && (shift == 56 || (key >> (shift + 8)) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        const Found<uint32_t> f = find_bin(hist, need);
-        prefix = (prefix << 8) | f.bin;
-        need -= f.above;
-        __syncthreads();
-        if (f.inside == need) return prefix << shift;
-    }
-    return prefix << (stop < 0 ? 0 : stop);
-}
-
 // One wave's candidates, CAP of them in LDS: the keys above `bound` that it has met.  Full, the wave
 // keeps the k largest and raises the bound to the smallest of them.
 template <int CAP>
@@ -139,10 +115,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
                 tm = fmaxf(tm, vm[u]);
             }
             run.raise(tm, c);
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-                for (int v = 0; v < V; ++v) run.add(x[u][v], c);
+            run.add(x, c);
             if (base == 0) {
                 // the first bound: k of the tile's vectors hold a score that reaches the k-th largest of
                 // their maxima
@@ -245,8 +218,7 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
     Running run;
     for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
         const float2 ms = part_ms[row * parts + p];
-        run.raise(ms.x, c);
-        run.s += ms.y * exp2_fast((ms.x - run.m) * c);
+        run.join(ms.x, ms.y, c);
     }
     float m;
     double s;
@@ -288,7 +260,7 @@ __global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, flo
         }
 #pragma unroll
         for (int i = 0; i < NMAX; ++i) {
-            run.add(x[i], c);
+            run.add_one(x[i], c);
 #pragma unroll
             for (int j = 0; j < i; ++j) {
                 const bool ahead = key[j] >= key[i];
@@ -302,7 +274,7 @@ __global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, flo
                 values[row * k + rank[i]] = key_score(key[i]);
                 index[row * k + rank[i]] = i;
             }
-        lse[row] = run.m == INFINITY ? INFINITY : (float)((double)run.m * inv_t + log((double)run.s));
+        lse[row] = run.m == INFINITY ? INFINITY : (float)((double)run.m * inv_t + log(run.s));
     }
 }
 
