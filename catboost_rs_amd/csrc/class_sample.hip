@@ -229,6 +229,110 @@ struct Entries {
     }
 };
 
+// ---- few classes: a row a thread ---------------------------------------------------------------
+// Scores and masses in registers.  A nucleus needs the mass ahead of every class: the pairs of classes, in
+// f64 (with S = 46 and at most 32 classes every sum is an integer below 2^53 and exact), each pair a
+// comparison and two multiply-adds with 0 or 1.
+constexpr int kFewShift = 46;
+template <class T, int NMAX>
+__global__ __launch_bounds__(256) void sample_few_kernel(Rows<T> X, Settings S, Out out) {
+    const uint32_t n = X.classes;
+    for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
+        const Row r = settings(S, row, n);
+        const T* x0 = X.data + (int64_t)row * X.rs;
+        const uint32_t bits = r.allowed ? r.allowed[0] : ~0u;
+        float x[NMAX], m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) {
+            x[i] = (uint32_t)i < n ? to_f32(x0[(int64_t)i * X.cs]) : -INFINITY;
+            x[i] = bits >> i & 1 && x[i] == x[i] ? x[i] : -INFINITY;
+            m = fmaxf(m, x[i]);
+        }
+        int first = -1;
+#pragma unroll
+        for (int i = NMAX - 1; i >= 0; --i) first = x[i] == m ? i : first;
+        if (m == -INFINITY) {
+            out.empty(row);
+            continue;
+        }
+        if (r.greedy) {
+            out.put(row, first, 0.0);
+            continue;
+        }
+        const bool inf = m == INFINITY;
+        const Masses M{inf ? 0.0 : (double)m, r.rt * 1.4426950408889634, kFewShift};
+        double w[NMAX], total = 0.0;
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) {
+            if (inf) x[i] = x[i] == m ? 0.0f : -INFINITY;
+            w[i] = __builtin_bit_cast(double, M.raw(x[i])) - 4503599627370496.0;
+            total += w[i];
+        }
+        uint32_t kept = ~0u;   // a bit a class
+        if (r.min_p > 1.0) {
+            kept = 1u << first;
+        } else if (r.k || r.p < 1.0) {
+            double ahead[NMAX], whole = total;
+            uint32_t place[NMAX];
+#pragma unroll
+            for (int i = 0; i < NMAX; ++i) {
+                ahead[i] = 0.0;
+                place[i] = 0;
+            }
+            const bool count = r.k != 0;
+#pragma unroll
+            for (int i = 1; i < NMAX; ++i)
+#pragma unroll
+                for (int j = 0; j < i; ++j) {
+                    const bool a = x[j] >= x[i];   // j is ahead of i
+                    ahead[i] = __builtin_fma(w[j], a ? 1.0 : 0.0, ahead[i]);
+                    ahead[j] = __builtin_fma(w[i], a ? 0.0 : 1.0, ahead[j]);
+                    if (count) {
+                        place[i] += a;
+                        place[j] += !a;
+                    }
+                }
+            if (count) {
+                whole = 0.0;
+#pragma unroll
+                for (int i = 0; i < NMAX; ++i) {
+                    const bool in = place[i] < r.k;
+                    whole += in ? w[i] : 0.0;
+                    kept = in ? kept : kept & ~(1u << i);
+                }
+            }
+            if (r.p < 1.0) {
+                const double want = r.p * whole;
+#pragma unroll
+                for (int i = 0; i < NMAX; ++i) kept = ahead[i] < want ? kept : kept & ~(1u << i);
+                kept |= 1u << first;
+            }
+        }
+        const double least = r.min_p > 0.0 && r.min_p <= 1.0 ? r.min_p * 70368744177664.0 : 0.0;
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) {
+            w[i] = kept >> i & 1 && w[i] >= least ? w[i] : 0.0;
+            sum += w[i];
+        }
+        const double target = r.u > 0.0 ? r.u * sum : 0.0;   // (NaN: 0)
+        int at = first;
+        double run = 0.0;
+        bool open = true;
+        float xs = m;
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) {
+            run += w[i];
+            if (open && w[i] > 0.0) {   // the last class with mass, unless the running mass passes the target before
+                at = i;
+                xs = x[i];
+                open = !(run > target);
+            }
+        }
+        out.put(row, at, (inf ? 0.0 : ((double)xs - (double)m) * r.rt) - log(total * 0x1p-46));
+    }
+}
+
 // ---- rows that fit the registers of a workgroup -----------------------------------------------
 // Thread t holds classes [t E, (t + 1) E).
 template <class T, bool kUnit, int THREADS>
@@ -841,7 +945,15 @@ template <class T, bool kUnit>
 int launch_sample(const Rows<T>& X, const Settings& S, const Out& out, hipStream_t st) {
     const uint32_t n = X.classes;
     const int shift = shift_of(n);
-    if (n <= 512) sample_short_kernel<T, kUnit, 64><<<row_grid(X.rows), 64, 0, st>>>(X, S, shift, out);
+    if (n <= 32) {
+        const unsigned grid = row_grid((X.rows + 255) / 256);
+        if (n <= 4) sample_few_kernel<T, 4><<<grid, 256, 0, st>>>(X, S, out);
+        else if (n <= 8) sample_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, S, out);
+        else if (n <= 12) sample_few_kernel<T, 12><<<grid, 256, 0, st>>>(X, S, out);
+        else if (n <= 16) sample_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, S, out);
+        else if (n <= 24) sample_few_kernel<T, 24><<<grid, 256, 0, st>>>(X, S, out);
+        else sample_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, S, out);
+    } else if (n <= 512) sample_short_kernel<T, kUnit, 64><<<row_grid(X.rows), 64, 0, st>>>(X, S, shift, out);
     else if (n <= 2048) sample_short_kernel<T, kUnit, 256><<<row_grid(X.rows), 256, 0, st>>>(X, S, shift, out);
     else if (n <= 8192) return launch_long<T, kUnit, 256>(X, S, shift, out, st);
     else return launch_long<T, kUnit, 1024>(X, S, shift, out, st);

@@ -528,8 +528,8 @@ int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint3
  * mass; logprob[r] its log probability before the cuts, (x - max x) / temperature - log sum w.  With
  * temperature <= 0 the first class is drawn, with logprob 0.  A row that allows no class has index -1 and
  * logprob -inf.
- * Masses are integers in units of 2^-51 of the row's largest weight (2^-(62 - b) beyond 2^b = 2^11
- * classes), so that sums are exact and the same for every launch shape.
+ * Masses are integers in units of 2^-S of the row's largest weight (S = 46 up to 32 classes, 51 up to 2^11,
+ * 62 - b up to 2^b), so that sums are exact and the same for every launch shape.
  *   uniform        [rows] f64 in [0, 1)
  *   temperature, top_k, top_p, min_p   values for every row; *_rows: nullable [rows], used in their place
  *   allowed        nullable; bit j & 31 of word allowed[r * allowed_stride + (j >> 5)] allows class j of row r
