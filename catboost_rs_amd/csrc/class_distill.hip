@@ -14,7 +14,6 @@ namespace {
 using namespace cbh::cls;
 
 constexpr uint32_t kMaxList = 1024;
-constexpr int kUnroll = 4;
 constexpr uint32_t kMaxSeg = 1u << 18;   // classes a workgroup takes: their marks are 32 KB of LDS
 
 struct Lists {   // the teacher's, and what weighs the rows
@@ -72,8 +71,8 @@ template <class T, bool kUnit, int THREADS, int kPhase>
 __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, float c, double it, double t,
                                                           uint32_t parts, uint32_t seg, float* __restrict__ loss,
                                                           Grad<T> G, float2* __restrict__ part_ms) {
-    constexpr int V = Pack<T>::V, W = THREADS / 64;
-    constexpr uint32_t kTile = THREADS * V * kUnroll;
+    constexpr int V = Pack<T>::V, U = kPacks<T>, W = THREADS / 64;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
     extern __shared__ uint32_t mark[];   // a bit a class of the segment
     __shared__ float tmp_f[W];
     __shared__ double tmp_d[W];
@@ -109,14 +108,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
                 if (j < n) atomicOr(&mark[j >> 5], 1u << (j & 31));
             }
             __syncthreads();
-            for (uint32_t base = 0; base < n; base += kTile) {
-                float x[kUnroll][V], tm = -INFINITY;
+            for (uint32_t base = wave * kSeg; base < n; base += W * kSeg) {
+                float x[U][V], tm = -INFINITY;
+                load_tile<T, kUnit>(x0, X.cs, base, n, -INFINITY, x);
 #pragma unroll
-                for (int q = 0; q < kUnroll; ++q)
-                    load_pack<T, kUnit>(x0, X.cs, base + (q * THREADS + threadIdx.x) * V, n, -INFINITY, x[q]);
-#pragma unroll
-                for (int q = 0; q < kUnroll; ++q) {
-                    const uint32_t i = base + (q * THREADS + threadIdx.x) * V;
+                for (int q = 0; q < U; ++q) {
+                    const uint32_t i = base + (q * 64 + lane) * V;
                     const uint32_t bits = i < n ? mark[i >> 5] >> (i & 31) : 0;
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
@@ -192,14 +189,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
         const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
         if (loss && first == 0 && threadIdx.x == 0) loss[row] = (float)o.loss;
         if (g0) {
-            for (uint32_t base = 0; base < n; base += kTile) {
-                float x[kUnroll][V];
+            for (uint32_t base = wave * kSeg; base < n; base += W * kSeg) {
+                float x[U][V];
+                load_tile<T, kUnit>(x0, X.cs, base, n, -INFINITY, x);
 #pragma unroll
-                for (int q = 0; q < kUnroll; ++q)
-                    load_pack<T, kUnit>(x0, X.cs, base + (q * THREADS + threadIdx.x) * V, n, -INFINITY, x[q]);
-#pragma unroll
-                for (int q = 0; q < kUnroll; ++q) {
-                    const uint32_t i = base + (q * THREADS + threadIdx.x) * V;
+                for (int q = 0; q < U; ++q) {
+                    const uint32_t i = base + (q * 64 + lane) * V;
 #pragma unroll
                     for (int v = 0; v < V; ++v) x[q][v] = exp2_fast((x[q][v] - o.M) * c) * o.others;
                     if (i < n) store_pack<T, kUnit>(g0, G.cs, i, n, x[q]);

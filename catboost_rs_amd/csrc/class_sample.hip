@@ -418,7 +418,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
 // histogram of counts or masses over the distance from the largest score; those, or those of the one
 // bin in which the cut lies, are listed, and the list cut exactly in registers.  Kept masses of the
 // bins above a nucleus's last are summed by segments, and the draw looks through one of them.
-constexpr uint32_t kSeg = 2048, kGroup = 32, kGroupSegs = 128;
+constexpr uint32_t kGroupSegs = 128;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
 constexpr float kBinsPerNat = 32.0f;
 __device__ __forceinline__ uint32_t bin_at(uint32_t b) { return b + (b >> 4); }   // (its place in LDS)
@@ -449,6 +449,23 @@ struct Long {
             for (int v = 0; v < V; ++v) x[v] = bits >> v & 1 ? x[v] : -INFINITY;
         }
     }
+    __device__ __forceinline__ void load(uint32_t seg, float (&x)[U][V]) const {
+        uint32_t bits[U];
+        if (r.allowed) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t i = at(seg, u, lane);
+                bits[u] = i < n ? r.allowed[i >> 5] >> (i & 31) : 0;
+            }
+        }
+        load_tile<T, kUnit>(x0, cs, seg * kSeg, n, -INFINITY, x);
+        if (r.allowed) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[u][v] = bits[u] >> v & 1 ? x[u][v] : -INFINITY;
+        }
+    }
     __device__ __forceinline__ float score(uint32_t i) const {
         if (i >= n || (r.allowed && !(r.allowed[i >> 5] >> (i & 31) & 1))) return -INFINITY;
         return to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * cs]);
@@ -471,8 +488,7 @@ struct Long {
         best_seg = s0;
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             float x[U][V], gm = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < U; ++u) load(at(seg, u, lane), x[u]);
+            load(seg, x);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -521,20 +537,20 @@ struct Long {
     template <bool kMass>
     __device__ __forceinline__ void histogram(uint32_t s0, uint32_t s1, const Masses& M, u64* hist) const {
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
-#pragma unroll 2
-            for (int u = 0; u < U; ++u) {
-                float x[V];
-                load(at(seg, u, lane), x);
+            float x[U][V];
+            load(seg, x);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
+                    const float y = x[u][v];
                     if (kMass) {
-                        const u64 w = M(x[v]);
-                        if (w) atomicAdd(&hist[bin_at(bin(x[v]))], w);
-                    } else if (x[v] > -INFINITY) {
-                        atomicAdd((uint32_t*)&hist[bin_at(bin(x[v]))], 1u);
+                        const u64 w = M(y);
+                        if (w) atomicAdd(&hist[bin_at(bin(y))], w);
+                    } else if (y > -INFINITY) {
+                        atomicAdd((uint32_t*)&hist[bin_at(bin(y))], 1u);
                     }
                 }
-            }
         }
     }
     // Kept masses of the segments: of all classes of at least `least` (cut = kBins), or of those in the bins
@@ -544,11 +560,12 @@ struct Long {
                                             u64* segs, u64* list, uint32_t* count) const {
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             u64 sum = 0;
-#pragma unroll 2
+            float xs[U][V];
+            load(seg, xs);
+#pragma unroll
             for (int u = 0; u < U; ++u) {
-                float x[V];
+                const float(&x)[V] = xs[u];
                 const uint32_t i = at(seg, u, lane);
-                load(i, x);
                 uint32_t hits = 0;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {

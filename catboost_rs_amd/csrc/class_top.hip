@@ -201,6 +201,106 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
     }
 }
 
+// Long rows and a k that is small beside them.  The pass over the scores takes nothing but the log-sum-exp
+// and the largest of every group of 32 classes (a lane's share of the 2048 classes a wave reads at a time), kept in
+// LDS.  The k-th largest of those maxima is a bound that at least k scores reach and hardly more (a k of a
+// quarter of the groups: 1.15 k of normal scores); the groups that reach it, which L2 still holds for the
+// most part, are read again and offered to the candidates.
+constexpr uint32_t kMaxGroupSegs = 64;
+template <class T, bool kUnit, int THREADS, int CAP>
+__global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t k, float c, double inv_t,
+                                                             uint32_t parts, uint32_t seg, float* __restrict__ values,
+                                                             int32_t* __restrict__ index, float* __restrict__ lse,
+                                                             u64* __restrict__ part_keys,
+                                                             float2* __restrict__ part_ms) {
+    constexpr int V = Pack<T>::V, U = kGroup / V, W = THREADS / 64, KMAX = CAP / 2;
+    extern __shared__ uint32_t groups[];
+    __shared__ u64 cand[W][CAP];
+    __shared__ u64 best[KMAX];
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t counts[W], nbest;
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
+    auto cand_at = [&](uint32_t i) -> u64 { return i % CAP < counts[i / CAP] ? cand[i / CAP][i % CAP] : 0; };
+
+    for (uint64_t job = blockIdx.x; job < X.rows * parts; job += gridDim.x) {
+        const uint64_t row = job / parts;
+        const uint32_t first = (uint32_t)(job % parts) * seg, n = min(X.classes - first, seg);
+        const T* x0 = X.data + (int64_t)row * X.rs + (int64_t)first * X.cs;
+        const uint32_t n_segs = (n + kSeg - 1) / kSeg;
+        Running run;
+        for (uint32_t s = wave; s < n_segs; s += W) {
+            float x[U][V], gm = -INFINITY;
+            load_tile<T, kUnit>(x0, X.cs, s * kSeg, n, -INFINITY, x);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) gm = fmaxf(gm, x[u][v]);
+            run.raise(gm, c);
+            run.add(x, c);
+            if (run.s != run.s) {   // since a NaN, which is the largest of its group, or +inf
+                bool nan = false;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) nan |= x[u][v] != x[u][v];
+                gm = nan ? NAN : gm;
+            }
+            groups[s * 64 + lane] = s * kSeg + lane * V < n ? order_key(gm) : 0;
+        }
+        __syncthreads();
+        const u64 kth_group = block_kth<THREADS>([&](uint32_t i) { return (u64)groups[i] << 32; }, n_segs * 64, k, 32, hist);
+        Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
+        C.set_bound(kth_group);
+        const uint32_t bound = (uint32_t)(kth_group >> 32);
+        for (uint32_t s = wave; s < n_segs; s += W) {
+            u64 hit = __ballot(groups[s * 64 + lane] >= bound);
+            while (hit) {   // two groups at a time, a class a lane
+                const uint32_t a = (uint32_t)__builtin_ctzll(hit);
+                hit &= hit - 1;
+                const uint32_t b = hit ? (uint32_t)__builtin_ctzll(hit) : 64;
+                hit &= hit - 1;
+                const uint32_t ln = lane < kGroup ? a : b, q = lane % kGroup;
+                const uint32_t i = s * kSeg + (q / V * 64 + ln) * V + q % V;
+                const bool have = ln < 64 && i < n;
+                const float x = have ? to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * X.cs]) : -INFINITY;
+                C.offer(x, first + i, have, k);
+            }
+        }
+        if ((threadIdx.x & 63) == 0) counts[wave] = C.count;
+        if (threadIdx.x == 0) nbest = 0;
+        float m;
+        double sum;
+        __syncthreads();
+        block_running<THREADS>(run, c, m, sum, tmp_f, tmp_d);
+        uint32_t total = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) total += counts[w];
+        u64 kth = 1;
+        if (total > k) kth = block_kth<THREADS>(cand_at, W * CAP, k, 0, hist);
+        for (uint32_t i = threadIdx.x; i < W * CAP; i += THREADS) {
+            const u64 key = cand_at(i);
+            if (key >= kth) best[atomicAdd(&nbest, 1u)] = key;
+        }
+        __syncthreads();
+        if (parts == 1) {
+            for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
+                const u64 key = best[i];
+                uint32_t rank = 0;
+                for (uint32_t j = 0; j < k; ++j) rank += best[j] > key;
+                values[row * k + rank] = key_score((uint32_t)(key >> 32));
+                index[row * k + rank] = (int32_t)~(uint32_t)key;
+            }
+            if (threadIdx.x == 0) lse[row] = m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(sum));
+        } else {
+            for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = best[i];
+            if (threadIdx.x == 0) part_ms[job] = float2{m, (float)sum};
+        }
+        __syncthreads();
+    }
+}
+
 // The segments of a row together.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ part_keys,
@@ -279,10 +379,12 @@ __global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, flo
 }
 
 // Segments of a row: one, unless the rows alone leave CUs idle and a row is long.
-constexpr uint32_t kMinSeg = 16384;
+constexpr uint32_t kMinSeg = 16384, kMaxSeg = kMaxGroupSegs * kSeg;
 uint32_t plan_parts(uint64_t rows, uint32_t classes) {
-    if (rows == 0 || rows >= 512 || classes < 2 * kMinSeg) return 1;
-    return (uint32_t)std::min<uint64_t>((512 + rows - 1) / rows, classes / kMinSeg);
+    uint32_t parts = (classes + kMaxSeg - 1) / kMaxSeg;
+    if (rows > 0 && rows < 512 && classes >= 2 * kMinSeg)
+        parts = std::max(parts, (uint32_t)std::min<uint64_t>((512 + rows - 1) / rows, classes / kMinSeg));
+    return parts;
 }
 
 template <class T, bool kUnit>
@@ -303,6 +405,13 @@ int launch_top(const Rows<T>& X, uint32_t k, double t, float* values, int32_t* i
     u64* pk = (u64*)workspace;
     float2* pm = parts > 1 ? (float2*)(pk + X.rows * parts * k) : nullptr;
     const unsigned grid = row_grid(X.rows * parts);
+    // by groups where k is at most a quarter of the shortest segment's
+    const uint32_t shortest = n - seg * (parts - 1);
+    if (n > 2048 && k * 4 <= shortest / kGroup && seg <= kMaxGroupSegs * kSeg) {
+        const size_t lds = sizeof(uint32_t) * 64 * ((seg + kSeg - 1) / kSeg);
+        if (k <= 128) top_groups_kernel<T, kUnit, 256, 256><<<grid, 256, lds, st>>>(X, k, c, it, parts, seg, values, index, lse, pk, pm);
+        else top_groups_kernel<T, kUnit, 256, 2048><<<grid, 256, lds, st>>>(X, k, c, it, parts, seg, values, index, lse, pk, pm);
+    } else
 #define TOP(TH, CAP) top_kernel<T, kUnit, TH, CAP><<<grid, TH, 0, st>>>(X, k, c, it, parts, seg, values, index, lse, pk, pm)
     if (n <= 2048) {
         if (k <= 128) TOP(64, 256);
