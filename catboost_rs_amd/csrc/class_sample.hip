@@ -418,12 +418,12 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
 // histogram of counts or masses over the distance from the largest score; those, or those of the one
 // bin in which the cut lies, are listed, and the list cut exactly in registers.  Kept masses of the
 // bins above a nucleus's last are summed by segments, and the draw looks through one of them.
-constexpr uint32_t kGroupSegs = 128;
+constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
 constexpr float kBinsPerNat = 32.0f;
 __device__ __forceinline__ uint32_t bin_at(uint32_t b) { return b + (b >> 4); }   // (its place in LDS)
 
-enum Mode : uint32_t { kGreedy, kWhole, kList, kNucleus, kSlow };
+enum Mode : uint32_t { kGreedy, kWhole, kList, kNucleus };   // (kWhole: a least weight above 1 as well)
 
 template <class T, bool kUnit, int THREADS>
 struct Long {
@@ -471,13 +471,14 @@ struct Long {
         return to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * cs]);
     }
     __device__ __forceinline__ Mode mode() const {
-        return r.greedy || r.min_p > 1.0 ? kGreedy : r.k ? kList : r.p < 1.0 ? kNucleus : kWhole;
+        return r.greedy ? kGreedy : r.min_p > 1.0 ? kWhole : r.k ? kList : r.p < 1.0 ? kNucleus : kWhole;
     }
     // top_k from the groups' maxes: a quarter of them at most, so that few classes beside the k largest reach
     // the k-th of the maxima; 2^18 classes at most (32 KB of maxima)
-    __device__ __forceinline__ bool by_groups(uint32_t segs) const {
-        return segs <= kGroupSegs && r.k <= segs * 16 && r.k * 4 <= (uint32_t)CAP;
+    __host__ __device__ static bool by_groups_of(uint32_t k, uint32_t segs) {
+        return segs <= kGroupSegs && k <= segs * 16 && k <= kMostByGroups;
     }
+    __device__ __forceinline__ bool by_groups(uint32_t segs) const { return by_groups_of(r.k, segs); }
 
     // Largest score of the segments [s0, s1) and the segment it was first met in, per thread; into `groups`
     // (nullable) every group's largest as an order key (0: nothing to draw); with `sums` the running softmax
@@ -550,14 +551,37 @@ struct Long {
                     } else if (y > -INFINITY) {
                         atomicAdd((uint32_t*)&hist[bin_at(bin(y))], 1u);
                     }
+                    if (v == V - 1) __builtin_amdgcn_sched_barrier(0);
                 }
         }
     }
-    // Kept masses of the segments: of all classes of at least `least` (cut = kBins), or of those in the bins
-    // before `cut`; the classes in bin `cut`, and with `all` those before, go to the list.
+    // Masses of the segments, of the classes of at least `least`; the mass of all classes, per thread.
+    __device__ __forceinline__ u64 weigh(uint32_t s0, uint32_t s1, const Masses& M, u64 least, u64* segs) const {
+        u64 all = 0;
+        for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
+            float x[U][V];
+            load(seg, x);
+            u64 sum = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const u64 w = M(x[u][v]);
+                    all += w;
+                    sum += w >= least ? w : 0;
+                }
+                __builtin_amdgcn_sched_barrier(0);   // (one vector's masses at a time: registers)
+            }
+            sum = wave_reduce(sum, Add());
+            if (lane == 0) segs[seg] = sum;
+        }
+        return all;
+    }
+    // The classes in bin `cut`, and with `all` those in the bins before, go to the list (at most cap; count goes
+    // on); with kSum the masses of the bins before go to their segments.
     template <bool kSum>
     __device__ __forceinline__ void collect(uint32_t s0, uint32_t s1, const Masses& M, uint32_t cut, bool all, u64 least,
-                                            u64* segs, u64* list, uint32_t* count) const {
+                                            u64* segs, u64* list, uint32_t* count, uint32_t cap) const {
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             u64 sum = 0;
             float xs[U][V];
@@ -569,12 +593,12 @@ struct Long {
                 uint32_t hits = 0;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const uint32_t b = cut < kBins ? bin(x[v]) : 0;
-                    if (kSum && (cut == kBins || b < cut)) {
+                    const uint32_t b = bin(x[v]);
+                    if (kSum && b < cut) {
                         const u64 w = M(x[v]);
                         sum += w >= least ? w : 0;
                     }
-                    if (cut < kBins && x[v] > -INFINITY && (b == cut || (all && b < cut))) hits |= 1u << v;
+                    if (x[v] > -INFINITY && (b == cut || (all && b < cut))) hits |= 1u << v;
                 }
                 while (__any(hits != 0)) {
                     const bool in = hits != 0;
@@ -586,7 +610,7 @@ struct Long {
                     uint32_t base = 0;
                     if (lane == 0) base = atomicAdd(count, (uint32_t)__popcll(b));
                     base = __builtin_amdgcn_readfirstlane(base) + (uint32_t)__popcll(b & ((1ull << lane) - 1));
-                    if (in && base < (uint32_t)CAP) list[base] = rank_key(z, i + v);
+                    if (in && base < cap) list[base] = rank_key(z, i + v);
                     hits &= hits - 1;
                 }
             }
@@ -708,6 +732,11 @@ struct Long {
         for (uint32_t i = threadIdx.x; i < n; i += THREADS)
             if (key_at(i)) total += mass(score(i));
         total = block_reduce<THREADS>(total, Add(), tmp);
+        if (r.min_p > 1.0) {
+            if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)total, -S)));
+            __syncthreads();
+            return;
+        }
         u64 from = 0;   // ranks below it are cut
         u64 have = 0, kept = total;
         for (uint32_t i = threadIdx.x; i < n; i += THREADS) have += key_at(i) != 0;
@@ -789,7 +818,7 @@ __device__ __forceinline__ Found<u64> find_cut(Get get, u64 want) {
     return Found<u64>{(uint32_t)__shfl(b, at), __shfl(above, at), __shfl(inside, at)};
 }
 
-// A workgroup a row, all steps in one launch.
+// Up to 8192 classes: a workgroup a row, all steps in one launch.
 template <class T, bool kUnit, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Settings S, int shift, Out out) {
     typedef Long<T, kUnit, THREADS> L;
@@ -822,12 +851,10 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
             if (threadIdx.x == 0) out.empty(row);
             continue;
         }
-        const bool slow_only = m == INFINITY;
+        bool slow = m == INFINITY;
         uint32_t first = 0;
-        if (mode == kGreedy) {
-            const uint32_t f = R.first_at(m, best, best_seg);
-            u64 lo = block_reduce<THREADS>((u64)f, [](u64 a, u64 b) { return a < b ? a : b; }, tmp);
-            first = (uint32_t)lo;
+        if (R.r.greedy || R.r.min_p > 1.0) {
+            first = (uint32_t)block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), [](u64 a, u64 b) { return a < b ? a : b; }, tmp);
             if (R.r.greedy) {
                 if (threadIdx.x == 0) out.put(row, first, 0.0);
                 continue;
@@ -835,39 +862,16 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
         }
         const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
         R.set_bins(m);
-        bool slow = slow_only;
-        if (!slow && mode == kGreedy) {   // (a least weight above 1: the first class, with its log probability)
-            u64 z = 0;
-            for (uint32_t seg = R.wave; seg < n_segs; seg += W)
-                for (int u = 0; u < L::U; ++u) {
-                    float x[L::V];
-                    R.load(R.at(seg, u, R.lane), x);
-#pragma unroll
-                    for (int v = 0; v < L::V; ++v) z += M(x[v]);
-                }
-            z = block_reduce<THREADS>(z, Add(), tmp);
-            if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)z, -shift)));
-            continue;
-        }
-        if (slow && mode == kGreedy) {
-            u64 z = 0;
-            for (uint32_t i = threadIdx.x; i < R.n; i += THREADS) z += R.score(i) == INFINITY;
-            z = block_reduce<THREADS>(z, Add(), tmp);
-            if (threadIdx.x == 0) out.put(row, first, -log((double)z));
-            continue;
-        }
         if (!slow && mode == kWhole) {
             const u64 least = least_mass(R.r.min_p, shift);
-            R.template collect<true>(0, n_segs, M, kBins, false, 0, segs, list, &count);
-            __syncthreads();
-            u64 z = 0;
-            for (uint32_t s = threadIdx.x; s < n_segs; s += THREADS) z += segs[s];
+            u64 z = R.weigh(0, n_segs, M, R.r.min_p > 1.0 ? 0 : least, segs);
             z = block_reduce<THREADS>(z, Add(), tmp);
-            if (least > 0) {
-                R.template collect<true>(0, n_segs, M, kBins, false, least, segs, list, &count);
-                __syncthreads();
+            __syncthreads();
+            if (R.r.min_p > 1.0) {
+                if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)z, -shift)));
+            } else {
+                R.finish_segments(segs, n_segs, M, kBins, 0, least, z, row, tmp, pick, out);
             }
-            R.finish_segments(segs, n_segs, M, kBins, 0, least, z, row, tmp, pick, out);
         } else if (!slow && mode == kNucleus) {
             R.template histogram<true>(0, n_segs, M, hist);
             __syncthreads();
@@ -876,7 +880,7 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
             z = block_reduce<THREADS>(z, Add(), tmp);
             const u64 want = nucleus_of(R.r.p, z), least = least_mass(R.r.min_p, shift);
             const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
-            R.template collect<true>(0, n_segs, M, f.bin, false, least, segs, list, &count);
+            R.template collect<true>(0, n_segs, M, f.bin, false, least, segs, list, &count, L::CAP);
             __syncthreads();
             if (count > (uint32_t)L::CAP) {
                 slow = true;
@@ -928,7 +932,7 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
                 if (f.above + f.inside > (u64)L::CAP) {
                     slow = true;
                 } else {
-                    R.template collect<false>(0, n_segs, M, f.bin, true, 0, segs, list, &count);
+                    R.template collect<false>(0, n_segs, M, f.bin, true, 0, nullptr, list, &count, L::CAP);
                     __syncthreads();
                 }
             }
@@ -939,6 +943,241 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
     }
 }
 
+// Rows of more than 8192 classes: the steps as launches of their own, `parts` workgroups a row, so that a few
+// rows fill the CUs and every step has the registers it needs (all steps in one launch of 1024 threads spilled
+// 110 registers: 256 x 131072 f32 with settings a row took 189 to 287 us).  Between the launches, per row:
+struct Top {      // of a part: its largest score (order key) over ~(its first class); the softmax denominator
+    u64 key;
+    float m, s;
+};
+struct Step {     // where the cut lies
+    u64 total, above;   // mass of all classes; weight of the bins before the cut's
+    uint32_t bin, state;
+};
+enum State : uint32_t { kCut, kOverflow };
+struct Space {    // the workspace of a chunk of rows
+    Top* tops;          // [rows][parts1]
+    uint32_t* groups;   // [rows][64 segs], nullable
+    u64* hist;          // [rows][parts2][kBins]
+    u64* segs;          // [rows][n_segs]
+    u64* list;          // [rows][kListCap]
+    uint32_t* count;    // [rows]
+    Step* steps;        // [rows]
+    u64* totals;        // [rows][parts2]
+    uint32_t parts1, per1, parts2, per2, n_segs;   // parts of a row and segments a part: of the scan, of the rest
+};
+constexpr uint32_t kListCap = 8192;
+
+template <int THREADS>
+__device__ __forceinline__ u64 row_top(const Space& P, uint64_t row, u64* tmp) {
+    u64 top = 0;
+    for (uint32_t p = threadIdx.x; p < P.parts1; p += THREADS) {
+        const u64 k = P.tops[row * P.parts1 + p].key;
+        top = k > top ? k : top;
+    }
+    return block_reduce<THREADS>(top, [](u64 a, u64 b) { return a > b ? a : b; }, tmp);
+}
+
+template <class T, bool kUnit>
+__global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
+    constexpr int THREADS = 256;
+    __shared__ float tmp_f[4];
+    __shared__ double tmp_d[4];
+    __shared__ u64 tmp[4];
+    const uint64_t row = blockIdx.x / P.parts1;
+    const uint32_t part = blockIdx.x % P.parts1, s0 = part * P.per1, s1 = min(P.n_segs, s0 + P.per1);
+    Long<T, kUnit, THREADS> R(X, S, row, shift);
+    const Mode mode = R.mode();
+    const float c = (float)(R.r.rt * 1.4426950408889634);
+    float best;
+    uint32_t best_seg;
+    Running run;
+    R.scan(s0, s1, mode == kList && R.by_groups(P.n_segs) ? P.groups + row * P.n_segs * 64 + s0 * 64 : nullptr, mode == kList,
+           c, best, best_seg, run);
+    const float m = block_reduce<THREADS>(best, MaxF(), tmp_f);
+    u64 first = 0xFFFFFFFFu;
+    if (R.r.greedy || R.r.min_p > 1.0)
+        first = block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), [](u64 a, u64 b) { return a < b ? a : b; }, tmp);
+    float rm = 0.0f;
+    double rs = 0.0;
+    if (mode == kList) block_running<THREADS>(run, c, rm, rs, tmp_f, tmp_d);
+    if (threadIdx.x == 0) {
+        P.tops[row * P.parts1 + part] = Top{m == -INFINITY ? 0 : (u64)order_key(m) << 32 | (uint32_t)~first, rm, (float)rs};
+        if (part == 0) P.count[row] = 0;
+    }
+}
+
+// Masses of the segments, or the part's histogram of masses or counts.
+template <class T, bool kUnit>
+__global__ __launch_bounds__(512) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
+    constexpr int THREADS = 512;
+    __shared__ u64 hist[kBinsPad];
+    __shared__ u64 tmp[THREADS / 64];
+    const uint64_t row = blockIdx.x / P.parts2;
+    const uint32_t part = blockIdx.x % P.parts2, s0 = part * P.per2, s1 = min(P.n_segs, s0 + P.per2);
+    Long<T, kUnit, THREADS> R(X, S, row, shift);
+    const Mode mode = R.mode();
+    if (mode == kGreedy || (mode == kList && P.groups && R.by_groups(P.n_segs))) return;
+    const u64 top = row_top<THREADS>(P, row, tmp);
+    const float m = key_score((uint32_t)(top >> 32));
+    if (top == 0 || m == INFINITY) return;
+    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+    if (mode == kWhole) {
+        u64 all = R.weigh(s0, s1, M, R.r.min_p > 1.0 ? 0 : least_mass(R.r.min_p, shift), P.segs + row * P.n_segs);
+        all = block_reduce<THREADS>(all, Add(), tmp);
+        if (threadIdx.x == 0) P.totals[row * P.parts2 + part] = all;
+        return;
+    }
+    for (uint32_t b = threadIdx.x; b < kBinsPad; b += THREADS) hist[b] = 0;
+    __syncthreads();
+    R.set_bins(m);
+    if (mode == kNucleus) R.template histogram<true>(s0, s1, M, hist);
+    else R.template histogram<false>(s0, s1, M, hist);
+    __syncthreads();
+    u64* to = P.hist + (row * P.parts2 + part) * kBins;
+    for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) to[b] = hist[bin_at(b)];
+}
+
+// The classes of the cut's bin (top_k: and of those before), and the segments' masses before it.
+template <class T, bool kUnit>
+__global__ __launch_bounds__(512) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
+    constexpr int THREADS = 512;
+    __shared__ u64 hist[kBinsPad];
+    __shared__ u64 tmp[THREADS / 64];
+    const uint64_t row = blockIdx.x / P.parts2;
+    const uint32_t part = blockIdx.x % P.parts2, s0 = part * P.per2, s1 = min(P.n_segs, s0 + P.per2);
+    Long<T, kUnit, THREADS> R(X, S, row, shift);
+    const Mode mode = R.mode();
+    if (mode != kNucleus && !(mode == kList && !(P.groups && R.by_groups(P.n_segs)))) return;
+    const u64 top = row_top<THREADS>(P, row, tmp);
+    const float m = key_score((uint32_t)(top >> 32));
+    if (top == 0 || m == INFINITY) return;
+    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+    R.set_bins(m);
+    u64 total = 0;
+    for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) {
+        u64 h = 0;
+        for (uint32_t p = 0; p < P.parts2; ++p) h += P.hist[(row * P.parts2 + p) * kBins + b];
+        hist[bin_at(b)] = h;
+        total += h;
+    }
+    total = block_reduce<THREADS>(total, Add(), tmp);
+    __syncthreads();
+    const u64 want = mode == kNucleus ? nucleus_of(R.r.p, total) : total < R.r.k ? total : (u64)R.r.k;
+    const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
+    const bool over = mode == kList && f.above + f.inside > kListCap;
+    if (part == 0 && threadIdx.x == 0) P.steps[row] = Step{total, f.above, f.bin, over ? kOverflow : kCut};
+    if (over) return;
+    u64* list = P.list + row * kListCap;
+    if (mode == kNucleus)
+        R.template collect<true>(s0, s1, M, f.bin, false, least_mass(R.r.min_p, shift), P.segs + row * P.n_segs, list, &P.count[row], kListCap);
+    else
+        R.template collect<false>(s0, s1, M, f.bin, true, 0, nullptr, list, &P.count[row], kListCap);
+}
+
+// A workgroup a row: the exact cut, and the draw.
+template <class T, bool kUnit>
+__global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
+    constexpr int THREADS = 1024, W = THREADS / 64;
+    typedef Long<T, kUnit, THREADS> L;
+    extern __shared__ u64 pool[];   // the row's groups and their list, or its segments' masses
+    __shared__ SelectLds lds;
+    __shared__ u64 tmp[W], pick[2];
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    __shared__ uint32_t count, khist[256];
+    const uint64_t row = blockIdx.x;
+    L R(X, S, row, shift);
+    const Mode mode = R.mode();
+    const u64 top = row_top<THREADS>(P, row, tmp);
+    if (top == 0) {
+        if (threadIdx.x == 0) out.empty(row);
+        return;
+    }
+    const float m = key_score((uint32_t)(top >> 32));
+    const uint32_t first = ~(uint32_t)top;
+    if (mode == kGreedy) {
+        if (threadIdx.x == 0) out.put(row, first, 0.0);
+        return;
+    }
+    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+    const bool by_groups = mode == kList && P.groups && R.by_groups(P.n_segs);
+    bool slow = m == INFINITY;
+    if (!slow && mode == kWhole) {
+        u64 total = 0;
+        for (uint32_t p = threadIdx.x; p < P.parts2; p += THREADS) total += P.totals[row * P.parts2 + p];
+        total = block_reduce<THREADS>(total, Add(), tmp);
+        if (R.r.min_p > 1.0) {
+            if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)total, -shift)));
+            return;
+        }
+        R.finish_segments(P.segs + row * P.n_segs, P.n_segs, M, kBins, 0, least_mass(R.r.min_p, shift), total, row, tmp, pick, out);
+        return;
+    }
+    if (!slow && mode == kNucleus) {
+        const Step step = P.steps[row];
+        const uint32_t n_list = P.count[row];
+        const u64 least = least_mass(R.r.min_p, shift);
+        slow = n_list > kListCap;
+        if (!slow) {
+            for (uint32_t s = threadIdx.x; s < P.n_segs; s += THREADS) pool[s] = P.segs[row * P.n_segs + s];
+            Entries<THREADS, 8> E;
+            R.read_list(E, P.list + row * kListCap, n_list);
+            E.weigh(M);
+            __syncthreads();
+            const Crossing x = select<THREADS, true, true>(
+                [&](auto g) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (E.key[e] && E.mass[e]) g(E.rank(e), E.mass[e]);
+                },
+                nucleus_of(R.r.p, step.total) - step.above, 56, &lds);
+            E.keep_from(x);
+            E.drop_below(least);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (E.key[e] && E.mass[e]) atomicAdd(&pool[E.idx[e] / kSeg], E.mass[e]);
+            __syncthreads();
+            R.set_bins(m);
+            R.finish_segments(pool, P.n_segs, M, step.bin, x.prefix << x.shift, least, step.total, row, tmp, pick, out);
+            return;
+        }
+    }
+    if (!slow && mode == kList) {
+        Running run;
+        for (uint32_t p = threadIdx.x; p < P.parts1; p += THREADS) {
+            const Top t = P.tops[row * P.parts1 + p];
+            run.join(t.m, t.s, (float)(R.r.rt * 1.4426950408889634));
+        }
+        float mr;
+        double sr;
+        block_running<THREADS>(run, (float)(R.r.rt * 1.4426950408889634), mr, sr, tmp_f, tmp_d);
+        const double log_z = log(sr);
+        if (by_groups) {
+            uint32_t* groups = (uint32_t*)(pool + kListCap);
+            u64 have = 0;
+            for (uint32_t g = threadIdx.x; g < P.n_segs * 64; g += THREADS) {
+                groups[g] = P.groups[row * P.n_segs * 64 + g];
+                have += groups[g] != 0;
+            }
+            if (threadIdx.x == 0) count = 0;
+            have = block_reduce<THREADS>(have, Add(), tmp);
+            __syncthreads();
+            u64 kth = 0;   // (fewer groups than k: all that is allowed is listed)
+            if (have >= R.r.k)
+                kth = block_kth<THREADS>([&](uint32_t i) { return (u64)groups[i] << 32; }, P.n_segs * 64, R.r.k, 32, khist);
+            R.gather(P.n_segs, groups, (uint32_t)(kth >> 32), pool, &count);
+            __syncthreads();
+            slow = count > kListCap;
+            if (!slow) R.finish_list(pool, count, M, log_z, row, &lds, tmp, out);
+        } else {
+            slow = P.steps[row].state == kOverflow;
+            if (!slow) R.finish_list(P.list + row * kListCap, P.count[row], M, log_z, row, &lds, tmp, out);
+        }
+    }
+    if (slow) R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
+}
+
 // Masses are sums of at most n weights of 1: they stay below 2^63.
 int shift_of(uint32_t n) {
     int b = 0;
@@ -946,20 +1185,99 @@ int shift_of(uint32_t n) {
     return std::min(51, 62 - b);
 }
 
-template <class T, bool kUnit, int THREADS>
-int launch_long(const Rows<T>& X, const Settings& S, int shift, const Out& out, hipStream_t st) {
-    typedef Long<T, kUnit, THREADS> L;
+template <class T, bool kUnit>
+int launch_mid(const Rows<T>& X, const Settings& S, int shift, const Out& out, hipStream_t st) {
+    typedef Long<T, kUnit, 256> L;
     const size_t n_segs = (X.classes + kSeg - 1) / kSeg;
-    const size_t lds = sizeof(u64) * (L::CAP + n_segs) + (n_segs <= kGroupSegs ? sizeof(uint32_t) * 64 * n_segs : 0);
-    CLS_TRY(hipFuncSetAttribute((const void*)sample_long_kernel<T, kUnit, THREADS>,
-                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    sample_long_kernel<T, kUnit, THREADS><<<row_grid(X.rows), THREADS, lds, st>>>(X, S, shift, out);
+    const size_t lds = sizeof(u64) * (L::CAP + n_segs) + sizeof(uint32_t) * 64 * n_segs;
+    sample_long_kernel<T, kUnit, 256><<<row_grid(X.rows), 256, lds, st>>>(X, S, shift, out);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
 
+// Long rows in chunks (the workspace stays below 64 MB up to 2^18 classes), each of at least 4 million scores.
+constexpr uint64_t kChunkRows = 512;
+constexpr uint32_t kMidClasses = 8192;
+size_t align64(size_t v) { return (v + 63) & ~(size_t)63; }
+// Parts of a row: the scan's workgroups of 4 waves take a tile each where the rows are few, 8 tiles where
+// they fill the chip; the others (8 waves) likewise, with histograms to pay for.
+Space plan(uint64_t rows, uint32_t n, unsigned char* base, size_t* bytes) {
+    Space P{};
+    P.n_segs = (n + kSeg - 1) / kSeg;
+    auto split = [&](uint64_t wgs, uint32_t waves, uint32_t& parts, uint32_t& per) {
+        const uint64_t want = std::max<uint64_t>(1, wgs / rows);
+        const uint32_t most = (P.n_segs + waves - 1) / waves;
+        parts = (uint32_t)std::min<uint64_t>(want, most);
+        per = (P.n_segs + parts - 1) / parts;
+        parts = (P.n_segs + per - 1) / per;
+    };
+    split(2048, 4, P.parts1, P.per1);
+    split(1024, 8, P.parts2, P.per2);
+    size_t at = 0;
+    auto take = [&](size_t size) {
+        const size_t a = at;
+        at += align64(size);
+        return base ? base + a : nullptr;
+    };
+    P.tops = (Top*)take(sizeof(Top) * rows * P.parts1);
+    P.groups = (uint32_t*)take(P.n_segs <= kGroupSegs ? sizeof(uint32_t) * 64 * P.n_segs * rows : 0);
+    if (P.n_segs > kGroupSegs) P.groups = nullptr;
+    P.hist = (u64*)take(sizeof(u64) * kBins * P.parts2 * rows);
+    P.segs = (u64*)take(sizeof(u64) * P.n_segs * rows);
+    P.list = (u64*)take(sizeof(u64) * kListCap * rows);
+    P.count = (uint32_t*)take(sizeof(uint32_t) * rows);
+    P.steps = (Step*)take(sizeof(Step) * rows);
+    P.totals = (u64*)take(sizeof(u64) * P.parts2 * rows);
+    *bytes = at;
+    return P;
+}
+
 template <class T, bool kUnit>
-int launch_sample(const Rows<T>& X, const Settings& S, const Out& out, hipStream_t st) {
+int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out, void* workspace, hipStream_t st) {
+    // what the settings can ask for (settings a row: anything)
+    const bool all_greedy = !S.t_rows && !(S.t > 0.0), any_list = S.k_rows || (S.k && S.k < X.classes);
+    const bool all_list = !S.k_rows && any_list && !(S.min_p_rows || S.min_p > 1.0);
+    const uint32_t n_segs = (X.classes + kSeg - 1) / kSeg;
+    const bool list_by_groups = all_list && Long<T, kUnit, 1024>::by_groups_of(S.k, n_segs);
+    const bool any_cut = S.k_rows || S.p_rows || S.p < 1.0 || any_list;
+    for (uint64_t r0 = 0; r0 < X.rows; r0 += kChunkRows) {
+        const uint64_t m = std::min(kChunkRows, X.rows - r0);
+        size_t bytes = 0;
+        const Space P = plan(m, X.classes, (unsigned char*)workspace, &bytes);
+        Rows<T> C = X;
+        C.data += (int64_t)r0 * X.rs;
+        C.rows = m;
+        Settings Q = S;
+        Q.uniform += r0;
+        if (Q.t_rows) Q.t_rows += r0;
+        if (Q.k_rows) Q.k_rows += r0;
+        if (Q.p_rows) Q.p_rows += r0;
+        if (Q.min_p_rows) Q.min_p_rows += r0;
+        if (Q.allowed) Q.allowed += (int64_t)r0 * Q.allowed_stride;
+        const Out o{out.index + r0, out.logprob ? out.logprob + r0 : nullptr};
+        scan_kernel<T, kUnit><<<(unsigned)(m * P.parts1), 256, 0, st>>>(C, Q, shift, o, P);
+        CLS_TRY(hipGetLastError());
+        if (!all_greedy && !list_by_groups) {
+            weigh_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 512, 0, st>>>(C, Q, shift, P);
+            CLS_TRY(hipGetLastError());
+            if (any_cut) {
+                collect_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 512, 0, st>>>(C, Q, shift, P);
+                CLS_TRY(hipGetLastError());
+            }
+        }
+        // LDS: a list and the groups, or the segments
+        size_t lds = any_list && P.groups ? sizeof(u64) * kListCap + sizeof(uint32_t) * 64 * P.n_segs : 0;
+        lds = std::max(lds, sizeof(u64) * P.n_segs);
+        if (lds > 32 * 1024)
+            CLS_TRY(hipFuncSetAttribute((const void*)draw_kernel<T, kUnit>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        draw_kernel<T, kUnit><<<(unsigned)m, 1024, lds, st>>>(C, Q, shift, o, P);
+        CLS_TRY(hipGetLastError());
+    }
+    return CBH_OK;
+}
+
+template <class T, bool kUnit>
+int launch_sample(const Rows<T>& X, const Settings& S, const Out& out, void* workspace, hipStream_t st) {
     const uint32_t n = X.classes;
     const int shift = shift_of(n);
     if (n <= 32) {
@@ -972,23 +1290,33 @@ int launch_sample(const Rows<T>& X, const Settings& S, const Out& out, hipStream
         else sample_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, S, out);
     } else if (n <= 512) sample_short_kernel<T, kUnit, 64><<<row_grid(X.rows), 64, 0, st>>>(X, S, shift, out);
     else if (n <= 2048) sample_short_kernel<T, kUnit, 256><<<row_grid(X.rows), 256, 0, st>>>(X, S, shift, out);
-    else if (n <= 8192) return launch_long<T, kUnit, 256>(X, S, shift, out, st);
-    else return launch_long<T, kUnit, 1024>(X, S, shift, out, st);
+    else if (n <= kMidClasses) return launch_mid<T, kUnit>(X, S, shift, out, st);
+    else return launch_split<T, kUnit>(X, S, shift, out, workspace, st);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
 
 template <class T>
 int run_sample(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t cs, const Settings& S, int32_t* index,
-               float* logprob, hipStream_t st) {
+               float* logprob, void* workspace, hipStream_t st) {
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
     const Out out{index, logprob};
-    return cs == 1 ? launch_sample<T, true>(X, S, out, st) : launch_sample<T, false>(X, S, out, st);
+    return cs == 1 ? launch_sample<T, true>(X, S, out, workspace, st) : launch_sample<T, false>(X, S, out, workspace, st);
 }
 
 }  // namespace
 
-extern "C" uint64_t cbh_sample_classes_workspace(uint64_t rows, uint32_t classes) { return 0; }
+extern "C" uint64_t cbh_sample_classes_workspace(uint64_t rows, uint32_t classes) {
+    if (rows == 0 || classes <= kMidClasses) return 0;
+    // a last chunk of fewer rows has more parts a row, and at most as many in all as a full one may have
+    size_t most = 0, bytes = 0;
+    (void)plan(std::min(rows, kChunkRows), classes, nullptr, &most);
+    if (rows > kChunkRows && rows % kChunkRows) {
+        (void)plan(rows % kChunkRows, classes, nullptr, &bytes);
+        most = std::max(most, bytes);
+    }
+    return most;
+}
 
 extern "C" int cbh_sample_classes(const void* scores, int32_t type, uint64_t rows, uint32_t classes,
                                   int64_t row_stride, int64_t class_stride, const double* uniform, double temperature,
@@ -1013,11 +1341,11 @@ extern "C" int cbh_sample_classes(const void* scores, int32_t type, uint64_t row
         hipStream_t st = (hipStream_t)stream;
         switch (type) {
             case CBH_TYPE_F32:
-                return run_sample<float>(scores, rows, classes, row_stride, class_stride, S, index, logprob, st);
+                return run_sample<float>(scores, rows, classes, row_stride, class_stride, S, index, logprob, workspace, st);
             case CBH_TYPE_F16:
-                return run_sample<_Float16>(scores, rows, classes, row_stride, class_stride, S, index, logprob, st);
+                return run_sample<_Float16>(scores, rows, classes, row_stride, class_stride, S, index, logprob, workspace, st);
             default:
-                return run_sample<bf16_t>(scores, rows, classes, row_stride, class_stride, S, index, logprob, st);
+                return run_sample<bf16_t>(scores, rows, classes, row_stride, class_stride, S, index, logprob, workspace, st);
         }
     } catch (const std::exception& e) {
         return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
