@@ -44,30 +44,34 @@ __device__ __forceinline__ Row settings(const Settings& S, uint64_t row, uint32_
 __device__ __forceinline__ uint32_t class_key(float x, bool allowed) {
     return allowed && x > -INFINITY ? order_key(x) : 0;
 }
-// 2^f for |f| <= 1/2: the terms (f ln 2)^i / i! up to i = 11 (what is left out is below 2^-47).
+// 2^f for |f| <= 1/2, within 2^-44, and exactly 1 at 0: 1 + f q(f), q the polynomial of degree 8 that meets
+// (2^f - 1) / f in the Chebyshev points of the interval.
 __device__ __forceinline__ double exp2_part(double f) {
-    double p = 4.4455382718708116e-10;
-    p = __builtin_fma(p, f, 7.0549116208011235e-09);
-    p = __builtin_fma(p, f, 1.0178086009239699e-07);
-    p = __builtin_fma(p, f, 1.3215486790144307e-06);
-    p = __builtin_fma(p, f, 1.5252733804059841e-05);
-    p = __builtin_fma(p, f, 1.5403530393381609e-04);
-    p = __builtin_fma(p, f, 1.3333558146428443e-03);
-    p = __builtin_fma(p, f, 9.6181291076284772e-03);
-    p = __builtin_fma(p, f, 5.5504108664821580e-02);
-    p = __builtin_fma(p, f, 2.4022650695910071e-01);
-    p = __builtin_fma(p, f, 6.9314718055994531e-01);
-    return __builtin_fma(p, f, 1.0);
+    double q = 1.0203121063391729e-07;
+    q = __builtin_fma(q, f, 1.3255224878668817e-06);
+    q = __builtin_fma(q, f, 1.525268684626772e-05);
+    q = __builtin_fma(q, f, 0.00015403455852453838);
+    q = __builtin_fma(q, f, 0.0013333558179043112);
+    q = __builtin_fma(q, f, 0.009618129159402558);
+    q = __builtin_fma(q, f, 0.055504108664760424);
+    q = __builtin_fma(q, f, 0.2402265069581299);
+    q = __builtin_fma(q, f, 0.6931471805599453);
+    return __builtin_fma(q, f, 1.0);
 }
 // The mass of a score: 2^((x - m) c) in units of 2^-S, rounded to an integer by the addition of 2^52
 // (S <= 51).  -inf and NaN have none (the maximum with a number drops NaN).  m is finite.
 struct Masses {
     double m, c;   // largest score, log2(e) / temperature
-    int S;
+    double big;    // 1.5 2^52 + S
+    __device__ __forceinline__ Masses(double m, double c, int S) : m(m), c(c), big(6755399441055744.0 + S) {}
     __device__ __forceinline__ u64 raw(float x) const {   // the mass plus kRaw
-        const double y = fmax(((double)x - m) * c, -1100.0);
-        const double k = rint(y);
-        return __builtin_bit_cast(u64, ldexp(exp2_part(y - k), (int)k + S) + 4503599627370496.0);
+        const double y = fmax(((double)x - m) * c, -120.0);   // (no mass below -53)
+        // y rounded to an integer k, and k + S in the low word of the sum: it goes to the exponent of a
+        // number in [0.7, 1.5]
+        const double t = y + big, k = t - big;
+        const uint32_t e = (uint32_t)__builtin_bit_cast(u64, t);
+        const u64 p = __builtin_bit_cast(u64, exp2_part(y - k)) + ((u64)e << 52);
+        return __builtin_bit_cast(u64, __builtin_bit_cast(double, p) + 4503599627370496.0);
     }
     static constexpr u64 kRaw = 0x4330000000000000ull;
     __device__ __forceinline__ u64 operator()(float x) const { return raw(x) - kRaw; }
@@ -90,64 +94,14 @@ __device__ __forceinline__ u64 least_mass(double min_p, int S) {
 }
 
 
-// ---- selection among entries in registers -----------------------------------------------------
-struct SelectLds {
-    u64 mass[256];
-    uint32_t count[256];
-};
-struct Crossing {
-    u64 prefix;   // the crossing entry's rank without its low `shift` bits
-    int shift;
-};
-
-// Entries have ranks (64 bits, their bits at top_shift + 8 and above all equal) and weights: 1, or their mass.
-// Taken from the largest rank down, where do the weights reach `want` (at most their sum)?  By bytes of
-// the rank; done as soon as one entry is left, or (kWhole) the ones left are all needed.
-template <int THREADS, bool kMass, bool kWhole, class ForEach>
-__device__ Crossing select(ForEach for_each, u64 want, int top_shift, SelectLds* lds) {
-    u64 prefix = 0;
-    for (int shift = top_shift; ; shift -= 8) {
-        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) {
-            lds->count[b] = 0;
-            if (kMass) lds->mass[b] = 0;
-        }
-        __syncthreads();
-        for_each([&](u64 rank, u64 mass) {
-            if (shift != top_shift && (rank >> shift >> 8) != prefix) return;
-            atomicAdd(&lds->count[rank >> shift & 255], 1u);
-            if (kMass) atomicAdd(&lds->mass[rank >> shift & 255], mass);
-        });
-        __syncthreads();
-        bool done;
-        if (kMass) {
-            const Found<u64> f = find_bin(lds->mass, want);
-            prefix = shift == top_shift ? f.bin : prefix << 8 | f.bin;
-            want -= f.above;
-            done = lds->count[f.bin] <= 1 || (kWhole && f.inside == want);
-        } else {
-            const Found<uint32_t> f = find_bin(lds->count, (uint32_t)want);
-            prefix = shift == top_shift ? f.bin : prefix << 8 | f.bin;
-            want -= f.above;
-            done = f.inside <= 1 || (kWhole && f.inside == want);
-        }
-        done = __builtin_amdgcn_readfirstlane((uint32_t)done) != 0 || shift == 0;
-        __syncthreads();
-        if (done) return Crossing{prefix, shift};
-    }
-}
-
+// ---- entries in registers ----------------------------------------------------------------------
 // Exclusive prefix sum over the workgroup, in thread order, and the sum of all.
 template <int THREADS>
 __device__ __forceinline__ u64 block_scan(u64 v, u64& all, u64* tmp) {
     const uint32_t lane = lane_id(), wave = threadIdx.x / 64;
-    u64 upto = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 t = __shfl_up(upto, o);
-        if (lane >= (uint32_t)o) upto += t;
-    }
+    const u64 upto = wave_scan(v, Add(), u64(0));
     if (THREADS == 64) {
-        all = __shfl(upto, 63);
+        all = read_lane(upto, 63);
         return upto - v;
     }
     if (lane == 63) tmp[wave] = upto;
@@ -187,7 +141,7 @@ struct Entries {
     __device__ __forceinline__ void keep_from(Crossing c) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if ((rank(e) >> c.shift) < c.prefix) key[e] = 0;
+            if (rank(e) < c.from) key[e] = 0;
     }
     __device__ void cut_count(uint32_t k, SelectLds* lds, u64* tmp) {
         uint32_t have = 0;
@@ -200,7 +154,7 @@ struct Entries {
                 for (int e = 0; e < E; ++e)
                     if (key[e]) f(rank(e), 0);
             },
-            k, 56, lds));
+            k, lds));
     }
     __device__ __forceinline__ void weigh(const Masses& M) {
 #pragma unroll
@@ -220,7 +174,7 @@ struct Entries {
                 for (int e = 0; e < E; ++e)
                     if (key[e] && mass[e]) f(rank(e), mass[e]);
             },
-            want, 56, lds));
+            want, lds));
     }
     __device__ __forceinline__ void drop_below(u64 least) {
 #pragma unroll
@@ -358,7 +312,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
             const u64 k = L.key[e] ? L.rank(e) : 0;
             top = k > top ? k : top;
         }
-        top = block_reduce<THREADS>(top, [](u64 a, u64 b) { return a > b ? a : b; }, tmp);
+        top = block_reduce<THREADS>(top, MaxU(), tmp);
         if (top == 0) {
             if (threadIdx.x == 0) out.empty(row);
             continue;
@@ -420,7 +374,11 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
 // bins above a nucleus's last are summed by segments, and the draw looks through one of them.
 constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
-constexpr float kBinsPerNat = 32.0f;
+// The bins reach from the largest score to a little below the lowest of a sample (the first score of every group),
+// 32 nats at most: 32 bins a nat, and more of them for the rows whose nucleus is wide, so that one bin holds
+// hundreds of classes and not thousands (64 x 200001 f16, bins of 1/32 nat: 79 us to list them, 28 for the
+// histogram's clashing atomics).
+constexpr float kMostNats = 32.0f;
 __device__ __forceinline__ uint32_t bin_at(uint32_t b) { return b + (b >> 4); }   // (its place in LDS)
 
 enum Mode : uint32_t { kGreedy, kWhole, kList, kNucleus };   // (kWhole: a least weight above 1 as well)
@@ -449,22 +407,29 @@ struct Long {
             for (int v = 0; v < V; ++v) x[v] = bits >> v & 1 ? x[v] : -INFINITY;
         }
     }
-    __device__ __forceinline__ void load(uint32_t seg, float (&x)[U][V]) const {
+    struct Tile {   // a segment's scores in their type; vector u becomes f32 where it is used
+        Pack<T> p[U];
         uint32_t bits[U];
-        if (r.allowed) {
+        bool masked;
+        __device__ __forceinline__ void get(int u, float (&x)[V]) const {
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = to_f32(p[u].v[v]);
+            if (masked) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[v] = bits[u] >> v & 1 ? x[v] : -INFINITY;
+            }
+        }
+    };
+    __device__ __forceinline__ void load(uint32_t seg, Tile& t) const {
+        t.masked = r.allowed != nullptr;
+        if (t.masked) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t i = at(seg, u, lane);
-                bits[u] = i < n ? r.allowed[i >> 5] >> (i & 31) : 0;
+                t.bits[u] = i < n ? r.allowed[i >> 5] >> (i & 31) : 0;
             }
         }
-        load_tile<T, kUnit>(x0, cs, seg * kSeg, n, -INFINITY, x);
-        if (r.allowed) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int v = 0; v < V; ++v) x[u][v] = bits[u] >> v & 1 ? x[u][v] : -INFINITY;
-        }
+        load_tile<T, kUnit>(x0, cs, seg * kSeg, n, -INFINITY, t.p);
     }
     __device__ __forceinline__ float score(uint32_t i) const {
         if (i >= n || (r.allowed && !(r.allowed[i >> 5] >> (i & 31) & 1))) return -INFINITY;
@@ -484,12 +449,16 @@ struct Long {
     // (nullable) every group's largest as an order key (0: nothing to draw); with `sums` the running softmax
     // denominator.
     __device__ __forceinline__ void scan(uint32_t s0, uint32_t s1, uint32_t* groups, bool sums, float c,
-                                         float& best, uint32_t& best_seg, Running& run) const {
+                                         float& best, uint32_t& best_seg, float& low, Running& run) const {
         best = -INFINITY;
+        low = INFINITY;
         best_seg = s0;
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
+            Tile t;
+            load(seg, t);
             float x[U][V], gm = -INFINITY;
-            load(seg, x);
+#pragma unroll
+            for (int u = 0; u < U; ++u) t.get(u, x[u]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -498,6 +467,7 @@ struct Long {
                 best = gm;
                 best_seg = seg;
             }
+            if (x[0][0] > -INFINITY) low = fminf(low, x[0][0]);
             if (groups) groups[(seg - s0) * 64 + lane] = gm > -INFINITY ? order_key(gm) : 0;
             if (sums) {
                 run.raise(gm, c);
@@ -526,9 +496,10 @@ struct Long {
 
     // ---- bins: monotone in the score, the largest in bin 0 ----
     float bm, bscale;
-    __device__ __forceinline__ void set_bins(float m) {
+    __device__ __forceinline__ void set_bins(float m, float low) {
         bm = m;
-        bscale = (float)(r.rt * kBinsPerNat);
+        const float range = fminf((m - low) * (float)r.rt * 1.25f + 1.0f, kMostNats);   // (NaN: the most)
+        bscale = (float)(r.rt * (double)((float)kBins / range));
     }
     __device__ __forceinline__ uint32_t bin(float x) const {
         const float z = (bm - x) * bscale;
@@ -538,44 +509,61 @@ struct Long {
     template <bool kMass>
     __device__ __forceinline__ void histogram(uint32_t s0, uint32_t s1, const Masses& M, u64* hist) const {
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
-            float x[U][V];
-            load(seg, x);
+            Tile t;
+            load(seg, t);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                float x[V];
+                t.get(u, x);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float y = x[u][v];
+                    const float y = x[v];
                     if (kMass) {
                         const u64 w = M(y);
                         if (w) atomicAdd(&hist[bin_at(bin(y))], w);
                     } else if (y > -INFINITY) {
                         atomicAdd((uint32_t*)&hist[bin_at(bin(y))], 1u);
                     }
-                    if (v == V - 1) __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_sched_barrier(0);   // (one vector's masses at a time: registers)
+            }
         }
     }
     // Masses of the segments, of the classes of at least `least`; the mass of all classes, per thread.
-    __device__ __forceinline__ u64 weigh(uint32_t s0, uint32_t s1, const Masses& M, u64 least, u64* segs) const {
+    template <bool kLeast>
+    __device__ __forceinline__ u64 weigh_segments(uint32_t s0, uint32_t s1, const Masses& M, u64 least, u64* segs) const {
         u64 all = 0;
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
-            float x[U][V];
-            load(seg, x);
+            Tile t;
+            load(seg, t);
             u64 sum = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                float x[V];
+                t.get(u, x);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const u64 w = M(x[u][v]);
-                    all += w;
-                    sum += w >= least ? w : 0;
+                    if (kLeast) {
+                        const u64 w = M(x[v]);
+                        all += w;
+                        sum += w >= least ? w : 0;
+                    } else {
+                        sum += M.raw(x[v]);
+                    }
                 }
-                __builtin_amdgcn_sched_barrier(0);   // (one vector's masses at a time: registers)
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!kLeast) {
+                sum -= kGroup * Masses::kRaw;
+                all += sum;
             }
             sum = wave_reduce(sum, Add());
             if (lane == 0) segs[seg] = sum;
         }
         return all;
+    }
+    __device__ __forceinline__ u64 weigh(uint32_t s0, uint32_t s1, const Masses& M, u64 least, u64* segs) const {
+        return least ? weigh_segments<true>(s0, s1, M, least, segs) : weigh_segments<false>(s0, s1, M, 0, segs);
     }
     // The classes in bin `cut`, and with `all` those in the bins before, go to the list (at most cap; count goes
     // on); with kSum the masses of the bins before go to their segments.
@@ -584,13 +572,13 @@ struct Long {
                                             u64* segs, u64* list, uint32_t* count, uint32_t cap) const {
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             u64 sum = 0;
-            float xs[U][V];
-            load(seg, xs);
+            uint32_t hits = 0;   // a bit a class of the lane's group
+            Tile t;
+            load(seg, t);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float(&x)[V] = xs[u];
-                const uint32_t i = at(seg, u, lane);
-                uint32_t hits = 0;
+                float x[V];
+                t.get(u, x);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const uint32_t b = bin(x[v]);
@@ -598,19 +586,19 @@ struct Long {
                         const u64 w = M(x[v]);
                         sum += w >= least ? w : 0;
                     }
-                    if (x[v] > -INFINITY && (b == cut || (all && b < cut))) hits |= 1u << v;
+                    if (x[v] > -INFINITY && (b == cut || (all && b < cut))) hits |= 1u << (u * V + v);
                 }
-                while (__any(hits != 0)) {
-                    const bool in = hits != 0;
-                    const uint32_t v = in ? (uint32_t)__builtin_ctz(hits) : 0;
-                    float z = x[0];
-#pragma unroll
-                    for (int q = 1; q < V; ++q) z = v == (uint32_t)q ? x[q] : z;
-                    const u64 b = __ballot(in);
-                    uint32_t base = 0;
-                    if (lane == 0) base = atomicAdd(count, (uint32_t)__popcll(b));
-                    base = __builtin_amdgcn_readfirstlane(base) + (uint32_t)__popcll(b & ((1ull << lane) - 1));
-                    if (in && base < cap) list[base] = rank_key(z, i + v);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__any(hits != 0)) {   // one place in the list for the segment's
+                const uint32_t mine = (uint32_t)__popc(hits), upto = wave_scan(mine, Add(), 0u);
+                uint32_t base = 0;
+                if (lane == 0) base = atomicAdd(count, read_lane(upto, 63));
+                base = __builtin_amdgcn_readfirstlane(base) + upto - mine;
+                while (hits) {
+                    const uint32_t q = (uint32_t)__builtin_ctz(hits), i = at(seg, (int)(q / V), lane) + q % V;
+                    if (base < cap) list[base] = rank_key(score(i), i);
+                    ++base;
                     hits &= hits - 1;
                 }
             }
@@ -620,23 +608,20 @@ struct Long {
             }
         }
     }
-    // Classes of the groups whose largest reaches the bound go to the list.
+    // Classes of the groups whose largest reaches the bound go to the list (count[0]): the groups are listed
+    // first (count[1]; as many as there are at most), then half a wave reads a group.  count starts as 0.
     __device__ __forceinline__ void gather(uint32_t segs, const uint32_t* groups, uint32_t bound, u64* list,
-                                           uint32_t* count) const {
-        for (uint32_t g0 = wave * 64; g0 < segs * 64; g0 += THREADS) {
-            u64 hit = __ballot(groups[g0 + lane] >= bound && groups[g0 + lane] != 0);
-            // a group at a time: lane l reads its class l
-            while (hit) {
-                const uint32_t ln = (uint32_t)__builtin_ctzll(hit);
-                hit &= hit - 1;
-                const uint32_t i = at(g0 / 64, (int)(lane % kGroup) / V, ln) + lane % V;
-                const float x = lane < kGroup ? score(i) : -INFINITY;
-                const bool in = x > -INFINITY && order_key(x) >= bound;
-                const u64 b = __ballot(in);
-                uint32_t base = 0;
-                if (lane == 0) base = atomicAdd(count, (uint32_t)__popcll(b));
-                base = __builtin_amdgcn_readfirstlane(base) + (uint32_t)__popcll(b & ((1ull << lane) - 1));
-                if (in && base < (uint32_t)CAP) list[base] = rank_key(x, i);
+                                           uint32_t* count, uint16_t* hits) const {
+        for (uint32_t g = threadIdx.x; g < segs * 64; g += THREADS)
+            if (groups[g] != 0 && groups[g] >= bound) hits[atomicAdd(&count[1], 1u)] = (uint16_t)g;
+        __syncthreads();
+        const uint32_t n_hits = count[1], q = threadIdx.x % kGroup;
+        for (uint32_t h = threadIdx.x / kGroup; h < n_hits; h += THREADS / kGroup) {
+            const uint32_t i = at(hits[h] / 64, (int)q / V, hits[h] % 64) + q % V;
+            const float x = score(i);
+            if (x > -INFINITY && order_key(x) >= bound) {
+                const uint32_t at = atomicAdd(&count[0], 1u);
+                if (at < (uint32_t)CAP) list[at] = rank_key(x, i);
             }
         }
     }
@@ -654,6 +639,10 @@ struct Long {
     // A list that holds every class that may be kept: top_k, top_p, min_p, and the draw.
     __device__ void finish_list(const u64* list, uint32_t count, const Masses& M, double log_z, uint64_t row, SelectLds* lds,
                                 u64* tmp, const Out& out) const {
+        if (count <= 256) {
+            finish_short(list, count, M, log_z, row, lds, tmp, out);
+            return;
+        }
         Entries<THREADS, 8> L;
         read_list(L, list, count);
         L.cut_count(r.k, lds, tmp);
@@ -667,11 +656,45 @@ struct Long {
                 for (int e = 0; e < 8; ++e)
                     if (L.key[e] && L.mass[e]) f((uint32_t)~L.idx[e], L.mass[e]);
             },
-            want, 24, lds);
+            want, lds);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (L.key[e] && L.mass[e] && ((u64)(uint32_t)~L.idx[e] >> c.shift) == c.prefix)
+            if (L.key[e] && L.mass[e] && (uint32_t)~L.idx[e] >= c.from && (uint32_t)~L.idx[e] <= c.last)
                 out.put(row, L.idx[e], ((double)key_score(L.key[e]) - M.m) * r.rt - log_z);
+    }
+    // The same for up to 256 classes: every entry counts those ahead of it, and later the mass before it.
+    __device__ void finish_short(const u64* list, uint32_t count, const Masses& M, double log_z, uint64_t row, SelectLds* lds,
+                                 u64* tmp, const Out& out) const {
+        const uint32_t t = threadIdx.x;
+        if (t < count) lds->mass[t] = list[t];
+        __syncthreads();
+        if (t < count) {
+            const u64 key = lds->mass[t];
+            uint32_t place = 0;
+            for (uint32_t j = 0; j < count; ++j) place += lds->mass[j] > key;
+            lds->rank[place] = key;
+        }
+        __syncthreads();
+        const uint32_t kept = min(count, r.k);
+        const u64 rank = t < kept ? lds->rank[t] : 0;
+        const float x = key_score((uint32_t)(rank >> 32));
+        u64 w = t < kept ? M(x) : 0, all;
+        const u64 ahead = block_scan<THREADS>(w, all, tmp);
+        if (r.p < 1.0 && ahead >= nucleus_of(r.p, all)) w = 0;
+        if (w < least_mass(r.min_p, S)) w = 0;
+        if (t < count) lds->mass[t] = w;
+        __syncthreads();
+        u64 before = 0, sum = 0;
+        if (t < kept) {
+            for (uint32_t j = 0; j < kept; ++j) {
+                const u64 wj = lds->mass[j];
+                before += (uint32_t)lds->rank[j] > (uint32_t)rank ? wj : 0;   // (~class: larger for a class before)
+                sum += wj;
+            }
+            const u64 target = target_of(r.u, sum);
+            if (w && target >= before && target - before < w) out.put(row, ~(uint32_t)rank, ((double)x - M.m) * r.rt - log_z);
+        }
+        __syncthreads();
     }
     // Segments' kept masses (and a nucleus's cut): the segment of the draw, then its class.
     __device__ void finish_segments(const u64* segs, uint32_t n_segs, const Masses& M, uint32_t cut, u64 from, u64 least,
@@ -747,8 +770,8 @@ struct Long {
                     for (uint32_t i = threadIdx.x; i < n; i += THREADS)
                         if (key_at(i)) f(rank_key(score(i), i), 0);
                 },
-                r.k, 56, lds);
-            from = c.prefix << c.shift;
+                r.k, lds);
+            from = c.from;
             kept = 0;
             for (uint32_t i = threadIdx.x; i < n; i += THREADS)
                 if (key_at(i) && rank_key(score(i), i) >= from) kept += mass(score(i));
@@ -763,9 +786,8 @@ struct Long {
                             if (w) f(rank_key(score(i), i), w);
                         }
                 },
-                nucleus_of(r.p, kept), 56, lds);
-            const u64 f = c.prefix << c.shift;
-            from = f > from ? f : from;
+                nucleus_of(r.p, kept), lds);
+            from = c.from > from ? c.from : from;
         }
         const u64 least = least_mass(r.min_p, S);
         // thread t holds the classes [t per, (t + 1) per)
@@ -795,12 +817,7 @@ __device__ __forceinline__ Found<u64> find_cut(Get get, u64 want) {
     const uint32_t l = lane_id();
     u64 sum = 0;
     for (uint32_t j = 0; j < kBins / 64; ++j) sum += get(l * (kBins / 64) + j);
-    u64 upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 v = __shfl_up(upto, o);
-        if (l >= (uint32_t)o) upto += v;
-    }
+    const u64 upto = wave_scan(sum, Add(), u64(0));
     u64 above = upto - sum, inside = 0;
     uint32_t b = l * (kBins / 64);
     const u64 cross = __ballot(upto >= want);
@@ -815,7 +832,7 @@ __device__ __forceinline__ Found<u64> find_cut(Get get, u64 want) {
             else if (j + 1 < kBins / 64) above += c;
         }
     }
-    return Found<u64>{(uint32_t)__shfl(b, at), __shfl(above, at), __shfl(inside, at)};
+    return Found<u64>{read_lane(b, at), read_lane(above, at), read_lane(inside, at)};
 }
 
 // Up to 8192 classes: a workgroup a row, all steps in one launch.
@@ -829,22 +846,24 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
     __shared__ u64 tmp[W], pick[2];
     __shared__ float tmp_f[W];
     __shared__ double tmp_d[W];
-    __shared__ uint32_t count, khist[256];
+    __shared__ uint32_t counts[2];
+    uint32_t& count = counts[0];
     const uint32_t n_segs = (X.classes + kSeg - 1) / kSeg;
     u64* list = pool;
     u64* segs = pool + L::CAP;
     uint32_t* groups = (uint32_t*)(segs + n_segs);
+    uint16_t* hits = (uint16_t*)(groups + n_segs * 64);
     for (uint64_t row = blockIdx.x; row < X.rows; row += gridDim.x) {
         L R(X, S, row, shift);
         const Mode mode = R.mode();
         const float c = (float)(R.r.rt * 1.4426950408889634);
         const bool by_groups = mode == kList && R.by_groups(n_segs);
-        float best;
+        float best, low;
         uint32_t best_seg;
         Running run;
-        R.scan(0, n_segs, by_groups ? groups : nullptr, mode == kList, c, best, best_seg, run);
+        R.scan(0, n_segs, by_groups ? groups : nullptr, mode == kList, c, best, best_seg, low, run);
         for (uint32_t b = threadIdx.x; b < kBinsPad; b += THREADS) hist[b] = 0;
-        if (threadIdx.x == 0) count = 0;
+        if (threadIdx.x < 2) counts[threadIdx.x] = 0;
         const float m = block_reduce<THREADS>(best, MaxF(), tmp_f);
         __syncthreads();
         if (m == -INFINITY) {
@@ -854,14 +873,14 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
         bool slow = m == INFINITY;
         uint32_t first = 0;
         if (R.r.greedy || R.r.min_p > 1.0) {
-            first = (uint32_t)block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), [](u64 a, u64 b) { return a < b ? a : b; }, tmp);
+            first = (uint32_t)block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), MinU(), tmp);
             if (R.r.greedy) {
                 if (threadIdx.x == 0) out.put(row, first, 0.0);
                 continue;
             }
         }
         const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
-        R.set_bins(m);
+        R.set_bins(m, -block_reduce<THREADS>(-low, MaxF(), tmp_f));
         if (!slow && mode == kWhole) {
             const u64 least = least_mass(R.r.min_p, shift);
             u64 z = R.weigh(0, n_segs, M, R.r.min_p > 1.0 ? 0 : least, segs);
@@ -894,14 +913,14 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
                         for (int e = 0; e < 8; ++e)
                             if (E.key[e] && E.mass[e]) g(E.rank(e), E.mass[e]);
                     },
-                    want - f.above, 56, &lds);
+                    want - f.above, &lds);
                 E.keep_from(x);
                 E.drop_below(least);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (E.key[e] && E.mass[e]) atomicAdd(&segs[E.idx[e] / kSeg], E.mass[e]);
                 __syncthreads();
-                R.finish_segments(segs, n_segs, M, f.bin, x.prefix << x.shift, least, z, row, tmp, pick, out);
+                R.finish_segments(segs, n_segs, M, f.bin, x.from, least, z, row, tmp, pick, out);
             }
         } else if (!slow) {
             float mr;
@@ -914,8 +933,8 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
                 for (uint32_t g = threadIdx.x; g < n_segs * 64; g += THREADS) have += groups[g] != 0;
                 have = block_reduce<THREADS>(have, Add(), tmp);
                 if (have >= R.r.k) {
-                    const u64 kth = block_kth<THREADS>([&](uint32_t i) { return (u64)groups[i] << 32; }, n_segs * 64, R.r.k, 32, khist);
-                    R.gather(n_segs, groups, (uint32_t)(kth >> 32), list, &count);
+                    const u64 kth = kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, n_segs * 64, R.r.k, &lds);
+                    R.gather(n_segs, groups, (uint32_t)kth, list, counts, hits);
                     __syncthreads();
                     listed = count <= (uint32_t)L::CAP;
                     __syncthreads();
@@ -946,9 +965,10 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
 // Rows of more than 8192 classes: the steps as launches of their own, `parts` workgroups a row, so that a few
 // rows fill the CUs and every step has the registers it needs (all steps in one launch of 1024 threads spilled
 // 110 registers: 256 x 131072 f32 with settings a row took 189 to 287 us).  Between the launches, per row:
-struct Top {      // of a part: its largest score (order key) over ~(its first class); the softmax denominator
+struct Top {      // of a part: its largest score (order key) over ~(its first class); the softmax denominator; a low score
     u64 key;
-    float m, s;
+    float m, s, low;
+    uint32_t unused;
 };
 struct Step {     // where the cut lies
     u64 total, above;   // mass of all classes; weight of the bins before the cut's
@@ -969,13 +989,16 @@ struct Space {    // the workspace of a chunk of rows
 constexpr uint32_t kListCap = 8192;
 
 template <int THREADS>
-__device__ __forceinline__ u64 row_top(const Space& P, uint64_t row, u64* tmp) {
+__device__ __forceinline__ u64 row_top(const Space& P, uint64_t row, u64* tmp, float& low) {
     u64 top = 0;
+    low = INFINITY;
     for (uint32_t p = threadIdx.x; p < P.parts1; p += THREADS) {
         const u64 k = P.tops[row * P.parts1 + p].key;
         top = k > top ? k : top;
+        low = fminf(low, P.tops[row * P.parts1 + p].low);
     }
-    return block_reduce<THREADS>(top, [](u64 a, u64 b) { return a > b ? a : b; }, tmp);
+    low = -block_reduce<THREADS>(-low, MaxF(), (float*)tmp);
+    return block_reduce<THREADS>(top, MaxU(), tmp);
 }
 
 template <class T, bool kUnit>
@@ -989,27 +1012,28 @@ __global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int sh
     Long<T, kUnit, THREADS> R(X, S, row, shift);
     const Mode mode = R.mode();
     const float c = (float)(R.r.rt * 1.4426950408889634);
-    float best;
+    float best, low;
     uint32_t best_seg;
     Running run;
     R.scan(s0, s1, mode == kList && R.by_groups(P.n_segs) ? P.groups + row * P.n_segs * 64 + s0 * 64 : nullptr, mode == kList,
-           c, best, best_seg, run);
+           c, best, best_seg, low, run);
+    low = -block_reduce<THREADS>(-low, MaxF(), tmp_f);
     const float m = block_reduce<THREADS>(best, MaxF(), tmp_f);
     u64 first = 0xFFFFFFFFu;
     if (R.r.greedy || R.r.min_p > 1.0)
-        first = block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), [](u64 a, u64 b) { return a < b ? a : b; }, tmp);
+        first = block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), MinU(), tmp);
     float rm = 0.0f;
     double rs = 0.0;
     if (mode == kList) block_running<THREADS>(run, c, rm, rs, tmp_f, tmp_d);
     if (threadIdx.x == 0) {
-        P.tops[row * P.parts1 + part] = Top{m == -INFINITY ? 0 : (u64)order_key(m) << 32 | (uint32_t)~first, rm, (float)rs};
+        P.tops[row * P.parts1 + part] = Top{m == -INFINITY ? 0 : (u64)order_key(m) << 32 | (uint32_t)~first, rm, (float)rs, low, 0};
         if (part == 0) P.count[row] = 0;
     }
 }
 
 // Masses of the segments, or the part's histogram of masses or counts.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(512) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
+__global__ __launch_bounds__(512, 4) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
     constexpr int THREADS = 512;
     __shared__ u64 hist[kBinsPad];
     __shared__ u64 tmp[THREADS / 64];
@@ -1018,7 +1042,8 @@ __global__ __launch_bounds__(512) void weigh_kernel(Rows<T> X, Settings S, int s
     Long<T, kUnit, THREADS> R(X, S, row, shift);
     const Mode mode = R.mode();
     if (mode == kGreedy || (mode == kList && P.groups && R.by_groups(P.n_segs))) return;
-    const u64 top = row_top<THREADS>(P, row, tmp);
+    float low;
+    const u64 top = row_top<THREADS>(P, row, tmp, low);
     const float m = key_score((uint32_t)(top >> 32));
     if (top == 0 || m == INFINITY) return;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
@@ -1030,7 +1055,7 @@ __global__ __launch_bounds__(512) void weigh_kernel(Rows<T> X, Settings S, int s
     }
     for (uint32_t b = threadIdx.x; b < kBinsPad; b += THREADS) hist[b] = 0;
     __syncthreads();
-    R.set_bins(m);
+    R.set_bins(m, low);
     if (mode == kNucleus) R.template histogram<true>(s0, s1, M, hist);
     else R.template histogram<false>(s0, s1, M, hist);
     __syncthreads();
@@ -1040,7 +1065,7 @@ __global__ __launch_bounds__(512) void weigh_kernel(Rows<T> X, Settings S, int s
 
 // The classes of the cut's bin (top_k: and of those before), and the segments' masses before it.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(512) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
+__global__ __launch_bounds__(512, 4) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
     constexpr int THREADS = 512;
     __shared__ u64 hist[kBinsPad];
     __shared__ u64 tmp[THREADS / 64];
@@ -1049,11 +1074,12 @@ __global__ __launch_bounds__(512) void collect_kernel(Rows<T> X, Settings S, int
     Long<T, kUnit, THREADS> R(X, S, row, shift);
     const Mode mode = R.mode();
     if (mode != kNucleus && !(mode == kList && !(P.groups && R.by_groups(P.n_segs)))) return;
-    const u64 top = row_top<THREADS>(P, row, tmp);
+    float low;
+    const u64 top = row_top<THREADS>(P, row, tmp, low);
     const float m = key_score((uint32_t)(top >> 32));
     if (top == 0 || m == INFINITY) return;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
-    R.set_bins(m);
+    R.set_bins(m, low);
     u64 total = 0;
     for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) {
         u64 h = 0;
@@ -1085,11 +1111,12 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
     __shared__ u64 tmp[W], pick[2];
     __shared__ float tmp_f[W];
     __shared__ double tmp_d[W];
-    __shared__ uint32_t count, khist[256];
+    __shared__ uint32_t count[2];
     const uint64_t row = blockIdx.x;
     L R(X, S, row, shift);
     const Mode mode = R.mode();
-    const u64 top = row_top<THREADS>(P, row, tmp);
+    float low;
+    const u64 top = row_top<THREADS>(P, row, tmp, low);
     if (top == 0) {
         if (threadIdx.x == 0) out.empty(row);
         return;
@@ -1131,15 +1158,15 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
                     for (int e = 0; e < 8; ++e)
                         if (E.key[e] && E.mass[e]) g(E.rank(e), E.mass[e]);
                 },
-                nucleus_of(R.r.p, step.total) - step.above, 56, &lds);
+                nucleus_of(R.r.p, step.total) - step.above, &lds);
             E.keep_from(x);
             E.drop_below(least);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (E.key[e] && E.mass[e]) atomicAdd(&pool[E.idx[e] / kSeg], E.mass[e]);
             __syncthreads();
-            R.set_bins(m);
-            R.finish_segments(pool, P.n_segs, M, step.bin, x.prefix << x.shift, least, step.total, row, tmp, pick, out);
+            R.set_bins(m, low);
+            R.finish_segments(pool, P.n_segs, M, step.bin, x.from, least, step.total, row, tmp, pick, out);
             return;
         }
     }
@@ -1155,21 +1182,22 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
         const double log_z = log(sr);
         if (by_groups) {
             uint32_t* groups = (uint32_t*)(pool + kListCap);
+            uint16_t* hits = (uint16_t*)(groups + P.n_segs * 64);
             u64 have = 0;
             for (uint32_t g = threadIdx.x; g < P.n_segs * 64; g += THREADS) {
                 groups[g] = P.groups[row * P.n_segs * 64 + g];
                 have += groups[g] != 0;
             }
-            if (threadIdx.x == 0) count = 0;
+            if (threadIdx.x < 2) count[threadIdx.x] = 0;
             have = block_reduce<THREADS>(have, Add(), tmp);
             __syncthreads();
             u64 kth = 0;   // (fewer groups than k: all that is allowed is listed)
             if (have >= R.r.k)
-                kth = block_kth<THREADS>([&](uint32_t i) { return (u64)groups[i] << 32; }, P.n_segs * 64, R.r.k, 32, khist);
-            R.gather(P.n_segs, groups, (uint32_t)(kth >> 32), pool, &count);
+                kth = kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, P.n_segs * 64, R.r.k, &lds);
+            R.gather(P.n_segs, groups, (uint32_t)kth, pool, count, hits);
             __syncthreads();
-            slow = count > kListCap;
-            if (!slow) R.finish_list(pool, count, M, log_z, row, &lds, tmp, out);
+            slow = count[0] > kListCap;
+            if (!slow) R.finish_list(pool, count[0], M, log_z, row, &lds, tmp, out);
         } else {
             slow = P.steps[row].state == kOverflow;
             if (!slow) R.finish_list(P.list + row * kListCap, P.count[row], M, log_z, row, &lds, tmp, out);
@@ -1189,7 +1217,7 @@ template <class T, bool kUnit>
 int launch_mid(const Rows<T>& X, const Settings& S, int shift, const Out& out, hipStream_t st) {
     typedef Long<T, kUnit, 256> L;
     const size_t n_segs = (X.classes + kSeg - 1) / kSeg;
-    const size_t lds = sizeof(u64) * (L::CAP + n_segs) + sizeof(uint32_t) * 64 * n_segs;
+    const size_t lds = sizeof(u64) * (L::CAP + n_segs) + (sizeof(uint32_t) + sizeof(uint16_t)) * 64 * n_segs;
     sample_long_kernel<T, kUnit, 256><<<row_grid(X.rows), 256, lds, st>>>(X, S, shift, out);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
@@ -1206,13 +1234,11 @@ Space plan(uint64_t rows, uint32_t n, unsigned char* base, size_t* bytes) {
     P.n_segs = (n + kSeg - 1) / kSeg;
     auto split = [&](uint64_t wgs, uint32_t waves, uint32_t& parts, uint32_t& per) {
         const uint64_t want = std::max<uint64_t>(1, wgs / rows);
-        const uint32_t most = (P.n_segs + waves - 1) / waves;
-        parts = (uint32_t)std::min<uint64_t>(want, most);
-        per = (P.n_segs + parts - 1) / parts;
+        per = (uint32_t)((P.n_segs + want - 1) / want + waves - 1) / waves * waves;
         parts = (P.n_segs + per - 1) / per;
     };
     split(2048, 4, P.parts1, P.per1);
-    split(1024, 8, P.parts2, P.per2);
+    split(768, 8, P.parts2, P.per2);
     size_t at = 0;
     auto take = [&](size_t size) {
         const size_t a = at;
@@ -1266,7 +1292,7 @@ int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out,
             }
         }
         // LDS: a list and the groups, or the segments
-        size_t lds = any_list && P.groups ? sizeof(u64) * kListCap + sizeof(uint32_t) * 64 * P.n_segs : 0;
+        size_t lds = any_list && P.groups ? sizeof(u64) * kListCap + (sizeof(uint32_t) + sizeof(uint16_t)) * 64 * P.n_segs : 0;
         lds = std::max(lds, sizeof(u64) * P.n_segs);
         if (lds > 32 * 1024)
             CLS_TRY(hipFuncSetAttribute((const void*)draw_kernel<T, kUnit>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));

@@ -84,22 +84,32 @@ template <class T>
 constexpr int kPacks = (int)kGroup / Pack<T>::V;
 template <class T, bool kUnit>
 __device__ __forceinline__ void load_tile(const T* row, int64_t cs, uint32_t base, uint32_t n, float fill,
-                                          float (&x)[kPacks<T>][Pack<T>::V]) {
+                                          Pack<T> (&p)[kPacks<T>]) {
     constexpr int V = Pack<T>::V, U = kPacks<T>;
     const uint32_t lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     if (kUnit && base + kSeg <= n) {
-        Pack<T> p[U];
         const Loose<T>* at = (const Loose<T>*)(row + base + lane * V);
 #pragma unroll
         for (int u = 0; u < U; ++u) p[u] = at[u * 64].p;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[u][v] = to_f32(p[u].v[v]);
     } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_pack<T, kUnit>(row, cs, base + (u * 64 + lane) * V, n, fill, x[u]);
+        for (int u = 0; u < U; ++u) {
+            float x[V];
+            load_pack<T, kUnit>(row, cs, base + (u * 64 + lane) * V, n, fill, x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) p[u].v[v] = from_f32<T>(x[v]);
+        }
     }
+}
+template <class T, bool kUnit>
+__device__ __forceinline__ void load_tile(const T* row, int64_t cs, uint32_t base, uint32_t n, float fill,
+                                          float (&x)[kPacks<T>][Pack<T>::V]) {
+    Pack<T> p[kPacks<T>];
+    load_tile<T, kUnit>(row, cs, base, n, fill, p);
+#pragma unroll
+    for (int u = 0; u < kPacks<T>; ++u)
+#pragma unroll
+        for (int v = 0; v < Pack<T>::V; ++v) x[u][v] = to_f32(p[u].v[v]);
 }
 template <class T, bool kUnit>
 __device__ __forceinline__ void store_pack(T* row, int64_t cs, uint32_t i, uint32_t n, const float (&x)[Pack<T>::V]) {
@@ -139,11 +149,47 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// A value from another lane by a data-parallel-primitive move (a register access, where a shuffle is a round
+// trip through LDS); lanes without a source get `none`.
+template <int kCtrl, int kRows, class V>
+__device__ __forceinline__ V dpp_move(V v, V none) {
+    static_assert(sizeof(V) == 4 || sizeof(V) == 8, "moved in words of 32 bits");
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                                                 kCtrl, kRows, 0xf, false));
+    } else {
+        const u64 a = __builtin_bit_cast(u64, v), b = __builtin_bit_cast(u64, none);
+        const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)b, (int)(uint32_t)a, kCtrl, kRows, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp((int)(b >> 32), (int)(a >> 32), kCtrl, kRows, 0xf, false);
+        return __builtin_bit_cast(V, (u64)hi << 32 | lo);
+    }
+}
+// Inclusive scan over the lanes, `none` the operation's neutral value: rows of 16 lanes, then across them.
+template <class V, class Op>
+__device__ __forceinline__ V wave_scan(V v, Op op, V none) {
+    v = op(dpp_move<0x111, 0xf>(v, none), v);   // from 1, 2, 4, 8 lanes below, within the row
+    v = op(dpp_move<0x112, 0xf>(v, none), v);
+    v = op(dpp_move<0x114, 0xf>(v, none), v);
+    v = op(dpp_move<0x118, 0xf>(v, none), v);
+    v = op(dpp_move<0x142, 0xa>(v, none), v);   // lane 15 of the row below to rows 1 and 3
+    v = op(dpp_move<0x143, 0xc>(v, none), v);   // lane 31 to rows 2 and 3
+    return v;
+}
+// (of a wave-uniform lane)
+template <class V>
+__device__ __forceinline__ V read_lane(V v, int lane) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        const u64 a = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)a, lane);
+        const uint32_t hi = __builtin_amdgcn_readlane((int)(a >> 32), lane);
+        return __builtin_bit_cast(V, (u64)hi << 32 | lo);
+    }
+}
 template <class V, class Op>
 __device__ __forceinline__ V wave_reduce(V v, Op op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
-    return v;
+    return read_lane(wave_scan(v, op, op.template none<V>()), 63);
 }
 // Reduction over a workgroup, in a fixed order; every thread gets it.  `tmp` holds a value a wave; the
 // call ends with a barrier after which tmp may be used again.
@@ -162,10 +208,26 @@ __device__ __forceinline__ V block_reduce(V v, Op op, V* tmp) {
 struct Add {
     template <class V>
     __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+    template <class V>
+    __device__ __forceinline__ V none() const { return V(0); }
 };
 struct MaxF {
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
     __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
+    template <class V>
+    __device__ __forceinline__ V none() const { return -(V)INFINITY; }
+};
+struct MaxU {
+    template <class V>
+    __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
+    template <class V>
+    __device__ __forceinline__ V none() const { return V(0); }
+};
+struct MinU {
+    template <class V>
+    __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; }
+    template <class V>
+    __device__ __forceinline__ V none() const { return ~V(0); }
 };
 
 // Where a sum over 256 bins in LDS, taken from bin 255 down, reaches `want`: the bin, what lies above it
@@ -186,12 +248,7 @@ __device__ __forceinline__ Found<V> find_bin(const V* hist, V want) {
         c[j] = hist[255 - 4 * l - j];
         sum += c[j];
     }
-    V upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const V v = __shfl_up(upto, o);
-        if (l >= (uint32_t)o) upto += v;
-    }
+    const V upto = wave_scan(sum, Add(), V(0));
     V above = upto - sum, inside = c[0];
     uint32_t b = 255 - 4 * l;
     const u64 cross = __ballot(upto >= want);
@@ -203,31 +260,99 @@ __device__ __forceinline__ Found<V> find_bin(const V* hist, V want) {
             inside = c[j];
             --b;
         }
-    return Found<V>{(uint32_t)__shfl(b, at), __shfl(above, at), __shfl(inside, at)};
+    return Found<V>{read_lane(b, at), read_lane(above, at), read_lane(inside, at)};
 }
 
-// The k-th largest of the keys get(0 .. n - 1) (0: no key; at least k are not 0), or any bound that
-// exactly k keys reach, by bytes from the top; `stop`: the lowest bit looked at.  All threads call it and get
-// the same value.  hist: 256 words of LDS.
-template <int THREADS, class Get>
-__device__ u64 block_kth(Get get, uint32_t n, uint32_t k, int stop, uint32_t* hist) {
-    u64 prefix = 0;
-    uint32_t need = k;
-    for (int shift = 56; shift >= stop; shift -= 8) {
-        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) hist[b] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-            const u64 key = get(i);
-            if (key != 0 && (shift == 56 || (key >> (shift + 8)) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
+struct CountLds {
+    u64 tmp[16], top[16];
+    uint32_t count[256];
+};
+struct SelectLds : CountLds {
+    u64 mass[256];
+    u64 rank[256];
+};
+// The bits of a rank's distance that are known before the digit at `shift`: from here up.
+__device__ __forceinline__ int prefix_shift(int shift, int bits) {
+    return shift == max(0, bits - 8) ? bits : shift == 0 ? (bits % 8 ? bits % 8 : 8) : shift + 8;
+}
+struct Crossing {
+    u64 from;    // ranks from here on are in the prefix
+    u64 last;    // and the lowest of them that may be there: the crossing entry's is in [from, last]
+};
+
+// Entries have ranks and weights: 1, or their mass (ranks are then all different).  Taken from the largest rank down, where do
+// the weights reach `want` (at most their sum)?  By digits of 8 bits of the ranks' distance from the lowest one, from
+// the highest bit that it has (the ranks of a list share their leading bits: as digits, every one of their atomics
+// would meet in one cell); done as soon as one entry is left, or (kWhole) the ones left are all needed.
+template <int THREADS, bool kMass, bool kWhole, class ForEach, class Lds>
+__device__ __forceinline__ Crossing select(ForEach for_each, u64 want, Lds* lds) {
+    u64 lo = ~0ull, hi = 0;
+    for_each([&](u64 rank, u64) {
+        lo = rank < lo ? rank : lo;
+        hi = rank > hi ? rank : hi;
+    });
+    lo = ~wave_reduce(~lo, MaxU());
+    hi = wave_reduce(hi, MaxU());
+    if (THREADS > 64) {
+        if (lane_id() == 0) {
+            lds->tmp[threadIdx.x / 64] = lo;
+            lds->top[threadIdx.x / 64] = hi;
         }
         __syncthreads();
-        const Found<uint32_t> f = find_bin(hist, need);
-        prefix = (prefix << 8) | f.bin;
-        need -= f.above;
-        __syncthreads();
-        if (f.inside == need) return prefix << shift;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) {
+            lo = lds->tmp[w] < lo ? lds->tmp[w] : lo;
+            hi = lds->top[w] > hi ? lds->top[w] : hi;
+        }
     }
-    return prefix << (stop < 0 ? 0 : stop);
+    const int bits = hi > lo ? 64 - __builtin_clzll(hi - lo) : 0;
+    u64 prefix = 0;
+    for (int shift = max(0, bits - 8); ; shift = max(0, shift - 8)) {
+        // (the last digit may repeat bits of the one before: those are equal among the entries left)
+        const int known = prefix_shift(shift, bits);
+        for (uint32_t b = threadIdx.x; b < 256; b += THREADS) {
+            lds->count[b] = 0;
+            if constexpr (kMass) lds->mass[b] = 0;
+        }
+        __syncthreads();
+        for_each([&](u64 rank, u64 mass) {
+            const u64 d = rank - lo;
+            if (known < bits && (d >> known) != (prefix >> known)) return;
+            atomicAdd(&lds->count[d >> shift & 255], 1u);
+            if constexpr (kMass) atomicAdd(&lds->mass[d >> shift & 255], mass);
+        });
+        __syncthreads();
+        bool done;
+        if constexpr (kMass) {
+            const Found<u64> f = find_bin(lds->mass, want);
+            prefix = (prefix & ~(255ull << shift)) | (u64)f.bin << shift;
+            want -= f.above;
+            done = lds->count[f.bin] <= 1 || (kWhole && f.inside == want);
+        } else {
+            const Found<uint32_t> f = find_bin(lds->count, (uint32_t)want);
+            prefix = (prefix & ~(255ull << shift)) | (u64)f.bin << shift;
+            want -= f.above;
+            done = f.inside <= 1 || (kWhole && f.inside == want);
+        }
+        done = __builtin_amdgcn_readfirstlane((uint32_t)done) != 0 || shift == 0;
+        __syncthreads();
+        if (done) return Crossing{lo + prefix, lo + (prefix | ((1ull << shift) - 1))};
+    }
+}
+
+// A bound that the k largest of the keys get(0 .. n - 1) reach and, unless there are equal ones, no others (0: no key;
+// at least k are not 0).
+template <int THREADS, class Get, class Lds>
+__device__ __forceinline__ u64 kth_of(Get get, uint32_t n, uint32_t k, Lds* lds) {
+    return select<THREADS, false, true>(
+               [&](auto f) {
+                   for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+                       const u64 key = get(i);
+                       if (key) f(key, 0);
+                   }
+               },
+               k, lds)
+        .from;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }

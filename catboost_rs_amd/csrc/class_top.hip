@@ -88,7 +88,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
     __shared__ u64 cand[W][CAP];
     __shared__ u64 best[KMAX];
     __shared__ uint32_t vmax[THREADS * kUnroll];
-    __shared__ uint32_t hist[256];
+    __shared__ CountLds lds;
     __shared__ uint32_t counts[W], nbest;
     __shared__ float tmp_f[W];
     __shared__ double tmp_d[W];
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
                 __syncthreads();
                 const uint32_t vecs = min((uint32_t)(THREADS * kUnroll), (n + V - 1) / V);
                 if (k <= vecs)
-                    C.set_bound(block_kth<THREADS>([&](uint32_t i) { return (u64)vmax[i] << 32; }, vecs, k, 32, hist));
+                    C.set_bound(kth_of<THREADS>([&](uint32_t i) { return (u64)vmax[i]; }, vecs, k, &lds) << 32);
             } else if (base == kTile || base == 3 * kTile) {
                 // the candidates of the first tiles give a better one
                 if ((threadIdx.x & 63) == 0) counts[wave] = C.count;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
 #pragma unroll
                 for (int w = 0; w < W; ++w) total += counts[w];
                 if (total >= k) {
-                    const u64 kth = block_kth<THREADS>(cand_at, W * CAP, k, 0, hist);
+                    const u64 kth = kth_of<THREADS>(cand_at, W * CAP, k, &lds);
                     C.set_bound(kth - 1);
                 }
                 __syncthreads();
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
 #pragma unroll
         for (int w = 0; w < W; ++w) total += counts[w];
         u64 kth = 1;
-        if (total > k) kth = block_kth<THREADS>(cand_at, W * CAP, k, 0, hist);
+        if (total > k) kth = kth_of<THREADS>(cand_at, W * CAP, k, &lds);
         for (uint32_t i = threadIdx.x; i < W * CAP; i += THREADS) {
             const u64 key = cand_at(i);
             if (key >= kth) best[atomicAdd(&nbest, 1u)] = key;
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
     extern __shared__ uint32_t groups[];
     __shared__ u64 cand[W][CAP];
     __shared__ u64 best[KMAX];
-    __shared__ uint32_t hist[256];
+    __shared__ CountLds lds;
     __shared__ uint32_t counts[W], nbest;
     __shared__ float tmp_f[W];
     __shared__ double tmp_d[W];
@@ -250,10 +250,9 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
             groups[s * 64 + lane] = s * kSeg + lane * V < n ? order_key(gm) : 0;
         }
         __syncthreads();
-        const u64 kth_group = block_kth<THREADS>([&](uint32_t i) { return (u64)groups[i] << 32; }, n_segs * 64, k, 32, hist);
+        const uint32_t bound = (uint32_t)kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, n_segs * 64, k, &lds);
         Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
-        C.set_bound(kth_group);
-        const uint32_t bound = (uint32_t)(kth_group >> 32);
+        C.set_bound((u64)bound << 32);
         for (uint32_t s = wave; s < n_segs; s += W) {
             u64 hit = __ballot(groups[s * 64 + lane] >= bound);
             while (hit) {   // two groups at a time, a class a lane
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
 #pragma unroll
         for (int w = 0; w < W; ++w) total += counts[w];
         u64 kth = 1;
-        if (total > k) kth = block_kth<THREADS>(cand_at, W * CAP, k, 0, hist);
+        if (total > k) kth = kth_of<THREADS>(cand_at, W * CAP, k, &lds);
         for (uint32_t i = threadIdx.x; i < W * CAP; i += THREADS) {
             const u64 key = cand_at(i);
             if (key >= kth) best[atomicAdd(&nbest, 1u)] = key;
@@ -308,7 +307,7 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
                                                         float c, double inv_t, float* __restrict__ values,
                                                         int32_t* __restrict__ index, float* __restrict__ lse) {
     __shared__ u64 best[kMaxTop];
-    __shared__ uint32_t hist[256];
+    __shared__ CountLds lds;
     __shared__ uint32_t nbest;
     __shared__ float tmp_f[THREADS / 64];
     __shared__ double tmp_d[THREADS / 64];
@@ -324,7 +323,7 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
     double s;
     __syncthreads();
     block_running<THREADS>(run, c, m, s, tmp_f, tmp_d);
-    const u64 kth = block_kth<THREADS>([&](uint32_t i) { return keys[i]; }, parts * k, k, 0, hist);
+    const u64 kth = kth_of<THREADS>([&](uint32_t i) { return keys[i]; }, parts * k, k, &lds);
     for (uint32_t i = threadIdx.x; i < parts * k; i += THREADS) {
         const u64 key = keys[i];
         if (key != 0 && key >= kth) best[atomicAdd(&nbest, 1u)] = key;
