@@ -44,34 +44,49 @@ __device__ __forceinline__ Row settings(const Settings& S, uint64_t row, uint32_
 __device__ __forceinline__ uint32_t class_key(float x, bool allowed) {
     return allowed && x > -INFINITY ? order_key(x) : 0;
 }
-// 2^f for |f| <= 1/2, within 2^-44, and exactly 1 at 0: 1 + f q(f), q the polynomial of degree 8 that meets
-// (2^f - 1) / f in the Chebyshev points of the interval.
-__device__ __forceinline__ double exp2_part(double f) {
-    double q = 1.0203121063391729e-07;
-    q = __builtin_fma(q, f, 1.3255224878668817e-06);
-    q = __builtin_fma(q, f, 1.525268684626772e-05);
-    q = __builtin_fma(q, f, 0.00015403455852453838);
-    q = __builtin_fma(q, f, 0.0013333558179043112);
-    q = __builtin_fma(q, f, 0.009618129159402558);
-    q = __builtin_fma(q, f, 0.055504108664760424);
-    q = __builtin_fma(q, f, 0.2402265069581299);
-    q = __builtin_fma(q, f, 0.6931471805599453);
-    return __builtin_fma(q, f, 1.0);
-}
 // The mass of a score: 2^((x - m) c) in units of 2^-S, rounded to an integer by the addition of 2^52
 // (S <= 51).  -inf and NaN have none (the maximum with a number drops NaN).  m is finite.
 struct Masses {
     double m, c;   // largest score, log2(e) / temperature
     double big;    // 1.5 2^52 + S
-    __device__ __forceinline__ Masses(double m, double c, int S) : m(m), c(c), big(6755399441055744.0 + S) {}
+    double q[9];
+    // 2^f for |f| <= 1/2, within 2^-44, and exactly 1 at 0: 1 + f q(f), q the polynomial of degree 8 that meets
+    // (2^f - 1) / f in the Chebyshev points of the interval.  Its coefficients are held in scalar registers (the
+    // compiler's own choice is 18 vector registers).
+    __device__ __forceinline__ Masses(double m, double c, int S) : m(m), c(c), big(6755399441055744.0 + S) {
+        const double k[9] = {0.6931471805599453, 0.2402265069581299, 0.055504108664760424,
+                             0.009618129159402558, 0.0013333558179043112, 0.00015403455852453838,
+                             1.525268684626772e-05, 1.3255224878668817e-06, 1.0203121063391729e-07};
+#pragma unroll
+        for (int i = 0; i < 9; ++i) {
+            q[i] = k[i];
+            asm("" : "+s"(q[i]));
+        }
+    }
+    __device__ __forceinline__ double exp2_part(double f) const {
+        double p = q[8];
+#pragma unroll
+        for (int i = 7; i >= 0; --i) p = __builtin_fma(p, f, q[i]);
+        return __builtin_fma(p, f, 1.0);
+    }
     __device__ __forceinline__ u64 raw(float x) const {   // the mass plus kRaw
-        const double y = fmax(((double)x - m) * c, -120.0);   // (no mass below -53)
+        // (the difference first: beside scores next to the lowest f32 the product's rounding would be more than it)
+        const double y = fmax(((double)x - m) * c, -120.0);   // no mass below -53
         // y rounded to an integer k, and k + S in the low word of the sum: it goes to the exponent of a
         // number in [0.7, 1.5]
         const double t = y + big, k = t - big;
         const uint32_t e = (uint32_t)__builtin_bit_cast(u64, t);
         const u64 p = __builtin_bit_cast(u64, exp2_part(y - k)) + ((u64)e << 52);
         return __builtin_bit_cast(u64, __builtin_bit_cast(double, p) + 4503599627370496.0);
+    }
+    // sums of masses against the largest's
+    __device__ __forceinline__ double log_of(u64 total) const { return log((double)total / (double)(*this)((float)m)); }
+    // the mass of a weight of min_p (0 and NaN: none; 1: the largest's own)
+    __device__ __forceinline__ u64 least(double min_p) const {
+        const u64 one = (*this)((float)m);
+        if (!(min_p > 0.0)) return 0;
+        const double v = ceil(min_p * (double)one);
+        return v < (double)one ? (u64)v : one;
     }
     static constexpr u64 kRaw = 0x4330000000000000ull;
     __device__ __forceinline__ u64 operator()(float x) const { return raw(x) - kRaw; }
@@ -88,11 +103,6 @@ __device__ __forceinline__ u64 nucleus_of(double p, u64 total) {
     const u64 v = d > 0.0 ? (u64)d : 0;
     return v < 1 ? 1 : v > total ? total : v;
 }
-// the mass of a weight of min_p (0 and NaN: none)
-__device__ __forceinline__ u64 least_mass(double min_p, int S) {
-    return min_p > 0.0 ? (u64)ceil(ldexp(min_p, S)) : 0;
-}
-
 
 // ---- entries in registers ----------------------------------------------------------------------
 // Exclusive prefix sum over the workgroup, in thread order, and the sum of all.
@@ -339,7 +349,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
         } else {
             if (r.k) L.cut_count(r.k, &lds, tmp);
             if (r.p < 1.0) L.cut_mass(nucleus_of(r.p, r.k ? L.sum(tmp) : total), &lds);
-            L.drop_below(least_mass(r.min_p, shift));
+            L.drop_below(M.least(r.min_p));
         }
         u64 mine = 0, all;
 #pragma unroll
@@ -360,19 +370,18 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
                 }
                 before += w;
             }
-            out.put(row, cls, (inf ? 0.0 : ((double)xs - (double)m) * r.rt) - log(ldexp((double)total, -shift)));
+            out.put(row, cls, (inf ? 0.0 : ((double)xs - (double)m) * r.rt) - M.log_of(total));
         }
         __syncthreads();
     }
 }
 
 // ---- long rows --------------------------------------------------------------------------------
-// A wave takes 2048 classes at a time (a segment), a lane 32 of them (a group): 16-byte vectors, lanes side by
-// side.  Which classes can be kept is found from the maxima of the groups (few of many: top_k), or from a
+// A wave takes 2048 classes at a time (a segment), in groups of 32.  Which classes can be kept is found from the maxima of the groups (few of many: top_k), or from a
 // histogram of counts or masses over the distance from the largest score; those, or those of the one
 // bin in which the cut lies, are listed, and the list cut exactly in registers.  Kept masses of the
 // bins above a nucleus's last are summed by segments, and the draw looks through one of them.
-constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024;
+constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024, kListCap = 8192, kShortList = 512;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
 // The bins reach from the largest score to a little below the lowest of a sample (the first score of every group),
 // 32 nats at most: 32 bins a nat, and more of them for the rows whose nucleus is wide, so that one bin holds
@@ -385,7 +394,8 @@ enum Mode : uint32_t { kGreedy, kWhole, kList, kNucleus };   // (kWhole: a least
 
 template <class T, bool kUnit, int THREADS>
 struct Long {
-    static constexpr int V = Pack<T>::V, U = kGroup / V, W = THREADS / 64, CAP = THREADS * 8;
+    static constexpr int V = Pack<T>::V, U = kGroup / V, W = THREADS / 64;
+    static constexpr int E = THREADS == 256 ? 8 : kListCap / THREADS, CAP = THREADS * E;   // a list's entries in registers
     const T* x0;
     int64_t cs;
     uint32_t n;
@@ -432,8 +442,10 @@ struct Long {
         load_tile<T, kUnit>(x0, cs, seg * kSeg, n, -INFINITY, t.p);
     }
     __device__ __forceinline__ float score(uint32_t i) const {
-        if (i >= n || (r.allowed && !(r.allowed[i >> 5] >> (i & 31) & 1))) return -INFINITY;
-        return to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * cs]);
+        const uint32_t j = min(i, n - 1);   // (a load that waits for no branch)
+        const float x = to_f32(x0[kUnit ? (int64_t)j : (int64_t)j * cs]);
+        const uint32_t bits = r.allowed ? r.allowed[j >> 5] >> (j & 31) : 1;
+        return i < n && (bits & 1) ? x : -INFINITY;
     }
     __device__ __forceinline__ Mode mode() const {
         return r.greedy ? kGreedy : r.min_p > 1.0 ? kWhole : r.k ? kList : r.p < 1.0 ? kNucleus : kWhole;
@@ -456,19 +468,25 @@ struct Long {
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             Tile t;
             load(seg, t);
-            float x[U][V], gm = -INFINITY;
+            float x[U][V], vm[U], gm = -INFINITY;
 #pragma unroll
             for (int u = 0; u < U; ++u) t.get(u, x[u]);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                vm[u] = -INFINITY;   // (NaN is no class)
 #pragma unroll
-                for (int v = 0; v < V; ++v) gm = fmaxf(gm, x[u][v]);
+                for (int v = 0; v < V; ++v) vm[u] = fmaxf(vm[u], x[u][v]);
+                gm = fmaxf(gm, vm[u]);
+            }
             if (gm > best) {
                 best = gm;
                 best_seg = seg;
             }
             if (x[0][0] > -INFINITY) low = fminf(low, x[0][0]);
-            if (groups) groups[(seg - s0) * 64 + lane] = gm > -INFINITY ? order_key(gm) : 0;
+            if (groups) {
+                const float g = group_max<V>(vm, lane, MaxF());
+                groups[(seg - s0) * 64 + group_of<V>(lane)] = g > -INFINITY ? order_key(g) : 0;
+            }
             if (sums) {
                 run.raise(gm, c);
 #pragma unroll
@@ -565,14 +583,39 @@ struct Long {
     __device__ __forceinline__ u64 weigh(uint32_t s0, uint32_t s1, const Masses& M, u64 least, u64* segs) const {
         return least ? weigh_segments<true>(s0, s1, M, least, segs) : weigh_segments<false>(s0, s1, M, 0, segs);
     }
+    // The lowest score whose bin is at most b (bins are monotone; by halving the order keys).
+    __device__ __forceinline__ float lowest_of(uint32_t b) const {
+        uint32_t lo = order_key(-INFINITY), hi = order_key(bm);   // (bin(lo) is above b, or lo is it; bin(hi) = 0)
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (bin(key_score(mid)) <= b) hi = mid;
+            else lo = mid;
+        }
+        return key_score(hi);
+    }
+    // Entries of a wave's staging area in LDS: at least two vectors of hits in all lanes.
+    static constexpr uint32_t kStage = 128 * V;
     // The classes in bin `cut`, and with `all` those in the bins before, go to the list (at most cap; count goes
     // on); with kSum the masses of the bins before go to their segments.
     template <bool kSum>
     __device__ __forceinline__ void collect(uint32_t s0, uint32_t s1, const Masses& M, uint32_t cut, bool all, u64 least,
-                                            u64* segs, u64* list, uint32_t* count, uint32_t cap) const {
+                                            u64* segs, u64* list, uint32_t* count, uint32_t cap, u64* stage) const {
+        stage += wave * kStage;
+        uint32_t staged = 0;
+        auto flush = [&]() {
+            wave_fence();
+            uint32_t base = 0;
+            if (lane == 0) base = atomicAdd(count, staged);
+            base = __builtin_amdgcn_readfirstlane(base);
+            for (uint32_t i = lane; i < staged; i += 64)
+                if (base + i < cap) list[base + i] = stage[i];
+            wave_fence();
+            staged = 0;
+        };
+        const float from = cut == kBins - 1 ? kLowest : lowest_of(cut);   // (the last bin takes all that is left)
+        const float above = all || cut == 0 ? INFINITY : lowest_of(cut - 1);
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             u64 sum = 0;
-            uint32_t hits = 0;   // a bit a class of the lane's group
             Tile t;
             load(seg, t);
 #pragma unroll
@@ -581,32 +624,27 @@ struct Long {
                 t.get(u, x);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const uint32_t b = bin(x[v]);
-                    if (kSum && b < cut) {
-                        const u64 w = M(x[v]);
+                    if (kSum) {
+                        const u64 w = M(x[v] >= above ? x[v] : -INFINITY);
                         sum += w >= least ? w : 0;
                     }
-                    if (x[v] > -INFINITY && (b == cut || (all && b < cut))) hits |= 1u << (u * V + v);
+                    const bool in = x[v] >= from && x[v] < above;
+                    const u64 who = __ballot(in);
+                    if (who) {
+                        if (in) stage[staged + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] =
+                            rank_key(x[v], at(seg, u, lane) + v);
+                        staged += (uint32_t)__popcll(who);
+                    }
                 }
+                if (staged > kStage - 64 * V) flush();
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            if (__any(hits != 0)) {   // one place in the list for the segment's
-                const uint32_t mine = (uint32_t)__popc(hits), upto = wave_scan(mine, Add(), 0u);
-                uint32_t base = 0;
-                if (lane == 0) base = atomicAdd(count, read_lane(upto, 63));
-                base = __builtin_amdgcn_readfirstlane(base) + upto - mine;
-                while (hits) {
-                    const uint32_t q = (uint32_t)__builtin_ctz(hits), i = at(seg, (int)(q / V), lane) + q % V;
-                    if (base < cap) list[base] = rank_key(score(i), i);
-                    ++base;
-                    hits &= hits - 1;
-                }
             }
             if (kSum) {
                 sum = wave_reduce(sum, Add());
                 if (lane == 0) segs[seg] = sum;
             }
         }
+        if (staged) flush();
     }
     // Classes of the groups whose largest reaches the bound go to the list (count[0]): the groups are listed
     // first (count[1]; as many as there are at most), then half a wave reads a group.  count starts as 0.
@@ -616,18 +654,27 @@ struct Long {
             if (groups[g] != 0 && groups[g] >= bound) hits[atomicAdd(&count[1], 1u)] = (uint16_t)g;
         __syncthreads();
         const uint32_t n_hits = count[1], q = threadIdx.x % kGroup;
-        for (uint32_t h = threadIdx.x / kGroup; h < n_hits; h += THREADS / kGroup) {
-            const uint32_t i = at(hits[h] / 64, (int)q / V, hits[h] % 64) + q % V;
-            const float x = score(i);
-            if (x > -INFINITY && order_key(x) >= bound) {
-                const uint32_t at = atomicAdd(&count[0], 1u);
-                if (at < (uint32_t)CAP) list[at] = rank_key(x, i);
+        constexpr int D = 8;   // groups a half wave has under way
+        for (uint32_t h0 = threadIdx.x / kGroup; h0 < n_hits; h0 += THREADS / kGroup * D) {
+            float x[D];
+            uint32_t i[D];
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const uint32_t h = h0 + d * (THREADS / kGroup), g = h < n_hits ? hits[h] : 0;
+                i[d] = h < n_hits ? g * kGroup + q : n;
+                x[d] = score(i[d]);
             }
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                if (x[d] > -INFINITY && order_key(x[d]) >= bound) {
+                    const uint32_t at = atomicAdd(&count[0], 1u);
+                    if (at < (uint32_t)CAP) list[at] = rank_key(x[d], i[d]);
+                }
         }
     }
-    __device__ __forceinline__ void read_list(Entries<THREADS, 8>& L, const u64* list, uint32_t count) const {
+    __device__ __forceinline__ void read_list(Entries<THREADS, E>& L, const u64* list, uint32_t count) const {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < E; ++e) {
             const uint32_t i = e * THREADS + threadIdx.x;
             const u64 k = i < count ? list[i] : 0;
             L.key[e] = (uint32_t)(k >> 32);
@@ -639,39 +686,44 @@ struct Long {
     // A list that holds every class that may be kept: top_k, top_p, min_p, and the draw.
     __device__ void finish_list(const u64* list, uint32_t count, const Masses& M, double log_z, uint64_t row, SelectLds* lds,
                                 u64* tmp, const Out& out) const {
-        if (count <= 256) {
+        if (count <= min(kShortList, (uint32_t)THREADS)) {
             finish_short(list, count, M, log_z, row, lds, tmp, out);
             return;
         }
-        Entries<THREADS, 8> L;
+        Entries<THREADS, E> L;
         read_list(L, list, count);
         L.cut_count(r.k, lds, tmp);
         L.weigh(M);
         if (r.p < 1.0) L.cut_mass(nucleus_of(r.p, L.sum(tmp)), lds);
-        L.drop_below(least_mass(r.min_p, S));
+        L.drop_below(M.least(r.min_p));
         const u64 want = target_of(r.u, L.sum(tmp)) + 1;
         const Crossing c = select<THREADS, true, false>(
             [&](auto f) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < E; ++e)
                     if (L.key[e] && L.mass[e]) f((uint32_t)~L.idx[e], L.mass[e]);
             },
             want, lds);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < E; ++e)
             if (L.key[e] && L.mass[e] && (uint32_t)~L.idx[e] >= c.from && (uint32_t)~L.idx[e] <= c.last)
                 out.put(row, L.idx[e], ((double)key_score(L.key[e]) - M.m) * r.rt - log_z);
     }
-    // The same for up to 256 classes: every entry counts those ahead of it, and later the mass before it.
+    // The same for up to 512 classes, one a thread: every entry counts those ahead of it, and later the mass before it.
     __device__ void finish_short(const u64* list, uint32_t count, const Masses& M, double log_z, uint64_t row, SelectLds* lds,
                                  u64* tmp, const Out& out) const {
         const uint32_t t = threadIdx.x;
-        if (t < count) lds->mass[t] = list[t];
+        if (t < kShortList) {
+            lds->mass[t] = t < count ? list[t] : 0;
+            lds->rank[t] = 0;
+        }
         __syncthreads();
         if (t < count) {
             const u64 key = lds->mass[t];
             uint32_t place = 0;
-            for (uint32_t j = 0; j < count; ++j) place += lds->mass[j] > key;
+            for (uint32_t j = 0; j < count; j += 8)   // (a read at a time would wait for LDS at each)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) place += lds->mass[j + q] > key;
             lds->rank[place] = key;
         }
         __syncthreads();
@@ -681,16 +733,18 @@ struct Long {
         u64 w = t < kept ? M(x) : 0, all;
         const u64 ahead = block_scan<THREADS>(w, all, tmp);
         if (r.p < 1.0 && ahead >= nucleus_of(r.p, all)) w = 0;
-        if (w < least_mass(r.min_p, S)) w = 0;
-        if (t < count) lds->mass[t] = w;
+        if (w < M.least(r.min_p)) w = 0;
+        if (t < kShortList) lds->mass[t] = w;
         __syncthreads();
         u64 before = 0, sum = 0;
         if (t < kept) {
-            for (uint32_t j = 0; j < kept; ++j) {
-                const u64 wj = lds->mass[j];
-                before += (uint32_t)lds->rank[j] > (uint32_t)rank ? wj : 0;   // (~class: larger for a class before)
-                sum += wj;
-            }
+            for (uint32_t j = 0; j < kept; j += 8)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const u64 wj = lds->mass[j + q];
+                    before += (uint32_t)lds->rank[j + q] > (uint32_t)rank ? wj : 0;   // (~class: larger for a class before)
+                    sum += wj;
+                }
             const u64 target = target_of(r.u, sum);
             if (w && target >= before && target - before < w) out.put(row, ~(uint32_t)rank, ((double)x - M.m) * r.rt - log_z);
         }
@@ -737,7 +791,7 @@ struct Long {
                 if (!found && target - before < w[q]) {
                     found = true;
                     const uint32_t i = seg * kSeg + threadIdx.x * Q + q;
-                    out.put(row, i, ((double)score(i) - M.m) * r.rt - log(ldexp((double)total, -S)));
+                    out.put(row, i, ((double)score(i) - M.m) * r.rt - M.log_of(total));
                 }
                 before += w[q];
             }
@@ -756,7 +810,7 @@ struct Long {
             if (key_at(i)) total += mass(score(i));
         total = block_reduce<THREADS>(total, Add(), tmp);
         if (r.min_p > 1.0) {
-            if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)total, -S)));
+            if (threadIdx.x == 0) out.put(row, first, -M.log_of(total));
             __syncthreads();
             return;
         }
@@ -789,7 +843,7 @@ struct Long {
                 nucleus_of(r.p, kept), lds);
             from = c.from > from ? c.from : from;
         }
-        const u64 least = least_mass(r.min_p, S);
+        const u64 least = M.least(r.min_p);
         // thread t holds the classes [t per, (t + 1) per)
         const uint32_t per = (n + THREADS - 1) / THREADS, a = min(n, threadIdx.x * per), b = min(n, a + per);
         auto weight = [&](uint32_t i) -> u64 {
@@ -805,7 +859,7 @@ struct Long {
         if (target >= before && target - before < mine) {
             uint32_t i = a;
             for (u64 w; target - before >= (w = weight(i)); ++i) before += w;
-            out.put(row, i, (inf ? 0.0 : ((double)score(i) - (double)m) * r.rt) - log(ldexp((double)total, -S)));
+            out.put(row, i, (inf ? 0.0 : ((double)score(i) - (double)m) * r.rt) - M.log_of(total));
         }
         __syncthreads();
     }
@@ -848,6 +902,7 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
     __shared__ double tmp_d[W];
     __shared__ uint32_t counts[2];
     uint32_t& count = counts[0];
+    __shared__ u64 stage[W * L::kStage];
     const uint32_t n_segs = (X.classes + kSeg - 1) / kSeg;
     u64* list = pool;
     u64* segs = pool + L::CAP;
@@ -882,12 +937,12 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
         const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
         R.set_bins(m, -block_reduce<THREADS>(-low, MaxF(), tmp_f));
         if (!slow && mode == kWhole) {
-            const u64 least = least_mass(R.r.min_p, shift);
+            const u64 least = M.least(R.r.min_p);
             u64 z = R.weigh(0, n_segs, M, R.r.min_p > 1.0 ? 0 : least, segs);
             z = block_reduce<THREADS>(z, Add(), tmp);
             __syncthreads();
             if (R.r.min_p > 1.0) {
-                if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)z, -shift)));
+                if (threadIdx.x == 0) out.put(row, first, -M.log_of(z));
             } else {
                 R.finish_segments(segs, n_segs, M, kBins, 0, least, z, row, tmp, pick, out);
             }
@@ -897,9 +952,9 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
             u64 z = 0;
             for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) z += hist[bin_at(b)];
             z = block_reduce<THREADS>(z, Add(), tmp);
-            const u64 want = nucleus_of(R.r.p, z), least = least_mass(R.r.min_p, shift);
+            const u64 want = nucleus_of(R.r.p, z), least = M.least(R.r.min_p);
             const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
-            R.template collect<true>(0, n_segs, M, f.bin, false, least, segs, list, &count, L::CAP);
+            R.template collect<true>(0, n_segs, M, f.bin, false, least, segs, list, &count, L::CAP, stage);
             __syncthreads();
             if (count > (uint32_t)L::CAP) {
                 slow = true;
@@ -951,7 +1006,7 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
                 if (f.above + f.inside > (u64)L::CAP) {
                     slow = true;
                 } else {
-                    R.template collect<false>(0, n_segs, M, f.bin, true, 0, nullptr, list, &count, L::CAP);
+                    R.template collect<false>(0, n_segs, M, f.bin, true, 0, nullptr, list, &count, L::CAP, stage);
                     __syncthreads();
                 }
             }
@@ -986,7 +1041,6 @@ struct Space {    // the workspace of a chunk of rows
     u64* totals;        // [rows][parts2]
     uint32_t parts1, per1, parts2, per2, n_segs;   // parts of a row and segments a part: of the scan, of the rest
 };
-constexpr uint32_t kListCap = 8192;
 
 template <int THREADS>
 __device__ __forceinline__ u64 row_top(const Space& P, uint64_t row, u64* tmp, float& low) {
@@ -1033,8 +1087,8 @@ __global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int sh
 
 // Masses of the segments, or the part's histogram of masses or counts.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(512, 4) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
-    constexpr int THREADS = 512;
+__global__ __launch_bounds__(256, 4) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
+    constexpr int THREADS = 256;
     __shared__ u64 hist[kBinsPad];
     __shared__ u64 tmp[THREADS / 64];
     const uint64_t row = blockIdx.x / P.parts2;
@@ -1048,7 +1102,7 @@ __global__ __launch_bounds__(512, 4) void weigh_kernel(Rows<T> X, Settings S, in
     if (top == 0 || m == INFINITY) return;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
     if (mode == kWhole) {
-        u64 all = R.weigh(s0, s1, M, R.r.min_p > 1.0 ? 0 : least_mass(R.r.min_p, shift), P.segs + row * P.n_segs);
+        u64 all = R.weigh(s0, s1, M, R.r.min_p > 1.0 ? 0 : M.least(R.r.min_p), P.segs + row * P.n_segs);
         all = block_reduce<THREADS>(all, Add(), tmp);
         if (threadIdx.x == 0) P.totals[row * P.parts2 + part] = all;
         return;
@@ -1065,8 +1119,8 @@ __global__ __launch_bounds__(512, 4) void weigh_kernel(Rows<T> X, Settings S, in
 
 // The classes of the cut's bin (top_k: and of those before), and the segments' masses before it.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(512, 4) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
-    constexpr int THREADS = 512;
+__global__ __launch_bounds__(256, 4) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
+    constexpr int THREADS = 256;
     __shared__ u64 hist[kBinsPad];
     __shared__ u64 tmp[THREADS / 64];
     const uint64_t row = blockIdx.x / P.parts2;
@@ -1094,26 +1148,23 @@ __global__ __launch_bounds__(512, 4) void collect_kernel(Rows<T> X, Settings S, 
     const bool over = mode == kList && f.above + f.inside > kListCap;
     if (part == 0 && threadIdx.x == 0) P.steps[row] = Step{total, f.above, f.bin, over ? kOverflow : kCut};
     if (over) return;
+    __shared__ u64 stage[THREADS / 64 * Long<T, kUnit, THREADS>::kStage];
     u64* list = P.list + row * kListCap;
     if (mode == kNucleus)
-        R.template collect<true>(s0, s1, M, f.bin, false, least_mass(R.r.min_p, shift), P.segs + row * P.n_segs, list, &P.count[row], kListCap);
+        R.template collect<true>(s0, s1, M, f.bin, false, M.least(R.r.min_p), P.segs + row * P.n_segs, list, &P.count[row], kListCap, stage);
     else
-        R.template collect<false>(s0, s1, M, f.bin, true, 0, nullptr, list, &P.count[row], kListCap);
+        R.template collect<false>(s0, s1, M, f.bin, true, 0, nullptr, list, &P.count[row], kListCap, stage);
 }
 
-// A workgroup a row: the exact cut, and the draw.
+// Rows that need no list: nothing allowed, the largest score, the whole row.  (Of 256 threads: 1024 with the
+// registers of the lists are one workgroup a CU.)
 template <class T, bool kUnit>
-__global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
-    constexpr int THREADS = 1024, W = THREADS / 64;
-    typedef Long<T, kUnit, THREADS> L;
-    extern __shared__ u64 pool[];   // the row's groups and their list, or its segments' masses
+__global__ __launch_bounds__(256) void draw_whole_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
+    constexpr int THREADS = 256, W = THREADS / 64;
     __shared__ SelectLds lds;
     __shared__ u64 tmp[W], pick[2];
-    __shared__ float tmp_f[W];
-    __shared__ double tmp_d[W];
-    __shared__ uint32_t count[2];
     const uint64_t row = blockIdx.x;
-    L R(X, S, row, shift);
+    Long<T, kUnit, THREADS> R(X, S, row, shift);
     const Mode mode = R.mode();
     float low;
     const u64 top = row_top<THREADS>(P, row, tmp, low);
@@ -1127,42 +1178,70 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
         if (threadIdx.x == 0) out.put(row, first, 0.0);
         return;
     }
+    if (mode != kWhole) return;
+    if (m == INFINITY) {
+        R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
+        return;
+    }
+    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+    u64 total = 0;
+    for (uint32_t p = threadIdx.x; p < P.parts2; p += THREADS) total += P.totals[row * P.parts2 + p];
+    total = block_reduce<THREADS>(total, Add(), tmp);
+    if (R.r.min_p > 1.0) {
+        if (threadIdx.x == 0) out.put(row, first, -M.log_of(total));
+        return;
+    }
+    R.finish_segments(P.segs + row * P.n_segs, P.n_segs, M, kBins, 0, M.least(R.r.min_p), total, row, tmp, pick, out);
+}
+
+// The others, a workgroup a row: the exact cut, and the draw.
+template <class T, bool kUnit>
+__global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int shift, Out out, Space P, bool alone) {
+    constexpr int THREADS = 1024, W = THREADS / 64;
+    typedef Long<T, kUnit, THREADS> L;
+    extern __shared__ u64 pool[];   // the row's groups and their list, or its segments' masses
+    __shared__ SelectLds lds;
+    __shared__ u64 tmp[W], pick[2];
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    __shared__ uint32_t count[2];
+    const uint64_t row = blockIdx.x;
+    L R(X, S, row, shift);
+    const Mode mode = R.mode();
+    float low;
+    const u64 top = row_top<THREADS>(P, row, tmp, low);
+    const float m = key_score((uint32_t)(top >> 32));
+    if (top == 0) {
+        if (alone && threadIdx.x == 0) out.empty(row);
+        return;
+    }
+    if (mode == kGreedy || mode == kWhole) return;
+    const uint32_t first = ~(uint32_t)top;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
     const bool by_groups = mode == kList && P.groups && R.by_groups(P.n_segs);
     bool slow = m == INFINITY;
-    if (!slow && mode == kWhole) {
-        u64 total = 0;
-        for (uint32_t p = threadIdx.x; p < P.parts2; p += THREADS) total += P.totals[row * P.parts2 + p];
-        total = block_reduce<THREADS>(total, Add(), tmp);
-        if (R.r.min_p > 1.0) {
-            if (threadIdx.x == 0) out.put(row, first, -log(ldexp((double)total, -shift)));
-            return;
-        }
-        R.finish_segments(P.segs + row * P.n_segs, P.n_segs, M, kBins, 0, least_mass(R.r.min_p, shift), total, row, tmp, pick, out);
-        return;
-    }
     if (!slow && mode == kNucleus) {
         const Step step = P.steps[row];
         const uint32_t n_list = P.count[row];
-        const u64 least = least_mass(R.r.min_p, shift);
+        const u64 least = M.least(R.r.min_p);
         slow = n_list > kListCap;
         if (!slow) {
             for (uint32_t s = threadIdx.x; s < P.n_segs; s += THREADS) pool[s] = P.segs[row * P.n_segs + s];
-            Entries<THREADS, 8> E;
+            Entries<THREADS, L::E> E;
             R.read_list(E, P.list + row * kListCap, n_list);
             E.weigh(M);
             __syncthreads();
             const Crossing x = select<THREADS, true, true>(
                 [&](auto g) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+                    for (int e = 0; e < L::E; ++e)
                         if (E.key[e] && E.mass[e]) g(E.rank(e), E.mass[e]);
                 },
                 nucleus_of(R.r.p, step.total) - step.above, &lds);
             E.keep_from(x);
             E.drop_below(least);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < L::E; ++e)
                 if (E.key[e] && E.mass[e]) atomicAdd(&pool[E.idx[e] / kSeg], E.mass[e]);
             __syncthreads();
             R.set_bins(m, low);
@@ -1238,7 +1317,7 @@ Space plan(uint64_t rows, uint32_t n, unsigned char* base, size_t* bytes) {
         parts = (P.n_segs + per - 1) / per;
     };
     split(2048, 4, P.parts1, P.per1);
-    split(768, 8, P.parts2, P.per2);
+    split(1024, 4, P.parts2, P.per2);
     size_t at = 0;
     auto take = [&](size_t size) {
         const size_t a = at;
@@ -1266,6 +1345,8 @@ int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out,
     const uint32_t n_segs = (X.classes + kSeg - 1) / kSeg;
     const bool list_by_groups = all_list && Long<T, kUnit, 1024>::by_groups_of(S.k, n_segs);
     const bool any_cut = S.k_rows || S.p_rows || S.p < 1.0 || any_list;
+    const bool any_whole = S.t_rows || !(S.t > 0.0) || S.min_p_rows || S.min_p > 1.0 ||
+                           ((S.k_rows || !any_list) && (S.p_rows || !(S.p < 1.0)));
     for (uint64_t r0 = 0; r0 < X.rows; r0 += kChunkRows) {
         const uint64_t m = std::min(kChunkRows, X.rows - r0);
         size_t bytes = 0;
@@ -1284,19 +1365,24 @@ int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out,
         scan_kernel<T, kUnit><<<(unsigned)(m * P.parts1), 256, 0, st>>>(C, Q, shift, o, P);
         CLS_TRY(hipGetLastError());
         if (!all_greedy && !list_by_groups) {
-            weigh_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 512, 0, st>>>(C, Q, shift, P);
+            weigh_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 256, 0, st>>>(C, Q, shift, P);
             CLS_TRY(hipGetLastError());
             if (any_cut) {
-                collect_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 512, 0, st>>>(C, Q, shift, P);
+                collect_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 256, 0, st>>>(C, Q, shift, P);
                 CLS_TRY(hipGetLastError());
             }
         }
+        if (any_whole) {
+            draw_whole_kernel<T, kUnit><<<(unsigned)m, 256, 0, st>>>(C, Q, shift, o, P);
+            CLS_TRY(hipGetLastError());
+        }
+        if (all_greedy || !any_cut) continue;
         // LDS: a list and the groups, or the segments
         size_t lds = any_list && P.groups ? sizeof(u64) * kListCap + (sizeof(uint32_t) + sizeof(uint16_t)) * 64 * P.n_segs : 0;
         lds = std::max(lds, sizeof(u64) * P.n_segs);
         if (lds > 32 * 1024)
             CLS_TRY(hipFuncSetAttribute((const void*)draw_kernel<T, kUnit>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        draw_kernel<T, kUnit><<<(unsigned)m, 1024, lds, st>>>(C, Q, shift, o, P);
+        draw_kernel<T, kUnit><<<(unsigned)m, 1024, lds, st>>>(C, Q, shift, o, P, !any_whole);
         CLS_TRY(hipGetLastError());
     }
     return CBH_OK;

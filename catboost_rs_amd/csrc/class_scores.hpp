@@ -230,6 +230,29 @@ struct MinU {
     __device__ __forceinline__ V none() const { return ~V(0); }
 };
 
+// The largest of 32 classes next to each other (a group), from the maxima of a lane's vectors: vector u of 32 / V
+// lanes side by side is a group.  Lane l gets that of group group_of<V>(l) of the tile, which holds the classes
+// [32 g, 32 g + 32): what is read again of a group is one run of memory.
+template <int V>
+__device__ __forceinline__ uint32_t group_of(uint32_t lane) {
+    constexpr uint32_t L = kGroup / V;
+    return lane % L * (64 / L) + lane / L;
+}
+template <int V, class K, class Op>
+__device__ __forceinline__ K group_max(const K (&vm)[kGroup / V], uint32_t lane, Op op) {
+    constexpr int L = (int)kGroup / V;   // lanes of a group, and vectors of a lane
+    K out = vm[0];
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+        K k = vm[u];
+        k = op(k, dpp_move<0xB1, 0xf>(k, k));                    // lanes 1 0 3 2
+        k = op(k, dpp_move<0x4E, 0xf>(k, k));                    // lanes 2 3 0 1
+        if constexpr (L == 8) k = op(k, dpp_move<0x141, 0xf>(k, k));   // mirrored within 8
+        out = lane % L == (uint32_t)u ? k : out;
+    }
+    return out;
+}
+
 // Where a sum over 256 bins in LDS, taken from bin 255 down, reaches `want`: the bin, what lies above it
 // and what it holds (the lowest non-zero place if the sum stays below).  Every wave finds it by itself: lane l
 // holds bins 255 - 4 l .. 252 - 4 l.  (Walked bin by bin with wave-uniform 64-bit sums, hipcc 7.2 selected
@@ -268,8 +291,8 @@ struct CountLds {
     uint32_t count[256];
 };
 struct SelectLds : CountLds {
-    u64 mass[256];
-    u64 rank[256];
+    u64 mass[512];   // (256 digits; or the entries of a short list)
+    u64 rank[512];
 };
 // The bits of a rank's distance that are known before the digit at `shift`: from here up.
 __device__ __forceinline__ int prefix_shift(int shift, int bits) {

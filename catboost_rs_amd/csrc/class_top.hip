@@ -202,8 +202,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
 }
 
 // Long rows and a k that is small beside them.  The pass over the scores takes nothing but the log-sum-exp
-// and the largest of every group of 32 classes (a lane's share of the 2048 classes a wave reads at a time), kept in
-// LDS.  The k-th largest of those maxima is a bound that at least k scores reach and hardly more (a k of a
+// and the largest of every group of 32 classes, kept in LDS.  The k-th largest of those maxima is a bound that at least k scores reach and hardly more (a k of a
 // quarter of the groups: 1.15 k of normal scores); the groups that reach it, which L2 still holds for the
 // most part, are read again and offered to the candidates.
 constexpr uint32_t kMaxGroupSegs = 64;
@@ -231,23 +230,29 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
         const uint32_t n_segs = (n + kSeg - 1) / kSeg;
         Running run;
         for (uint32_t s = wave; s < n_segs; s += W) {
-            float x[U][V], gm = -INFINITY;
+            float x[U][V], vm[U], gm = -INFINITY;
             load_tile<T, kUnit>(x0, X.cs, s * kSeg, n, -INFINITY, x);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int v = 0; v < V; ++v) gm = fmaxf(gm, x[u][v]);
+                for (int v = 0; v < V; ++v) vm[u] = v ? fmaxf(vm[u], x[u][v]) : x[u][v];
+#pragma unroll
+            for (int u = 0; u < U; ++u) gm = fmaxf(gm, vm[u]);
             run.raise(gm, c);
             run.add(x, c);
-            if (run.s != run.s) {   // since a NaN, which is the largest of its group, or +inf
-                bool nan = false;
+            const uint32_t g = s * 64 + group_of<V>(lane);
+            uint32_t key = order_key(group_max<V>(vm, lane, MaxF()));
+            if (__any(run.s != run.s)) {   // since a NaN, which is the largest of its group, or +inf
+                uint32_t keys[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u) {
+                    keys[u] = 0;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) nan |= x[u][v] != x[u][v];
-                gm = nan ? NAN : gm;
+                    for (int v = 0; v < V; ++v) keys[u] = max(keys[u], order_key(x[u][v]));
+                }
+                key = group_max<V>(keys, lane, MaxU());
             }
-            groups[s * 64 + lane] = s * kSeg + lane * V < n ? order_key(gm) : 0;
+            groups[g] = g * kGroup < n ? key : 0;
         }
         __syncthreads();
         const uint32_t bound = (uint32_t)kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, n_segs * 64, k, &lds);
@@ -261,7 +266,7 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
                 const uint32_t b = hit ? (uint32_t)__builtin_ctzll(hit) : 64;
                 hit &= hit - 1;
                 const uint32_t ln = lane < kGroup ? a : b, q = lane % kGroup;
-                const uint32_t i = s * kSeg + (q / V * 64 + ln) * V + q % V;
+                const uint32_t i = s * kSeg + ln * kGroup + q;
                 const bool have = ln < 64 && i < n;
                 const float x = have ? to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * X.cs]) : -INFINITY;
                 C.offer(x, first + i, have, k);
