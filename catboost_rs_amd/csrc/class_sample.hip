@@ -381,7 +381,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
 // histogram of counts or masses over the distance from the largest score; those, or those of the one
 // bin in which the cut lies, are listed, and the list cut exactly in registers.  Kept masses of the
 // bins above a nucleus's last are summed by segments, and the draw looks through one of them.
-constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024, kListCap = 8192, kShortList = 512;
+constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024, kListCap = 8192, kShortList = 128;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
 // The bins reach from the largest score to a little below the lowest of a sample (the first score of every group),
 // 32 nats at most: 32 bins a nat, and more of them for the rows whose nucleus is wide, so that one bin holds
@@ -395,7 +395,7 @@ enum Mode : uint32_t { kGreedy, kWhole, kList, kNucleus };   // (kWhole: a least
 template <class T, bool kUnit, int THREADS>
 struct Long {
     static constexpr int V = Pack<T>::V, U = kGroup / V, W = THREADS / 64;
-    static constexpr int E = THREADS == 256 ? 8 : kListCap / THREADS, CAP = THREADS * E;   // a list's entries in registers
+    static constexpr int E = THREADS == 1024 ? 8 : 2048 / THREADS, CAP = THREADS * E;   // a list's entries in registers
     const T* x0;
     int64_t cs;
     uint32_t n;
@@ -542,8 +542,8 @@ struct Long {
                     } else if (y > -INFINITY) {
                         atomicAdd((uint32_t*)&hist[bin_at(bin(y))], 1u);
                     }
+                    if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (four masses at a time: registers)
                 }
-                __builtin_amdgcn_sched_barrier(0);   // (one vector's masses at a time: registers)
             }
         }
     }
@@ -568,8 +568,8 @@ struct Long {
                     } else {
                         sum += M.raw(x[v]);
                     }
+                    if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
             if (!kLeast) {
                 sum -= kGroup * Masses::kRaw;
@@ -583,22 +583,29 @@ struct Long {
     __device__ __forceinline__ u64 weigh(uint32_t s0, uint32_t s1, const Masses& M, u64 least, u64* segs) const {
         return least ? weigh_segments<true>(s0, s1, M, least, segs) : weigh_segments<false>(s0, s1, M, 0, segs);
     }
-    // The lowest score whose bin is at most b (bins are monotone; by halving the order keys).
+    // The lowest score whose bin is at most b (bins are monotone): the order keys' range is cut into 64 by the lanes.
     __device__ __forceinline__ float lowest_of(uint32_t b) const {
         uint32_t lo = order_key(-INFINITY), hi = order_key(bm);   // (bin(lo) is above b, or lo is it; bin(hi) = 0)
         while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (bin(key_score(mid)) <= b) hi = mid;
-            else lo = mid;
+            const uint32_t step = (hi - lo + 63) / 64, probe = min(hi, lo + step * (lane + 1));   // (the last is hi)
+            const u64 yes = __ballot(bin(key_score(probe)) <= b);
+            const uint32_t at = yes ? (uint32_t)__builtin_ctzll(yes) : 63;
+            hi = min(hi, lo + step * (at + 1));
+            lo = lo + step * at;
         }
         return key_score(hi);
     }
-    // Entries of a wave's staging area in LDS: at least two vectors of hits in all lanes.
-    static constexpr uint32_t kStage = 128 * V;
-    // The classes in bin `cut`, and with `all` those in the bins before, go to the list (at most cap; count goes
-    // on); with kSum the masses of the bins before go to their segments.
+    // The scores of the bins at the cut: [from, above); with `all`, all from there up.
+    __device__ __forceinline__ void cut_scores(uint32_t cut, bool all, float& from, float& above) const {
+        from = cut == kBins - 1 ? kLowest : lowest_of(cut);   // (the last bin takes all that is left)
+        above = all || cut == 0 ? INFINITY : lowest_of(cut - 1);
+    }
+    // Entries of a wave's staging area in LDS.
+    static constexpr uint32_t kStage = 256;
+    // The classes of scores in [from, above) go to the list (at most cap; count goes on); with kSum the masses of
+    // those above go to their segments.
     template <bool kSum>
-    __device__ __forceinline__ void collect(uint32_t s0, uint32_t s1, const Masses& M, uint32_t cut, bool all, u64 least,
+    __device__ __forceinline__ void collect(uint32_t s0, uint32_t s1, const Masses& M, float from, float above, u64 least,
                                             u64* segs, u64* list, uint32_t* count, uint32_t cap, u64* stage) const {
         stage += wave * kStage;
         uint32_t staged = 0;
@@ -612,8 +619,6 @@ struct Long {
             wave_fence();
             staged = 0;
         };
-        const float from = cut == kBins - 1 ? kLowest : lowest_of(cut);   // (the last bin takes all that is left)
-        const float above = all || cut == 0 ? INFINITY : lowest_of(cut - 1);
         for (uint32_t seg = s0 + wave; seg < s1; seg += W) {
             u64 sum = 0;
             Tile t;
@@ -634,10 +639,10 @@ struct Long {
                         if (in) stage[staged + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] =
                             rank_key(x[v], at(seg, u, lane) + v);
                         staged += (uint32_t)__popcll(who);
+                        if (staged > kStage - 64) flush();
                     }
+                    if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
-                if (staged > kStage - 64 * V) flush();
-                __builtin_amdgcn_sched_barrier(0);
             }
             if (kSum) {
                 sum = wave_reduce(sum, Add());
@@ -646,12 +651,9 @@ struct Long {
         }
         if (staged) flush();
     }
-    // Classes of the groups whose largest reaches the bound go to the list (count[0]): the groups are listed
-    // first (count[1]; as many as there are at most), then half a wave reads a group.  count starts as 0.
-    __device__ __forceinline__ void gather(uint32_t segs, const uint32_t* groups, uint32_t bound, u64* list,
-                                           uint32_t* count, uint16_t* hits) const {
-        for (uint32_t g = threadIdx.x; g < segs * 64; g += THREADS)
-            if (groups[g] != 0 && groups[g] >= bound) hits[atomicAdd(&count[1], 1u)] = (uint16_t)g;
+    // Classes that reach the bound, of the groups listed in hits (count[1] of them; written without a barrier since),
+    // go to the list (count[0]); half a wave reads a group.
+    __device__ __forceinline__ void gather(uint32_t bound, u64* list, uint32_t* count, const uint16_t* hits) const {
         __syncthreads();
         const uint32_t n_hits = count[1], q = threadIdx.x % kGroup;
         constexpr int D = 8;   // groups a half wave has under way
@@ -709,23 +711,27 @@ struct Long {
             if (L.key[e] && L.mass[e] && (uint32_t)~L.idx[e] >= c.from && (uint32_t)~L.idx[e] <= c.last)
                 out.put(row, L.idx[e], ((double)key_score(L.key[e]) - M.m) * r.rt - log_z);
     }
-    // The same for up to 512 classes, one a thread: every entry counts those ahead of it, and later the mass before it.
+    // The same for up to 128 classes: every entry counts those ahead of it, and later the mass of the classes
+    // before it; several threads share an entry's counting.
     __device__ void finish_short(const u64* list, uint32_t count, const Masses& M, double log_z, uint64_t row, SelectLds* lds,
                                  u64* tmp, const Out& out) const {
         const uint32_t t = threadIdx.x;
-        if (t < kShortList) {
-            lds->mass[t] = t < count ? list[t] : 0;
-            lds->rank[t] = 0;
+        const uint32_t slots = (count + 63) / 64 * 64, shares = (uint32_t)THREADS / slots, share = t / slots, e = t % slots;
+        const uint32_t each = ((slots + shares - 1) / shares + 7) / 8 * 8;   // (of the entries, by eights)
+        const uint32_t j0 = min(slots, share * each), j1 = share < shares ? min(slots, j0 + each) : j0;
+        for (uint32_t i = t; i < slots; i += THREADS) {
+            lds->mass[i] = i < count ? list[i] : 0;
+            lds->place[i] = 0;
         }
         __syncthreads();
-        if (t < count) {
-            const u64 key = lds->mass[t];
-            uint32_t place = 0;
-            for (uint32_t j = 0; j < count; j += 8)   // (a read at a time would wait for LDS at each)
+        const u64 key = lds->mass[e];
+        uint32_t place = 0;
+        for (uint32_t j = j0; j < j1; j += 8)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) place += lds->mass[j + q] > key;
-            lds->rank[place] = key;
-        }
+            for (int q = 0; q < 8; ++q) place += lds->mass[j + q] > key;
+        if (j0 < j1 && e < count) atomicAdd(&lds->place[e], place);
+        __syncthreads();
+        if (t < count) lds->rank[lds->place[t]] = key;   // (t < slots: e is t)
         __syncthreads();
         const uint32_t kept = min(count, r.k);
         const u64 rank = t < kept ? lds->rank[t] : 0;
@@ -734,19 +740,27 @@ struct Long {
         const u64 ahead = block_scan<THREADS>(w, all, tmp);
         if (r.p < 1.0 && ahead >= nucleus_of(r.p, all)) w = 0;
         if (w < M.least(r.min_p)) w = 0;
-        if (t < kShortList) lds->mass[t] = w;
+        const u64 sum = block_reduce<THREADS>(w, Add(), tmp);
+        // before the draw's class lie the classes whose masses come to no more than the target
+        for (uint32_t i = t; i < slots; i += THREADS) lds->mass[i] = 0;
         __syncthreads();
-        u64 before = 0, sum = 0;
-        if (t < kept) {
-            for (uint32_t j = 0; j < kept; j += 8)
+        u64 mine = t < kept ? w : 0;
+        if (t < slots) {
+            lds->rank[t] = t < kept ? rank : 0;
+            lds->weight[t] = mine;
+        }
+        __syncthreads();
+        const uint32_t cls = (uint32_t)lds->rank[e];   // (~class: larger for a class before)
+        u64 before = 0;
+        for (uint32_t j = j0; j < j1; j += 8)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const u64 wj = lds->mass[j + q];
-                    before += (uint32_t)lds->rank[j + q] > (uint32_t)rank ? wj : 0;   // (~class: larger for a class before)
-                    sum += wj;
-                }
+            for (int q = 0; q < 8; ++q) before += (uint32_t)lds->rank[j + q] > cls ? lds->weight[j + q] : 0;
+        if (j0 < j1 && e < kept) atomicAdd(&lds->mass[e], before);
+        __syncthreads();
+        if (mine) {
             const u64 target = target_of(r.u, sum);
-            if (w && target >= before && target - before < w) out.put(row, ~(uint32_t)rank, ((double)x - M.m) * r.rt - log_z);
+            before = lds->mass[t];
+            if (target >= before && target - before < mine) out.put(row, ~(uint32_t)rank, ((double)x - M.m) * r.rt - log_z);
         }
         __syncthreads();
     }
@@ -954,7 +968,9 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
             z = block_reduce<THREADS>(z, Add(), tmp);
             const u64 want = nucleus_of(R.r.p, z), least = M.least(R.r.min_p);
             const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
-            R.template collect<true>(0, n_segs, M, f.bin, false, least, segs, list, &count, L::CAP, stage);
+            float from, above;
+            R.cut_scores(f.bin, false, from, above);
+            R.template collect<true>(0, n_segs, M, from, above, least, segs, list, &count, L::CAP, stage);
             __syncthreads();
             if (count > (uint32_t)L::CAP) {
                 slow = true;
@@ -989,7 +1005,9 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
                 have = block_reduce<THREADS>(have, Add(), tmp);
                 if (have >= R.r.k) {
                     const u64 kth = kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, n_segs * 64, R.r.k, &lds);
-                    R.gather(n_segs, groups, (uint32_t)kth, list, counts, hits);
+                    for (uint32_t g = threadIdx.x; g < n_segs * 64; g += THREADS)
+                        if (groups[g] != 0 && groups[g] >= (uint32_t)kth) hits[atomicAdd(&counts[1], 1u)] = (uint16_t)g;
+                    R.gather((uint32_t)kth, list, counts, hits);
                     __syncthreads();
                     listed = count <= (uint32_t)L::CAP;
                     __syncthreads();
@@ -1006,7 +1024,9 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
                 if (f.above + f.inside > (u64)L::CAP) {
                     slow = true;
                 } else {
-                    R.template collect<false>(0, n_segs, M, f.bin, true, 0, nullptr, list, &count, L::CAP, stage);
+                    float from, above;
+                    R.cut_scores(f.bin, true, from, above);
+                    R.template collect<false>(0, n_segs, M, from, above, 0, nullptr, list, &count, L::CAP, stage);
                     __syncthreads();
                 }
             }
@@ -1028,8 +1048,10 @@ struct Top {      // of a part: its largest score (order key) over ~(its first c
 struct Step {     // where the cut lies
     u64 total, above;   // mass of all classes; weight of the bins before the cut's
     uint32_t bin, state;
+    float m, from, up_to;   // the largest score; the scores that are listed
+    uint32_t unused;
 };
-enum State : uint32_t { kCut, kOverflow };
+enum State : uint32_t { kNone, kCut, kOverflow };
 struct Space {    // the workspace of a chunk of rows
     Top* tops;          // [rows][parts1]
     uint32_t* groups;   // [rows][64 segs], nullable
@@ -1087,7 +1109,7 @@ __global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int sh
 
 // Masses of the segments, or the part's histogram of masses or counts.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(256, 4) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void weigh_kernel(Rows<T> X, Settings S, int shift, Space P) {
     constexpr int THREADS = 256;
     __shared__ u64 hist[kBinsPad];
     __shared__ u64 tmp[THREADS / 64];
@@ -1117,89 +1139,67 @@ __global__ __launch_bounds__(256, 4) void weigh_kernel(Rows<T> X, Settings S, in
     for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) to[b] = hist[bin_at(b)];
 }
 
-// The classes of the cut's bin (top_k: and of those before), and the segments' masses before it.
+// The bin of the cut, once a row (by each of a row's workgroups in the pass after, it took longer than the pass).
 template <class T, bool kUnit>
-__global__ __launch_bounds__(256, 4) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
-    constexpr int THREADS = 256;
+__global__ __launch_bounds__(1024) void cut_kernel(Rows<T> X, Settings S, int shift, Space P) {
+    constexpr int THREADS = 1024;
     __shared__ u64 hist[kBinsPad];
     __shared__ u64 tmp[THREADS / 64];
-    const uint64_t row = blockIdx.x / P.parts2;
-    const uint32_t part = blockIdx.x % P.parts2, s0 = part * P.per2, s1 = min(P.n_segs, s0 + P.per2);
-    Long<T, kUnit, THREADS> R(X, S, row, shift);
-    const Mode mode = R.mode();
-    if (mode != kNucleus && !(mode == kList && !(P.groups && R.by_groups(P.n_segs)))) return;
-    float low;
-    const u64 top = row_top<THREADS>(P, row, tmp, low);
-    const float m = key_score((uint32_t)(top >> 32));
-    if (top == 0 || m == INFINITY) return;
-    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
-    R.set_bins(m, low);
-    u64 total = 0;
-    for (uint32_t b = threadIdx.x; b < kBins; b += THREADS) {
-        u64 h = 0;
-        for (uint32_t p = 0; p < P.parts2; ++p) h += P.hist[(row * P.parts2 + p) * kBins + b];
-        hist[bin_at(b)] = h;
-        total += h;
-    }
-    total = block_reduce<THREADS>(total, Add(), tmp);
-    __syncthreads();
-    const u64 want = mode == kNucleus ? nucleus_of(R.r.p, total) : total < R.r.k ? total : (u64)R.r.k;
-    const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
-    const bool over = mode == kList && f.above + f.inside > kListCap;
-    if (part == 0 && threadIdx.x == 0) P.steps[row] = Step{total, f.above, f.bin, over ? kOverflow : kCut};
-    if (over) return;
-    __shared__ u64 stage[THREADS / 64 * Long<T, kUnit, THREADS>::kStage];
-    u64* list = P.list + row * kListCap;
-    if (mode == kNucleus)
-        R.template collect<true>(s0, s1, M, f.bin, false, M.least(R.r.min_p), P.segs + row * P.n_segs, list, &P.count[row], kListCap, stage);
-    else
-        R.template collect<false>(s0, s1, M, f.bin, true, 0, nullptr, list, &P.count[row], kListCap, stage);
-}
-
-// Rows that need no list: nothing allowed, the largest score, the whole row.  (Of 256 threads: 1024 with the
-// registers of the lists are one workgroup a CU.)
-template <class T, bool kUnit>
-__global__ __launch_bounds__(256) void draw_whole_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
-    constexpr int THREADS = 256, W = THREADS / 64;
-    __shared__ SelectLds lds;
-    __shared__ u64 tmp[W], pick[2];
     const uint64_t row = blockIdx.x;
     Long<T, kUnit, THREADS> R(X, S, row, shift);
     const Mode mode = R.mode();
     float low;
     const u64 top = row_top<THREADS>(P, row, tmp, low);
-    if (top == 0) {
-        if (threadIdx.x == 0) out.empty(row);
-        return;
-    }
     const float m = key_score((uint32_t)(top >> 32));
-    const uint32_t first = ~(uint32_t)top;
-    if (mode == kGreedy) {
-        if (threadIdx.x == 0) out.put(row, first, 0.0);
+    const bool list = mode == kList && !(P.groups && R.by_groups(P.n_segs));
+    if ((mode != kNucleus && !list) || top == 0 || m == INFINITY) {
+        if (threadIdx.x == 0) P.steps[row].state = kNone;
         return;
     }
-    if (mode != kWhole) return;
-    if (m == INFINITY) {
-        R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
-        return;
-    }
-    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+    R.set_bins(m, low);
     u64 total = 0;
-    for (uint32_t p = threadIdx.x; p < P.parts2; p += THREADS) total += P.totals[row * P.parts2 + p];
+    static_assert(THREADS == kBins, "a bin a thread");
+#pragma unroll 8
+    for (uint32_t p = 0; p < P.parts2; ++p) total += P.hist[(row * P.parts2 + p) * kBins + threadIdx.x];
+    hist[bin_at(threadIdx.x)] = total;
     total = block_reduce<THREADS>(total, Add(), tmp);
-    if (R.r.min_p > 1.0) {
-        if (threadIdx.x == 0) out.put(row, first, -M.log_of(total));
-        return;
-    }
-    R.finish_segments(P.segs + row * P.n_segs, P.n_segs, M, kBins, 0, M.least(R.r.min_p), total, row, tmp, pick, out);
+    __syncthreads();
+    const u64 want = !list ? nucleus_of(R.r.p, total) : total < R.r.k ? total : (u64)R.r.k;
+    const Found<u64> f = find_cut([&](uint32_t b) { return hist[bin_at(b)]; }, want);
+    const bool over = list && f.above + f.inside > kListCap;
+    Step step{total, f.above, f.bin, over ? kOverflow : kCut, m, 0.0f, 0.0f, 0};
+    R.cut_scores(f.bin, list, step.from, step.up_to);
+    if (threadIdx.x == 0) P.steps[row] = step;
 }
 
-// The others, a workgroup a row: the exact cut, and the draw.
+// The classes of the cut's bin (top_k: and of those before), and the segments' masses before it.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int shift, Out out, Space P, bool alone) {
-    constexpr int THREADS = 1024, W = THREADS / 64;
+__global__ __launch_bounds__(256, 4) void collect_kernel(Rows<T> X, Settings S, int shift, Space P) {
+    constexpr int THREADS = 256;
+    __shared__ u64 stage[THREADS / 64 * Long<T, kUnit, THREADS>::kStage];
+    const uint64_t row = blockIdx.x / P.parts2;
+    const Step step = P.steps[row];
+    if (step.state != kCut) return;
+    const uint32_t part = blockIdx.x % P.parts2, s0 = part * P.per2, s1 = min(P.n_segs, s0 + P.per2);
+    Long<T, kUnit, THREADS> R(X, S, row, shift);
+    const Masses M{(double)step.m, R.r.rt * 1.4426950408889634, shift};
+    u64* list = P.list + row * kListCap;
+    if (R.mode() == kNucleus)
+        R.template collect<true>(s0, s1, M, step.from, step.up_to, M.least(R.r.min_p), P.segs + row * P.n_segs, list,
+                                 &P.count[row], kListCap, stage);
+    else
+        R.template collect<false>(s0, s1, M, step.from, step.up_to, 0, nullptr, list, &P.count[row], kListCap, stage);
+}
+
+// Rows whose cut needs no pass over the row: nothing allowed, the largest score, the whole row, and a small top_k
+// from the maxima of the groups.  512 threads: what these steps wait for is barriers and LDS, and 8 waves
+// wait less than 16.
+template <class T, bool kUnit>
+__global__ __launch_bounds__(512) void draw_direct_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
+    constexpr int THREADS = 512, W = THREADS / 64;
     typedef Long<T, kUnit, THREADS> L;
-    extern __shared__ u64 pool[];   // the row's groups and their list, or its segments' masses
+    __shared__ u64 list[L::CAP];
+    __shared__ uint16_t hits[kGroupSegs * 64];
     __shared__ SelectLds lds;
     __shared__ u64 tmp[W], pick[2];
     __shared__ float tmp_f[W];
@@ -1208,17 +1208,97 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
     const uint64_t row = blockIdx.x;
     L R(X, S, row, shift);
     const Mode mode = R.mode();
+    const bool by_groups = mode == kList && R.by_groups(P.n_segs);
+    constexpr int kGroupsEach = (int)(kGroupSegs * 64 / THREADS);
+    uint32_t groups[kGroupsEach];   // (under way while the rest of the row's state is read)
+#pragma unroll
+    for (int j = 0; j < kGroupsEach; ++j) {
+        const uint32_t g = j * THREADS + threadIdx.x;
+        groups[j] = by_groups && g < P.n_segs * 64 ? P.groups[row * P.n_segs * 64 + g] : 0;
+    }
+    float low;
+    const u64 top = row_top<THREADS>(P, row, tmp, low);
+    if (top == 0) {
+        if (threadIdx.x == 0) out.empty(row);
+        return;
+    }
+    const float m = key_score((uint32_t)(top >> 32)), c = (float)(R.r.rt * 1.4426950408889634);
+    const uint32_t first = ~(uint32_t)top;
+    if (mode == kGreedy) {
+        if (threadIdx.x == 0) out.put(row, first, 0.0);
+        return;
+    }
+    if (mode != kWhole && !by_groups) return;
+    if (m == INFINITY) {
+        R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
+        return;
+    }
+    const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
+    if (mode == kWhole) {
+        u64 total = 0;
+        for (uint32_t p = threadIdx.x; p < P.parts2; p += THREADS) total += P.totals[row * P.parts2 + p];
+        total = block_reduce<THREADS>(total, Add(), tmp);
+        if (R.r.min_p > 1.0) {
+            if (threadIdx.x == 0) out.put(row, first, -M.log_of(total));
+            return;
+        }
+        R.finish_segments(P.segs + row * P.n_segs, P.n_segs, M, kBins, 0, M.least(R.r.min_p), total, row, tmp, pick, out);
+        return;
+    }
+    Running run;
+    for (uint32_t p = threadIdx.x; p < P.parts1; p += THREADS) {
+        const Top t = P.tops[row * P.parts1 + p];
+        run.join(t.m, t.s, c);
+    }
+    float mr;
+    double sr;
+    block_running<THREADS>(run, c, mr, sr, tmp_f, tmp_d);
+    const double log_z = log(sr);
+    u64 have = 0;
+#pragma unroll
+    for (int j = 0; j < kGroupsEach; ++j) have += groups[j] != 0;
+    if (threadIdx.x < 2) count[threadIdx.x] = 0;
+    have = block_reduce<THREADS>(have, Add(), tmp);
+    u64 kth = 0;   // (fewer groups than k: all that is allowed is listed)
+    if (have >= R.r.k)
+        kth = select<THREADS, false, true>(
+                  [&](auto f) {
+#pragma unroll
+                      for (int j = 0; j < kGroupsEach; ++j)
+                          if (groups[j]) f((u64)groups[j], 0);
+                  },
+                  R.r.k, &lds)
+                  .from;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kGroupsEach; ++j)
+        if (groups[j] != 0 && groups[j] >= (uint32_t)kth) hits[atomicAdd(&count[1], 1u)] = (uint16_t)(j * THREADS + threadIdx.x);
+    R.gather((uint32_t)kth, list, count, hits);
+    __syncthreads();
+    const bool slow = count[0] > (uint32_t)L::CAP;
+    if (!slow) R.finish_list(list, count[0], M, log_z, row, &lds, tmp, out);
+    else R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
+}
+
+// The others, a workgroup a row: the exact cut, and the draw.
+template <class T, bool kUnit>
+__global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
+    constexpr int THREADS = 1024, W = THREADS / 64;
+    typedef Long<T, kUnit, THREADS> L;
+    extern __shared__ u64 pool[];   // its segments' masses
+    __shared__ SelectLds lds;
+    __shared__ u64 tmp[W], pick[2];
+    __shared__ float tmp_f[W];
+    __shared__ double tmp_d[W];
+    const uint64_t row = blockIdx.x;
+    L R(X, S, row, shift);
+    const Mode mode = R.mode();
     float low;
     const u64 top = row_top<THREADS>(P, row, tmp, low);
     const float m = key_score((uint32_t)(top >> 32));
-    if (top == 0) {
-        if (alone && threadIdx.x == 0) out.empty(row);
-        return;
-    }
-    if (mode == kGreedy || mode == kWhole) return;
+    if (top == 0 || mode == kGreedy || mode == kWhole || (mode == kList && P.groups && R.by_groups(P.n_segs))) return;
     const uint32_t first = ~(uint32_t)top;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
-    const bool by_groups = mode == kList && P.groups && R.by_groups(P.n_segs);
     bool slow = m == INFINITY;
     if (!slow && mode == kNucleus) {
         const Step step = P.steps[row];
@@ -1259,28 +1339,8 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
         double sr;
         block_running<THREADS>(run, (float)(R.r.rt * 1.4426950408889634), mr, sr, tmp_f, tmp_d);
         const double log_z = log(sr);
-        if (by_groups) {
-            uint32_t* groups = (uint32_t*)(pool + kListCap);
-            uint16_t* hits = (uint16_t*)(groups + P.n_segs * 64);
-            u64 have = 0;
-            for (uint32_t g = threadIdx.x; g < P.n_segs * 64; g += THREADS) {
-                groups[g] = P.groups[row * P.n_segs * 64 + g];
-                have += groups[g] != 0;
-            }
-            if (threadIdx.x < 2) count[threadIdx.x] = 0;
-            have = block_reduce<THREADS>(have, Add(), tmp);
-            __syncthreads();
-            u64 kth = 0;   // (fewer groups than k: all that is allowed is listed)
-            if (have >= R.r.k)
-                kth = kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, P.n_segs * 64, R.r.k, &lds);
-            R.gather(P.n_segs, groups, (uint32_t)kth, pool, count, hits);
-            __syncthreads();
-            slow = count[0] > kListCap;
-            if (!slow) R.finish_list(pool, count[0], M, log_z, row, &lds, tmp, out);
-        } else {
-            slow = P.steps[row].state == kOverflow;
-            if (!slow) R.finish_list(P.list + row * kListCap, P.count[row], M, log_z, row, &lds, tmp, out);
-        }
+        slow = P.steps[row].state == kOverflow;
+        if (!slow) R.finish_list(P.list + row * kListCap, P.count[row], M, log_z, row, &lds, tmp, out);
     }
     if (slow) R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
 }
@@ -1343,10 +1403,8 @@ int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out,
     const bool all_greedy = !S.t_rows && !(S.t > 0.0), any_list = S.k_rows || (S.k && S.k < X.classes);
     const bool all_list = !S.k_rows && any_list && !(S.min_p_rows || S.min_p > 1.0);
     const uint32_t n_segs = (X.classes + kSeg - 1) / kSeg;
-    const bool list_by_groups = all_list && Long<T, kUnit, 1024>::by_groups_of(S.k, n_segs);
+    const bool list_by_groups = all_list && Long<T, kUnit, 512>::by_groups_of(S.k, n_segs);
     const bool any_cut = S.k_rows || S.p_rows || S.p < 1.0 || any_list;
-    const bool any_whole = S.t_rows || !(S.t > 0.0) || S.min_p_rows || S.min_p > 1.0 ||
-                           ((S.k_rows || !any_list) && (S.p_rows || !(S.p < 1.0)));
     for (uint64_t r0 = 0; r0 < X.rows; r0 += kChunkRows) {
         const uint64_t m = std::min(kChunkRows, X.rows - r0);
         size_t bytes = 0;
@@ -1368,21 +1426,19 @@ int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out,
             weigh_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 256, 0, st>>>(C, Q, shift, P);
             CLS_TRY(hipGetLastError());
             if (any_cut) {
+                cut_kernel<T, kUnit><<<(unsigned)m, 1024, 0, st>>>(C, Q, shift, P);
+                CLS_TRY(hipGetLastError());
                 collect_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 256, 0, st>>>(C, Q, shift, P);
                 CLS_TRY(hipGetLastError());
             }
         }
-        if (any_whole) {
-            draw_whole_kernel<T, kUnit><<<(unsigned)m, 256, 0, st>>>(C, Q, shift, o, P);
-            CLS_TRY(hipGetLastError());
-        }
-        if (all_greedy || !any_cut) continue;
-        // LDS: a list and the groups, or the segments
-        size_t lds = any_list && P.groups ? sizeof(u64) * kListCap + (sizeof(uint32_t) + sizeof(uint16_t)) * 64 * P.n_segs : 0;
-        lds = std::max(lds, sizeof(u64) * P.n_segs);
+        draw_direct_kernel<T, kUnit><<<(unsigned)m, 512, 0, st>>>(C, Q, shift, o, P);
+        CLS_TRY(hipGetLastError());
+        if (all_greedy || !any_cut || list_by_groups) continue;
+        const size_t lds = sizeof(u64) * P.n_segs;
         if (lds > 32 * 1024)
             CLS_TRY(hipFuncSetAttribute((const void*)draw_kernel<T, kUnit>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        draw_kernel<T, kUnit><<<(unsigned)m, 1024, lds, st>>>(C, Q, shift, o, P, !any_whole);
+        draw_kernel<T, kUnit><<<(unsigned)m, 1024, lds, st>>>(C, Q, shift, o, P);
         CLS_TRY(hipGetLastError());
     }
     return CBH_OK;

@@ -291,8 +291,9 @@ struct CountLds {
     uint32_t count[256];
 };
 struct SelectLds : CountLds {
-    u64 mass[512];   // (256 digits; or the entries of a short list)
-    u64 rank[512];
+    u64 mass[256];   // (digits; or the entries of a short list)
+    u64 rank[128], weight[128];
+    uint32_t place[128];
 };
 // The bits of a rank's distance that are known before the digit at `shift`: from here up.
 __device__ __forceinline__ int prefix_shift(int shift, int bits) {
