@@ -14,6 +14,10 @@ namespace {
 using namespace cbh::cls;
 
 constexpr uint32_t kMaxList = 1024;
+// Rows from 256 KB on are taken by 512 threads, one workgroup a CU: with four of 256 threads a CU the rows that are
+// under way pass the 256 MB of the last cache, and the second read comes from HBM (1500 x 100003 f32: 320 against
+// 372 us; 4096 x 65536 bf16, 128 KB a row: 349 against 278).
+constexpr size_t kWideRow = (size_t)1 << 18;
 constexpr uint32_t kMaxSeg = 1u << 18;   // classes a workgroup takes: their marks are 32 KB of LDS
 
 struct Lists {   // the teacher's, and what weighs the rows
@@ -67,7 +71,7 @@ __device__ __forceinline__ double times_log(double q, double l) { return q == 0.
 
 // A workgroup takes a row (kPhase 0), or a segment of one (few rows of many classes): phase 1 leaves the
 // segment's (m, s) of its others, phase 2 reads all of the row's and writes its part of the gradient.
-template <class T, bool kUnit, int THREADS, int kPhase>
+template <class T, bool kUnit, int THREADS, int LE /* list entries a thread */, int kPhase>
 __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, float c, double it, double t,
                                                           uint32_t parts, uint32_t seg, float* __restrict__ loss,
                                                           Grad<T> G, float2* __restrict__ part_ms) {
@@ -75,8 +79,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
     extern __shared__ uint32_t mark[];   // a bit a class of the segment
     __shared__ float tmp_f[W];
-    __shared__ double tmp_d[W];
-    __shared__ uint32_t tmp_u[W];
+    __shared__ double tmp_d[W * 5];
     const uint32_t words = (min(seg, X.classes) + 31) / 32;
 
     for (uint64_t job = blockIdx.x; job < X.rows * parts; job += gridDim.x) {
@@ -99,13 +102,27 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
             }
             continue;
         }
+        // the list, once: the teacher's log probabilities and the student's scores stay in registers
+        uint32_t cls[LE];   // (a class past all: no entry)
+        float xl[LE];
+        double lq[LE];
+        const T* xr = X.data + (int64_t)row * X.rs;
+#pragma unroll
+        for (int e = 0; e < LE; ++e) {
+            const uint32_t i = e * THREADS + threadIdx.x;
+            cls[e] = i < L.k ? (uint32_t)ix[i] : ~0u;
+            if (cls[e] >= X.classes) cls[e] = ~0u;
+            lq[e] = cls[e] != ~0u ? (double)u[i] * it : -INFINITY;
+            xl[e] = cls[e] != ~0u ? to_f32(xr[(int64_t)cls[e] * X.cs]) : -INFINITY;
+        }
         Running run;
         if (kPhase != 2) {
             for (uint32_t i = threadIdx.x; i < words; i += THREADS) mark[i] = 0;
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
-                const uint32_t j = (uint32_t)ix[i] - first;
-                if (j < n) atomicOr(&mark[j >> 5], 1u << (j & 31));
+#pragma unroll
+            for (int e = 0; e < LE; ++e) {
+                const uint32_t j = cls[e] - first;
+                if (cls[e] != ~0u && j < n) atomicOr(&mark[j >> 5], 1u << (j & 31));
             }
             __syncthreads();
             for (uint32_t base = wave * kSeg; base < n; base += W * kSeg) {
@@ -137,54 +154,49 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
             if (threadIdx.x == 0) part_ms[job] = float2{mo, (float)so};
             continue;
         }
-        // the list: the teacher's sums, the student's largest listed score
-        RowSums r{};
         float lmax = kLowest;
         double umax = -INFINITY;
-        const T* xr = X.data + (int64_t)row * X.rs;
-        uint32_t listed = 0;
-        for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
-            const uint32_t j = (uint32_t)ix[i];
-            if (j >= X.classes) continue;
-            ++listed;
-            umax = fmax(umax, (double)u[i] * it);
-            lmax = fmaxf(lmax, to_f32(xr[(int64_t)j * X.cs]));
+#pragma unroll
+        for (int e = 0; e < LE; ++e) {
+            lmax = fmaxf(lmax, xl[e]);
+            umax = fmax(umax, lq[e]);
         }
-        r.listed = block_reduce<THREADS>(listed, Add(), tmp_u);
         const float M = fmaxf(mo, block_reduce<THREADS>(lmax, MaxF(), tmp_f));
+        RowSums r{};
         if (L.lse) {
             r.base = (double)L.lse[row];
         } else {
-            umax = block_reduce<THREADS>(umax, MaxF(), tmp_d);
-            double s = 0.0;
-            for (uint32_t i = threadIdx.x; i < L.k; i += THREADS)
-                if ((uint32_t)ix[i] < X.classes) s += exp((double)u[i] * it - umax);
-            r.base = umax;
-            r.base_log = log(block_reduce<THREADS>(s, Add(), tmp_d));
+            r.base = umax = block_reduce<THREADS>(umax, MaxF(), tmp_d);
+            double s[1] = {0.0};
+#pragma unroll
+            for (int e = 0; e < LE; ++e) s[0] += cls[e] != ~0u ? exp(lq[e] - umax) : 0.0;
+            block_sums<THREADS>(s, tmp_d);
+            r.base_log = log(s[0]);
         }
-        double held = 0.0, entropy = 0.0, sl = 0.0;
-        for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
-            const uint32_t j = (uint32_t)ix[i];
-            if (j >= X.classes) continue;
-            const double lq = log_q(u[i], it, r), q = exp(lq);
-            held += q;
-            entropy += times_log(q, lq);
-            sl += exp(((double)to_f32(xr[(int64_t)j * X.cs]) - (double)M) * it);
+        // sums over the list: q, q log q, the student's exponentials, q (x - M) / t, entries
+        double s[5] = {};
+        double el[LE];
+#pragma unroll
+        for (int e = 0; e < LE; ++e) {
+            el[e] = 0.0;
+            if (cls[e] == ~0u) continue;
+            const double l = (lq[e] - r.base) - r.base_log, q = exp(l), d = ((double)xl[e] - (double)M) * it;
+            el[e] = exp(d);
+            lq[e] = q;   // (from here on: q)
+            s[0] += q;
+            s[1] += times_log(q, l);
+            s[2] += el[e];
+            s[3] += times_log(q, d);
+            s[4] += 1.0;
         }
-        r.held = block_reduce<THREADS>(held, Add(), tmp_d);
-        r.entropy = block_reduce<THREADS>(entropy, Add(), tmp_d);
-        sl = block_reduce<THREADS>(sl, Add(), tmp_d);
+        block_sums<THREADS>(s, tmp_d);
+        r.held = s[0];
+        r.entropy = s[1];
+        r.listed = (uint32_t)s[4];
+        const double sl = s[2];
         so = so == 0.0 ? 0.0 : so * exp(((double)mo - (double)M) * it);   // (in f64: far below M it must not vanish)
-        const double log_s = log(so + sl);
-        double lin = 0.0;
-        for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
-            const uint32_t j = (uint32_t)ix[i];
-            if (j >= X.classes) continue;
-            const float x = to_f32(xr[(int64_t)j * X.cs]);
-            const double q = exp(log_q(u[i], it, r));
-            lin += times_log(q, x == -INFINITY ? -(double)INFINITY : ((double)x - (double)M) * it - log_s);
-        }
-        lin = block_reduce<THREADS>(lin, Add(), tmp_d);
+        // sum q log p; a row without a score above -inf gives its classes no probability
+        const double lin = so + sl == 0.0 ? (r.held > 0.0 ? -(double)INFINITY : 0.0) : s[3] - times_log(r.held, log(so + sl));
         const double rest = row_rest(r, L.lse != nullptr, X.classes);
         const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
         if (loss && first == 0 && threadIdx.x == 0) loss[row] = (float)o.loss;
@@ -201,11 +213,11 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
                 }
             }
             __syncthreads();   // the listed classes are written over
-            for (uint32_t i = threadIdx.x; i < L.k; i += THREADS) {
-                const uint32_t j = (uint32_t)ix[i];
-                if (j - first >= n) continue;
-                const double p = exp(((double)to_f32(xr[(int64_t)j * X.cs]) - (double)M) * it) * o.inv_s;
-                g0[(int64_t)(j - first) * G.cs] = from_f32<T>((float)(w * t * (p * o.whole - exp(log_q(u[i], it, r)))));
+#pragma unroll
+            for (int e = 0; e < LE; ++e) {
+                const uint32_t j = cls[e] - first;
+                if (cls[e] == ~0u || j >= n) continue;
+                g0[(int64_t)j * G.cs] = from_f32<T>((float)(w * t * (el[e] * o.inv_s * o.whole - lq[e])));
             }
         }
         __syncthreads();
@@ -302,7 +314,7 @@ uint32_t plan_parts(uint64_t rows, uint32_t classes) {
 // Segments start at a multiple of 32 classes: a vector's marks lie in one word.
 uint32_t segment(uint32_t classes, uint32_t parts) { return ((classes + parts - 1) / parts + 31) / 32 * 32; }
 
-template <class T, bool kUnit, int THREADS>
+template <class T, bool kUnit, int THREADS, int LE>
 int launch_rows(const Rows<T>& X, const Lists& L, float c, double t, uint32_t parts, float* loss, const Grad<T>& G,
                 void* workspace, hipStream_t st) {
     const uint32_t seg = segment(X.classes, parts);
@@ -311,11 +323,11 @@ int launch_rows(const Rows<T>& X, const Lists& L, float c, double t, uint32_t pa
     float2* ms = (float2*)workspace;
     const double it = 1.0 / t;
     if (parts == 1) {
-        distill_kernel<T, kUnit, THREADS, 0><<<grid, THREADS, lds, st>>>(X, L, c, it, t, 1, seg, loss, G, ms);
+        distill_kernel<T, kUnit, THREADS, LE, 0><<<grid, THREADS, lds, st>>>(X, L, c, it, t, 1, seg, loss, G, ms);
     } else {
-        distill_kernel<T, kUnit, THREADS, 1><<<grid, THREADS, lds, st>>>(X, L, c, it, t, parts, seg, loss, G, ms);
+        distill_kernel<T, kUnit, THREADS, LE, 1><<<grid, THREADS, lds, st>>>(X, L, c, it, t, parts, seg, loss, G, ms);
         CLS_TRY(hipGetLastError());
-        distill_kernel<T, kUnit, THREADS, 2><<<grid, THREADS, 0, st>>>(X, L, c, it, t, parts, seg, loss, G, ms);
+        distill_kernel<T, kUnit, THREADS, LE, 2><<<grid, THREADS, 0, st>>>(X, L, c, it, t, parts, seg, loss, G, ms);
     }
     CLS_TRY(hipGetLastError());
     return CBH_OK;
@@ -337,11 +349,12 @@ int run_distill(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64
         return CBH_OK;
     }
     const bool unit = cs == 1 && (!grad || gcs == 1);
-    if (n <= 2048)
-        return unit ? launch_rows<T, true, 64>(X, L, c, t, parts, loss, G, workspace, st)
-                    : launch_rows<T, false, 64>(X, L, c, t, parts, loss, G, workspace, st);
-    return unit ? launch_rows<T, true, 256>(X, L, c, t, parts, loss, G, workspace, st)
-                : launch_rows<T, false, 256>(X, L, c, t, parts, loss, G, workspace, st);
+#define ROWS(TH, LE) (unit ? launch_rows<T, true, TH, LE>(X, L, c, t, parts, loss, G, workspace, st) \
+                           : launch_rows<T, false, TH, LE>(X, L, c, t, parts, loss, G, workspace, st))
+    if (n <= 2048) return L.k <= 64 ? ROWS(64, 1) : L.k <= 256 ? ROWS(64, 4) : ROWS(64, 16);
+    if (n * sizeof(T) < kWideRow) return L.k <= 256 ? ROWS(256, 1) : ROWS(256, 4);
+    return L.k <= 512 ? ROWS(512, 1) : ROWS(512, 2);
+#undef ROWS
 }
 
 }  // namespace

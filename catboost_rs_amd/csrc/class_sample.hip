@@ -423,7 +423,7 @@ struct Long {
         bool masked;
         __device__ __forceinline__ void get(int u, float (&x)[V]) const {
 #pragma unroll
-            for (int v = 0; v < V; ++v) x[v] = to_f32(p[u].v[v]);
+            for (int v = 0; v < V; ++v) x[v] = p[u].get(v);
             if (masked) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) x[v] = bits[u] >> v & 1 ? x[v] : -INFINITY;

@@ -41,14 +41,34 @@ __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) {
 
 // One vector load or store moves 16 bytes; the address needs the element's alignment only (rows of odd
 // length start anywhere).
+// A vector stays in its four words until a score of it is used: as separate 16-bit values the compiler gives each
+// a register.
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
 template <class T>
 struct Pack {
     static constexpr int V = 16 / (int)sizeof(T);
-    T v[V];
+    Words w;
+    __device__ __forceinline__ float get(int v) const {
+        const uint32_t word = w[v * (int)sizeof(T) / 4];
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, word);
+        else if constexpr (__is_same(T, bf16_t)) return __builtin_bit_cast(float, v % 2 ? word & 0xFFFF0000u : word << 16);
+        else return (float)__builtin_bit_cast(_Float16, (uint16_t)(word >> (v % 2 * 16)));
+    }
+    __device__ __forceinline__ void set(const float (&x)[V]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[v] = __builtin_bit_cast(uint32_t, x[v]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v += 2)
+                w[v / 2] = (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(x[v])) |
+                           (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(x[v + 1])) << 16;
+        }
+    }
 };
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Loose {
-    Pack<T> p;
+    Words w;
 };
 
 // Scores as the kernels take them.
@@ -66,9 +86,9 @@ __device__ __forceinline__ void load_pack(const T* row, int64_t cs, uint32_t i, 
                                           float (&x)[Pack<T>::V]) {
     constexpr int V = Pack<T>::V;
     if (kUnit && i + V <= n) {
-        const Pack<T> p = ((const Loose<T>*)(row + i))->p;
+        const Pack<T> p{((const Loose<T>*)(row + i))->w};
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[v] = to_f32(p.v[v]);
+        for (int v = 0; v < V; ++v) x[v] = p.get(v);
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v)
@@ -90,14 +110,13 @@ __device__ __forceinline__ void load_tile(const T* row, int64_t cs, uint32_t bas
     if (kUnit && base + kSeg <= n) {
         const Loose<T>* at = (const Loose<T>*)(row + base + lane * V);
 #pragma unroll
-        for (int u = 0; u < U; ++u) p[u] = at[u * 64].p;
+        for (int u = 0; u < U; ++u) p[u].w = at[u * 64].w;
     } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float x[V];
             load_pack<T, kUnit>(row, cs, base + (u * 64 + lane) * V, n, fill, x);
-#pragma unroll
-            for (int v = 0; v < V; ++v) p[u].v[v] = from_f32<T>(x[v]);
+            p[u].set(x);
         }
     }
 }
@@ -109,16 +128,15 @@ __device__ __forceinline__ void load_tile(const T* row, int64_t cs, uint32_t bas
 #pragma unroll
     for (int u = 0; u < kPacks<T>; ++u)
 #pragma unroll
-        for (int v = 0; v < Pack<T>::V; ++v) x[u][v] = to_f32(p[u].v[v]);
+        for (int v = 0; v < Pack<T>::V; ++v) x[u][v] = p[u].get(v);
 }
 template <class T, bool kUnit>
 __device__ __forceinline__ void store_pack(T* row, int64_t cs, uint32_t i, uint32_t n, const float (&x)[Pack<T>::V]) {
     constexpr int V = Pack<T>::V;
     if (kUnit && i + V <= n) {
         Pack<T> p;
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.v[v] = from_f32<T>(x[v]);
-        ((Loose<T>*)(row + i))->p = p;
+        p.set(x);
+        ((Loose<T>*)(row + i))->w = p.w;
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v)
@@ -380,6 +398,26 @@ __device__ __forceinline__ u64 kth_of(Get get, uint32_t n, uint32_t k, Lds* lds)
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Sums of N values at once.  tmp: N values a wave.
+template <int THREADS, int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double* tmp) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_reduce(v[i], Add());
+    if (THREADS == 64) return;
+    if (lane_id() == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) tmp[threadIdx.x / 64 * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = 0.0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) v[i] += tmp[w * N + i];
+    }
+    __syncthreads();
+}
 
 // A running softmax denominator: sum over the scores seen of 2^((x - m) c), c = log2(e) / temperature.
 // m starts at the lowest finite value, so that a score of -inf adds 0 and a row of nothing else
