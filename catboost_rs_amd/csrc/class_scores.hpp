@@ -136,7 +136,9 @@ __device__ __forceinline__ void store_pack(T* row, int64_t cs, uint32_t i, uint3
     if (kUnit && i + V <= n) {
         Pack<T> p;
         p.set(x);
-        ((Loose<T>*)(row + i))->w = p.w;
+        // (past the caches: nobody reads a gradient before the pass ends, and the rows' second read shares them)
+        typedef uint32_t Unaligned __attribute__((ext_vector_type(4), aligned(2)));
+        __builtin_nontemporal_store(p.w, (Unaligned*)(row + i));
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v)
