@@ -69,6 +69,10 @@ __device__ __forceinline__ double log_q(float u, double it, const RowSums& r) { 
 // q log q and q log p, 0 where q is
 __device__ __forceinline__ double times_log(double q, double l) { return q == 0.0 ? 0.0 : q * l; }
 
+// Two passes over a row, the second from the last cache while the rows under way fit it, one of them writing.
+// 4096 x 65536 bf16, k 64: 269 us, 1.07 GB of reads and writes at 4.0 TB/s (a copy: 5.2); 1500 x 100003 f32, k 20: 297
+// us, 1.2 GB at 4.0 TB/s.  Bound by memory and the second read.  Holding a row's tiles in registers between the
+// passes was built and spilled (the f32 forms of a tile are twice its registers): not kept.
 // A workgroup takes a row (kPhase 0), or a segment of one (few rows of many classes): phase 1 leaves the
 // segment's (m, s) of its others, phase 2 reads all of the row's and writes its part of the gradient.
 template <class T, bool kUnit, int THREADS, int LE /* list entries a thread */, int kPhase>
@@ -224,7 +228,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
     }
 }
 
-// Few classes: a row a thread, its scores in registers, the listed classes a bit mask.
+// Few classes: a row a thread, its scores in registers, the listed classes a bit mask.  1M x 10 f32, k 3, class-major:
+// 64 us, 112 MB at 1.75 TB/s; bound by the f64 exponentials and logarithms of the lists.
 template <class T, int NMAX>
 __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, float c, double it, double t,
                                                           float* __restrict__ loss, Grad<T> G) {

@@ -148,6 +148,25 @@ def check_refusals():
     refuses(ValueError, cb.sample_classes, x, u, top_k=torch.zeros(4, device="cuda"))
 
 
+def check_example():
+    """The example trains a teacher, distils it and draws answers."""
+    from examples import distill_classes
+    losses, agree, drawn = distill_classes.main(rows=4000, steps=40)
+    assert losses[-1] < 0.5 * losses[0] and agree > 0.5 and drawn.shape == (4000,)
+    assert 0 <= int(drawn.min()) and int(drawn.max()) < 10
+
+
+def check_split_settings():
+    """Settings a row and one setting for all rows draw the same, over more rows than one pass of the long path takes."""
+    x, _, u = case(700, 9001, torch.bfloat16, 8)
+    full = torch.full((700,), 1.0, device="cuda")
+    for k, p in ((0, 1.0), (0, 0.875), (40, 0.875), (3000, 1.0)):
+        one = cb.sample_classes(x, u, top_k=k, top_p=p)
+        row = cb.sample_classes(x, u, temperature=full, top_k=(full * k).int(), top_p=full * p, min_p=full * 0)
+        for a, b in zip(one, row):
+            assert torch.equal(a, b), (k, p)
+
+
 if __name__ == "__main__":
     for name, f in list(globals().items()):
         if name.startswith("check_"):
