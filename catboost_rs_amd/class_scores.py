@@ -34,7 +34,7 @@ def _bind():
     _state.update(torch=torch, lib=L, check=cb._check, top=L.cbh_top_classes, top_ws=L.cbh_top_classes_workspace,
                   distill=L.cbh_distill_gradients, distill_ws=L.cbh_distill_gradients_workspace,
                   sample=L.cbh_sample_classes, sample_ws=L.cbh_sample_classes_workspace,
-                  stream=torch.cuda.current_stream)
+                  raw_stream=getattr(torch._C, "_cuda_getCurrentRawStream", None))
     return torch
 
 
@@ -53,7 +53,7 @@ def _scores(torch, x, what="scores"):
 
 def _vector(torch, x, shape, dtype, like, what):
     """`x` as a contiguous tensor of this shape and type beside `like`; its address."""
-    if not isinstance(x, torch.Tensor) or tuple(x.shape) != shape:
+    if not isinstance(x, torch.Tensor) or x.shape != shape:
         raise ValueError(f"{what} must be a torch tensor of shape {list(shape)}")
     if x.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, not {x.dtype}")
@@ -70,9 +70,27 @@ def _addr(x):
     return None if x is None else x.data_ptr()
 
 
+class _Stay:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_STAY = _Stay()
+
+
 def _on(x):
-    """The device of `x` made current for the call (a no-op where it is)."""
-    return _state["torch"].cuda.device(x.device)
+    """The device of `x` made current for the call (nothing where it is: the context costs a small call 2 us)."""
+    cuda = _state["torch"].cuda
+    return _STAY if cuda.current_device() == x.device.index else cuda.device(x.device)
+
+
+def _stream(x):
+    """torch's current stream on the device of `x`, as an address."""
+    raw = _state["raw_stream"]
+    return raw(x.device.index) if raw else _state["torch"].cuda.current_stream(x.device).cuda_stream
 
 
 def top_classes(scores, k, temperature=1.0):
@@ -91,7 +109,7 @@ def top_classes(scores, k, temperature=1.0):
         size = _state["top_ws"](n, m, max(k, 0))
         ws = _workspace(torch, size, scores)
         _state["check"](_state["top"](scores.data_ptr(), t, n, m, rs, cs, max(k, 0), float(temperature), values.data_ptr(),
-                                      index.data_ptr(), lse.data_ptr(), _addr(ws), size, _state["stream"]().cuda_stream))
+                                      index.data_ptr(), lse.data_ptr(), _addr(ws), size, _stream(scores)))
     return values, index, lse
 
 
@@ -119,7 +137,7 @@ def distill_gradients(scores, top_scores, top_index, *, top_lse=None, temperatur
         ws = _workspace(torch, size, scores)
         _state["check"](_state["distill"](scores.data_ptr(), t, n, m, rs, cs, u.data_ptr(), ix.data_ptr(), k, _addr(base),
                                           float(temperature), _addr(w), loss.data_ptr(), grad.data_ptr(), grs, gcs,
-                                          _addr(ws), size, _state["stream"]().cuda_stream))
+                                          _addr(ws), size, _stream(scores)))
     return loss, grad
 
 
@@ -157,5 +175,5 @@ def sample_classes(scores, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_
         _state["check"](_state["sample"](scores.data_ptr(), t, n, m, rs, cs, uniform.data_ptr(), float(tv), _addr(tr),
                                          max(int(kv), 0), _addr(kr), float(pv), _addr(pr), float(mv), _addr(mr),
                                          _addr(allowed), astride, index.data_ptr(), logprob.data_ptr(), _addr(ws), size,
-                                         _state["stream"]().cuda_stream))
+                                         _stream(scores)))
     return index, logprob

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
             r.base = umax = block_reduce<THREADS>(umax, MaxF(), tmp_d);
             double s[1] = {0.0};
 #pragma unroll
-            for (int e = 0; e < LE; ++e) s[0] += cls[e] != ~0u ? exp(lq[e] - umax) : 0.0;
+            for (int e = 0; e < LE; ++e) s[0] += cls[e] != ~0u ? exp_f64(lq[e] - umax) : 0.0;
             block_sums<THREADS>(s, tmp_d);
             r.base_log = log(s[0]);
         }
@@ -184,8 +184,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
         for (int e = 0; e < LE; ++e) {
             el[e] = 0.0;
             if (cls[e] == ~0u) continue;
-            const double l = (lq[e] - r.base) - r.base_log, q = exp(l), d = ((double)xl[e] - (double)M) * it;
-            el[e] = exp(d);
+            const double l = (lq[e] - r.base) - r.base_log, q = exp_f64(l), d = ((double)xl[e] - (double)M) * it;
+            el[e] = exp_f64(d);
             lq[e] = q;   // (from here on: q)
             s[0] += q;
             s[1] += times_log(q, l);
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
         r.entropy = s[1];
         r.listed = (uint32_t)s[4];
         const double sl = s[2];
-        so = so == 0.0 ? 0.0 : so * exp(((double)mo - (double)M) * it);   // (in f64: far below M it must not vanish)
+        so = so == 0.0 ? 0.0 : so * exp_f64(((double)mo - (double)M) * it);   // (in f64: far below M it must not vanish)
         // sum q log p; a row without a score above -inf gives its classes no probability
         const double lin = so + sl == 0.0 ? (r.held > 0.0 ? -(double)INFINITY : 0.0) : s[3] - times_log(r.held, log(so + sl));
         const double rest = row_rest(r, L.lse != nullptr, X.classes);
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
         } else {
             double s = 0.0;
             for (uint32_t i = 0; i < L.k; ++i)
-                if ((uint32_t)ix[i] < n) s += exp((double)u[i] * it - umax);
+                if ((uint32_t)ix[i] < n) s += exp_f64((double)u[i] * it - umax);
             r.base = umax;
             r.base_log = log(s);
         }
@@ -278,15 +278,15 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             const float e = exp2_fast((x[j] - mo) * c);
             s += mask >> j & 1 ? 0.0f : e;
         }
-        const double so = s == 0.0f ? 0.0 : (double)s * exp(((double)mo - (double)M) * it);
+        const double so = s == 0.0f ? 0.0 : (double)s * exp_f64(((double)mo - (double)M) * it);
         double sl = 0.0;
         for (uint32_t i = 0; i < L.k; ++i)
-            if ((uint32_t)ix[i] < n) sl += exp(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it);
+            if ((uint32_t)ix[i] < n) sl += exp_f64(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it);
         const double log_s = log(so + sl);
         double lin = 0.0;
         for (uint32_t i = 0; i < L.k; ++i)
             if ((uint32_t)ix[i] < n) {
-                const double lq = log_q(u[i], it, r), q = exp(lq);
+                const double lq = log_q(u[i], it, r), q = exp_f64(lq);
                 const float xl = to_f32(x0[(int64_t)ix[i] * X.cs]);
                 r.held += q;
                 r.entropy += times_log(q, lq);
@@ -302,8 +302,8 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
                     g0[(int64_t)j * G.cs] = from_f32<T>(exp2_fast((x[j] - o.M) * c) * o.others);
             for (uint32_t i = 0; i < L.k; ++i)
                 if ((uint32_t)ix[i] < n) {
-                    const double p = exp(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it) * o.inv_s;
-                    g0[(int64_t)ix[i] * G.cs] = from_f32<T>((float)(w * t * (p * o.whole - exp(log_q(u[i], it, r)))));
+                    const double p = exp_f64(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it) * o.inv_s;
+                    g0[(int64_t)ix[i] * G.cs] = from_f32<T>((float)(w * t * (p * o.whole - exp_f64(log_q(u[i], it, r)))));
                 }
         }
     }
@@ -347,7 +347,9 @@ int run_distill(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64
     if (n <= 32) {
         const unsigned grid = row_grid((rows + 255) / 256);
         const double it = 1.0 / t;
-        if (n <= 8) distill_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+        if (n <= 4) distill_few_kernel<T, 4><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+        else if (n <= 8) distill_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+        else if (n <= 12) distill_few_kernel<T, 12><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
         else if (n <= 16) distill_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
         else distill_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
         CLS_TRY(hipGetLastError());

@@ -50,13 +50,9 @@ struct Masses {
     double m, c;   // largest score, log2(e) / temperature
     double big;    // 1.5 2^52 + S
     double q[9];
-    // 2^f for |f| <= 1/2, within 2^-44, and exactly 1 at 0: 1 + f q(f), q the polynomial of degree 8 that meets
-    // (2^f - 1) / f in the Chebyshev points of the interval.  Its coefficients are held in scalar registers (the
-    // compiler's own choice is 18 vector registers).
+    // The polynomial's coefficients are held in scalar registers (the compiler's own choice is 18 vector registers).
     __device__ __forceinline__ Masses(double m, double c, int S) : m(m), c(c), big(6755399441055744.0 + S) {
-        const double k[9] = {0.6931471805599453, 0.2402265069581299, 0.055504108664760424,
-                             0.009618129159402558, 0.0013333558179043112, 0.00015403455852453838,
-                             1.525268684626772e-05, 1.3255224878668817e-06, 1.0203121063391729e-07};
+        const double k[9] = {CBH_EXP2_TERMS};
 #pragma unroll
         for (int i = 0; i < 9; ++i) {
             q[i] = k[i];
@@ -1457,8 +1453,11 @@ int launch_sample(const Rows<T>& X, const Settings& S, const Out& out, void* wor
     const int shift = shift_of(n);
     if (n <= 32) {
         const unsigned grid = row_grid((X.rows + 255) / 256);
+        // (the pairs grow with the square: places in twos up to 12, then in fours and eights)
         if (n <= 4) sample_few_kernel<T, 4><<<grid, 256, 0, st>>>(X, S, out);
+        else if (n <= 6) sample_few_kernel<T, 6><<<grid, 256, 0, st>>>(X, S, out);
         else if (n <= 8) sample_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, S, out);
+        else if (n <= 10) sample_few_kernel<T, 10><<<grid, 256, 0, st>>>(X, S, out);
         else if (n <= 12) sample_few_kernel<T, 12><<<grid, 256, 0, st>>>(X, S, out);
         else if (n <= 16) sample_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, S, out);
         else if (n <= 24) sample_few_kernel<T, 24><<<grid, 256, 0, st>>>(X, S, out);

@@ -399,6 +399,24 @@ __device__ __forceinline__ u64 kth_of(Get get, uint32_t n, uint32_t k, Lds* lds)
         .from;
 }
 
+// (2^f - 1) / f for |f| <= 1/2 as a polynomial of degree 8, lowest term first: it meets the function in the Chebyshev
+// points of the interval; 1 + f q(f) is 2^f within 2^-44, and exactly 1 at 0.
+#define CBH_EXP2_TERMS                                                                            \
+    0.6931471805599453, 0.2402265069581299, 0.055504108664760424,                   \
+        0.009618129159402558, 0.0013333558179043112, 0.00015403455852453838,           \
+        1.525268684626772e-05, 1.3255224878668817e-06, 1.0203121063391729e-07
+// e^z within 2^-43, for what is held in f64 (half the instructions of exp()); 0 from -760 down, NaN stays.
+__device__ __forceinline__ double exp_f64(double z) {
+    const double q[9] = {CBH_EXP2_TERMS};
+    double y = z * 1.4426950408889634;
+    y = y < -1100.0 ? -1100.0 : y;
+    const double k = rint(y), f = y - k;
+    double p = q[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) p = __builtin_fma(p, f, q[i]);
+    return ldexp(__builtin_fma(p, f, 1.0), (int)k);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Sums of N values at once.  tmp: N values a wave.
