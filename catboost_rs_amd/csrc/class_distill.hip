@@ -229,8 +229,9 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
 }
 
 // Few classes: a row a thread, its scores in registers, the listed classes a bit mask.  1M x 10 f32, k 3, class-major:
-// 64 us, 112 MB at 1.75 TB/s; bound by the f64 exponentials and logarithms of the lists.
-template <class T, int NMAX>
+// 41 us, 112 MB at 2.8 TB/s; bound by the f64 exponentials and logarithms of the lists, and their loads.
+// Lists of up to KM entries are held in registers as well (KM 0: read again in every step; k 3 that way 59 us).
+template <class T, int NMAX, int KM>
 __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, float c, double it, double t,
                                                           float* __restrict__ loss, Grad<T> G) {
     const uint32_t n = X.classes;
@@ -244,26 +245,63 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
                 for (uint32_t j = 0; j < n; ++j) g0[(int64_t)j * G.cs] = from_f32<T>(0.0f);
             continue;
         }
+        const float* u = L.scores + row * L.k;
+        const int32_t* ix = L.index + row * L.k;
+        struct Entry {   // of the list: class (n and more: none), teacher's score / t, then the student's, q, e^(x - M)
+            uint32_t cls;
+            double ut;
+            float x;
+            double q, e;
+        };
+        Entry kept[KM ? KM : 1];
+        if constexpr (KM > 0) {
+#pragma unroll
+            for (int i = 0; i < KM; ++i) {
+                const uint32_t at = min((uint32_t)i, L.k - 1);
+                kept[i].cls = (uint32_t)i < L.k ? (uint32_t)ix[at] : ~0u;
+                kept[i].ut = (double)u[at] * it;
+            }
+        }
         float x[NMAX], M = kLowest, mo = kLowest;
 #pragma unroll
         for (int j = 0; j < NMAX; ++j) x[j] = (uint32_t)j < n ? to_f32(x0[(int64_t)j * X.cs]) : -INFINITY;
-        const float* u = L.scores + row * L.k;
-        const int32_t* ix = L.index + row * L.k;
+        if constexpr (KM > 0) {
+#pragma unroll
+            for (int i = 0; i < KM; ++i) {
+                kept[i].x = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NMAX; ++j) kept[i].x = kept[i].cls == (uint32_t)j ? x[j] : kept[i].x;
+            }
+        }
+        auto each = [&](auto f) {
+            if constexpr (KM > 0) {
+#pragma unroll
+                for (int i = 0; i < KM; ++i)
+                    if (kept[i].cls < n) f(kept[i]);
+            } else {
+                for (uint32_t i = 0; i < L.k; ++i) {
+                    Entry en;
+                    en.cls = (uint32_t)ix[i];
+                    if (en.cls >= n) continue;
+                    en.ut = (double)u[i] * it;
+                    en.x = to_f32(x0[(int64_t)en.cls * X.cs]);
+                    f(en);
+                }
+            }
+        };
         uint32_t mask = 0;
         double umax = -INFINITY;
-        for (uint32_t i = 0; i < L.k; ++i)
-            if ((uint32_t)ix[i] < n) {
-                mask |= 1u << ix[i];
-                umax = fmax(umax, (double)u[i] * it);
-            }
+        each([&](Entry& en) {
+            mask |= 1u << en.cls;
+            umax = fmax(umax, en.ut);
+        });
         RowSums r{};
         r.listed = (uint32_t)__popc(mask);
         if (L.lse) {
             r.base = (double)L.lse[row];
         } else {
             double s = 0.0;
-            for (uint32_t i = 0; i < L.k; ++i)
-                if ((uint32_t)ix[i] < n) s += exp_f64((double)u[i] * it - umax);
+            each([&](Entry& en) { s += exp_f64(en.ut - umax); });
             r.base = umax;
             r.base_log = log(s);
         }
@@ -279,19 +317,20 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             s += mask >> j & 1 ? 0.0f : e;
         }
         const double so = s == 0.0f ? 0.0 : (double)s * exp_f64(((double)mo - (double)M) * it);
-        double sl = 0.0;
-        for (uint32_t i = 0; i < L.k; ++i)
-            if ((uint32_t)ix[i] < n) sl += exp_f64(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it);
-        const double log_s = log(so + sl);
-        double lin = 0.0;
-        for (uint32_t i = 0; i < L.k; ++i)
-            if ((uint32_t)ix[i] < n) {
-                const double lq = log_q(u[i], it, r), q = exp_f64(lq);
-                const float xl = to_f32(x0[(int64_t)ix[i] * X.cs]);
-                r.held += q;
-                r.entropy += times_log(q, lq);
-                lin += times_log(q, xl == -INFINITY ? -(double)INFINITY : ((double)xl - (double)M) * it - log_s);
-            }
+        auto weigh = [&](Entry& en) {
+            en.q = exp_f64((en.ut - r.base) - r.base_log);
+            en.e = exp_f64(((double)en.x - (double)M) * it);
+        };
+        double sl = 0.0, cross = 0.0;   // sum q (x - M) / t
+        each([&](Entry& en) {
+            weigh(en);
+            sl += en.e;
+            r.held += en.q;
+            r.entropy += times_log(en.q, (en.ut - r.base) - r.base_log);
+            cross += times_log(en.q, ((double)en.x - (double)M) * it);
+        });
+        // (a row without a score above -inf gives its classes no probability)
+        const double lin = so + sl == 0.0 ? (r.held > 0.0 ? -(double)INFINITY : 0.0) : cross - times_log(r.held, log(so + sl));
         const double rest = row_rest(r, L.lse != nullptr, n);
         const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
         if (loss) loss[row] = (float)o.loss;
@@ -300,11 +339,10 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             for (int j = 0; j < NMAX; ++j)
                 if ((uint32_t)j < n && !(mask >> j & 1))
                     g0[(int64_t)j * G.cs] = from_f32<T>(exp2_fast((x[j] - o.M) * c) * o.others);
-            for (uint32_t i = 0; i < L.k; ++i)
-                if ((uint32_t)ix[i] < n) {
-                    const double p = exp_f64(((double)to_f32(x0[(int64_t)ix[i] * X.cs]) - (double)M) * it) * o.inv_s;
-                    g0[(int64_t)ix[i] * G.cs] = from_f32<T>((float)(w * t * (p * o.whole - exp_f64(log_q(u[i], it, r)))));
-                }
+            each([&](Entry& en) {
+                if constexpr (KM == 0) weigh(en);
+                g0[(int64_t)en.cls * G.cs] = from_f32<T>((float)(w * t * (en.e * o.inv_s * o.whole - en.q)));
+            });
         }
     }
 }
@@ -347,11 +385,14 @@ int run_distill(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64
     if (n <= 32) {
         const unsigned grid = row_grid((rows + 255) / 256);
         const double it = 1.0 / t;
-        if (n <= 4) distill_few_kernel<T, 4><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
-        else if (n <= 8) distill_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
-        else if (n <= 12) distill_few_kernel<T, 12><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
-        else if (n <= 16) distill_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
-        else distill_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G);
+#define FEW(N) (L.k <= 4 ? distill_few_kernel<T, N, 4><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G) \
+                         : distill_few_kernel<T, N, 0><<<grid, 256, 0, st>>>(X, L, c, it, t, loss, G))
+        if (n <= 4) FEW(4);
+        else if (n <= 8) FEW(8);
+        else if (n <= 12) FEW(12);
+        else if (n <= 16) FEW(16);
+        else FEW(32);
+#undef FEW
         CLS_TRY(hipGetLastError());
         return CBH_OK;
     }
