@@ -193,8 +193,8 @@ struct Entries {
 // Scores and masses in registers.  A nucleus needs the mass ahead of every class: the pairs of classes, in
 // f64 (with S = 46 and at most 32 classes every sum is an integer below 2^53 and exact), each pair a
 // comparison and two multiply-adds with 0 or 1.
-// 1M x 10 f32, top_p 0.9, class-major: 46 us, 64 MB at 1.4 TB/s; bound by f64 instructions (the masses, and
-// the pairs of 12 places).  A wave a row took 3.2 ms.
+// 1M x 10 f32, top_p 0.9, class-major: 37 us, 64 MB at 1.7 TB/s; bound by f64 instructions (the masses, and
+// the pairs of 10 places; 46 us with 12).  A wave a row took 3.2 ms.
 constexpr int kFewShift = 46;
 template <class T, int NMAX>
 __global__ __launch_bounds__(256) void sample_few_kernel(Rows<T> X, Settings S, Out out) {
@@ -1077,7 +1077,7 @@ __device__ __forceinline__ u64 row_top(const Space& P, uint64_t row, u64* tmp, f
 }
 
 template <class T, bool kUnit>
-__global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int shift, Out out, Space P) {
+__global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int shift, Space P) {
     constexpr int THREADS = 256;
     __shared__ float tmp_f[4];
     __shared__ double tmp_d[4];
@@ -1423,7 +1423,7 @@ int launch_split(const Rows<T>& X, const Settings& S, int shift, const Out& out,
         if (Q.min_p_rows) Q.min_p_rows += r0;
         if (Q.allowed) Q.allowed += (int64_t)r0 * Q.allowed_stride;
         const Out o{out.index + r0, out.logprob ? out.logprob + r0 : nullptr};
-        scan_kernel<T, kUnit><<<(unsigned)(m * P.parts1), 256, 0, st>>>(C, Q, shift, o, P);
+        scan_kernel<T, kUnit><<<(unsigned)(m * P.parts1), 256, 0, st>>>(C, Q, shift, P);
         CLS_TRY(hipGetLastError());
         if (!all_greedy && !list_by_groups) {
             weigh_kernel<T, kUnit><<<(unsigned)(m * P.parts2), 256, 0, st>>>(C, Q, shift, P);

@@ -97,7 +97,7 @@ __device__ __forceinline__ void load_pack(const T* row, int64_t cs, uint32_t i, 
 }
 // A wave's 2048 classes from `base` on (a multiple of 2048, the same in all lanes): vector u of a lane holds
 // the classes from base + (u 64 + lane) V on.  The loads of a whole tile are all under way before the first is
-// waited for (guarded one by one, each was waited for in its branch: 203 against 135 us for the top classes of
+// waited for (guarded one by one, each was waited for in its branch: 203 against 175 us for the top classes of
 // 4096 x 65536 bf16).
 constexpr uint32_t kSeg = 2048, kGroup = 32;   // classes of a wave's tile, and of a lane in it
 template <class T>

@@ -75,6 +75,13 @@ def test_sample_arguments_are_checked(lib):
     assert sample(u=None) == -5 and sample(index=None) == -5
     assert sample(allowed=P, stride=3) == -2 and sample(allowed=P, stride=-3) == -2
     assert sample(allowed=P + 2) == -5
+    need = lib.cbh_sample_classes_workspace(1, 200_000)
+    assert need > 0 and lib.cbh_sample_classes_workspace(10 ** 9, 2048) == 0
+    assert sample(rows=1, classes=200_000) == -1
+    assert sample(rows=1, classes=200_000, ws=P, size=need - 1) == -1
+    assert sample(rows=1, classes=200_000, ws=P + 4, size=need) == -1
+    # the workspace does not grow with the rows beyond a chunk of them
+    assert lib.cbh_sample_classes_workspace(2 ** 31 - 1, 200_000) < 128 << 20
 
 
 def test_no_rows_are_no_work(lib):

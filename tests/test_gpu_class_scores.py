@@ -352,6 +352,18 @@ def test_sample_values(values):
             check_sample(x, g.random(rows), kind="bf16" if n == 500 else "f32", tag=(n, how), **how)
 
 
+def test_rows_of_more_classes_than_have_groups():
+    """Beyond 2^18 classes the draws take top_k from a histogram, and the top classes split every row."""
+    g = np.random.default_rng(17)
+    rows, n = 2, 600_011
+    x = O.scores(g, rows, n, "normal")
+    for how in (dict(k=50), dict(k=50, p=0.9), dict(k=3001), dict(p=0.9), dict(), dict(min_p=0.1), dict(t=0.0)):
+        check_sample(x, g.random(rows), kind="f16", tag=how, **how)
+    check_top(x, 40, 1.0, "f16", "rows")
+    u, ix, lse = teacher(g, x, 40, 1.0)
+    check_distill(x, u, ix, lse, 1.0, None, "f16", "rows")
+
+
 def test_sample_ends_of_the_uniform_range():
     g = np.random.default_rng(14)
     for rows, n in ((9, 10), (9, 3000), (9, 40000)):
