@@ -383,9 +383,8 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
 constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024, kListCap = 8192, kShortList = 128;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
 // The bins reach from the largest score to a little below the lowest of a sample (the first score of every group),
-// 32 nats at most: 32 bins a nat, and more of them for the rows whose nucleus is wide, so that one bin holds
-// hundreds of classes and not thousands (64 x 200001 f16, bins of 1/32 nat: 79 us to list them, 28 for the
-// histogram's clashing atomics).
+// 32 nats at most: 32 bins a nat, and more of them for the rows of a narrow range, whose nucleus is wide: one bin
+// then holds hundreds of classes and not thousands, which the list has to take.
 constexpr float kMostNats = 32.0f;
 __device__ __forceinline__ uint32_t bin_at(uint32_t b) { return b + (b >> 4); }   // (its place in LDS)
 
