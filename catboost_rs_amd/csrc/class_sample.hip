@@ -31,7 +31,7 @@ __device__ __forceinline__ Row settings(const Settings& S, uint64_t row, uint32_
     r.u = S.uniform[row];
     const double t = S.t_rows ? (double)S.t_rows[row] : S.t;
     r.greedy = !(t > 0.0);
-    r.rt = 1.0 / t;
+    r.rt = fmin(1.0 / t, 1e308);   // (finite: the largest score's own exponent is 0 times it)
     r.p = S.p_rows ? (double)S.p_rows[row] : S.p;
     r.min_p = S.min_p_rows ? (double)S.min_p_rows[row] : S.min_p;
     const uint32_t k = S.k_rows ? (uint32_t)max(S.k_rows[row], 0) : S.k;
@@ -510,7 +510,14 @@ struct Long {
         return first;
     }
 
-    // ---- bins: monotone in the score, the largest in bin 0 ----
+    // Rows that slow() takes whatever their settings: those of +inf, and those whose cut goes by bins or by f32
+    // exponentials at a temperature beyond [1e-30, 1e36], whose reciprocal's products leave f32 (an infinite scale of
+    // the bins puts the largest score, at distance 0, into the last).  Masses are f64 at any temperature.
+    __device__ __forceinline__ bool whole_row(float m, Mode mode) const {
+        return m == INFINITY || (mode != kWhole && !(r.rt >= 1e-36 && r.rt <= 1e30));
+    }
+
+    // ---- bins: monotone in the score, the largest in bin 0 (whole_row() keeps the scale finite) ----
     float bm, bscale;
     __device__ __forceinline__ void set_bins(float m, float low) {
         bm = m;
@@ -586,7 +593,7 @@ struct Long {
         uint32_t lo = order_key(-INFINITY), hi = order_key(bm);   // (bin(lo) is above b, or lo is it; bin(hi) = 0)
         while (hi - lo > 1) {
             const uint32_t step = (hi - lo + 63) / 64, probe = min(hi, lo + step * (lane + 1));   // (the last is hi)
-            const u64 yes = __ballot(bin(key_score(probe)) <= b);
+            const u64 yes = __ballot(probe == hi || bin(key_score(probe)) <= b);   // (hi is one: the range shrinks)
             const uint32_t at = yes ? (uint32_t)__builtin_ctzll(yes) : 63;
             hi = min(hi, lo + step * (at + 1));
             lo = lo + step * at;
@@ -809,8 +816,8 @@ struct Long {
             }
         }
     }
-    // Any row, by selection over the whole of it: rows of +inf, and those whose cut lies among more classes than
-    // a list holds (equal scores).
+    // Any row, by selection over the whole of it: rows of +inf or of far temperatures (whole_row()), and those whose
+    // cut lies among more classes than a list holds (equal scores).
     __device__ void slow(uint32_t top_key, uint32_t first, uint64_t row, SelectLds* lds, u64* tmp, u64* pick, const Out& out) const {
         const float m = key_score(top_key);
         const bool inf = m == INFINITY;
@@ -937,7 +944,7 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
             if (threadIdx.x == 0) out.empty(row);
             continue;
         }
-        bool slow = m == INFINITY;
+        bool slow = R.whole_row(m, mode);
         uint32_t first = 0;
         if (R.r.greedy || R.r.min_p > 1.0) {
             first = (uint32_t)block_reduce<THREADS>((u64)R.first_at(m, best, best_seg), MinU(), tmp);
@@ -1121,7 +1128,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) void weigh_kernel(Rows
     float low;
     const u64 top = row_top<THREADS>(P, row, tmp, low);
     const float m = key_score((uint32_t)(top >> 32));
-    if (top == 0 || m == INFINITY) return;
+    if (top == 0 || R.whole_row(m, mode)) return;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
     if (mode == kWhole) {
         u64 all = R.weigh(s0, s1, M, R.r.min_p > 1.0 ? 0 : M.least(R.r.min_p), P.segs + row * P.n_segs);
@@ -1152,7 +1159,7 @@ __global__ __launch_bounds__(1024) void cut_kernel(Rows<T> X, Settings S, int sh
     const u64 top = row_top<THREADS>(P, row, tmp, low);
     const float m = key_score((uint32_t)(top >> 32));
     const bool list = mode == kList && !(P.groups && R.by_groups(P.n_segs));
-    if ((mode != kNucleus && !list) || top == 0 || m == INFINITY) {
+    if ((mode != kNucleus && !list) || top == 0 || R.whole_row(m, mode)) {
         if (threadIdx.x == 0) P.steps[row].state = kNone;
         return;
     }
@@ -1230,7 +1237,7 @@ __global__ __launch_bounds__(512) void draw_direct_kernel(Rows<T> X, Settings S,
         return;
     }
     if (mode != kWhole && !by_groups) return;
-    if (m == INFINITY) {
+    if (R.whole_row(m, mode)) {
         R.slow((uint32_t)(top >> 32), first, row, &lds, tmp, pick, out);
         return;
     }
@@ -1301,7 +1308,7 @@ __global__ __launch_bounds__(1024) void draw_kernel(Rows<T> X, Settings S, int s
     if (top == 0 || mode == kGreedy || mode == kWhole || (mode == kList && P.groups && R.by_groups(P.n_segs))) return;
     const uint32_t first = ~(uint32_t)top;
     const Masses M{(double)m, R.r.rt * 1.4426950408889634, shift};
-    bool slow = m == INFINITY;
+    bool slow = R.whole_row(m, mode);
     if (!slow && mode == kNucleus) {
         const Step step = P.steps[row];
         const uint32_t n_list = P.count[row];

@@ -532,7 +532,9 @@ int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint3
  * Masses are integers in units of 2^-S of the row's largest weight (S = 46 up to 32 classes, 51 up to 2^11,
  * 62 - b up to 2^b), so that sums are exact and the same for every launch shape.
  *   uniform        [rows] f64 in [0, 1)
- *   temperature, top_k, top_p, min_p   values for every row; *_rows: nullable [rows], used in their place
+ *   temperature, top_k, top_p, min_p   values for every row; *_rows: nullable [rows], used in their place.  Any
+ *                  positive temperature is taken, infinity too (a row beyond [1e-30, 1e36] of more than 2048 classes
+ *                  with top_k or top_p takes several passes over it)
  *   allowed        nullable; bit j & 31 of word allowed[r * allowed_stride + (j >> 5)] allows class j of row r
  *                  (allowed_stride 0: one list for all rows)
  *   index [rows] i32, logprob nullable [rows] f32 */
