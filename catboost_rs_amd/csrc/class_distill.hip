@@ -5,9 +5,12 @@
 //   loss = w t^2 [ sum_l q_l (log q_l - log p_l) + rest (log rest - log sum_others p) ]
 //   grad = w t [ p_j H - q_j ] (listed),  w t p_j (H - rest / sum_others p) (others),  H = sum q + rest
 // The others' softmax mass is summed over the others themselves (the listed classes are marked in
-// an LDS bit mask and read as -inf), never as the difference 1 - listed: a student that is
-// sure of its answer leaves the others a mass that such a difference would lose.  What belongs to the
-// listed classes is f64: their gradient is a difference of nearly equal probabilities.
+// an LDS bit mask and read as -inf), never as the difference 1 - listed, and relative to the others' own
+// largest score m: a student that is sure of its answer leaves the others a mass that such a difference would
+// lose, and that no number relative to the row's largest score M holds (e^((m - M) / t) is 0 in f32 from a gap of 87
+// temperatures on, in f64 from 745).  With s the others' sum of e^((x - m) / t) and S all classes' of e^((x - M) / t):
+//   sum_others p = s e^((m - M) / t) / S,  p_j (H - rest / sum_others p) = e^((x_j - m) / t) (H e^((m - M) / t) / S - rest / s)
+// What belongs to the listed classes is f64: their gradient is a difference of nearly equal probabilities.
 #include "class_scores.hpp"
 
 namespace {
@@ -41,33 +44,34 @@ struct RowSums {
 };
 struct Outcome {
     double loss;
-    float M, others;   // gradient of an other class: 2^((x - M) c) * others
+    float others;          // gradient of an other class: 2^((x - m) c) * others, m the largest of them
     double whole, inv_s;   // of a listed one: wt (2^((x - M) c) * inv_s * whole - q)
 };
 
-// (M, S_o): running maximum and sum of the others; S_l the listed classes' sum at the same M; lin = sum q
-// log p_l.  t, w as in the loss.
 __device__ __forceinline__ double row_rest(const RowSums& r, bool has_lse, uint32_t n) {
     return has_lse && r.listed < n ? fmax(0.0, 1.0 - r.held) : 0.0;
 }
-__device__ __forceinline__ Outcome outcome(const RowSums& r, double rest, double M, double s_others, double s_listed,
-                                           double lin, double t, double w) {
+// q log q and q log p, 0 where q is
+__device__ __forceinline__ double times_log(double q, double l) { return q == 0.0 ? 0.0 : q * l; }
+// gap: (m - M) / t; s_others: the others' sum at m; s_listed: the listed classes' at M; cross: sum q (x - M) / t.  t, w as
+// in the loss.
+__device__ __forceinline__ Outcome outcome(const RowSums& r, double rest, double gap, double s_others, double s_listed,
+                                           double cross, double t, double w) {
     Outcome o;
-    const double S = s_others + s_listed;
-    o.M = (float)M;
+    const double fade = s_others == 0.0 ? 0.0 : exp_f64(gap), S = s_others * fade + s_listed;
+    const double share = s_others > 0.0 ? rest / s_others : 0.0, log_s = log(S);
     o.whole = r.held + rest;
     o.inv_s = S > 0.0 ? 1.0 / S : S == 0.0 ? 0.0 : S;   // (NaN stays)
-    // share of the others in the gradient: whole / S - rest / s_others
-    o.others = (float)(w * t * (o.whole * o.inv_s - (s_others > 0.0 ? rest / s_others : 0.0)));
+    o.others = (float)(w * t * (o.whole * o.inv_s * fade - share));
+    // sum q log p; a row without a score above -inf gives its classes no probability
+    const double lin = S == 0.0 ? (r.held > 0.0 ? -(double)INFINITY : 0.0) : cross - times_log(r.held, log_s);
     double loss = r.entropy - lin;
-    if (rest > 0.0) loss += rest * (log(rest) - log(s_others * o.inv_s));
+    if (rest > 0.0) loss += s_others == 0.0 ? (double)INFINITY : rest * (log(rest / s_others) - gap + log_s);
     o.loss = w * t * t * loss;
     return o;
 }
 // (the list's own log-sum-exp stays in two parts: next to the lowest f32 one number would lose the logarithm)
 __device__ __forceinline__ double log_q(float u, double it, const RowSums& r) { return ((double)u * it - r.base) - r.base_log; }
-// q log q and q log p, 0 where q is
-__device__ __forceinline__ double times_log(double q, double l) { return q == 0.0 ? 0.0 : q * l; }
 
 // Two passes over a row, the second from the last cache while the rows under way fit it, one of them writing.
 // 4096 x 65536 bf16, k 64: 269 us, 1.07 GB of reads and writes at 4.0 TB/s (a copy: 5.2); 1500 x 100003 f32, k 20: 297
@@ -197,12 +201,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
         r.held = s[0];
         r.entropy = s[1];
         r.listed = (uint32_t)s[4];
-        const double sl = s[2];
-        so = so == 0.0 ? 0.0 : so * exp_f64(((double)mo - (double)M) * it);   // (in f64: far below M it must not vanish)
-        // sum q log p; a row without a score above -inf gives its classes no probability
-        const double lin = so + sl == 0.0 ? (r.held > 0.0 ? -(double)INFINITY : 0.0) : s[3] - times_log(r.held, log(so + sl));
         const double rest = row_rest(r, L.lse != nullptr, X.classes);
-        const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
+        const Outcome o = outcome(r, rest, ((double)mo - (double)M) * it, so, s[2], s[3], t, w);
         if (loss && first == 0 && threadIdx.x == 0) loss[row] = (float)o.loss;
         if (g0) {
             for (uint32_t base = wave * kSeg; base < n; base += W * kSeg) {
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
                 for (int q = 0; q < U; ++q) {
                     const uint32_t i = base + (q * 64 + lane) * V;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) x[q][v] = exp2_fast((x[q][v] - o.M) * c) * o.others;
+                    for (int v = 0; v < V; ++v) x[q][v] = exp2_fast((x[q][v] - mo) * c) * o.others;
                     if (i < n) store_pack<T, kUnit>(g0, G.cs, i, n, x[q]);
                 }
             }
@@ -316,7 +316,6 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             const float e = exp2_fast((x[j] - mo) * c);
             s += mask >> j & 1 ? 0.0f : e;
         }
-        const double so = s == 0.0f ? 0.0 : (double)s * exp_f64(((double)mo - (double)M) * it);
         auto weigh = [&](Entry& en) {
             en.q = exp_f64((en.ut - r.base) - r.base_log);
             en.e = exp_f64(((double)en.x - (double)M) * it);
@@ -329,16 +328,14 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             r.entropy += times_log(en.q, (en.ut - r.base) - r.base_log);
             cross += times_log(en.q, ((double)en.x - (double)M) * it);
         });
-        // (a row without a score above -inf gives its classes no probability)
-        const double lin = so + sl == 0.0 ? (r.held > 0.0 ? -(double)INFINITY : 0.0) : cross - times_log(r.held, log(so + sl));
         const double rest = row_rest(r, L.lse != nullptr, n);
-        const Outcome o = outcome(r, rest, (double)M, so, sl, lin, t, w);
+        const Outcome o = outcome(r, rest, ((double)mo - (double)M) * it, (double)s, sl, cross, t, w);
         if (loss) loss[row] = (float)o.loss;
         if (g0) {
 #pragma unroll
             for (int j = 0; j < NMAX; ++j)
                 if ((uint32_t)j < n && !(mask >> j & 1))
-                    g0[(int64_t)j * G.cs] = from_f32<T>(exp2_fast((x[j] - o.M) * c) * o.others);
+                    g0[(int64_t)j * G.cs] = from_f32<T>(exp2_fast((x[j] - mo) * c) * o.others);
             each([&](Entry& en) {
                 if constexpr (KM == 0) weigh(en);
                 g0[(int64_t)en.cls * G.cs] = from_f32<T>((float)(w * t * (en.e * o.inv_s * o.whole - en.q)));

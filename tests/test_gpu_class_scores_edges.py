@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from tests import class_scores_oracle as O
-from tests.test_gpu_class_scores import run_sample
+from tests.test_gpu_class_scores import run_distill, run_sample
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,112 @@ def test_sample_far_temperatures_of_rows(rows, n):
         check_far(O.scores(g, rows, n, values), g.random(rows), t=g.choice([0.0, 1.0, 1e-37, 1e-40, 1e37, np.inf], rows),
                      k=g.choice([0, 0, 3, 300], rows), p=g.choice([1.0, 0.8, 0.5], rows), min_p=g.choice([0.0, 0.1], rows),
                      allowed=g.random((rows, n)) < 0.7, tag=values)
+
+
+# ---- students that are sure of their answer --------------------------------------------------
+
+def mass_of(z):
+    """The largest of some z (0 if all are -inf) and the sum of exp(z - largest): a log-sum-exp in two parts (next to
+    the lowest f32 one number would lose the logarithm)."""
+    m = z.max() if z.size and z.max() > -np.inf else 0.0
+    return m, np.exp(z - m).sum()
+
+
+def distill_in_logs(x, u, ix, base, t, w):
+    """Loss and gradient by the formulas with every softmax mass as a logarithm, and what the bars count against: a
+    row's gradient terms before they are subtracted, and the others' largest distance in temperatures."""
+    rows, n = x.shape
+    loss, grad, size, far = np.zeros(rows), np.zeros((rows, n)), np.zeros((rows, n)), np.zeros(rows)
+    with np.errstate(all="ignore"):
+        for r in range(rows):
+            z = x[r].astype(np.float64) / t
+            ok = (ix[r] >= 0) & (ix[r] < n)
+            at, lu = ix[r][ok].astype(int), u[r][ok].astype(np.float64) / t
+            free = np.ones(n, bool)
+            free[at] = False
+            big, total = mass_of(z)
+            um, us = mass_of(lu) if base is None else (float(base[r]), 1.0)
+            lq = np.where(lu > -np.inf, (lu - um) - np.log(us), -np.inf)
+            q = np.exp(lq)
+            g = np.exp(z - big) / total * q.sum()
+            loss[r] = (q[q > 0] * (lq - (z[at] - big) + np.log(total))[q > 0]).sum()
+            rest = max(0.0, 1.0 - q.sum()) if base is not None and free.any() else 0.0
+            size[r] = g
+            if rest > 0:
+                om, others = mass_of(z[free])
+                loss[r] += rest * (np.log(rest) - (np.log(others) + (om - big) - np.log(total)))
+                g = g + np.exp(z - big) / total * rest
+                share = np.where(free & (others > 0), rest * np.exp(np.where(free, z - om, 0.0)) / others, 0.0)
+                g, size[r] = g - share, g + share
+                near = z[free][z[free] > -np.inf]
+                far[r] = min(near.max() - near.min(), 110.0) if near.size else 0.0
+            g[at] -= q
+            size[r][at] += q
+            loss[r] *= w * t * t
+            grad[r], size[r] = w * t * g, w * t * size[r]
+    return loss, grad, size, far
+
+
+def check_distill_in_logs(x, u, ix, base, t, w, kind, order, tag):
+    rows, n = x.shape
+    weight = None if w == 1.0 else np.full(rows, w, np.float32)
+    loss, grad = run_distill(x, u, ix, base, t, weight, kind, order)
+    el, eg, size, far = distill_in_logs(O.round_to(x, kind), u, ix, base, t, w)
+    # a mass is a sum of f32 exponentials of d, |d| <= far: off by 3 |d| 2^-24 (difference, scale, product) and 2^-23
+    # each, by the f32 additions of 32 of them and by at most a factor of that kind for every tile; a class's
+    # gradient is such an exponential times f64 factors of masses, rounded to f32 three times and to the type
+    rel = (32 + 4 + 4 * far) * 2.0 ** -24
+    fin = np.isfinite(el)
+    assert np.array_equal(np.where(fin, 0, loss), np.where(fin, 0, el), equal_nan=True), (tag, loss, el)
+    bar = w * t * t * rel * 3 + np.abs(el) * 2.0 ** -23
+    assert (np.abs(loss - el)[fin] <= bar[fin]).all(), (tag, loss, el)
+    # (an exponential below the normal range may be 0)
+    bar = size * 2 * rel[:, None] + np.abs(eg) * O.half_step(kind) + O.smallest(kind) * max(1.0, w * t) * 2
+    off = np.abs(grad - eg)
+    at = np.unravel_index(np.nanargmax(off - bar), off.shape)
+    assert (off <= bar).all(), (tag, at, grad[at], eg[at])
+
+
+GAPS = [60.0, 86.0, 88.0, 95.0, 120.0, 700.0, 760.0, 2000.0, 1e4]
+
+
+def sure(g, rows, n, k, t, gap, how):
+    """Students whose listed classes (all of them, or one) lie `gap` temperatures above every other class, and
+    teachers that leave a tenth of their mass to the others."""
+    x = O.scores(g, rows, n, "normal")
+    ix = np.stack([g.permutation(n)[:k] for _ in range(rows)]).astype(np.int32)
+    raised = ix if how == "all" else ix[:, :1]
+    lift = gap * t + x.max(1, keepdims=True) - np.take_along_axis(x, raised, 1).min(1, keepdims=True)
+    np.put_along_axis(x, raised, (np.take_along_axis(x, raised, 1) + lift).astype(np.float32), 1)
+    q = g.random((rows, k)) + 0.1
+    q = 0.9 * q / q.sum(1, keepdims=True)
+    base = g.standard_normal(rows).astype(np.float32)
+    return x, (t * (np.log(q) + base[:, None])).astype(np.float32), ix, base
+
+
+@pytest.mark.parametrize("rows,n,k", [(24, 20, 6), (24, 10, 3), (6, 500, 20), (4, 9001, 40), (3, 40000, 30), (2, 140001, 20)])
+def test_distill_sure_students(rows, n, k):
+    """However far the others lie below a student's answer, they share what the teacher leaves them."""
+    g = np.random.default_rng(n + k)
+    for how in ("all", "one"):
+        for t, w in ((1.0, 1.0), (0.1, 2.0)):
+            for gap in GAPS:
+                x, u, ix, base = sure(g, rows, n, k, t, gap, how)
+                for kind in ("f32", "bf16"):
+                    order = "rows" if kind == "f32" else "padded"
+                    check_distill_in_logs(x, u, ix, base, t, w, kind, order, (how, t, gap, kind))
+
+
+@pytest.mark.parametrize("rows,n,k", [(24, 20, 6), (24, 10, 3), (6, 500, 20), (4, 9001, 40), (3, 40000, 30)])
+def test_distill_masked_others(rows, n, k):
+    """Others at a mask's finite value: -1e4, or the lowest of the type, some of them -inf; and all of them -inf (the
+    loss is infinite)."""
+    g = np.random.default_rng(n - k)
+    for low in (-1e4, O.LOWEST, -np.inf):
+        x, u, ix, base = sure(g, rows, n, k, 1.0, 1.0, "all")
+        free = np.ones((rows, n), bool)
+        np.put_along_axis(free, ix, False, 1)
+        x[free] = low
+        if low > -np.inf:
+            x[free & (g.random((rows, n)) < 0.3)] = -np.inf
+        check_distill_in_logs(x, u, ix, base, 1.0, 1.0, "f32", "rows", low)
