@@ -70,8 +70,11 @@ __device__ __forceinline__ Outcome outcome(const RowSums& r, double rest, double
     o.loss = w * t * t * loss;
     return o;
 }
-// (the list's own log-sum-exp stays in two parts: next to the lowest f32 one number would lose the logarithm)
-__device__ __forceinline__ double log_q(float u, double it, const RowSums& r) { return ((double)u * it - r.base) - r.base_log; }
+// (the list's own log-sum-exp stays in two parts: next to the lowest f32 one number would lose the logarithm; an entry
+// of -inf has no mass beside a log-sum-exp of -inf either)
+__device__ __forceinline__ double log_q(double ut, const RowSums& r) {
+    return ut == -(double)INFINITY ? ut : (ut - r.base) - r.base_log;
+}
 
 // Two passes over a row, the second from the last cache while the rows under way fit it, one of them writing.
 // 4096 x 65536 bf16, k 64: 269 us, 1.07 GB of reads and writes at 4.0 TB/s (a copy: 5.2); 1500 x 100003 f32, k 20: 297
@@ -177,7 +180,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
             r.base = umax = block_reduce<THREADS>(umax, MaxF(), tmp_d);
             double s[1] = {0.0};
 #pragma unroll
-            for (int e = 0; e < LE; ++e) s[0] += cls[e] != ~0u ? exp_f64(lq[e] - umax) : 0.0;
+            for (int e = 0; e < LE; ++e) s[0] += lq[e] == -INFINITY ? 0.0 : exp_f64(lq[e] - umax);   // (no entry: -inf)
             block_sums<THREADS>(s, tmp_d);
             r.base_log = log(s[0]);
         }
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
         for (int e = 0; e < LE; ++e) {
             el[e] = 0.0;
             if (cls[e] == ~0u) continue;
-            const double l = (lq[e] - r.base) - r.base_log, q = exp_f64(l), d = ((double)xl[e] - (double)M) * it;
+            const double l = log_q(lq[e], r), q = exp_f64(l), d = ((double)xl[e] - (double)M) * it;
             el[e] = exp_f64(d);
             lq[e] = q;   // (from here on: q)
             s[0] += q;
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             r.base = (double)L.lse[row];
         } else {
             double s = 0.0;
-            each([&](Entry& en) { s += exp_f64(en.ut - umax); });
+            each([&](Entry& en) { s += en.ut == -INFINITY ? 0.0 : exp_f64(en.ut - umax); });
             r.base = umax;
             r.base_log = log(s);
         }
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             s += mask >> j & 1 ? 0.0f : e;
         }
         auto weigh = [&](Entry& en) {
-            en.q = exp_f64((en.ut - r.base) - r.base_log);
+            en.q = exp_f64(log_q(en.ut, r));
             en.e = exp_f64(((double)en.x - (double)M) * it);
         };
         double sl = 0.0, cross = 0.0;   // sum q (x - M) / t
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, fl
             weigh(en);
             sl += en.e;
             r.held += en.q;
-            r.entropy += times_log(en.q, (en.ut - r.base) - r.base_log);
+            r.entropy += times_log(en.q, log_q(en.ut, r));
             cross += times_log(en.q, ((double)en.x - (double)M) * it);
         });
         const double rest = row_rest(r, L.lse != nullptr, n);

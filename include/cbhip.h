@@ -510,7 +510,8 @@ int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t cl
  *   weight         nullable [rows]; a row of weight 0 gives 0 whatever its scores hold
  *   loss           nullable [rows] f32; grad nullable, with strides of its own (not both null); neither may
  *                  overlap an input
- * A teacher's entry of -inf has q = 0.  A student's row of -inf alone has p = 0 everywhere and an
+ * A teacher's entry of -inf has q = 0, all of a row's too (with a top_lse of -inf the others then hold all mass).
+ * A student's row of -inf alone has p = 0 everywhere and an
  * infinite loss; NaN or +inf in a student's row makes that row's loss and gradient NaN. */
 uint64_t cbh_distill_gradients_workspace(uint64_t rows, uint32_t classes);
 int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,

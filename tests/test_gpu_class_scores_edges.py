@@ -188,3 +188,18 @@ def test_distill_masked_others(rows, n, k):
         if low > -np.inf:
             x[free & (g.random((rows, n)) < 0.3)] = -np.inf
         check_distill_in_logs(x, u, ix, base, 1.0, 1.0, "f32", "rows", low)
+
+
+@pytest.mark.parametrize("rows,n,k", [(24, 20, 6), (24, 10, 3), (6, 500, 20), (4, 9001, 40), (3, 40000, 30)])
+def test_distill_teacher_without_mass(rows, n, k):
+    """A teacher's entries of -inf hold no mass, all of a row's among them: without top_lse nothing pulls at the
+    student, with one of -inf the others hold everything."""
+    g = np.random.default_rng(n * k)
+    x = O.scores(g, rows, n, "normal")
+    ix = np.stack([g.permutation(n)[:k] for _ in range(rows)]).astype(np.int32)
+    u = np.full((rows, k), -np.inf, np.float32)
+    u[0, 1:] = 0.5
+    for base in (None, np.full(rows, -np.inf, np.float32)):
+        if base is not None:
+            base[0] = 3.0
+        check_distill_in_logs(x, u, ix, base, 1.5, 1.0, "f32", "rows", base is None)
