@@ -76,6 +76,12 @@ struct Candidates {
     }
 };
 
+// A row's log-sum-exp from its (m, s), once its largest score `top` is known: a NaN ranks first, and only then is a
+// NaN in s more than the +inf - +inf of a row with +inf.
+__device__ __forceinline__ float row_lse(float m, double s, float top, double inv_t) {
+    return m == INFINITY && top == top ? INFINITY : (float)((double)m * inv_t + log(s));
+}
+
 // Short rows, and a k that is large beside the row: candidates are taken in the pass itself (4 x 1000 f32, k 5:
 // 6.8 us, latency).
 // A workgroup takes a row, or one of the `parts` segments of `seg` classes of a row (few rows of many
@@ -191,10 +197,11 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
                 const u64 key = best[i];
                 uint32_t rank = 0;
                 for (uint32_t j = 0; j < got; ++j) rank += best[j] > key;
-                values[row * k + rank] = key_score((uint32_t)(key >> 32));
+                const float x = key_score((uint32_t)(key >> 32));
+                values[row * k + rank] = x;
                 index[row * k + rank] = (int32_t)~(uint32_t)key;
+                if (rank == 0) lse[row] = row_lse(m, s, x, inv_t);
             }
-            if (threadIdx.x == 0) lse[row] = m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(s));
         } else {
             for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = i < got ? best[i] : 0;
             if (threadIdx.x == 0) part_ms[job] = float2{m, (float)s};
@@ -299,10 +306,11 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
                 const u64 key = best[i];
                 uint32_t rank = 0;
                 for (uint32_t j = 0; j < k; ++j) rank += best[j] > key;
-                values[row * k + rank] = key_score((uint32_t)(key >> 32));
+                const float x = key_score((uint32_t)(key >> 32));
+                values[row * k + rank] = x;
                 index[row * k + rank] = (int32_t)~(uint32_t)key;
+                if (rank == 0) lse[row] = row_lse(m, sum, x, inv_t);
             }
-            if (threadIdx.x == 0) lse[row] = m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(sum));
         } else {
             for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = best[i];
             if (threadIdx.x == 0) part_ms[job] = float2{m, (float)sum};
@@ -344,10 +352,11 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
         const u64 key = best[i];
         uint32_t rank = 0;
         for (uint32_t j = 0; j < k; ++j) rank += best[j] > key;
-        values[row * k + rank] = key_score((uint32_t)(key >> 32));
+        const float x = key_score((uint32_t)(key >> 32));
+        values[row * k + rank] = x;
         index[row * k + rank] = (int32_t)~(uint32_t)key;
+        if (rank == 0) lse[row] = row_lse(m, s, x, inv_t);
     }
-    if (threadIdx.x == 0) lse[row] = m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(s));
 }
 
 // Few classes: a row a thread, its scores in registers; a score's place is the count of those ahead.
@@ -378,13 +387,16 @@ __global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, flo
                 rank[j] += !ahead;
             }
         }
+        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NMAX; ++i)
+        for (int i = 0; i < NMAX; ++i) {
             if ((uint32_t)i < n && rank[i] < k) {
                 values[row * k + rank[i]] = key_score(key[i]);
                 index[row * k + rank[i]] = i;
             }
-        lse[row] = run.m == INFINITY ? INFINITY : (float)((double)run.m * inv_t + log(run.s));
+            top = rank[i] == 0 ? key_score(key[i]) : top;
+        }
+        lse[row] = row_lse(run.m, run.s, top, inv_t);
     }
 }
 

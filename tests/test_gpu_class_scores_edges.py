@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from tests import class_scores_oracle as O
-from tests.test_gpu_class_scores import run_distill, run_sample
+from tests.test_gpu_class_scores import run_distill, run_sample, run_top
 
 pytestmark = pytest.mark.gpu
 
@@ -203,3 +203,22 @@ def test_distill_teacher_without_mass(rows, n, k):
         if base is not None:
             base[0] = 3.0
         check_distill_in_logs(x, u, ix, base, 1.5, 1.0, "f32", "rows", base is None)
+
+
+# ---- sums of parts, infinities beside NaN ------------------------------------------------------
+
+def test_top_nan_beside_infinity():
+    """A NaN makes a row's log-sum-exp NaN, +inf in the row or not."""
+    g = np.random.default_rng(21)
+    for rows, n, k in ((5, 20, 9), (5, 3000, 100), (5, 20000, 50), (5, 70000, 100), (5, 70000, 1000)):
+        x = O.scores(g, rows, n, "normal")
+        x[0, [n // 2, 1]] = np.nan, np.inf
+        x[1, [1, n - 1]] = np.nan, np.inf
+        x[2, 3] = np.inf
+        x[3, n // 3] = np.nan
+        x[4, [0, 2]] = -np.inf, np.inf
+        for kind in ("f32", "f16", "bf16"):
+            v, i, s = run_top(x, k, 1.0, kind, "rows")
+            ev, ei, _ = O.top(O.round_to(x, kind), k, 1.0)
+            assert np.array_equal(i, ei) and np.array_equal(v.astype(np.float64), ev, equal_nan=True), (n, kind)
+            assert np.isnan(s[[0, 1, 3]]).all() and (s[[2, 4]] == np.inf).all(), (n, kind, s)
