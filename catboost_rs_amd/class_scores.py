@@ -97,7 +97,7 @@ def top_classes(scores, k, temperature=1.0):
     """The ``k`` largest scores of every row (``cbh_top_classes``): ``values`` [rows][k] f32, largest
     first, their classes ``index`` [rows][k] i32 (the lowest first among equal scores), and
     ``lse`` [rows] f32, the row's log-sum-exp of ``scores / temperature``: what
-    :func:`distill_gradients` takes of a teacher.  1 <= k <= min(classes, 1024)."""
+    :func:`distill_gradients` takes of a teacher.  1 <= k <= min(classes, 1024); 1e-38 <= temperature <= 1e36."""
     torch = _state.get("torch") or _bind()
     t, n, m, rs, cs = _scores(torch, scores)
     k = int(k)

@@ -423,7 +423,7 @@ extern "C" int cbh_distill_gradients(const void* scores, int32_t type, uint64_t 
         if (rc != CBH_OK) return rc;
         if (k < 1 || k > kMaxList) return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "k must be in 1 .. 1024");
         if (!good_temperature(temperature))
-            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "temperature must be positive and finite");
+            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, kBadTemperature);
         if (rows == 0) return CBH_OK;
         if (!top_scores || !top_index) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "the teacher's lists are null");
         if (!loss && !grad) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "loss and grad are both null");

@@ -509,7 +509,10 @@ inline int check_scores(const void* scores, int32_t type, uint64_t rows, uint32_
         return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "strides pass the address range");
     return CBH_OK;
 }
-inline bool good_temperature(double t) { return t > 0.0 && std::isfinite(t) && std::isfinite(1.0 / t); }
+// The exponent of a score, (x - m) log2(e) / t, is taken in f32: log2(e) / t is finite and normal there from 1e-38 on,
+// and up to 1e36 a difference that leaves f32 has no weight (e^-340).
+inline bool good_temperature(double t) { return t >= 1e-38 && t <= 1e36; }
+constexpr const char* kBadTemperature = "temperature must be in 1e-38 .. 1e36";
 
 // The grid of a kernel whose workgroups walk over the rows: a launch holds fewer than 2^32 threads.
 inline unsigned row_grid(uint64_t blocks) { return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(blocks, 1u << 20)); }

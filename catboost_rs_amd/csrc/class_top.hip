@@ -477,7 +477,7 @@ extern "C" int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, 
         if (k < 1 || k > classes || k > kMaxTop)
             return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "k must be in 1 .. min(classes, 1024)");
         if (!good_temperature(temperature))
-            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "temperature must be positive and finite");
+            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, kBadTemperature);
         if (rows == 0) return CBH_OK;
         if (!values || !index || !lse) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "outputs are null");
         const uint64_t need = cbh_top_classes_workspace(rows, classes, k);

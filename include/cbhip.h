@@ -487,7 +487,7 @@ int cbh_ctr_columns(const uint32_t* buckets, uint32_t n_buckets, uint64_t n, con
 enum { CBH_TYPE_F32 = 0, CBH_TYPE_F16 = 1, CBH_TYPE_BF16 = 2 };
 
 /* The k largest scores of every row, largest first, the lowest class first among equal ones, and the row's
- * log-sum-exp of scores / temperature (temperature > 0):
+ * log-sum-exp of scores / temperature (1e-38 <= temperature <= 1e36):
  *   values [rows][k] f32, index [rows][k], lse [rows] f32;  1 <= k <= min(classes, 1024)
  * -0 and +0 are equal (and come back as 0); NaN counts as larger than +inf and makes the row's lse NaN; a
  * row of -inf alone has lse = -inf. */
@@ -497,7 +497,7 @@ int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t cl
                     float* lse, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Distillation of a student's scores x from a teacher's top classes: loss and its gradient in one call.
- * With t = temperature, p = softmax(x / t), u_i = top_scores[r][i] the teacher's score of class
+ * With t = temperature (1e-38 .. 1e36), p = softmax(x / t), u_i = top_scores[r][i] the teacher's score of class
  * top_index[r][i], and q_i = exp(u_i / t - top_lse[r]) (the teacher's probability, top_lse its log-sum-exp
  * at t; NULL: over the listed classes alone, which then hold the whole mass):
  *   rest  = max(0, 1 - sum q) when top_lse is given and a class is not listed, else 0

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from tests import class_scores_oracle as O
-from tests.test_gpu_class_scores import run_distill, run_sample, run_top
+from tests.test_gpu_class_scores import check_top, run_distill, run_sample, run_top
 
 pytestmark = pytest.mark.gpu
 
@@ -222,3 +222,12 @@ def test_top_nan_beside_infinity():
             ev, ei, _ = O.top(O.round_to(x, kind), k, 1.0)
             assert np.array_equal(i, ei) and np.array_equal(v.astype(np.float64), ev, equal_nan=True), (n, kind)
             assert np.isnan(s[[0, 1, 3]]).all() and (s[[2, 4]] == np.inf).all(), (n, kind, s)
+
+
+@pytest.mark.parametrize("t", [1e-38, 1e-37, 1e36])
+def test_top_at_the_ends_of_the_temperatures(t):
+    """Scores of the temperature's size keep their weights beside each other."""
+    g = np.random.default_rng(22)
+    for rows, n, k in ((40, 20, 7), (6, 3000, 20), (2, 70000, 20)):
+        x = (O.scores(g, rows, n, "normal").astype(np.float64) * t).astype(np.float32)
+        check_top(x, k, t, "f32", "rows", (n, t))
