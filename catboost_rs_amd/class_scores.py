@@ -31,7 +31,7 @@ def _bind():
     if len(_runtimes()) > 1:
         raise RuntimeError("two HIP runtimes are loaded: import torch before the first call of catboost_rs_amd")
     _TYPE.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-    _state.update(torch=torch, lib=L, check=cb._check, top=L.cbh_top_classes, top_ws=L.cbh_top_classes_workspace,
+    _state.update(torch=torch, lib=L, check=cb._check, error=cb.CbhError, top=L.cbh_top_classes, top_ws=L.cbh_top_classes_workspace,
                   distill=L.cbh_distill_gradients, distill_ws=L.cbh_distill_gradients_workspace,
                   sample=L.cbh_sample_classes, sample_ws=L.cbh_sample_classes_workspace,
                   raw_stream=getattr(torch._C, "_cuda_getCurrentRawStream", None))
@@ -48,6 +48,8 @@ def _scores(torch, x, what="scores"):
     if not x.is_cuda:
         raise ValueError(f"{what} must be on the GPU")
     (n, m), (rs, cs) = x.shape, x.stride()
+    if m > 1 << 24:   # (before anything of that size is allocated, and before 32 bits cut it off)
+        raise _state["error"](-2, f"{what}: classes must be in 1 .. 2^24")
     return t, n, m, rs, cs
 
 
@@ -101,14 +103,15 @@ def top_classes(scores, k, temperature=1.0):
     torch = _state.get("torch") or _bind()
     t, n, m, rs, cs = _scores(torch, scores)
     k = int(k)
+    k = k if 1 <= k <= 1024 else 0   # (0: refused below)
     with _on(scores):
         dev = scores.device
-        values = torch.empty((n, max(k, 0)), dtype=torch.float32, device=dev)
-        index = torch.empty((n, max(k, 0)), dtype=torch.int32, device=dev)
+        values = torch.empty((n, k), dtype=torch.float32, device=dev)
+        index = torch.empty((n, k), dtype=torch.int32, device=dev)
         lse = torch.empty(n, dtype=torch.float32, device=dev)
-        size = _state["top_ws"](n, m, max(k, 0))
+        size = _state["top_ws"](n, m, k)
         ws = _workspace(torch, size, scores)
-        _state["check"](_state["top"](scores.data_ptr(), t, n, m, rs, cs, max(k, 0), float(temperature), values.data_ptr(),
+        _state["check"](_state["top"](scores.data_ptr(), t, n, m, rs, cs, k, float(temperature), values.data_ptr(),
                                       index.data_ptr(), lse.data_ptr(), _addr(ws), size, _stream(scores)))
     return values, index, lse
 
@@ -173,7 +176,7 @@ def sample_classes(scores, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_
         size = _state["sample_ws"](n, m)
         ws = _workspace(torch, size, scores)
         _state["check"](_state["sample"](scores.data_ptr(), t, n, m, rs, cs, uniform.data_ptr(), float(tv), _addr(tr),
-                                         max(int(kv), 0), _addr(kr), float(pv), _addr(pr), float(mv), _addr(mr),
+                                         min(max(int(kv), 0), m), _addr(kr), float(pv), _addr(pr), float(mv), _addr(mr),
                                          _addr(allowed), astride, index.data_ptr(), logprob.data_ptr(), _addr(ws), size,
                                          _stream(scores)))
     return index, logprob

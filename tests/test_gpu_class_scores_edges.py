@@ -3,6 +3,10 @@ their answer, infinities beside NaN, teachers without mass, sums of parts.
 
 Scores, buffers and calls are those of test_gpu_class_scores.py.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -231,3 +235,13 @@ def test_top_at_the_ends_of_the_temperatures(t):
     for rows, n, k in ((40, 20, 7), (6, 3000, 20), (2, 70000, 20)):
         x = (O.scores(g, rows, n, "normal").astype(np.float64) * t).astype(np.float32)
         check_top(x, k, t, "f32", "rows", (n, t))
+
+
+def test_torch_tensors_at_their_ends():
+    """In a process of its own: torch brings its own copy of the HIP runtime, and one serves a process."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-u", os.path.join(here, "torch_class_scores_edges.py")], cwd=os.path.dirname(here),
+                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+    print(r.stdout)
+    assert r.returncode == 0, r.stdout[-3000:]
+    assert r.stdout.rstrip().endswith("all checks passed")
