@@ -6,6 +6,9 @@ They take torch tensors on the GPU and enqueue on torch's current stream; what t
 is made by torch on that stream.  Scores are [rows][classes], f32, f16 or bf16, of any
 strides: the [classes][rows] scores of a trained model go in as ``scores.t()``.
 
+They record no autograd graph, also where the scores require a gradient: a loss is a value to look at, and the
+gradient goes on with ``scores.backward(grad)``.
+
 One HIP runtime serves a process: import torch before the first call of this package (a library
 that was loaded before torch runs on another copy of the runtime, which cannot take torch's
 tensors; these functions then raise).
@@ -122,7 +125,8 @@ def distill_gradients(scores, top_scores, top_index, *, top_lse=None, temperatur
     ``top_index`` [rows][k] i32 are the teacher's (an index outside the classes is no entry);
     ``top_lse`` [rows] f32 its log-sum-exp at this temperature, so that the classes it did not list
     share what is left of its mass, or None: the listed classes hold all of it.  ``weight`` [rows] f32
-    scales a row's loss and gradient; 0 leaves the row out whatever it holds."""
+    scales a row's loss and gradient; 0 leaves the row out whatever it holds.  The loss carries no graph:
+    a model's scores pass the gradient on with ``scores.backward(grad)``."""
     torch = _state.get("torch") or _bind()
     t, n, m, rs, cs = _scores(torch, scores)
     if not isinstance(top_scores, torch.Tensor) or top_scores.dim() != 2:

@@ -37,6 +37,29 @@ def check_sizes_beyond_32_bits():
             assert torch.equal(a, b), k
 
 
+def check_scores_of_a_model():
+    """Scores that require a gradient: nothing is recorded, and backward(grad) gives the model's."""
+    inputs = torch.randn(50, 8, device="cuda")
+    v, i, s = cb.top_classes(torch.randn(50, 12, device="cuda"), 3, temperature=2.0)
+    weight = torch.randn(8, 12, device="cuda", requires_grad=True)
+    scores = inputs @ weight
+    loss, grad = cb.distill_gradients(scores, v, i, top_lse=s, temperature=2.0)
+    assert not loss.requires_grad and not grad.requires_grad
+    scores.backward(grad)
+    torch.testing.assert_close(weight.grad, inputs.t() @ grad, rtol=1e-5, atol=1e-5)
+    # against autograd through the formulas
+    leaf = scores.detach().double().requires_grad_()
+    lp = torch.log_softmax(leaf / 2.0, 1)
+    q = torch.exp(v.double() / 2.0 - s.double()[:, None])
+    rest = 1 - q.sum(1)
+    others = torch.logsumexp(lp.scatter(1, i.long(), float("-inf")), 1)
+    want = 4.0 * ((q * (torch.log(q) - lp.gather(1, i.long()))).sum(1) + rest * (torch.log(rest) - others))
+    want.sum().backward()
+    # (12 classes: f32 exponentials of |d| <= 20, off by 62 roundings, and the roundings of sums)
+    assert (grad - leaf.grad).abs().max().item() <= 2.0 * 100 * 2.0 ** -24
+    assert (loss - want).abs().max().item() <= 4.0 * 300 * 2.0 ** -24
+
+
 if __name__ == "__main__":
     for name, f in list(globals().items()):
         if name.startswith("check_"):
