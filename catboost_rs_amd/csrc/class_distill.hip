@@ -85,7 +85,7 @@ __device__ __forceinline__ double log_q(double ut, const RowSums& r) {
 template <class T, bool kUnit, int THREADS, int LE /* list entries a thread */, int kPhase>
 __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, float c, double it, double t,
                                                           uint32_t parts, uint32_t seg, float* __restrict__ loss,
-                                                          Grad<T> G, float2* __restrict__ part_ms) {
+                                                          Grad<T> G, PartSum* __restrict__ part_ms) {
     constexpr int V = Pack<T>::V, U = kPacks<T>, W = THREADS / 64;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
     extern __shared__ uint32_t mark[];   // a bit a class of the segment
@@ -154,15 +154,15 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
             }
         } else {
             for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
-                const float2 ms = part_ms[row * parts + p];
-                run.join(ms.x, ms.y, c);
+                const PartSum ms = part_ms[row * parts + p];
+                run.join(ms.m, ms.s, c);
             }
         }
         float mo;
         double so;
         block_running<THREADS>(run, c, mo, so, tmp_f, tmp_d);
         if (kPhase == 1) {
-            if (threadIdx.x == 0) part_ms[job] = float2{mo, (float)so};
+            if (threadIdx.x == 0) part_ms[job] = PartSum{so, mo};
             continue;
         }
         float lmax = kLowest;
@@ -363,7 +363,7 @@ int launch_rows(const Rows<T>& X, const Lists& L, float c, double t, uint32_t pa
     const uint32_t seg = segment(X.classes, parts);
     const unsigned grid = row_grid(X.rows * parts);
     const size_t lds = 4 * (size_t)((std::min(seg, X.classes) + 31) / 32);
-    float2* ms = (float2*)workspace;
+    PartSum* ms = (PartSum*)workspace;
     const double it = 1.0 / t;
     if (parts == 1) {
         distill_kernel<T, kUnit, THREADS, LE, 0><<<grid, THREADS, lds, st>>>(X, L, c, it, t, 1, seg, loss, G, ms);
@@ -409,7 +409,7 @@ int run_distill(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64
 
 extern "C" uint64_t cbh_distill_gradients_workspace(uint64_t rows, uint32_t classes) {
     const uint32_t parts = plan_parts(rows, classes);
-    return parts <= 1 ? 0 : rows * parts * 8;
+    return parts <= 1 ? 0 : rows * parts * sizeof(PartSum);
 }
 
 extern "C" int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes,

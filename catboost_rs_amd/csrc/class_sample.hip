@@ -1047,8 +1047,8 @@ __global__ __launch_bounds__(THREADS) void sample_long_kernel(Rows<T> X, Setting
 // 110 registers: 256 x 131072 f32 with settings a row took 189 to 287 us).  Between the launches, per row:
 struct Top {      // of a part: its largest score (order key) over ~(its first class); the softmax denominator; a low score
     u64 key;
-    float m, s, low;
-    uint32_t unused;
+    double s;
+    float m, low;
 };
 struct Step {     // where the cut lies
     u64 total, above;   // mass of all classes; weight of the bins before the cut's
@@ -1107,7 +1107,7 @@ __global__ __launch_bounds__(256) void scan_kernel(Rows<T> X, Settings S, int sh
     double rs = 0.0;
     if (mode == kList) block_running<THREADS>(run, c, rm, rs, tmp_f, tmp_d);
     if (threadIdx.x == 0) {
-        P.tops[row * P.parts1 + part] = Top{m == -INFINITY ? 0 : (u64)order_key(m) << 32 | (uint32_t)~first, rm, (float)rs, low, 0};
+        P.tops[row * P.parts1 + part] = Top{m == -INFINITY ? 0 : (u64)order_key(m) << 32 | (uint32_t)~first, rs, rm, low};
         if (part == 0) P.count[row] = 0;
     }
 }

@@ -476,6 +476,12 @@ struct Running {
         s += s2 * (double)exp2_fast((m2 - m) * c);
     }
 };
+// That of a part of a row, between launches: the sum stays in f64 (rounded to f32, what the other classes add to a
+// largest weight of 1 would lose up to 2^-25 a part).
+struct PartSum {
+    double s;
+    float m;
+};
 // (m, s) pairs of several threads together: the largest m, and the sums in f64.
 template <int THREADS>
 __device__ __forceinline__ void block_running(Running r, float c, float& m, double& s, float* tmp_f, double* tmp_d) {

@@ -90,7 +90,7 @@ template <class T, bool kUnit, int THREADS, int CAP>
 __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, float c, double inv_t, uint32_t parts,
                                                       uint32_t seg, float* __restrict__ values,
                                                       int32_t* __restrict__ index, float* __restrict__ lse,
-                                                      u64* __restrict__ part_keys, float2* __restrict__ part_ms) {
+                                                      u64* __restrict__ part_keys, PartSum* __restrict__ part_ms) {
     constexpr int V = Pack<T>::V, W = THREADS / 64, KMAX = CAP / 2;
     constexpr uint32_t kTile = THREADS * V * kUnroll;
     __shared__ u64 cand[W][CAP];
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
             }
         } else {
             for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = i < got ? best[i] : 0;
-            if (threadIdx.x == 0) part_ms[job] = float2{m, (float)s};
+            if (threadIdx.x == 0) part_ms[job] = PartSum{s, m};
         }
         __syncthreads();
     }
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
                                                              uint32_t parts, uint32_t seg, float* __restrict__ values,
                                                              int32_t* __restrict__ index, float* __restrict__ lse,
                                                              u64* __restrict__ part_keys,
-                                                             float2* __restrict__ part_ms) {
+                                                             PartSum* __restrict__ part_ms) {
     constexpr int V = Pack<T>::V, U = kGroup / V, W = THREADS / 64, KMAX = CAP / 2;
     extern __shared__ uint32_t groups[];
     __shared__ u64 cand[W][CAP];
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
             }
         } else {
             for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = best[i];
-            if (threadIdx.x == 0) part_ms[job] = float2{m, (float)sum};
+            if (threadIdx.x == 0) part_ms[job] = PartSum{sum, m};
         }
         __syncthreads();
     }
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
 // The segments of a row together.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ part_keys,
-                                                        const float2* __restrict__ part_ms, uint32_t parts, uint32_t k,
+                                                        const PartSum* __restrict__ part_ms, uint32_t parts, uint32_t k,
                                                         float c, double inv_t, float* __restrict__ values,
                                                         int32_t* __restrict__ index, float* __restrict__ lse) {
     __shared__ u64 best[kMaxTop];
@@ -335,8 +335,8 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
     if (threadIdx.x == 0) nbest = 0;
     Running run;
     for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
-        const float2 ms = part_ms[row * parts + p];
-        run.join(ms.x, ms.y, c);
+        const PartSum ms = part_ms[row * parts + p];
+        run.join(ms.m, ms.s, c);
     }
     float m;
     double s;
@@ -425,7 +425,7 @@ int launch_top(const Rows<T>& X, uint32_t k, double t, float* values, int32_t* i
     }
     const uint32_t seg = (n + parts - 1) / parts;
     u64* pk = (u64*)workspace;
-    float2* pm = parts > 1 ? (float2*)(pk + X.rows * parts * k) : nullptr;
+    PartSum* pm = parts > 1 ? (PartSum*)(pk + X.rows * parts * k) : nullptr;
     const unsigned grid = row_grid(X.rows * parts);
     // by groups where k is at most a quarter of the shortest segment's
     const uint32_t shortest = n - seg * (parts - 1);
@@ -465,7 +465,7 @@ int run_top(const void* scores, uint64_t rows, uint32_t classes, int64_t rs, int
 
 extern "C" uint64_t cbh_top_classes_workspace(uint64_t rows, uint32_t classes, uint32_t k) {
     const uint32_t parts = plan_parts(rows, classes);
-    return parts == 1 ? 0 : rows * parts * (8 * (uint64_t)k + 8);
+    return parts == 1 ? 0 : rows * parts * (8 * (uint64_t)k + sizeof(PartSum));
 }
 
 extern "C" int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,

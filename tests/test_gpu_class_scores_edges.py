@@ -245,3 +245,29 @@ def test_torch_tensors_at_their_ends():
     print(r.stdout)
     assert r.returncode == 0, r.stdout[-3000:]
     assert r.stdout.rstrip().endswith("all checks passed")
+
+
+def small_beside_one(n, t):
+    """A row of one 0, the 4095 classes beside it (a thread adds up the scores of a tile in f32) -inf and the others
+    -30, at the temperature where a unit is a factor of 2: every f32 exponential is a power of two, and the sum is
+    1 + 2^-30 (n - 4096) without rounding in any thread."""
+    x = np.full((1, n), -30.0, np.float32)
+    x[0, :4096] = -np.inf
+    x[0, 0] = 0.0
+    return x, np.log1p((n - 4096) * 2.0 ** -30)
+
+
+@pytest.mark.parametrize("n", [70001, 300000])
+def test_sums_of_parts_keep_their_bits(n):
+    """What is little beside 1 in a part of a row still counts: the log-sum-exp, and the log probability of a drawn
+    class, are right to a rounding."""
+    t = 1.0 / np.log(2.0)
+    x, lse = small_beside_one(n, t)
+    _, _, s = run_top(x, 3, t, "f32", "rows")
+    assert abs(s[0] - lse) <= lse * 2.0 ** -23, (s[0], lse)
+    for k in (5, 1000):
+        index, lp = run_sample(x, np.zeros(1), t=t, k=k)
+        assert index[0] == 0 and abs(lp[0] + lse) <= lse * 2.0 ** -23, (k, lp[0], lse)
+    # the teacher is sure of class 0: the loss is -log p of it
+    loss, _ = run_distill(x, np.zeros((1, 1)), np.zeros((1, 1), np.int32), None, t, None, "f32", "rows")
+    assert abs(loss[0] - t * t * lse) <= t * t * lse * 2.0 ** -23, (loss[0], t * t * lse)
