@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 from tests import class_scores_oracle as O
-from tests.test_gpu_class_scores import check_top, run_distill, run_sample, run_top
+from tests.test_gpu_class_scores import check_sample, check_top, reach, run_distill, run_sample, run_top, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -271,3 +271,66 @@ def test_sums_of_parts_keep_their_bits(n):
     # the teacher is sure of class 0: the loss is -log p of it
     loss, _ = run_distill(x, np.zeros((1, 1)), np.zeros((1, 1), np.int32), None, t, None, "f32", "rows")
     assert abs(loss[0] - t * t * lse) <= t * t * lse * 2.0 ** -23, (loss[0], t * t * lse)
+
+
+# ---- routes --------------------------------------------------------------------------------------
+
+def check_tiled(got, want, rows, what):
+    """Rows repeat with the period of `want`."""
+    for r in range(rows):
+        assert np.array_equal(got[r], want[r % len(want)], equal_nan=True), (what, r)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,n,k", [(512, 40000, 20), (512, 40000, 256), (520, 130001, 1000), (2, 35002, 130)])
+def test_top_long_rows_by_groups(rows, n, k, kind):
+    """Rows of many classes that a workgroup takes whole (512 of them and more), for short and long lists, and parts
+    of rows with lists beyond 128."""
+    g = np.random.default_rng(n + k)
+    few = np.concatenate([O.scores(g, 1, n, v) for v in ("normal", "ties", "rising", "normal")])
+    few[3, [5, n // 2]] = np.nan, np.inf
+    few = O.round_to(few, kind)
+    ev, ei, es = O.top(few, k, 1.5)
+    x = few[np.arange(rows) % 4]
+    v, i, s = run_top(x, k, 1.5, kind, "rows")
+    check_tiled(i, ei.astype(np.int32), rows, "index")
+    check_tiled(v, ev.astype(np.float32), rows, "values")
+    for r in range(rows):
+        if r % 4 == 3:
+            assert np.isnan(s[r])
+        else:
+            assert abs(s[r] - es[r % 4]) <= (n / 64 + 16 + reach(few[:3], 1.5)) * 2.0 ** -23 + abs(es[r % 4]) * 2.0 ** -24, r
+
+
+@pytest.mark.parametrize("kind,n", [("f32", 70001), ("bf16", 140003)])
+@pytest.mark.parametrize("rows,k", [(512, 20), (512, 700), (3, 700)])
+def test_distill_wide_rows(rows, k, kind, n):
+    """Rows of 256 KB and more: whole (512 rows) and in parts, with lists of one and of two entries a thread."""
+    g = np.random.default_rng(n + k)
+    few = O.scores(g, 3, n, "normal")
+    u, ix, lse = teacher(g, few, k, 1.0)
+    at = np.arange(rows) % 3
+    for base in (lse, None):
+        b = None if base is None else base[at]
+        loss, grad = run_distill(few[at], u[at], ix[at], b, 1.0, None, kind, "rows")
+        for r in range(3, rows):
+            assert loss[r] == loss[r % 3] and np.array_equal(grad[r], grad[r % 3]), r
+        el, eg, size, far = distill_in_logs(O.round_to(few, kind), u, ix, base, 1.0, 1.0)
+        rel = (n / 512 + 36 + 4 * 110) * 2.0 ** -24
+        assert (np.abs(loss[:3] - el) <= 3 * rel + np.abs(el) * 2.0 ** -23).all(), (loss[:3], el)
+        bar = size * 2 * rel + np.abs(eg) * O.half_step(kind) + O.smallest(kind) * 2
+        assert (np.abs(grad[:3] - eg) <= bar).all()
+
+
+def test_rows_of_the_most_classes():
+    """2^24 classes, the most that are taken."""
+    g = np.random.default_rng(24)
+    n = 1 << 24
+    x = g.standard_normal((1, n)).astype(np.float32)
+    v, i, s = run_top(x, 40, 1.0, "f32", "rows")
+    by = np.argsort(-x[0], kind="stable")[:40]
+    assert np.array_equal(i[0], by) and np.array_equal(v[0], x[0][by])
+    # exponentials of d, |d| <= 12 (off by 3 |d| 2^-24 + 2^-23), f32 additions of 32 of them, and a rounding
+    assert abs(s[0] - O.log_sum_exp(x.astype(np.float64))[0]) <= (3 * 12 + 2 + 10 + s[0]) * 2.0 ** -24
+    for how in (dict(p=0.9), dict(k=50)):
+        check_sample(x, g.random(1), tag=how, **how)
