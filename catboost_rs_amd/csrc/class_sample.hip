@@ -382,9 +382,10 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(Rows<T> X, Settin
 // bins above a nucleus's last are summed by segments, and the draw looks through one of them.
 constexpr uint32_t kGroupSegs = 128, kMostByGroups = 1024, kListCap = 8192, kShortList = 128;
 constexpr uint32_t kBins = 1024, kBinsPad = kBins + kBins / 16;
-// The bins reach from the largest score to a little below the lowest of a sample (the first score of every group),
-// 32 nats at most: 32 bins a nat, and more of them for the rows of a narrow range, whose nucleus is wide: one bin
-// then holds hundreds of classes and not thousands, which the list has to take.
+// The bins reach from the largest score to a little below the lowest of a sample (the first class of every lane's
+// tile, 64 of 2048), 32 nats at most and where the sample holds no class (all of them masked): 32 bins a nat, and more of
+// them for the rows of a narrow range, whose nucleus is wide: one bin then holds hundreds of classes and not
+// thousands, which the list has to take.
 constexpr float kMostNats = 32.0f;
 __device__ __forceinline__ uint32_t bin_at(uint32_t b) { return b + (b >> 4); }   // (its place in LDS)
 
@@ -521,7 +522,7 @@ struct Long {
     float bm, bscale;
     __device__ __forceinline__ void set_bins(float m, float low) {
         bm = m;
-        const float range = fminf((m - low) * (float)r.rt * 1.25f + 1.0f, kMostNats);   // (NaN: the most)
+        const float range = low < INFINITY ? fminf((m - low) * (float)r.rt * 1.25f + 1.0f, kMostNats) : kMostNats;
         bscale = (float)(r.rt * (double)((float)kBins / range));
     }
     __device__ __forceinline__ uint32_t bin(float x) const {

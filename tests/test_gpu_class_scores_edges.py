@@ -334,3 +334,19 @@ def test_rows_of_the_most_classes():
     assert abs(s[0] - O.log_sum_exp(x.astype(np.float64))[0]) <= (3 * 12 + 2 + 10 + s[0]) * 2.0 ** -24
     for how in (dict(p=0.9), dict(k=50)):
         check_sample(x, g.random(1), tag=how, **how)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(6, 5003), (4, 70001)])
+def test_sample_masks_that_bar_the_sampled_classes(rows, n, kind):
+    """The bins' range is taken from a lane's first class of every tile: a list of allowed classes without any of
+    those (or with one alone) draws as any other."""
+    g = np.random.default_rng(n + 2)
+    each = 4 if kind == "f32" else 8
+    j = np.arange(n)
+    for one in (False, True):
+        allowed = np.broadcast_to((j % 2048 >= 64 * each) | (j % each != 0) | (one & (j == 2048)), (rows, n))
+        for values in ("normal", "ties", "masked"):
+            x = O.scores(g, rows, n, values)
+            for how in (dict(p=0.9), dict(k=2000), dict(k=n // 3, p=0.5), dict(t=3.0, p=0.99, min_p=0.01)):
+                check_sample(x, g.random(rows), allowed=allowed, kind=kind, tag=(one, values, how), **how)
