@@ -76,10 +76,25 @@ struct Candidates {
     }
 };
 
-// A row's log-sum-exp from its (m, s), once its largest score `top` is known: a NaN ranks first, and only then is a
-// NaN in s more than the +inf - +inf of a row with +inf.
-__device__ __forceinline__ float row_lse(float m, double s, float top, double inv_t) {
-    return m == INFINITY && top == top ? INFINITY : (float)((double)m * inv_t + log(s));
+// A row's log-sum-exp from its (m, s).  A row of +inf has NaN in s (+inf - +inf), as one of NaN; which it is is known when the
+// row's largest are ranked: a NaN is among them, and its thread then writes NaN in place of +inf.  (The
+// log-sum-exp is written first and its registers are free from there: written last, by the thread that knows the
+// largest, it took top_groups_kernel to 97 registers and a wave a SIMD less, 167 against 155 us.)
+__device__ __forceinline__ float row_lse(float m, double s, double inv_t) {
+    return m == INFINITY ? INFINITY : (float)((double)m * inv_t + log(s));
+}
+// The `got` keys of best, the largest first, and NaN to lse if there is one.
+template <int THREADS>
+__device__ __forceinline__ void write_ranked(const u64* best, uint32_t got, float* values, int32_t* index, float* lse) {
+    for (uint32_t i = threadIdx.x; i < got; i += THREADS) {
+        const u64 key = best[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < got; ++j) rank += best[j] > key;
+        const float x = key_score((uint32_t)(key >> 32));
+        values[rank] = x;
+        index[rank] = (int32_t)~(uint32_t)key;
+        if (x != x) *lse = x;
+    }
 }
 
 // Short rows, and a k that is large beside the row: candidates are taken in the pass itself (4 x 1000 f32, k 5:
@@ -181,6 +196,10 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
         double s;
         __syncthreads();
         block_running<THREADS>(run, c, m, s, tmp_f, tmp_d);
+        if (threadIdx.x == 0) {
+            if (parts == 1) lse[row] = row_lse(m, s, inv_t);
+            else part_ms[job] = PartSum{s, m};
+        }
         uint32_t total = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) total += counts[w];
@@ -192,20 +211,10 @@ __global__ __launch_bounds__(THREADS) void top_kernel(Rows<T> X, uint32_t k, flo
         }
         __syncthreads();
         const uint32_t got = nbest;   // k, or all of a segment of fewer
-        if (parts == 1) {
-            for (uint32_t i = threadIdx.x; i < got; i += THREADS) {
-                const u64 key = best[i];
-                uint32_t rank = 0;
-                for (uint32_t j = 0; j < got; ++j) rank += best[j] > key;
-                const float x = key_score((uint32_t)(key >> 32));
-                values[row * k + rank] = x;
-                index[row * k + rank] = (int32_t)~(uint32_t)key;
-                if (rank == 0) lse[row] = row_lse(m, s, x, inv_t);
-            }
-        } else {
+        if (parts == 1)
+            write_ranked<THREADS>(best, got, values + row * k, index + row * k, lse + row);
+        else
             for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = i < got ? best[i] : 0;
-            if (threadIdx.x == 0) part_ms[job] = PartSum{s, m};
-        }
         __syncthreads();
     }
 }
@@ -291,6 +300,10 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
         double sum;
         __syncthreads();
         block_running<THREADS>(run, c, m, sum, tmp_f, tmp_d);
+        if (threadIdx.x == 0) {
+            if (parts == 1) lse[row] = row_lse(m, sum, inv_t);
+            else part_ms[job] = PartSum{sum, m};
+        }
         uint32_t total = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) total += counts[w];
@@ -301,20 +314,10 @@ __global__ __launch_bounds__(THREADS) void top_groups_kernel(Rows<T> X, uint32_t
             if (key >= kth) best[atomicAdd(&nbest, 1u)] = key;
         }
         __syncthreads();
-        if (parts == 1) {
-            for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
-                const u64 key = best[i];
-                uint32_t rank = 0;
-                for (uint32_t j = 0; j < k; ++j) rank += best[j] > key;
-                const float x = key_score((uint32_t)(key >> 32));
-                values[row * k + rank] = x;
-                index[row * k + rank] = (int32_t)~(uint32_t)key;
-                if (rank == 0) lse[row] = row_lse(m, sum, x, inv_t);
-            }
-        } else {
+        if (parts == 1)
+            write_ranked<THREADS>(best, k, values + row * k, index + row * k, lse + row);
+        else
             for (uint32_t i = threadIdx.x; i < k; i += THREADS) part_keys[job * k + i] = best[i];
-            if (threadIdx.x == 0) part_ms[job] = PartSum{sum, m};
-        }
         __syncthreads();
     }
 }
@@ -342,21 +345,14 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
     double s;
     __syncthreads();
     block_running<THREADS>(run, c, m, s, tmp_f, tmp_d);
+    if (threadIdx.x == 0) lse[row] = row_lse(m, s, inv_t);
     const u64 kth = kth_of<THREADS>([&](uint32_t i) { return keys[i]; }, parts * k, k, &lds);
     for (uint32_t i = threadIdx.x; i < parts * k; i += THREADS) {
         const u64 key = keys[i];
         if (key != 0 && key >= kth) best[atomicAdd(&nbest, 1u)] = key;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
-        const u64 key = best[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < k; ++j) rank += best[j] > key;
-        const float x = key_score((uint32_t)(key >> 32));
-        values[row * k + rank] = x;
-        index[row * k + rank] = (int32_t)~(uint32_t)key;
-        if (rank == 0) lse[row] = row_lse(m, s, x, inv_t);
-    }
+    write_ranked<THREADS>(best, k, values + row * k, index + row * k, lse + row);
 }
 
 // Few classes: a row a thread, its scores in registers; a score's place is the count of those ahead.
@@ -378,25 +374,27 @@ __global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, flo
             run.m = fmaxf(run.m, x[i]);
         }
 #pragma unroll
-        for (int i = 0; i < NMAX; ++i) {
-            run.add_one(x[i], c);
+        for (int i = 0; i < NMAX; ++i) run.add_one(x[i], c);
+        float z = row_lse(run.m, run.s, inv_t);
+        if (run.m == INFINITY) {   // (beside a NaN: it)
+#pragma unroll
+            for (int i = 0; i < NMAX; ++i) z = x[i] != x[i] ? x[i] : z;
+        }
+        lse[row] = z;
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i)
 #pragma unroll
             for (int j = 0; j < i; ++j) {
                 const bool ahead = key[j] >= key[i];
                 rank[i] += ahead;
                 rank[j] += !ahead;
             }
-        }
-        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NMAX; ++i) {
+        for (int i = 0; i < NMAX; ++i)
             if ((uint32_t)i < n && rank[i] < k) {
                 values[row * k + rank[i]] = key_score(key[i]);
                 index[row * k + rank[i]] = i;
             }
-            top = rank[i] == 0 ? key_score(key[i]) : top;
-        }
-        lse[row] = row_lse(run.m, run.s, top, inv_t);
     }
 }
 
