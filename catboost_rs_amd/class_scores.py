@@ -4,7 +4,8 @@ classes drawn from given random numbers.
 
 They take torch tensors on the GPU and enqueue on torch's current stream; what they return
 is made by torch on that stream.  Scores are [rows][classes], f32, f16 or bf16, of any
-strides: the [classes][rows] scores of a trained model go in as ``scores.t()``.
+strides.  A trained model's scores ([classes][rows] f64 on the host, from ``Trainer.approx`` or
+``apply_oblivious``) go in as f32 on the GPU: ``torch.from_numpy(raw).float().cuda().t()``.
 
 They record no autograd graph, also where the scores require a gradient: a loss is a value to look at, and the
 gradient goes on with ``scores.backward(grad)``.

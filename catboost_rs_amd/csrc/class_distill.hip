@@ -232,7 +232,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(Rows<T> X, Lists L, fl
 }
 
 // Few classes: a row a thread, its scores in registers, the listed classes a bit mask.  1M x 10 f32, k 3, class-major:
-// 41 us, 112 MB at 2.8 TB/s; bound by the f64 exponentials and logarithms of the lists, and their loads.
+// 39 us, 112 MB at 2.9 TB/s; bound by the f64 exponentials and logarithms of the lists, their loads, and scalar registers
+// that do not fit (108 put aside at 12 classes and 4 entries, 286 at 32).
 // Lists of up to KM entries are held in registers as well (KM 0: read again in every step; k 3 that way 59 us).
 template <class T, int NMAX, int KM>
 __global__ __launch_bounds__(256) void distill_few_kernel(Rows<T> X, Lists L, float c, double it, double t,

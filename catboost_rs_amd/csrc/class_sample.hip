@@ -193,8 +193,10 @@ struct Entries {
 // Scores and masses in registers.  A nucleus needs the mass ahead of every class: the pairs of classes, in
 // f64 (with S = 46 and at most 32 classes every sum is an integer below 2^53 and exact), each pair a
 // comparison and two multiply-adds with 0 or 1.
-// 1M x 10 f32, top_p 0.9, class-major: 37 us, 64 MB at 1.7 TB/s; bound by f64 instructions (the masses, and
-// the pairs of 10 places; 46 us with 12).  A wave a row took 3.2 ms.
+// 1M x 10 f32, top_p 0.9, class-major: 35 us, 56 MB at 1.6 TB/s; bound by f64 instructions (the masses, and
+// the pairs of 10 places; 46 us with 12) and by scalar registers that do not fit: the pairs' comparisons are masks in
+// pairs of them, and each that the compiler puts aside costs vector instructions (119 at 10 places, 1133 at 32:
+// 500k x 32 271 us).  A wave a row took 3.2 ms.
 constexpr int kFewShift = 46;
 template <class T, int NMAX>
 __global__ __launch_bounds__(256) void sample_few_kernel(Rows<T> X, Settings S, Out out) {
@@ -458,7 +460,9 @@ struct Long {
 
     // Largest score of the segments [s0, s1) and the segment it was first met in, per thread; into `groups`
     // (nullable) every group's largest as an order key (0: nothing to draw); with `sums` the running softmax
-    // denominator.
+    // denominator: what a top_k row's log probability takes of the classes that are cut.  Its exponentials are f32 (off by
+    // 3 |d| 2^-24 + 2^-23, d = (x - max) / t, the sum f64): the pass stays bound by memory with them, at 24 us for 256 x
+    // 131072 f32, where f64 masses, which need the maximum first, take a pass of 27 to 34 us more.
     __device__ __forceinline__ void scan(uint32_t s0, uint32_t s1, uint32_t* groups, bool sums, float c,
                                          float& best, uint32_t& best_seg, float& low, Running& run) const {
         best = -INFINITY;
@@ -817,8 +821,11 @@ struct Long {
             }
         }
     }
-    // Any row, by selection over the whole of it: rows of +inf or of far temperatures (whole_row()), and those whose
-    // cut lies among more classes than a list holds (equal scores).
+    // Any row, by selection over the whole of it, read again for every digit: rows of +inf or of far temperatures
+    // (whole_row()), and those whose cut needs more classes than a list holds: a nucleus that ends among so many of
+    // one bin (equal scores, or few of the bins' sample allowed), a top_k and what shares its last bin beyond 8192 (2048 in
+    // rows of 2049 to 8192 classes).  256 x 131072 f32: top_k 5000 126 us, 8000 138, 9000 700, 100000 706; 256 x 6000: top_k
+    // 2000 28 us, 2100 84.
     __device__ void slow(uint32_t top_key, uint32_t first, uint64_t row, SelectLds* lds, u64* tmp, u64* pick, const Out& out) const {
         const float m = key_score(top_key);
         const bool inf = m == INFINITY;

@@ -355,7 +355,9 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(const u64* __restrict__ 
     write_ranked<THREADS>(best, k, values + row * k, index + row * k, lse + row);
 }
 
-// Few classes: a row a thread, its scores in registers; a score's place is the count of those ahead.
+// Few classes: a row a thread, its scores in registers; a score's place is the count of those ahead.  1M x 10 f32, k 3: 35 us
+// class-major, 36 by rows, 68 MB at 1.9 TB/s; 500k x 32, k 5: 67 and 77 us.  Bound by the comparisons of all pairs, whose masks
+// do not fit the scalar registers (116 put aside at 16 places, 696 at 32), and by stores to scattered places.
 template <class T, int NMAX>
 __global__ __launch_bounds__(256) void top_few_kernel(Rows<T> X, uint32_t k, float c, double inv_t,
                                                       float* __restrict__ values, int32_t* __restrict__ index,

@@ -473,13 +473,13 @@ int cbh_ctr_columns(const uint32_t* buckets, uint32_t n_buckets, uint64_t n, con
 
 /* ---- class scores: top classes, distillation, drawn classes (no counterpart in the reference) ----
  *
- * Operators on a matrix of class scores (the raw approximant of a MultiClass model, or any other
- * classifier's logits).  All pointers are DEVICE pointers; the work is enqueued on `stream` (a
- * hipStream_t, NULL = the default stream) and not waited for; nothing is allocated, so the calls may be
- * captured into a graph.
+ * Operators on a matrix of class scores in device memory (a MultiClass model's, converted from the f64 that
+ * cbh_session_read_approx and cbh_apply_oblivious write to the host, or any other classifier's logits).  All
+ * pointers are DEVICE pointers; the work is enqueued on `stream` (a hipStream_t, NULL = the default stream) and not
+ * waited for; nothing is allocated, so the calls may be captured into a graph.
  *   scores         score of row r, class j at scores[r * row_stride + j * class_stride], of `type`; strides
  *                  in elements (class_stride 1: a row's classes next to each other; row_stride 1: the
- *                  [classes][rows] layout of cbh_session_read_approx and cbh_apply_oblivious)
+ *                  [classes][rows] order in which a model's scores are read)
  *   rows, classes  0 <= rows < 2^31 (no rows: nothing is done), 1 <= classes <= 2^24
  *   workspace      device memory of at least cbh_*_workspace() bytes, aligned to 8; its content is not
  *                  kept.  NULL where that is 0.
@@ -511,8 +511,8 @@ int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t cl
  *   loss           nullable [rows] f32; grad nullable, with strides of its own (not both null); neither may
  *                  overlap an input
  * A teacher's entry of -inf has q = 0, all of a row's too (with a top_lse of -inf the others then hold all mass).
- * A student's row of -inf alone has p = 0 everywhere and an
- * infinite loss; NaN or +inf in a student's row makes that row's loss and gradient NaN. */
+ * A student's row of -inf alone has p = 0 everywhere and an infinite loss (so has one whose unlisted classes are all
+ * -inf where rest > 0; at a finite value, however low, the loss is finite); NaN or +inf in a student's row makes that row's loss and gradient NaN. */
 uint64_t cbh_distill_gradients_workspace(uint64_t rows, uint32_t classes);
 int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
                           int64_t class_stride, const float* top_scores, const int32_t* top_index, uint32_t k,
@@ -531,7 +531,8 @@ int cbh_distill_gradients(const void* scores, int32_t type, uint64_t rows, uint3
  * temperature <= 0 the first class is drawn, with logprob 0.  A row that allows no class has index -1 and
  * logprob -inf.
  * Masses are integers in units of 2^-S of the row's largest weight (S = 46 up to 32 classes, 51 up to 2^11,
- * 62 - b up to 2^b), so that sums are exact and the same for every launch shape.
+ * 62 - b up to 2^b), so that sums are exact and the same for every launch shape; in rows of more than 2048 classes
+ * with top_k, log sum w is of f32 exponentials added up in f64.
  *   uniform        [rows] f64 in [0, 1)
  *   temperature, top_k, top_p, min_p   values for every row; *_rows: nullable [rows], used in their place.  Any
  *                  positive temperature is taken, infinity too (a row beyond [1e-30, 1e36] of more than 2048 classes
