@@ -490,7 +490,8 @@ enum { CBH_TYPE_F32 = 0, CBH_TYPE_F16 = 1, CBH_TYPE_BF16 = 2 };
  * log-sum-exp of scores / temperature (1e-38 <= temperature <= 1e36):
  *   values [rows][k] f32, index [rows][k], lse [rows] f32;  1 <= k <= min(classes, 1024)
  * -0 and +0 are equal (and come back as 0); NaN counts as larger than +inf and makes the row's lse NaN; a
- * row of -inf alone has lse = -inf. */
+ * row of -inf alone has lse = -inf, and lse is infinite where its value leaves f32 (scores near the ends of f32 at a
+ * temperature below 1). */
 uint64_t cbh_top_classes_workspace(uint64_t rows, uint32_t classes, uint32_t k);
 int cbh_top_classes(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
                     int64_t class_stride, uint32_t k, double temperature, float* values, int32_t* index,
