@@ -72,9 +72,10 @@ def draw(rng):
             return dict(case, k=rng.choice([0, 1, min(classes, _log(rng, 1, 256))]))
         return dict(case, entropy=rng.random() < 0.5)
     if kind == "adamw":
-        tensors, values = _log(rng, 1, 200), _log(rng, 1000, 60_000_000)
+        state = rng.choice(["f32", "f8"])
+        tensors, values = _log(rng, 1, 150 if state == "f32" else 24), _log(rng, 1000, 38_000_000)
         return dict(kind=kind, tensors=tensors, values=max(values, tensors), type=rng.choice(["f32", "f32", "bf16", "f16"]),
-                    grad=rng.choice(kinds), state=rng.choice(["f32", "f8"]), flags=rng.random() < 0.4)
+                    grad=rng.choice(kinds), state=state, flags=rng.random() < 0.4)
     entries, dim = _log(rng, 16, 300_000), _log(rng, 1, 1024)
     many = 1 if rng.random() < 0.6 else _log(rng, 2, 100)
     entries = min(entries, 30_000_000 // dim)
@@ -222,34 +223,37 @@ def _masked(s):
 
 
 def _statistics(s):
-    """The distances d of a row's scores from the largest, and its statistics [m, log Z, E]."""
+    """The distances d of a row's scores from the largest, and its statistics [m, log Z, E]: -inf, -inf and 0 of a
+    row that allows nothing."""
     x = _masked(s)
     m = x.amax(1, keepdim=True)
-    d = (x - m) / s["temperature"]
+    d = (x - torch.where(m > float("-inf"), m, 0.0)) / s["temperature"]
     e = torch.exp(d)
     z = e.sum(1, keepdim=True)
-    far = -torch.where(e > 0, e * d, 0.0).sum(1, keepdim=True) / z
-    return d, torch.cat([m, torch.log(z), far], 1)
+    far = torch.where(e > 0, e * d, 0.0).sum(1, keepdim=True)
+    return d, torch.cat([m, torch.log(z), torch.where(z > 0, -far / z, 0.0)], 1)
 
 
 def _plain_logprobs(s):
     d, stats = _statistics(s)
     given = s["given"].long()
     some = (given >= 0) & (given < s["classes"])
-    logprob = torch.where(some, d.gather(1, torch.where(some, given, 0)) - stats[:, 1:2], 0.0)
-    out = {"logprob": logprob, "entropy": stats[:, 1] + stats[:, 2], "stats": stats}
+    log_z = torch.where(stats[:, 1:2] > float("-inf"), stats[:, 1:2], 0.0)   # (a row that allows nothing: d is -inf)
+    logprob = torch.where(some, d.gather(1, torch.where(some, given, 0)) - log_z, 0.0)
+    out = {"logprob": logprob, "entropy": log_z[:, 0] + stats[:, 2], "stats": stats}
     if s["k"]:
         values, index = torch.sort(d, dim=1, descending=True, stable=True)   # ties: the lowest class first
         values, index = values[:, :s["k"]], index[:, :s["k"]]
-        out["top_logprob"] = values - stats[:, 1:2]
+        out["top_logprob"] = values - log_z
         out["top_index"] = torch.where(values > float("-inf"), index, -1).int()
     return out
 
 
 def _plain_gradients(s):
     m, log_z, far = s["stats"][:, :, None].unbind(1)
-    d = (_masked(s) - m) / s["temperature"]
-    p = torch.exp(d - log_z)
+    some = m > float("-inf")   # (a row that allows nothing)
+    d = (_masked(s) - torch.where(some, m, 0.0)) / s["temperature"]
+    p = torch.exp(d - torch.where(some, log_z, 0.0))
     given = s["given"].long()
     some = (given >= 0) & (given < s["classes"])
     g = torch.where(some, s["logprob_grad"], 0.0)
@@ -426,7 +430,7 @@ def _exact_scores(s, a, b):
     if free is not None:
         z = z.masked_fill(~free, float("-inf"))
     lse = torch.logsumexp(z, 1, keepdim=True)
-    logp = z - lse
+    logp = torch.where(lse > float("-inf"), z - lse, float("-inf"))   # (a row that allows nothing)
     p = torch.exp(logp)
     entropy = -torch.nan_to_num(p * logp, nan=0.0).sum(1, keepdim=True)
     given = s["given"][a:b].long()
@@ -434,8 +438,9 @@ def _exact_scores(s, a, b):
     at = torch.where(some, given, 0)
     if s["kind"] == "logprobs":
         best = z.amax(1, keepdim=True)
+        log_z = torch.where(best > float("-inf"), lse - best, best)
         out = {"logprob": torch.where(some, logp.gather(1, at), 0.0), "entropy": entropy[:, 0],
-               "stats": torch.cat([best * s["temperature"], lse - best, entropy - (lse - best)], 1)}
+               "stats": torch.cat([best * s["temperature"], log_z, torch.where(log_z > float("-inf"), entropy - log_z, 0.0)], 1)}
         if s["k"]:
             out["top_logprob"], out["top_index"] = torch.topk(logp, s["k"], dim=1).values, None
         return out
