@@ -11,7 +11,9 @@ thin ctypes front-end used by the tests and ``bench.py``:
   (crates/cb-train/src/boosting.rs:6532-7300) through ``cbt_*``.
 
 The operators on class scores (:func:`top_classes`, :func:`distill_gradients`,
-:func:`sample_classes`) take torch tensors on the GPU.
+:func:`sample_classes`, :func:`class_logprobs`, :func:`logprob_gradients`) and what trains a student
+beside a boosted model (:func:`lookup_rows`, :func:`lookup_gradients`, :class:`AdamW`) take torch
+tensors on the GPU.
 
 There is no CPU fallback: if the library is missing or no GPU is present, calls raise.
 """
@@ -133,7 +135,9 @@ EXPORTS = ["cbh_session_begin", "cbh_session_begin_u8", "cbh_session_grow",
            "cbt_open_ctr", "cbh_hist_build_noalloc", "cbh_session_capture_hists", "cbh_session_level_hist",
            "cbh_columns_from_rows", "cbh_session_fill_tile", "cbt_fill_tile", "cbh_top_classes",
            "cbh_top_classes_workspace", "cbh_distill_gradients", "cbh_distill_gradients_workspace",
-           "cbh_sample_classes", "cbh_sample_classes_workspace"]
+           "cbh_sample_classes", "cbh_sample_classes_workspace", "cbh_class_logprobs",
+           "cbh_class_logprobs_workspace", "cbh_logprob_gradients", "cbh_lookup_rows", "cbh_lookup_gradients",
+           "cbh_lookup_gradients_workspace", "cbh_adamw_step"]
 
 _lib = None
 
@@ -205,6 +209,14 @@ def load(path: str = LIB_PATH):
     L.cbh_distill_gradients_workspace.argtypes = L.cbh_sample_classes_workspace.argtypes = [U64, U32]
     for fn in (L.cbh_top_classes_workspace, L.cbh_distill_gradients_workspace, L.cbh_sample_classes_workspace):
         fn.restype = U64
+    L.cbh_class_logprobs.argtypes = scores + [P, U32, F64, P, I64, U32, P, P, P, P, P, P, U64, P]
+    L.cbh_class_logprobs_workspace.argtypes = [U64, U32, U32]
+    L.cbh_logprob_gradients.argtypes = scores + [P, U32, P, P, P, F64, P, I64, P, I64, I64, P]
+    L.cbh_lookup_rows.argtypes = [P, I32, U32, U32, I64, I64, P, U64, U32, F64, P, P]
+    L.cbh_lookup_gradients.argtypes = [P, I32, U64, U32, I64, I64, P, U32, U32, F64, P, I32, P, U64, P]
+    L.cbh_lookup_gradients_workspace.argtypes = [U64, U32, U32, U32]
+    L.cbh_class_logprobs_workspace.restype = L.cbh_lookup_gradients_workspace.restype = U64
+    L.cbh_adamw_step.argtypes = [P, U32, P, P]
     L.cbt_close.argtypes = [P]
     L.cbt_close.restype = None
     _lib = L
@@ -221,7 +233,11 @@ def _ptr(a):
 
 
 # operators on class scores that live on the GPU (torch tensors; torch is imported at the first call)
-from .class_scores import distill_gradients, sample_classes, top_classes  # noqa: E402
+from .class_scores import (class_logprobs, distill_gradients, logprob_gradients, sample_classes,  # noqa: E402
+                           top_classes)
+# and what trains a student on them
+from .adamw import AdamW  # noqa: E402
+from .lookup import lookup_gradients, lookup_rows  # noqa: E402
 
 # ---------------------------------------------------------------------------------------
 # kernel-level entry points

@@ -1,0 +1,151 @@
+"""AdamW steps over many tensors on the GPU at once, with states in 32 or 8 bits: the update of a student that
+:func:`distill_gradients`, :func:`logprob_gradients` and :func:`lookup_gradients` give gradients for."""
+from __future__ import annotations
+
+import ctypes as C
+
+from .class_scores import _TYPE, _bind, _on, _state, _stream
+
+BLOCK = 256   # values of an 8-bit state that share a scale
+
+
+class _Tensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p), ("copy", C.c_void_p), ("n", C.c_uint64),
+                ("param_type", C.c_int32), ("grad_type", C.c_int32), ("copy_type", C.c_int32), ("number", C.c_uint32)]
+
+
+class _Settings(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("step", C.c_int64), ("step_device", C.c_void_p), ("lr_device", C.c_void_p),
+                ("grad_scale", C.c_void_p), ("skip", C.c_void_p), ("seed", C.c_uint32), ("state", C.c_int32)]
+
+
+class AdamW:
+    """Weights ``params`` (torch tensors f32, f16 or bf16 on one GPU, contiguous) with the states that AdamW keeps of
+    them; :meth:`step` takes their gradients and updates weights and states in place (``cbh_adamw_step``: the formulas are
+    there).
+
+    ``state``: ``"f32"`` (``exp_avg`` and ``exp_avg_sq``, f32 of the weights' shapes) or ``"f8"`` (float8_e4m3fn codes
+    of the first moment and of the square root of the second, with the scales ``exp_avg_scale`` and
+    ``exp_avg_sq_scale`` f32 of every 256 values; rounded by random bits of ``seed`` and the step).  States of an
+    earlier run are given by those names, as lists of tensors, and kept, not copied; with ``steps``, the number of steps
+    that they are after.  ``copies``: a list of tensors (or None) that get the new weights rounded to their type: 16-bit
+    weights beside f32 ones.
+
+    ``steps`` is a number, or an i64 tensor of one value on the GPU: then every step adds 1 to it on the stream (not
+    where ``skip`` holds a step back), and a step may be captured into a graph.
+    """
+
+    def __init__(self, params, *, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state="f32", exp_avg=None,
+                 exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None, copies=None, steps=0, seed=0):
+        torch = _state.get("torch") or _bind()
+        self.params = list(params)
+        if state not in ("f32", "f8"):
+            raise ValueError("state must be 'f32' or 'f8'")
+        for p in self.params:
+            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.device != self.params[0].device:
+                raise ValueError("params must be torch tensors on one GPU")
+            if p.dtype not in _TYPE:
+                raise ValueError(f"params must be float32, float16 or bfloat16, not {p.dtype}")
+            if not p.is_contiguous():
+                raise ValueError("params must be contiguous")
+        self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
+        self.state, self.steps, self.seed = state, steps, int(seed) & 0xFFFFFFFF
+        small = state == "f8"
+        kind = torch.float8_e4m3fn if small else torch.float32
+        self.exp_avg = self._states(torch, exp_avg, kind, None, "exp_avg")
+        self.exp_avg_sq = self._states(torch, exp_avg_sq, kind, None, "exp_avg_sq")
+        blocks = [((p.numel() + BLOCK - 1) // BLOCK,) for p in self.params]
+        self.exp_avg_scale = self._states(torch, exp_avg_scale, torch.float32, blocks, "exp_avg_scale") if small else None
+        self.exp_avg_sq_scale = self._states(torch, exp_avg_sq_scale, torch.float32, blocks, "exp_avg_sq_scale") if small else None
+        if not small and (exp_avg_scale is not None or exp_avg_sq_scale is not None):
+            raise ValueError("states in f32 have no scales")
+        self.copies = [None] * len(self.params) if copies is None else list(copies)
+        if len(self.copies) != len(self.params):
+            raise ValueError("copies must be a tensor or None for every weight")
+        for c, p in zip(self.copies, self.params):
+            if c is not None and (not isinstance(c, torch.Tensor) or c.dtype not in _TYPE or c.shape != p.shape
+                                  or c.device != p.device or not c.is_contiguous()):
+                raise ValueError("a copy must be a contiguous float32, float16 or bfloat16 tensor of its weight's shape and device")
+        if isinstance(steps, torch.Tensor):
+            if steps.dtype != torch.int64 or steps.numel() != 1 or (self.params and steps.device != self.params[0].device):
+                raise ValueError("steps must be a number, or an int64 tensor of one value beside the weights")
+        elif steps < 0:
+            raise ValueError("steps must not be negative")
+        self._shapes = [p.shape for p in self.params]
+        self._types = [p.dtype for p in self.params]
+        self._records = (_Tensor * max(1, len(self.params)))()
+        for r, i in zip(self._records, range(len(self.params))):
+            r.n, r.number, r.param_type = self.params[i].numel(), i, _TYPE[self._types[i]]
+
+    def _states(self, torch, given, dtype, shapes, what):
+        shapes = [p.shape for p in self.params] if shapes is None else shapes
+        if given is None:
+            return [torch.zeros(s, dtype=torch.float32, device=p.device).to(dtype) for s, p in zip(shapes, self.params)]
+        given = list(given)
+        if len(given) != len(self.params):
+            raise ValueError(f"{what} must be a tensor for every weight")
+        for x, s, p in zip(given, shapes, self.params):
+            if not isinstance(x, torch.Tensor) or x.shape != s or x.dtype != dtype or x.device != p.device or not x.is_contiguous():
+                raise ValueError(f"{what} must be contiguous {dtype} tensors of shape {[list(s) for s in shapes]}")
+        return given
+
+    def _scalar(self, torch, x, dtype, what):
+        if x.numel() != 1 or x.dtype != dtype or x.device != self.params[0].device:
+            raise ValueError(f"{what} must be a {dtype} tensor of one value beside the weights")
+        return x.data_ptr()
+
+    def step(self, grads=None, *, lr=None, grad_scale=None, skip=None):
+        """One step with ``grads``, a list of tensors (f32, f16 or bf16 of the weights' shapes; None leaves its weight as it
+        is), by default the weights' ``.grad``.  ``lr`` replaces the rate for this step: a number, or an f32 tensor of one
+        value on the GPU.  ``grad_scale``: an f32 tensor of one value by which gradients are multiplied.
+        ``skip``: an i32 tensor of one value; where it is not 0, nothing is changed (a number in ``steps`` still counts
+        the step)."""
+        torch = _state["torch"]
+        params = self.params
+        grads = [p.grad for p in params] if grads is None else list(grads)
+        if len(grads) != len(params):
+            raise ValueError("grads must be a tensor or None for every weight")
+        if not params:
+            return
+        dev, records, kept = params[0].device, self._records, []
+        for i, g in enumerate(grads):
+            r, p = records[i], params[i]
+            if g is None:
+                r.n = 0
+                continue
+            if not isinstance(g, torch.Tensor) or g.shape != self._shapes[i] or g.dtype not in _TYPE or g.device != dev:
+                raise ValueError(f"gradient {i} must be a float32, float16 or bfloat16 tensor of its weight's shape and device")
+            if p.shape != self._shapes[i] or p.dtype != self._types[i] or p.device != dev or not p.is_contiguous():
+                raise ValueError(f"weight {i} is not what it was: shape, type, device or layout changed")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                kept.append(g)
+            r.n, r.param, r.grad, r.grad_type = p.numel(), p.data_ptr(), g.data_ptr(), _TYPE[g.dtype]
+            r.exp_avg, r.exp_avg_sq = self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr()
+            if self.exp_avg_scale is not None:
+                r.exp_avg_scale, r.exp_avg_sq_scale = self.exp_avg_scale[i].data_ptr(), self.exp_avg_sq_scale[i].data_ptr()
+            c = self.copies[i]
+            if c is not None:
+                r.copy, r.copy_type = c.data_ptr(), _TYPE[c.dtype]
+        s = _Settings(beta1=self.beta1, beta2=self.beta2, eps=self.eps, weight_decay=self.weight_decay, seed=self.seed,
+                      state=1 if self.state == "f8" else 0)
+        lr = self.lr if lr is None else lr
+        if isinstance(lr, torch.Tensor):
+            s.lr_device = self._scalar(torch, lr, torch.float32, "lr")
+        else:
+            s.lr = lr
+        if grad_scale is not None:
+            s.grad_scale = self._scalar(torch, grad_scale, torch.float32, "grad_scale")
+        if skip is not None:
+            s.skip = self._scalar(torch, skip, torch.int32, "skip")
+        with _on(params[0]):
+            if isinstance(self.steps, torch.Tensor):
+                self.steps.add_(1 if skip is None else (skip.view(self.steps.shape) == 0))
+                s.step_device = self.steps.data_ptr()
+            else:
+                s.step = self.steps + 1
+            _state["check"](_state["adamw"](records, len(params), C.byref(s), _stream(params[0])))
+        if not isinstance(self.steps, torch.Tensor):
+            self.steps += 1

@@ -1,6 +1,6 @@
 """Operators on class scores that live on the GPU: the top classes of a row with its
-log-sum-exp, distillation of a student from a teacher's top classes (loss and gradient), and
-classes drawn from given random numbers.
+log-sum-exp, distillation of a student from a teacher's top classes (loss and gradient),
+classes drawn from given random numbers, and log probabilities of given classes with their gradient.
 
 They take torch tensors on the GPU and enqueue on torch's current stream; what they return
 is made by torch on that stream.  Scores are [rows][classes], f32, f16 or bf16, of any
@@ -16,7 +16,7 @@ tensors; these functions then raise).
 """
 from __future__ import annotations
 
-import ctypes as C
+from collections import namedtuple
 
 _TYPE = {}      # torch dtype -> CBH_TYPE_*
 _state = {}     # the bound library functions, once the runtime was looked at
@@ -38,6 +38,9 @@ def _bind():
     _state.update(torch=torch, lib=L, check=cb._check, error=cb.CbhError, top=L.cbh_top_classes, top_ws=L.cbh_top_classes_workspace,
                   distill=L.cbh_distill_gradients, distill_ws=L.cbh_distill_gradients_workspace,
                   sample=L.cbh_sample_classes, sample_ws=L.cbh_sample_classes_workspace,
+                  logprobs=L.cbh_class_logprobs, logprobs_ws=L.cbh_class_logprobs_workspace,
+                  logprob_grad=L.cbh_logprob_gradients, lookup=L.cbh_lookup_rows, table_grad=L.cbh_lookup_gradients,
+                  table_grad_ws=L.cbh_lookup_gradients_workspace, adamw=L.cbh_adamw_step,
                   raw_stream=getattr(torch._C, "_cuda_getCurrentRawStream", None))
     return torch
 
@@ -185,3 +188,72 @@ def sample_classes(scores, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_
                                          _addr(allowed), astride, index.data_ptr(), logprob.data_ptr(), _addr(ws), size,
                                          _stream(scores)))
     return index, logprob
+
+
+ClassLogprobs = namedtuple("ClassLogprobs", "logprob entropy stats top_logprob top_index")
+
+
+def _given(torch, given, n, like, what="given"):
+    """Classes [rows] or [rows][m] i32, and their shape."""
+    if not isinstance(given, torch.Tensor) or given.dim() not in (1, 2) or given.shape[0] != n:
+        raise ValueError(f"{what} must be a torch tensor [rows] or [rows][m]")
+    return _vector(torch, given, given.shape, torch.int32, like, what), given.shape[1] if given.dim() == 2 else 1
+
+
+def _allowed(torch, allowed, n, m, like):
+    """Words of allowed classes and their stride (0: one list for all rows)."""
+    if allowed is None:
+        return None, 0
+    words = (m + 31) // 32
+    one = isinstance(allowed, torch.Tensor) and allowed.dim() == 2 and allowed.shape[0] == 1
+    return _vector(torch, allowed, (1 if one else n, words), torch.int32, like, "allowed"), 0 if one else words
+
+
+def class_logprobs(scores, given=None, *, temperature=1.0, k=0, allowed=None):
+    """Log probabilities of given classes with the entropy and the ``k`` most probable classes of every row
+    (``cbh_class_logprobs``: the formulas are there), over the allowed classes at a temperature.  ``given``: i32
+    [rows] or [rows][m], or None; an index outside the classes is no entry and has 0.  ``allowed`` as in
+    :func:`sample_classes`.  Gives ``logprob`` f32 of given's shape, ``entropy`` [rows] f32 in nats, ``stats`` [rows][3]
+    f32 (what :func:`logprob_gradients` takes), ``top_logprob`` [rows][k] f32, largest first, and ``top_index``
+    [rows][k] i32 (-1 where fewer classes have a probability); 0 <= k <= min(classes, 1024)."""
+    torch = _state.get("torch") or _bind()
+    t, n, m, rs, cs = _scores(torch, scores)
+    given, count = (None, 0) if given is None else _given(torch, given, n, scores)
+    allowed, astride = _allowed(torch, allowed, n, m, scores)
+    k = int(k)
+    k = k if 0 <= k <= 1024 else 1 << 30   # (refused below, before anything of that size is allocated)
+    with _on(scores):
+        dev, f32 = scores.device, torch.float32
+        logprob = torch.empty((n, 0) if given is None else given.shape, dtype=f32, device=dev)
+        entropy, stats = torch.empty(n, dtype=f32, device=dev), torch.empty((n, 3), dtype=f32, device=dev)
+        shape = (n, k if k <= 1024 else 0)
+        top_logprob, top_index = torch.empty(shape, dtype=f32, device=dev), torch.empty(shape, dtype=torch.int32, device=dev)
+        size = _state["logprobs_ws"](n, m, k) if k <= 1024 else 0
+        ws = _workspace(torch, size, scores)
+        _state["check"](_state["logprobs"](scores.data_ptr(), t, n, m, rs, cs, _addr(given), count, float(temperature),
+                                           _addr(allowed), astride, k, logprob.data_ptr(), entropy.data_ptr(),
+                                           stats.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), _addr(ws),
+                                           size, _stream(scores)))
+    return ClassLogprobs(logprob, entropy, stats, top_logprob, top_index)
+
+
+def logprob_gradients(scores, given, logprob_grad, stats, *, entropy_grad=None, temperature=1.0, allowed=None):
+    """Gradient by the scores, in their type and layout, of a function of what :func:`class_logprobs` gave for
+    them (``cbh_logprob_gradients``): ``logprob_grad`` f32 of given's shape and ``entropy_grad`` [rows] f32 are its
+    derivatives by the log probabilities and the entropy, ``stats`` what the forward call returned;
+    ``temperature`` and ``allowed`` are those of that call.  A row of zeros in both gives 0 whatever its scores
+    hold."""
+    torch = _state.get("torch") or _bind()
+    t, n, m, rs, cs = _scores(torch, scores)
+    given, count = _given(torch, given, n, scores)
+    g = _vector(torch, logprob_grad, given.shape, torch.float32, scores, "logprob_grad")
+    h = None if entropy_grad is None else _vector(torch, entropy_grad, (n,), torch.float32, scores, "entropy_grad")
+    stats = _vector(torch, stats, (n, 3), torch.float32, scores, "stats")
+    allowed, astride = _allowed(torch, allowed, n, m, scores)
+    with _on(scores):
+        grad = torch.empty_like(scores)
+        grs, gcs = grad.stride()
+        _state["check"](_state["logprob_grad"](scores.data_ptr(), t, n, m, rs, cs, given.data_ptr(), count, g.data_ptr(),
+                                               _addr(h), stats.data_ptr(), float(temperature), _addr(allowed), astride,
+                                               grad.data_ptr(), grs, gcs, _stream(scores)))
+    return grad

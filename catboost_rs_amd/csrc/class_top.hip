@@ -16,66 +16,6 @@ using namespace cbh::cls;
 constexpr uint32_t kMaxTop = 1024;
 constexpr int kUnroll = 4;   // 16-byte loads a thread has in flight
 
-// One wave's candidates, CAP of them in LDS: the keys above `bound` that it has met.  Full, the wave
-// keeps the k largest and raises the bound to the smallest of them.
-template <int CAP>
-struct Candidates {
-    u64* keys;
-    uint32_t count;   // wave-uniform
-    u64 bound;        // keys at or below it are not among the k largest
-    float fbound;     // no score below it passes (NaN: all pass)
-    __device__ __forceinline__ void set_bound(u64 b) {
-        if (b > bound) {
-            bound = b;
-            fbound = key_score((uint32_t)(b >> 32));
-        }
-    }
-    __device__ __forceinline__ void compact(uint32_t k) {
-        constexpr int R = CAP / 64;
-        wave_fence();
-        const uint32_t l = lane_id();
-        u64 key[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const uint32_t i = r * 64 + l;
-            key[r] = i < count ? keys[i] : 0;
-        }
-        u64 kth = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const u64 t = kth | (1ull << bit);
-            uint32_t c = 0;
-#pragma unroll
-            for (int r = 0; r < R; ++r) c += (uint32_t)__popcll(__ballot(key[r] >= t));
-            if (c >= k) kth = t;
-            if (c == k) break;
-        }
-        uint32_t kept = 0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const u64 b = __ballot(key[r] >= kth);
-            if (key[r] >= kth) keys[kept + (uint32_t)__popcll(b & ((1ull << l) - 1))] = key[r];
-            kept += (uint32_t)__popcll(b);
-        }
-        count = kept;
-        wave_fence();
-        set_bound(kth - 1);   // (the smallest kept key is in; a key equal to it does not come again)
-    }
-    // x: this lane's score of class cls, or no score
-    __device__ __forceinline__ void offer(float x, uint32_t cls, bool have, uint32_t k) {
-        const u64 key = rank_key(x, cls);
-        bool in = have && key > bound;
-        u64 b = __ballot(in);
-        if (!b) return;
-        if (count + (uint32_t)__popcll(b) > (uint32_t)CAP) {
-            compact(k);
-            in = in && key > bound;
-            b = __ballot(in);
-        }
-        if (in) keys[count + (uint32_t)__popcll(b & ((1ull << lane_id()) - 1))] = key;
-        count += (uint32_t)__popcll(b);
-    }
-};
-
 // A row's log-sum-exp from its (m, s).  A row of +inf has NaN in s (+inf - +inf), as one of NaN; which it is is known when the
 // row's largest are ranked: a NaN is among them, and its thread then writes NaN in place of +inf.  (The
 // log-sum-exp is written first and its registers are free from there: written last, by the thread that knows the

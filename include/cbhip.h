@@ -549,6 +549,109 @@ int cbh_sample_classes(const void* scores, int32_t type, uint64_t rows, uint32_t
                        int64_t allowed_stride, int32_t* index, float* logprob, void* workspace,
                        uint64_t workspace_bytes, void* stream);
 
+/* ---- a student beside a boosted model: log probabilities, looked-up rows, AdamW (no counterpart in the reference) ----
+ *
+ * As the operators on class scores above: DEVICE pointers, work enqueued on `stream` and not waited for, nothing
+ * allocated (the calls may be captured into a graph; two graphs that may run at once need a workspace each), f32 or
+ * wider arithmetic, results that do not depend on the order of execution. */
+
+/* Log probabilities of given classes, the entropy of every row, and its k most probable classes.  With x the scores of
+ * the allowed classes, m the largest and t = temperature (1e-38 .. 1e36):
+ *   d_j = (x_j - m) / t,  Z = sum exp d_j,  E = -sum exp(d_j) d_j / Z
+ *   logprob[r][i] = d_c - log Z of c = given[r][i] (0 where c is outside [0, classes): no entry)
+ *   entropy[r]    = log Z + E
+ *   stats[r]      = m, log Z, E: what cbh_logprob_gradients takes
+ *   top_logprob, top_index [rows][k]: the largest scores first, the lowest class first among equal ones
+ *   given          [rows][n_given], 0 <= n_given <= 1024 (NULL with 0)
+ *   allowed        nullable; bit j & 31 of word allowed[r * allowed_stride + (j >> 5)] allows class j of row r
+ *                  (allowed_stride 0: one list for all rows); a class that is not allowed counts as a score of -inf
+ *                  whatever its score holds
+ *   k              0 <= k <= min(classes, 1024)
+ * A class of -inf has log probability -inf and is not among the k (index -1 and log probability -inf behind the last
+ * one).  A row of -inf alone has entropy 0 and stats -inf, -inf, 0.  A row with NaN or +inf has NaN in logprob (of an
+ * entry), entropy, stats and top_logprob; its top_index is ordered as in cbh_top_classes.  entropy, stats, logprob are
+ * nullable. */
+uint64_t cbh_class_logprobs_workspace(uint64_t rows, uint32_t classes, uint32_t k);
+int cbh_class_logprobs(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                       int64_t class_stride, const int32_t* given, uint32_t n_given, double temperature,
+                       const uint32_t* allowed, int64_t allowed_stride, uint32_t k, float* logprob, float* entropy,
+                       float* stats, float* top_logprob, int32_t* top_index, void* workspace,
+                       uint64_t workspace_bytes, void* stream);
+
+/* The gradient by the scores of a function of the log probabilities and the entropy, from its derivatives by them,
+ * g = logprob_grad [rows][n_given] and h = entropy_grad [rows] (nullable: 0), and the stats that cbh_class_logprobs
+ * gave for these scores, temperature and allowed classes.  With p_j = exp(d_j - log Z), G = sum g of the entries:
+ *   grad_j = (sum of g_i of the entries i with class j - p_j (G + h (d_j + E))) / t, 0 where j is not allowed
+ * rounded once to the scores' type.  Entries of one class add up.  A row whose g (of entries) and h are all 0 gives 0
+ * whatever its scores hold, and is not read; a row of -inf alone gives its entries' g / t alone where they are
+ * allowed; NaN or +inf in a row makes its gradient NaN where allowed.  `grad` has strides of its own and may not overlap
+ * an input. */
+int cbh_logprob_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
+                          int64_t class_stride, const int32_t* given, uint32_t n_given, const float* logprob_grad,
+                          const float* entropy_grad, const float* stats, double temperature, const uint32_t* allowed,
+                          int64_t allowed_stride, void* grad, int64_t grad_row_stride, int64_t grad_class_stride,
+                          void* stream);
+
+/* Sums of rows of a table: what whole-number inputs (bins of cbh_quantize, buckets of cbh_perfect_hash, leaves of
+ * trees) are to a model that is trained by gradients.
+ *   out[r][c] = scale * sum_i table[index[r][i]][c], the sum in f32 in the order of i, rounded once to the type
+ *   table          element (v, c) at table[v * row_stride + c * column_stride]; 1 <= entries < 2^31, 1 <= dim <= 2^24
+ *   index          [rows][list], rows * list < 2^31; an index outside [0, entries) is no entry and adds nothing
+ *   out            [rows][dim] of the table's type; may not overlap an input */
+int cbh_lookup_rows(const void* table, int32_t type, uint32_t entries, uint32_t dim, int64_t row_stride,
+                    int64_t column_stride, const int32_t* index, uint64_t rows, uint32_t list, double scale, void* out,
+                    void* stream);
+
+/* Its gradient by the table, from that by `out`:
+ *   table_grad[v][c] = scale * sum over the places (r, i) with index[r][i] = v of grad[r][c]
+ * in f32, by parts of the sorted places joined in their order (the same for every run), rounded once; 0 for an entry that does not occur.
+ *   grad           element (r, c) at grad[r * row_stride + c * column_stride] (strides of 0: one value for many), of `type`
+ *   table_grad     [entries][dim] of grad_type (CBH_TYPE_*)
+ *   workspace      aligned to 16 */
+uint64_t cbh_lookup_gradients_workspace(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim);
+int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t rows, uint32_t dim, int64_t row_stride,
+                         int64_t column_stride, const int32_t* index, uint32_t list, uint32_t entries, double scale,
+                         void* table_grad, int32_t grad_type, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* One AdamW step over many tensors, in place.  For every value, with s the number of this step (from 1), in f32:
+ *   g = grad * *grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - m lr / (1 - beta1^s) / (sqrt(v) / sqrt(1 - beta2^s) + eps)
+ * rounded once to the parameter's type.  States of CBH_STATE_F32 are m and v.  States of CBH_STATE_F8 are m and
+ * sqrt(v) as OCP e4m3 codes, times a power of two for every 256 values of a tensor, which takes the largest into (224, 448]
+ * (0: all of them are 0; the largest m below 2^-100 too).  A value is rounded to one of its two neighbours by 16 bits u: up where
+ * u 2^-16 and the fraction reach 1 together, so that states that change by less than a code's step a step still follow; a v above 0
+ * keeps a code above 0.  u is of the low (m) and high (v) half of
+ *   mix(i + mix(seed ^ mix(s)) + number 0x9E3779B9), all of 32 bits,
+ *   mix(x): x ^= x >> 16; x *= 0x5851F42D; x ^= x >> 15; x *= 0x4C957F2D; x ^= x >> 16
+ * of value i of tensor `number`.  NaN or infinity in m or v is held as NaN and leaves the other values of its block as they are. */
+enum { CBH_STATE_F32 = 0, CBH_STATE_F8 = 1 };
+typedef struct {
+    void* param;               /* [n] of param_type */
+    const void* grad;          /* [n] of grad_type */
+    void* exp_avg;             /* [n] f32, or codes u8 */
+    void* exp_avg_sq;          /* [n] f32 (v), or codes u8 (of sqrt(v)) */
+    float* exp_avg_scale;      /* [ceil(n / 256)], CBH_STATE_F8 */
+    float* exp_avg_sq_scale;   /* [ceil(n / 256)], CBH_STATE_F8 */
+    void* copy;                /* nullable [n]: the new parameter, rounded to copy_type */
+    uint64_t n;                /* 0: nothing is done */
+    int32_t param_type;        /* CBH_TYPE_* */
+    int32_t grad_type;
+    int32_t copy_type;
+    uint32_t number;
+} cbh_adamw_tensor;
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;   /* 0 <= beta < 1, eps >= 0 */
+    int64_t step;                 /* >= 1 */
+    const int64_t* step_device;   /* nullable DEVICE pointer: the step, in place of `step` (graphs) */
+    const float* lr_device;       /* nullable DEVICE pointer: the rate, in place of `lr` */
+    const float* grad_scale;      /* nullable DEVICE pointer: 1 */
+    const int32_t* skip;          /* nullable DEVICE pointer: where it is not 0, nothing is changed */
+    uint32_t seed;
+    int32_t state;                /* CBH_STATE_* */
+} cbh_adamw_settings;
+/* tensors: HOST array [count].  Parameters, states and copies may not overlap one another (refused). */
+int cbh_adamw_step(const cbh_adamw_tensor* tensors, uint32_t count, const cbh_adamw_settings* settings, void* stream);
+
 /* Version / build information. */
 const char* cbh_version(void);
 const char* cbh_last_error(void);
