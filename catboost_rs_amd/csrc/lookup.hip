@@ -40,108 +40,183 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table
 }
 
 // ---- sort -----------------------------------------------------------------------------------
-// Stable radix sort of (entry, place), least significant digits first, of up to 11 bits.  A workgroup ranks 4096 keys.
-constexpr uint32_t kSortKeys = 4096, kSortWaves = 4, kMaxDigitBits = 11, kWaveKeys = kSortKeys / kSortWaves;
+// What is summed up comes as (entry, row), sorted by entry and stable by place.  A place without an entry sorts behind all, as
+// `entries`.
 struct Sort {
-    uint32_t n, entries;      // keys; a place without an entry sorts behind all, as `entries`
-    uint32_t blocks, digits;  // of a pass; digits a power of two
+    const int32_t* index;
+    uint32_t n, entries, list;
+    uint32_t blocks, digits;   // of a pass by digits; digits a power of two
     int shift, bits;
+    uint8_t* mark;             // [entries]: cleared here, set where an entry's sum is taken
 };
-__device__ __forceinline__ u64 first_key(const int32_t* index, uint32_t i, uint32_t entries) {
-    return (u64)min((uint32_t)index[i], entries) << 32 | i;
+__device__ __forceinline__ uint32_t place_entry(const Sort& S, uint32_t i) { return min((uint32_t)S.index[i], S.entries); }
+__device__ __forceinline__ void clear_marks(const Sort& S, uint32_t block, uint32_t blocks) {
+    for (uint64_t v = (uint64_t)block * 256 + threadIdx.x; v < S.entries; v += (uint64_t)blocks * 256) S.mark[v] = 0;
 }
-template <bool kFirst>
-__device__ __forceinline__ u64 sort_key(const void* in, uint32_t i, uint32_t entries) {
-    return kFirst ? first_key((const int32_t*)in, i, entries) : ((const u64*)in)[i];
-}
-template <bool kFirst>
-__device__ __forceinline__ void count_digits(const void* in, const Sort& S, uint32_t from, uint32_t to, uint32_t* count) {
-    for (uint32_t i = from + lane_id(); i < to; i += 64)
-        atomicAdd(&count[(uint32_t)(sort_key<kFirst>(in, i, S.entries) >> 32 >> S.shift) & (S.digits - 1)], 1u);
-}
-// Keys of every digit in every block: counts [block][digit].  The first pass clears the marks of entries that occur.
-template <bool kFirst>
-__global__ __launch_bounds__(256) void sort_count_kernel(const void* __restrict__ in, Sort S, uint32_t* __restrict__ counts,
-                                                         uint8_t* __restrict__ mark) {
-    __shared__ uint32_t count[1 << kMaxDigitBits];
-    if (kFirst)
-        for (uint64_t v = (uint64_t)blockIdx.x * 256 + threadIdx.x; v < S.entries; v += (uint64_t)gridDim.x * 256) mark[v] = 0;
-    for (uint32_t d = threadIdx.x; d < S.digits; d += 256) count[d] = 0;
+
+// Few places: a workgroup takes 64 of them and counts, over all places, those ahead of each; a wave a quarter of them.
+constexpr uint32_t kRankMost = 8192;
+__global__ __launch_bounds__(256) void rank_kernel(Sort S, u64* __restrict__ out) {
+    __shared__ uint32_t entry[kRankMost];
+    __shared__ uint32_t ahead[4][64];
+    const uint32_t blocks = (S.n + 63) / 64;
+    if (blockIdx.x >= blocks) return clear_marks(S, blockIdx.x - blocks, gridDim.x - blocks);
+    const uint32_t n4 = (S.n + 15) / 16 * 16;   // (four quarters of whole vectors; what lies behind the places is behind all)
+    for (uint32_t i = threadIdx.x; i < n4; i += 256) entry[i] = i < S.n ? place_entry(S, i) : ~0u;
     __syncthreads();
-    const uint32_t wave = threadIdx.x / 64, from = blockIdx.x * kSortKeys + wave * kWaveKeys;
-    if (from < S.n) count_digits<kFirst>(in, S, from, min(S.n, from + kWaveKeys), count);
+    const uint32_t wave = threadIdx.x / 64, lane = lane_id(), at = blockIdx.x * 64 + lane;
+    const uint32_t mine = at < S.n ? entry[at] : ~0u;
+    const uint32_t from = wave * (n4 / 4), to = from + n4 / 4;
+    // places before this workgroup's go ahead of an equal one, those behind it do not
+    uint32_t count = 0;
+    const uint32_t own0 = min(max(blockIdx.x * 64, from), to), own1 = min(max(min(blockIdx.x * 64 + 64, n4), from), to);
+    typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+    const Quad* q = (const Quad*)entry;
+#pragma unroll 4
+    for (uint32_t i = from / 4; i < own0 / 4; ++i) {
+        const Quad e = q[i];
+        count += (e[0] <= mine) + (e[1] <= mine) + (e[2] <= mine) + (e[3] <= mine);
+    }
+    for (uint32_t i = own0; i < own1; ++i) count += entry[i] < mine || (entry[i] == mine && i < at);
+#pragma unroll 4
+    for (uint32_t i = own1 / 4; i < to / 4; ++i) {
+        const Quad e = q[i];
+        count += (e[0] < mine) + (e[1] < mine) + (e[2] < mine) + (e[3] < mine);
+    }
+    ahead[wave][lane] = count;
+    __syncthreads();
+    if (wave == 0 && at < S.n)
+        out[ahead[0][lane] + ahead[1][lane] + ahead[2][lane] + ahead[3][lane]] = (u64)mine << 32 | at / S.list;
+}
+
+// Many places: radix sort of (entry, place), least significant digits first, of up to 11 bits.  A workgroup ranks
+// 256 ROUNDS keys, held in registers; the last pass writes rows for places.
+constexpr uint32_t kMaxDigitBits = 11;
+template <bool kFirst>
+__device__ __forceinline__ u64 sort_key(const u64* in, const Sort& S, uint32_t i) {
+    return kFirst ? (u64)place_entry(S, i) << 32 | i : in[i];
+}
+__device__ __forceinline__ uint32_t digit_of(u64 key, const Sort& S) { return (uint32_t)(key >> 32 >> S.shift) & (S.digits - 1); }
+// Keys of every digit in every block: counts [block][digit].
+template <bool kFirst, int ROUNDS>
+__global__ __launch_bounds__(256) void sort_count_kernel(const u64* __restrict__ in, Sort S, uint32_t* __restrict__ counts) {
+    __shared__ uint32_t count[1 << kMaxDigitBits];
+    if (kFirst) clear_marks(S, blockIdx.x, gridDim.x);
+    for (uint32_t d = threadIdx.x; d < S.digits; d += 256) count[d] = 0;
+    uint32_t digit[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const uint32_t i = (blockIdx.x * ROUNDS + r) * 256 + threadIdx.x;
+        digit[r] = i < S.n ? digit_of(sort_key<kFirst>(in, S, i), S) : ~0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        if (digit[r] != ~0u) atomicAdd(&count[digit[r]], 1u);
     __syncthreads();
     for (uint32_t d = threadIdx.x; d < S.digits; d += 256) counts[(uint64_t)blockIdx.x * S.digits + d] = count[d];
 }
 // For every digit the running sum over the blocks, in place, and its total.  A workgroup takes 64 digits, its waves
-// a quarter of the blocks each.
-__global__ __launch_bounds__(256) void sort_scan_kernel(Sort S, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
-    __shared__ uint32_t part[4][64];
+// a part of the blocks each.
+constexpr uint32_t kScanWaves = 16;
+__global__ __launch_bounds__(1024) void sort_scan_kernel(Sort S, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
+    __shared__ uint32_t part[kScanWaves][64];
     const uint32_t wave = threadIdx.x / 64, lane = lane_id(), d = blockIdx.x * 64 + lane;
-    const uint32_t each = (S.blocks + 3) / 4, b0 = min(S.blocks, wave * each), b1 = min(S.blocks, b0 + each);
+    const uint32_t each = (S.blocks + kScanWaves - 1) / kScanWaves, b0 = min(S.blocks, wave * each), b1 = min(S.blocks, b0 + each);
     uint32_t sum = 0;
-    if (d < S.digits)
+    if (d < S.digits) {
+#pragma unroll 8
         for (uint32_t b = b0; b < b1; ++b) sum += counts[(uint64_t)b * S.digits + d];
+    }
     part[wave][lane] = sum;
     __syncthreads();
     uint32_t at = 0;
     for (uint32_t w = 0; w < wave; ++w) at += part[w][lane];
     if (d >= S.digits) return;
-    for (uint32_t b = b0; b < b1; ++b) {
-        const uint32_t c = counts[(uint64_t)b * S.digits + d];
-        counts[(uint64_t)b * S.digits + d] = at;
-        at += c;
+    for (uint32_t b = b0; b < b1; b += 8) {
+        uint32_t c[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) c[j] = b + j < b1 ? counts[(uint64_t)(b + j) * S.digits + d] : 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            if (b + j < b1) counts[(uint64_t)(b + j) * S.digits + d] = at;
+            at += c[j];
+        }
     }
-    if (wave == 3) totals[d] = at;
+    if (wave == kScanWaves - 1) totals[d] = at;
 }
 // Keys to their places: the digits below, then the blocks before, then the waves before, then the rounds before, then the lanes
-// before.  The last pass marks the entries that occur.
-template <bool kFirst, bool kLast>
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const void* __restrict__ in, Sort S, const uint32_t* __restrict__ counts,
-                                                           const uint32_t* __restrict__ totals, u64* __restrict__ out,
-                                                           uint8_t* __restrict__ mark) {
-    __shared__ uint32_t at[kSortWaves][1 << kMaxDigitBits];
+// before.  Without `totals` the counts are as they were counted, and few blocks': each adds them up for itself.
+template <bool kFirst, bool kLast, int ROUNDS>
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict__ in, Sort S, const uint32_t* __restrict__ counts,
+                                                           const uint32_t* __restrict__ totals, u64* __restrict__ out) {
+    __shared__ uint32_t at[4][1 << kMaxDigitBits];
     __shared__ uint32_t sums[4];
-    const uint32_t wave = threadIdx.x / 64, lane = lane_id(), from = blockIdx.x * kSortKeys + wave * kWaveKeys;
-    for (uint32_t i = threadIdx.x; i < kSortWaves * S.digits; i += 256) at[i / S.digits][i % S.digits] = 0;
+    const uint32_t wave = threadIdx.x / 64, lane = lane_id(), from = (blockIdx.x * 4 + wave) * ROUNDS * 64;
+    u64 key[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const uint32_t i = from + r * 64 + lane;
+        key[r] = i < S.n ? sort_key<kFirst>(in, S, i) : 0;
+    }
+    for (uint32_t i = threadIdx.x; i < 4 * S.digits; i += 256) at[i / S.digits][i % S.digits] = 0;
     __syncthreads();
-    const uint32_t to = from < S.n ? min(S.n, from + kWaveKeys) : from;
-    count_digits<kFirst>(in, S, from, to, at[wave]);
-    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        if (from + r * 64 + lane < S.n) atomicAdd(&at[wave][digit_of(key[r], S)], 1u);
     // digits in ascending order by threads: each takes a run of them
+    constexpr uint32_t kRun = (1u << kMaxDigitBits) / 256;
     const uint32_t run = (S.digits + 255) / 256, d0 = threadIdx.x * run;
-    uint32_t mine = 0;
-    for (uint32_t d = d0; d < min(S.digits, d0 + run); ++d) mine += totals[d];
+    uint32_t total[kRun], before[kRun], mine = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kRun; ++j) {
+        const uint32_t d = d0 + j;
+        total[j] = before[j] = 0;
+        if (j >= run || d >= S.digits) continue;
+        if (totals) {
+            total[j] = totals[d];
+            before[j] = counts[(uint64_t)blockIdx.x * S.digits + d];
+        } else {
+#pragma unroll 8
+            for (uint32_t b = 0; b < S.blocks; ++b) {
+                const uint32_t c = counts[(uint64_t)b * S.digits + d];
+                total[j] += c;
+                before[j] += b < blockIdx.x ? c : 0;
+            }
+        }
+        mine += total[j];
+    }
     const uint32_t upto = wave_scan(mine, Add(), 0u);
     if (lane == 63) sums[wave] = upto;
     __syncthreads();
     uint32_t base = upto - mine;
     for (uint32_t w = 0; w < wave; ++w) base += sums[w];
-    for (uint32_t d = d0; d < min(S.digits, d0 + run); ++d) {
-        uint32_t a = base + counts[(uint64_t)blockIdx.x * S.digits + d];
 #pragma unroll
-        for (uint32_t w = 0; w < kSortWaves; ++w) {
+    for (uint32_t j = 0; j < kRun; ++j) {
+        const uint32_t d = d0 + j;
+        if (j >= run || d >= S.digits) continue;
+        uint32_t a = base + before[j];
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
             const uint32_t c = at[w][d];
             at[w][d] = a;
             a += c;
         }
-        base += totals[d];
+        base += total[j];
     }
     __syncthreads();
-    for (uint32_t i0 = from; i0 < to; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        const bool have = i < to;
-        const u64 key = have ? sort_key<kFirst>(in, i, S.entries) : 0;
-        const uint32_t d = (uint32_t)(key >> 32 >> S.shift) & (S.digits - 1);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const uint32_t i = from + r * 64 + lane, d = digit_of(key[r], S);
+        const bool have = i < S.n;
         u64 same = __ballot(have);
         for (int b = 0; b < S.bits; ++b) {
             const u64 set = __ballot(d >> b & 1);
             same &= d >> b & 1 ? set : ~set;
         }
         if (have) {
-            const uint32_t ahead = (uint32_t)__popcll(same & ((1ull << lane) - 1));
-            out[at[wave][d] + ahead] = key;
-            if (kLast && (uint32_t)(key >> 32) < S.entries) mark[key >> 32] = 1;
+            const uint32_t place = at[wave][d] + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+            out[place] = kLast ? key[r] >> 32 << 32 | (uint32_t)key[r] / S.list : key[r];
         }
         wave_fence();
         if (have && (same >> lane) == 1) at[wave][d] += (uint32_t)__popcll(same);   // (the last of the equal ones)
@@ -150,102 +225,202 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const void* __restric
 }
 
 // ---- sums -----------------------------------------------------------------------------------
+constexpr uint32_t kSumThreads = 512;
 struct Table {
-    const u64* sorted;   // (entry, place)
-    uint32_t n, entries, dim, list, chunk, chunks;
+    const u64* sorted;   // (entry, row)
+    uint32_t n, entries, dim;
+    uint32_t lanes, places;    // of a group: lanes that hold a row's vectors, and places that it adds up
+    uint32_t chunk, chunks;    // places of a workgroup
     float scale;
     float* part;         // [chunks][2][dim]: of the first run, where it began before; of the last, where it goes on
+    uint8_t* mark;
 };
 __device__ __forceinline__ uint32_t entry_at(const Table& B, uint32_t i) { return (uint32_t)(B.sorted[i] >> 32); }
 
-// A group of `lanes` lanes takes a chunk of the list and its vectors of the rows.
-template <class T, class O, bool kUnit>
-__global__ __launch_bounds__(256) void table_sum_kernel(const T* __restrict__ grad, int64_t rs, int64_t cs, Table B, uint32_t lanes,
-                                                        O* __restrict__ out) {
-    constexpr int V = Pack<T>::V;
-    const uint32_t tiles = (B.dim + lanes * V - 1) / (lanes * V), per = 256 / lanes;
-    const uint64_t groups = ((uint64_t)B.chunks + per - 1) / per;
-    for (uint64_t job = blockIdx.x; job < groups * tiles; job += gridDim.x) {
-        const uint32_t chunk = (uint32_t)(job / tiles) * per + threadIdx.x / lanes;
-        const uint32_t c = ((uint32_t)(job % tiles) * lanes + threadIdx.x % lanes) * V;
-        if (chunk >= B.chunks || c >= B.dim) continue;
-        const uint32_t from = chunk * B.chunk, to = min(B.n, from + B.chunk);
-        uint32_t cur = entry_at(B, from);
-        bool before = from > 0 && entry_at(B, from - 1) == cur;
-        float acc[V];
+// V values from column c on, in the output's type.
+template <class O, int V>
+__device__ __forceinline__ void store_values(O* row, uint32_t c, uint32_t dim, const float (&y)[V]) {
+    constexpr int N = V * (int)sizeof(O) / 4;   // words
+    typedef uint32_t Some __attribute__((ext_vector_type(N), aligned(sizeof(O))));
+    if (c + V <= dim) {
+        Some w;
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        auto flush = [&](bool after) {
-            if (cur >= B.entries) return;
-            if (before || after) {
-                float* p = B.part + ((uint64_t)chunk * 2 + !before) * B.dim;
-                store_pack<float, true>(p, 1, c, B.dim, *(const float(*)[4])&acc[0]);
-                if constexpr (V == 8)
-                    if (c + 4 < B.dim) store_pack<float, true>(p, 1, c + 4, B.dim, *(const float(*)[4])&acc[4]);
-            } else {
-                O* o = out + (uint64_t)cur * B.dim;
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (c + v < B.dim) o[c + v] = from_f32<O>(acc[v] * B.scale);
-            }
-        };
-        for (uint32_t i = from; i < to; ++i) {
-            const u64 key = B.sorted[i];
-            const uint32_t e = (uint32_t)(key >> 32);
-            if (e != cur) {
-                flush(false);
-                before = false;
-                cur = e;
-#pragma unroll
-                for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-            }
-            if (e >= B.entries) break;   // (sorted behind all)
-            float x[V];
-            load_pack<T, kUnit>(grad + (int64_t)((uint32_t)key / B.list) * rs, cs, c, B.dim, 0.0f, x);
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] += x[v];
+        for (int i = 0; i < N; ++i) {
+            if constexpr (sizeof(O) == 4)
+                w[i] = __builtin_bit_cast(uint32_t, y[i]);
+            else
+                w[i] = (uint32_t)__builtin_bit_cast(uint16_t, from_f32<O>(y[2 * i])) |
+                       (uint32_t)__builtin_bit_cast(uint16_t, from_f32<O>(y[2 * i + 1])) << 16;
         }
-        flush(to < B.n && entry_at(B, to) == cur);
+        *(Some*)(row + c) = w;
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (c + v < dim) row[c + v] = from_f32<O>(y[v]);
     }
 }
 
-// Runs of several chunks, by the workgroup of the chunk in which they begin; and the entries that do not occur.
-constexpr uint32_t kJoinWaves = 4;
+// A group of lanes takes `places` of the list, eight rows on their way at a time, and writes the runs that lie within them.
+// What of a run lies in several groups goes to LDS and is added up there, in the groups' order, a column a thread; what lies in several
+// workgroups, by join_kernel.
+enum { kHead = 1, kHeadEnds = 2, kTail = 4, kGoesOn = 8 };
+template <class T, class O, bool kUnit>
+__global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restrict__ grad, int64_t rs, int64_t cs, Table B,
+                                                                O* __restrict__ out) {
+    constexpr int V = Pack<T>::V, kFly = 8;
+    __shared__ float slot[2][kSumThreads * V];   // [head, tail][group][column]
+    __shared__ uint32_t flags[kSumThreads], head[kSumThreads], tail[kSumThreads];
+    const uint32_t width = B.lanes * V, tiles = (B.dim + width - 1) / width, per = kSumThreads / B.lanes;
+    const uint32_t group = threadIdx.x / B.lanes, in = threadIdx.x % B.lanes;
+    for (uint64_t job = blockIdx.x; job < (uint64_t)B.chunks * tiles; job += gridDim.x) {
+        const uint32_t chunk = (uint32_t)(job / tiles), c0 = (uint32_t)(job % tiles) * width, c = c0 + in * V;
+        const uint32_t from = min(B.n, chunk * B.chunk + group * B.places), to = min(B.n, from + B.places);
+        uint32_t cur = B.entries, flag = 0;
+        bool before = false;
+        float acc[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        auto keep = [&](uint32_t which) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) slot[which][threadIdx.x * V + v] = acc[v];
+        };
+        auto finish = [&] {   // the run of cur ends within the group
+            if (before) {
+                keep(0);
+                flag |= kHead | kHeadEnds;
+            } else if (cur < B.entries && c < B.dim) {
+                float y[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = acc[v] * B.scale;
+                store_values<O, V>(out + (uint64_t)cur * B.dim, c, B.dim, y);
+                if (c == 0) B.mark[cur] = 1;
+            }
+        };
+        if (from < to) {
+            cur = entry_at(B, from);
+            before = from > 0 && cur < B.entries && entry_at(B, from - 1) == cur;
+            if (in == 0) head[group] = cur;
+            for (uint32_t i0 = from; i0 < to; i0 += kFly) {
+                uint32_t e[kFly];
+                Pack<T> p[kFly];
+#pragma unroll
+                for (int u = 0; u < kFly; ++u) {
+                    const u64 key = B.sorted[min(i0 + u, to - 1)];
+                    e[u] = i0 + u < to ? (uint32_t)(key >> 32) : B.entries;
+                    const T* row = grad + (int64_t)(uint32_t)key * rs;
+                    if (e[u] >= B.entries) {
+                        p[u].w = Words{};
+                    } else if (kUnit && c + V <= B.dim) {
+                        p[u].w = ((const Loose<T>*)(row + c))->w;
+                    } else {
+                        float x[V];
+                        load_pack<T, kUnit>(row, cs, c, B.dim, 0.0f, x);
+                        p[u].set(x);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kFly; ++u) {
+                    if (i0 + u < to && e[u] != cur) {
+                        finish();
+                        before = false;
+                        cur = e[u];
+#pragma unroll
+                        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+                    }
+#pragma unroll
+                    for (int v = 0; v < V; ++v) acc[v] += p[u].get(v);
+                }
+            }
+            const bool after = cur < B.entries && to < B.n && entry_at(B, to) == cur;
+            if (!after) {
+                finish();
+            } else {
+                keep(before ? 0 : 1);
+                flag |= before ? kHead | kGoesOn : kTail | kGoesOn;
+            }
+        }
+        if (in == 0) {
+            flags[group] = flag;
+            tail[group] = cur;
+        }
+        __syncthreads();
+        for (uint32_t q = threadIdx.x; q < width; q += kSumThreads) {
+            if (c0 + q >= B.dim) break;
+            float sum = 0.0f;
+            bool began = false, on = false;   // the run began in this workgroup; goes on from the last group
+            for (uint32_t a = 0; a < per; ++a) {
+                const uint32_t f = flags[a];
+                if (f & kHead) {
+                    sum += slot[0][a * width + q];
+                    if (f & kHeadEnds) {
+                        if (began) out[(uint64_t)head[a] * B.dim + c0 + q] = from_f32<O>(sum * B.scale);
+                        else B.part[(uint64_t)chunk * 2 * B.dim + c0 + q] = sum;
+                        if (c0 + q == 0) B.mark[head[a]] = 1;
+                    }
+                }
+                if (f & kTail) {
+                    sum = slot[1][a * width + q];
+                    began = true;
+                }
+                on = f & kGoesOn;
+            }
+            if (on) {   // (past this workgroup: a run that goes on from a group has its next part in the one behind)
+                B.part[((uint64_t)chunk * 2 + began) * B.dim + c0 + q] = sum;
+                if (c0 + q == 0) B.mark[tail[per - 1]] = 1;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Runs of several workgroups, by that of the chunk in which they begin; and the entries that do not occur.
+constexpr uint32_t kZeroRows = 256;
 template <class O>
-__global__ __launch_bounds__(256) void table_join_kernel(Table B, const uint8_t* __restrict__ mark, uint32_t join_blocks,
-                                                         O* __restrict__ out) {
+__global__ __launch_bounds__(256) void table_join_kernel(Table B, uint32_t join_blocks, O* __restrict__ out) {
+    __shared__ uint32_t list[kZeroRows], count;
+    __shared__ float sum[4][64];
+    const uint32_t wave = threadIdx.x / 64, lane = lane_id();
     if (blockIdx.x >= join_blocks) {
-        const uint64_t all = (uint64_t)B.entries * B.dim, step = (uint64_t)(gridDim.x - join_blocks) * 256;
-        for (uint64_t i = (uint64_t)(blockIdx.x - join_blocks) * 256 + threadIdx.x; i < all; i += step)
-            if (!mark || !mark[i / B.dim]) out[i] = from_f32<O>(0.0f);
+        constexpr uint32_t V = 16 / sizeof(O);
+        const uint32_t vecs = (B.dim + V - 1) / V;
+        for (uint64_t row0 = (uint64_t)(blockIdx.x - join_blocks) * kZeroRows; row0 < B.entries;
+             row0 += (uint64_t)(gridDim.x - join_blocks) * kZeroRows) {
+            __syncthreads();
+            if (threadIdx.x == 0) count = 0;
+            __syncthreads();
+            const uint64_t row = row0 + threadIdx.x;
+            if (row < B.entries && (!B.n || !B.mark[row])) list[atomicAdd(&count, 1u)] = threadIdx.x;   // (their order does not matter)
+            __syncthreads();
+            float z[V] = {};
+            for (uint32_t j = threadIdx.x; j < count * vecs; j += 256)
+                store_pack<O, true>(out + (row0 + list[j / vecs]) * B.dim, 1, (uint32_t)(j % vecs) * V, B.dim, z);
+        }
         return;
     }
-    __shared__ uint32_t last;
-    __shared__ float sum[kJoinWaves][64];
-    const uint32_t wave = threadIdx.x / 64, lane = lane_id();
     for (uint32_t chunk = blockIdx.x; chunk + 1 < B.chunks; chunk += join_blocks) {
         const uint32_t from = chunk * B.chunk, next = from + B.chunk, e = entry_at(B, next - 1);
         if (e >= B.entries || entry_at(B, next) != e) continue;
         if (from > 0 && entry_at(B, from) == e && entry_at(B, from - 1) == e) continue;   // began before
         // the last chunk that the run reaches
         __syncthreads();
-        if (threadIdx.x == 0) last = B.chunks - 1;
+        if (threadIdx.x == 0) count = B.chunks - 1;
         __syncthreads();
         for (uint32_t c0 = chunk + 1;; c0 += 256) {
             const uint32_t c = c0 + threadIdx.x;
             const bool ends = c < B.chunks && (c == B.chunks - 1 || entry_at(B, (c + 1) * B.chunk) != e);
-            if (ends) atomicMin(&last, c);
+            if (ends) atomicMin(&count, c);
             if (__syncthreads_or(ends) || c0 + 256 >= B.chunks) break;
         }
         __syncthreads();
-        const uint32_t upto = last, count = upto - chunk;   // chunks behind the first
-        const uint32_t each = (count + kJoinWaves - 1) / kJoinWaves;
-        const uint32_t a = chunk + 1 + min(count, wave * each), b = min(upto + 1, a + each);
+        const uint32_t upto = count, behind = upto - chunk;   // chunks behind the first
+        const uint32_t each = (behind + 3) / 4;
+        const uint32_t a = chunk + 1 + min(behind, wave * each), b = min(upto + 1, a + each);
         for (uint32_t c0 = 0; c0 < B.dim; c0 += 64) {
             const uint32_t c = c0 + lane;
             float s = 0.0f;
             if (c < B.dim) {
                 if (wave == 0) s = B.part[((uint64_t)chunk * 2 + 1) * B.dim + c];
+#pragma unroll 8
                 for (uint32_t q = a; q < b; ++q) s += B.part[(uint64_t)q * 2 * B.dim + c];
             }
             sum[wave][lane] = s;
@@ -259,18 +434,23 @@ __global__ __launch_bounds__(256) void table_join_kernel(Table B, const uint8_t*
 
 // ---- host -----------------------------------------------------------------------------------
 struct Layout {
-    uint32_t n, passes, bits, blocks, chunk, chunks;
+    uint32_t n, passes, bits, rounds, blocks;
+    uint32_t lanes, places, chunk, chunks;
     uint64_t keys, counts, totals, mark, part, bytes;   // offsets; keys: two arrays
 };
-Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim) {
+Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint32_t vec) {
     Layout L{};
     L.n = (uint32_t)(rows * list);
     uint32_t bits = 1;
     while (entries >> bits) ++bits;   // keys are 0 .. entries
-    L.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-    L.bits = (bits + L.passes - 1) / L.passes;
-    L.blocks = (L.n + kSortKeys - 1) / kSortKeys;
-    L.chunk = L.n <= 1u << 14 ? 16 : L.n <= 1u << 18 ? 32 : 64;
+    L.passes = L.n <= kRankMost ? 0 : (bits + kMaxDigitBits - 1) / kMaxDigitBits;
+    L.bits = L.passes ? (bits + L.passes - 1) / L.passes : 0;
+    L.rounds = L.n <= 1u << 19 ? 4 : 16;
+    L.blocks = (L.n + L.rounds * 256 - 1) / (L.rounds * 256);
+    L.lanes = 1;
+    while (L.lanes < 64 && L.lanes * vec < dim) L.lanes *= 2;
+    L.places = L.n <= 1u << 17 ? 16 : 32;
+    L.chunk = L.places * (kSumThreads / L.lanes);
     L.chunks = (L.n + L.chunk - 1) / L.chunk;
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
@@ -278,60 +458,59 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim) {
         at += (bytes + 15) / 16 * 16;
         return p;
     };
-    L.keys = take(16 * (uint64_t)L.n);
-    L.counts = take(4ull * L.blocks << L.bits);
-    L.totals = take(4ull << L.bits);
-    L.mark = take(entries);
+    L.keys = take((L.passes > 1 ? 16 : 8) * (uint64_t)L.n);
+    L.counts = take(L.passes ? 4ull * L.blocks << L.bits : 0);
+    L.totals = take(L.passes ? 4ull << L.bits : 0);
+    L.mark = take(L.n ? entries : 0);
     L.part = take(8ull * L.chunks * dim);
     L.bytes = at;
     return L;
 }
 
 template <class T, class O>
-int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const uint8_t* mark, void* out, hipStream_t st) {
-    constexpr uint32_t V = Pack<T>::V;
-    uint32_t lanes = 1;
-    while (lanes < 64 && lanes * V < B.dim) lanes *= 2;
-    const uint32_t tiles = (B.dim + lanes * V - 1) / (lanes * V), per = 256 / lanes;
-    if (B.chunks) {
-        const unsigned grid = row_grid(((uint64_t)B.chunks + per - 1) / per * tiles);
-        if (cs == 1) table_sum_kernel<T, O, true><<<grid, 256, 0, st>>>((const T*)grad, rs, cs, B, lanes, (O*)out);
-        else table_sum_kernel<T, O, false><<<grid, 256, 0, st>>>((const T*)grad, rs, cs, B, lanes, (O*)out);
+int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, void* out, hipStream_t st) {
+    const uint32_t tiles = (B.dim + B.lanes * Pack<T>::V - 1) / (B.lanes * Pack<T>::V);
+    if (B.n) {
+        const unsigned grid = row_grid((uint64_t)B.chunks * tiles);
+        if (cs == 1) table_sum_kernel<T, O, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, (O*)out);
+        else table_sum_kernel<T, O, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, (O*)out);
         CLS_TRY(hipGetLastError());
     }
-    const uint32_t join = std::min<uint32_t>(B.chunks, 1u << 16);
-    const uint32_t zero = (uint32_t)std::min<uint64_t>(((uint64_t)B.entries * B.dim + 1023) / 1024, 4096);
-    table_join_kernel<O><<<join + zero, 256, 0, st>>>(B, mark, join, (O*)out);
+    const uint32_t join = B.chunks > 1 ? std::min<uint32_t>(B.chunks - 1, 1u << 14) : 0;
+    const uint32_t zero = std::min<uint32_t>((B.entries + kZeroRows - 1) / kZeroRows, 1u << 14);
+    table_join_kernel<O><<<join + zero, 256, 0, st>>>(B, join, (O*)out);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
 template <class T>
-int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const uint8_t* mark, void* out, int32_t type,
-                hipStream_t st) {
+int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, void* out, int32_t type, hipStream_t st) {
     switch (type) {
-        case CBH_TYPE_F32: return launch_sums<T, float>(grad, rs, cs, B, mark, out, st);
-        case CBH_TYPE_F16: return launch_sums<T, _Float16>(grad, rs, cs, B, mark, out, st);
-        default: return launch_sums<T, bf16_t>(grad, rs, cs, B, mark, out, st);
+        case CBH_TYPE_F32: return launch_sums<T, float>(grad, rs, cs, B, out, st);
+        case CBH_TYPE_F16: return launch_sums<T, _Float16>(grad, rs, cs, B, out, st);
+        default: return launch_sums<T, bf16_t>(grad, rs, cs, B, out, st);
     }
 }
 
-int sort_places(const int32_t* index, uint32_t entries, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
-    Sort S{L.n, entries, L.blocks, 1u << L.bits, 0, (int)L.bits};
+// Counts of so few blocks are added up by every block of the scatter, without a launch for them.
+constexpr uint32_t kOwnScan = 32;
+template <int ROUNDS>
+int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
     u64* a = (u64*)(ws + L.keys);
     u64* b = a + L.n;
-    uint32_t *counts = (uint32_t*)(ws + L.counts), *totals = (uint32_t*)(ws + L.totals);
-    uint8_t* mark = (uint8_t*)(ws + L.mark);
-    const unsigned scan = (S.digits + 63) / 64;
-    const void* in = index;
+    const u64* in = nullptr;
+    uint32_t* counts = (uint32_t*)(ws + L.counts);
+    uint32_t* totals = L.blocks <= kOwnScan ? nullptr : (uint32_t*)(ws + L.totals);
     for (uint32_t p = 0; p < L.passes; ++p) {
         S.shift = (int)(p * L.bits);
         const bool first = p == 0, last = p + 1 == L.passes;
-        if (first) sort_count_kernel<true><<<L.blocks, 256, 0, st>>>(in, S, counts, mark);
-        else sort_count_kernel<false><<<L.blocks, 256, 0, st>>>(in, S, counts, mark);
+        if (first) sort_count_kernel<true, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts);
+        else sort_count_kernel<false, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts);
         CLS_TRY(hipGetLastError());
-        sort_scan_kernel<<<scan, 256, 0, st>>>(S, counts, totals);
-        CLS_TRY(hipGetLastError());
-#define SCATTER(F, L_) sort_scatter_kernel<F, L_><<<L.blocks, 256, 0, st>>>(in, S, counts, totals, a, mark)
+        if (totals) {
+            sort_scan_kernel<<<(S.digits + 63) / 64, 64 * kScanWaves, 0, st>>>(S, counts, totals);
+            CLS_TRY(hipGetLastError());
+        }
+#define SCATTER(F, L_) sort_scatter_kernel<F, L_, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts, totals, a)
         if (first) last ? SCATTER(true, true) : SCATTER(true, false);
         else last ? SCATTER(false, true) : SCATTER(false, false);
 #undef SCATTER
@@ -340,6 +519,15 @@ int sort_places(const int32_t* index, uint32_t entries, const Layout& L, char* w
         in = a;
         std::swap(a, b);
     }
+    return CBH_OK;
+}
+int sort_places(const int32_t* index, uint32_t entries, uint32_t list, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
+    const Sort S{index, L.n, entries, list, L.blocks, 1u << L.bits, 0, (int)L.bits, (uint8_t*)(ws + L.mark)};
+    *sorted = (u64*)(ws + L.keys);
+    if (L.passes) return L.rounds == 4 ? sort_by_digits<4>(S, L, ws, sorted, st) : sort_by_digits<16>(S, L, ws, sorted, st);
+    const uint32_t clear = std::min<uint32_t>((entries + 4095) / 4096, 1024);
+    rank_kernel<<<(L.n + 63) / 64 + clear, 256, 0, st>>>(S, *sorted);
+    CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
 
@@ -404,7 +592,7 @@ extern "C" int cbh_lookup_rows(const void* table, int32_t type, uint32_t entries
 
 extern "C" uint64_t cbh_lookup_gradients_workspace(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim) {
     if (rows > 0x7FFFFFFFull || rows * list > 0x7FFFFFFFull || entries < 1 || entries >= 1u << 31 || dim > kMaxClasses) return 0;
-    return layout(rows, list, entries, dim).bytes;
+    return std::max(layout(rows, list, entries, dim, 4).bytes, layout(rows, list, entries, dim, 8).bytes);
 }
 
 extern "C" int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t rows, uint32_t dim, int64_t row_stride,
@@ -416,23 +604,24 @@ extern "C" int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t row
         if (rc == CBH_OK) rc = check_matrix(table_grad, grad_type, "the table's gradient", entries, dim, dim, 1);
         if (rc == CBH_OK) rc = check_scale(scale);
         if (rc != CBH_OK) return rc;
-        const Layout L = layout(rows, list, entries, dim);
-        if (L.bytes > workspace_bytes || !workspace || (uintptr_t)workspace % 16)
-            return cbh_internal_fail(CBH_ERR_LENGTH_MISMATCH, "the workspace needs " + std::to_string(L.bytes) +
+        const uint64_t need = cbh_lookup_gradients_workspace(rows, list, entries, dim);
+        if (need > workspace_bytes || (need && (!workspace || (uintptr_t)workspace % 16)))
+            return cbh_internal_fail(CBH_ERR_LENGTH_MISMATCH, "the workspace needs " + std::to_string(need) +
                                                                   " bytes, aligned to 16");
+        const Layout L = layout(rows, list, entries, dim, 16 / (uint32_t)type_bytes(type));
         hipStream_t st = (hipStream_t)stream;
         char* ws = (char*)workspace;
-        u64* sorted = (u64*)(ws + L.keys);
+        u64* sorted = nullptr;
         if (L.n) {
-            rc = sort_places(index, entries, L, ws, &sorted, st);
+            rc = sort_places(index, entries, list, L, ws, &sorted, st);
             if (rc != CBH_OK) return rc;
         }
-        const Table B{sorted, L.n, entries, dim, list, L.chunk, L.chunks, (float)scale, (float*)(ws + L.part)};
-        const uint8_t* mark = L.n ? (const uint8_t*)(ws + L.mark) : nullptr;   // (no rows: no entry occurs)
+        const Table B{sorted,  L.n,          entries,                dim,                    L.lanes, L.places, L.chunk,
+                      L.chunks, (float)scale, (float*)(ws + L.part), (uint8_t*)(ws + L.mark)};
         switch (type) {
-            case CBH_TYPE_F32: return launch_sums<float>(grad, row_stride, column_stride, B, mark, table_grad, grad_type, st);
-            case CBH_TYPE_F16: return launch_sums<_Float16>(grad, row_stride, column_stride, B, mark, table_grad, grad_type, st);
-            default: return launch_sums<bf16_t>(grad, row_stride, column_stride, B, mark, table_grad, grad_type, st);
+            case CBH_TYPE_F32: return launch_sums<float>(grad, row_stride, column_stride, B, table_grad, grad_type, st);
+            case CBH_TYPE_F16: return launch_sums<_Float16>(grad, row_stride, column_stride, B, table_grad, grad_type, st);
+            default: return launch_sums<bf16_t>(grad, row_stride, column_stride, B, table_grad, grad_type, st);
         }
     } catch (const std::exception& e) {
         return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
