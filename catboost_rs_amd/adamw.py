@@ -3,10 +3,14 @@
 from __future__ import annotations
 
 import ctypes as C
+from operator import attrgetter
+
+import numpy as np
 
 from .class_scores import _TYPE, _bind, _on, _state, _stream
 
 BLOCK = 256   # values of an 8-bit state that share a scale
+_SHAPE, _DTYPE, _DEVICE = attrgetter("shape"), attrgetter("dtype"), attrgetter("device")
 
 
 class _Tensor(C.Structure):
@@ -44,12 +48,11 @@ class AdamW:
         if state not in ("f32", "f8"):
             raise ValueError("state must be 'f32' or 'f8'")
         for p in self.params:
-            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.device != self.params[0].device:
-                raise ValueError("params must be torch tensors on one GPU")
-            if p.dtype not in _TYPE:
-                raise ValueError(f"params must be float32, float16 or bfloat16, not {p.dtype}")
-            if not p.is_contiguous():
-                raise ValueError("params must be contiguous")
+            if not isinstance(p, torch.Tensor):
+                raise ValueError("params must be torch tensors")
+        self._shapes, self._types = [p.shape for p in self.params], [p.dtype for p in self.params]
+        self._records = np.zeros(len(self.params), np.dtype(_Tensor))
+        self._look_at_weights(torch)
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
         self.state, self.steps, self.seed = state, steps, int(seed) & 0xFFFFFFFF
         small = state == "f8"
@@ -73,11 +76,32 @@ class AdamW:
                 raise ValueError("steps must be a number, or an int64 tensor of one value beside the weights")
         elif steps < 0:
             raise ValueError("steps must not be negative")
-        self._shapes = [p.shape for p in self.params]
-        self._types = [p.dtype for p in self.params]
-        self._records = (_Tensor * max(1, len(self.params)))()
-        for r, i in zip(self._records, range(len(self.params))):
-            r.n, r.number, r.param_type = self.params[i].numel(), i, _TYPE[self._types[i]]
+        # what of the library's records of the tensors does not change from step to step; the states' memory stays alive and in
+        # place with its storage
+        self._fixed = [x for x in (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale) if x is not None]
+        self._fixed = [t.untyped_storage() for x in self._fixed + [self.copies] for t in x if t is not None]
+        for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+            if getattr(self, name) is not None:
+                self._records[name] = [t.data_ptr() for t in getattr(self, name)]
+        self._records["copy"] = [0 if c is None else c.data_ptr() for c in self.copies]
+        self._records["copy_type"] = [0 if c is None else _TYPE[c.dtype] for c in self.copies]
+        self._records["param_type"] = [_TYPE[t] for t in self._types]
+        self._records["number"] = range(len(self.params))
+        self._sizes = np.array([p.numel() for p in self.params], np.uint64)
+
+    def _look_at_weights(self, torch):
+        for p, shape, dtype in zip(self.params, self._shapes, self._types):
+            if p.shape != shape or p.dtype != dtype:
+                raise ValueError("a weight is not what it was: its shape or type changed")
+            if not p.is_cuda or p.device != self.params[0].device:
+                raise ValueError("params must be on one GPU")
+            if p.dtype not in _TYPE:
+                raise ValueError(f"params must be float32, float16 or bfloat16, not {p.dtype}")
+            if not p.is_contiguous():
+                raise ValueError("params must be contiguous")
+        self._addresses = [p.data_ptr() for p in self.params]
+        self._weights = [p.untyped_storage() for p in self.params]
+        self._records["param"] = self._addresses
 
     def _states(self, torch, given, dtype, shapes, what):
         shapes = [p.shape for p in self.params] if shapes is None else shapes
@@ -109,26 +133,27 @@ class AdamW:
             raise ValueError("grads must be a tensor or None for every weight")
         if not params:
             return
-        dev, records, kept = params[0].device, self._records, []
-        for i, g in enumerate(grads):
-            r, p = records[i], params[i]
-            if g is None:
-                r.n = 0
-                continue
-            if not isinstance(g, torch.Tensor) or g.shape != self._shapes[i] or g.dtype not in _TYPE or g.device != dev:
-                raise ValueError(f"gradient {i} must be a float32, float16 or bfloat16 tensor of its weight's shape and device")
-            if p.shape != self._shapes[i] or p.dtype != self._types[i] or p.device != dev or not p.is_contiguous():
-                raise ValueError(f"weight {i} is not what it was: shape, type, device or layout changed")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept.append(g)
-            r.n, r.param, r.grad, r.grad_type = p.numel(), p.data_ptr(), g.data_ptr(), _TYPE[g.dtype]
-            r.exp_avg, r.exp_avg_sq = self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr()
-            if self.exp_avg_scale is not None:
-                r.exp_avg_scale, r.exp_avg_sq_scale = self.exp_avg_scale[i].data_ptr(), self.exp_avg_sq_scale[i].data_ptr()
-            c = self.copies[i]
-            if c is not None:
-                r.copy, r.copy_type = c.data_ptr(), _TYPE[c.dtype]
+        dev, records = params[0].device, self._records
+        # (attribute by attribute over all tensors: a loop over them would cost more than the step of small ones)
+        try:
+            shapes, records["n"] = list(map(_SHAPE, grads)), self._sizes
+        except AttributeError:   # (a weight without a gradient: nothing of it is touched)
+            records["n"] = np.where([g is None for g in grads], 0, self._sizes)
+            grads = [p if g is None else g for g, p in zip(grads, params)]
+            shapes = [getattr(g, "shape", None) for g in grads]
+        try:
+            same = shapes == self._shapes and set(map(torch.Tensor.get_device, grads)) == {dev.index}
+            records["grad_type"] = list(map(_TYPE.__getitem__, map(_DTYPE, grads)))
+        except (KeyError, TypeError, AttributeError):
+            same = False
+        if not same:
+            raise ValueError("a gradient must be a float32, float16 or bfloat16 tensor of its weight's shape and device")
+        if not all(map(torch.Tensor.is_contiguous, grads)):
+            grads = [g.contiguous() for g in grads]
+        addresses = list(map(torch.Tensor.data_ptr, params))
+        if addresses != self._addresses:   # (weights that moved; the memory of the old ones is kept until then, so that it is nobody else's)
+            self._look_at_weights(torch)
+        records["grad"] = list(map(torch.Tensor.data_ptr, grads))
         s = _Settings(beta1=self.beta1, beta2=self.beta2, eps=self.eps, weight_decay=self.weight_decay, seed=self.seed,
                       state=1 if self.state == "f8" else 0)
         lr = self.lr if lr is None else lr
@@ -146,6 +171,6 @@ class AdamW:
                 s.step_device = self.steps.data_ptr()
             else:
                 s.step = self.steps + 1
-            _state["check"](_state["adamw"](records, len(params), C.byref(s), _stream(params[0])))
+            _state["check"](_state["adamw"](records.ctypes.data, len(params), C.byref(s), _stream(params[0])))
         if not isinstance(self.steps, torch.Tensor):
             self.steps += 1

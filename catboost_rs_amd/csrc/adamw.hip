@@ -16,20 +16,23 @@ using namespace cbh::cls;
 constexpr uint32_t kBlock = 256;      // values that share a scale: a wave's
 constexpr uint32_t kBlocks = 4;       // blocks a wave has in flight
 constexpr uint32_t kTile = kBlock * kBlocks * 4;   // values of a workgroup's step
-constexpr uint32_t kBatch = 44;       // tensors of a launch: their addresses are kernel arguments (4 KB at most)
 
+// Tensors of a launch: their addresses are kernel arguments (4 KB at most with the settings).
+template <bool kSmall, bool kCopy>
 struct Batch {
-    void* param[kBatch];
-    const void* grad[kBatch];
-    void* m[kBatch];
-    void* v[kBatch];
-    float* m_scale[kBatch];
-    float* v_scale[kBatch];
-    void* copy[kBatch];
-    uint64_t n[kBatch];
-    uint64_t tiles[kBatch];   // of this tensor and those before
-    uint32_t number[kBatch];
+    static constexpr uint32_t N = kCopy ? 44 : kSmall ? 56 : 76;
+    void* param[N];
+    const void* grad[N];
+    void* m[N];
+    void* v[N];
+    float* m_scale[kSmall ? N : 1];
+    float* v_scale[kSmall ? N : 1];
+    void* copy[kCopy ? N : 1];
+    uint64_t n[N];
+    uint32_t tiles[N];   // of this tensor and those before
+    uint32_t number[N];
     uint32_t count;
+    int32_t copy_type;
 };
 struct Factors {
     float decay, rate, root;   // 1 - lr wd, lr / (1 - b1^s), 1 / sqrt(1 - b2^s)
@@ -67,29 +70,27 @@ __host__ __device__ inline uint32_t mix(uint32_t x) {
 }
 
 // ---- e4m3 --------------------------------------------------------------------------------------
-__device__ __forceinline__ float from_code(uint32_t c) {
-    const uint32_t u = c & 0x7F;
-    // normal codes are the top bits of an f32 with another exponent bias; below, multiples of 2^-9
-    float x = u >= 8 ? __builtin_bit_cast(float, (u + (120u << 3)) << 20) : (float)u * 0x1p-9f;
-    x = u == 0x7F ? NAN : x;
-    return c & 0x80 ? -x : x;
-}
-// |x| times the block's inverse scale (at most 448), rounded up or down by 16 random bits.
-__device__ __forceinline__ uint32_t to_code(float x, float inv, uint32_t random, bool least) {
+// |x| times the block's inverse scale (at most 448), rounded up or down by 16 random bits.  Normal values: the bits that an f32
+// has below the code's carry into it; below 2^-6: a multiple of 2^-9.  What comes out has a code, which the conversion
+// then finds (NaN stays NaN).
+__device__ __forceinline__ float round_code(float x, float inv, uint32_t random, bool least) {
     const float y = fabsf(x) * inv;
-    uint32_t c;
-    if (y < 0x1p-6f) c = (uint32_t)(y * 512.0f + (float)random * 0x1p-16f);
-    else c = ((__builtin_bit_cast(uint32_t, y) + (random << 4)) >> 20) - (120u << 3);
-    if (least) c = x > 0.0f ? max(c, 1u) : c;
-    c = y > 0.0f ? c : 0;
-    if (!(fabsf(x) < INFINITY)) c = 0x7F;
-    return c | (x < 0.0f ? 0x80u : 0u);
+    const float small = truncf(y * 512.0f + (float)random * 0x1p-16f);
+    const float large = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y) + (random << 4)) & 0xFFF00000u);
+    float c = y < 0x1p-6f ? (least ? fmaxf(small, 1.0f) : small) * 0x1p-9f : large;
+    if (!(y > 0.0f)) c = 0.0f;
+    if (!(fabsf(x) < INFINITY)) c = NAN;
+    return c;
 }
 // The power of two that takes the block's largest finite value into (224, 448]; 0 below 2^-100.
 __device__ __forceinline__ float block_scale(float largest) {
     const uint32_t bits = __builtin_bit_cast(uint32_t, largest);
     const uint32_t e = (bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000);
     return largest < 0x1p-100f ? 0.0f : __builtin_bit_cast(float, e << 23);
+}
+// Of a power of two, or 0 for 0.
+__device__ __forceinline__ float inverse(float s) {
+    return s > 0.0f ? __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, s)) : 0.0f;
 }
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
@@ -98,68 +99,103 @@ __device__ __forceinline__ float finite_abs(float x) {
 
 // ---- four values of a lane -----------------------------------------------------------------------
 template <class T>
-struct __attribute__((packed, aligned(sizeof(T)))) Four {
-    T v[4];
+struct Words4 {   // four values in words
+    static constexpr int N = (int)sizeof(T);
+    typedef uint32_t Type __attribute__((ext_vector_type(N)));
+    struct __attribute__((packed, aligned(sizeof(T)))) Any {
+        Type w;
+    };
+};
+template <>
+struct Words4<uint8_t> {
+    typedef uint32_t Type;
+    struct __attribute__((packed, aligned(1))) Any {
+        uint32_t w;
+    };
 };
 template <class T>
-__device__ __forceinline__ void load4(const T* p, uint64_t i, uint64_t n, Four<T>& q) {
-    if (i + 4 <= n) {
-        q = *(const Four<T>*)(p + i);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q.v[k] = i + k < n ? p[i + k] : T{};
+struct Four {
+    typename Words4<T>::Type w;
+    __device__ __forceinline__ float get(int k) const {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t word = w[k];   // (the cast of a vector's element itself takes the first)
+            return __builtin_bit_cast(float, word);
+        } else if constexpr (sizeof(T) == 1) {
+            return k == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0)
+                   : k == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
+                   : k == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2)
+                            : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+        } else {
+            const uint32_t word = w[k / 2];
+            if constexpr (__is_same(T, bf16_t)) return __builtin_bit_cast(float, k % 2 ? word & 0xFFFF0000u : word << 16);
+            else return (float)__builtin_bit_cast(_Float16, (uint16_t)(word >> (k % 2 * 16)));
+        }
     }
-}
-template <class T>
-__device__ __forceinline__ void store4(T* p, uint64_t i, uint64_t n, const Four<T>& q) {
-    if (i + 4 <= n) {
-        *(Four<T>*)(p + i) = q;
-    } else {
+    // (8 bits: values that have a code)
+    __device__ __forceinline__ void set(const float (&x)[4]) {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k < n) p[i + k] = q.v[k];
+            for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(uint32_t, x[k]);
+        } else if constexpr (sizeof(T) == 1) {
+            int q = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+            w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], q, true);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k += 2)
+                w[k / 2] = (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(x[k])) |
+                           (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(x[k + 1])) << 16;
+        }
     }
-}
-template <class T>
-__device__ __forceinline__ void store_copy(void* copy, uint64_t i, uint64_t n, const float (&x)[4]) {
-    Four<T> q;
+    // (kWhole: all four are there)
+    template <bool kWhole>
+    __device__ __forceinline__ void load(const T* p, uint64_t i, uint64_t n) {
+        if constexpr (kWhole) {
+            w = ((const typename Words4<T>::Any*)(p + i))->w;
+        } else {
+            T t[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) q.v[k] = from_f32<T>(x[k]);
-    store4((T*)copy, i, n, q);
-}
+            for (int k = 0; k < 4; ++k) t[k] = i + k < n ? p[i + k] : T{};
+            w = __builtin_bit_cast(typename Words4<T>::Type, t);
+        }
+    }
+    template <bool kWhole>
+    __device__ __forceinline__ void store(T* p, uint64_t i, uint64_t n) const {
+        if constexpr (kWhole) {
+            ((typename Words4<T>::Any*)(p + i))->w = w;
+        } else {
+            struct Values {
+                T v[4];
+            };
+            const Values t = __builtin_bit_cast(Values, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < n) p[i + k] = t.v[k];
+        }
+    }
+};
 
-template <class P, class G, bool kSmall>
-__global__ __launch_bounds__(256) void adamw_kernel(Batch B, Step S, int32_t copy_type) {
+// A wave's blocks: all loads under way before the first is waited for.
+template <class P, class G, bool kSmall, bool kCopy, bool kWhole, int BLOCKS>
+__device__ __forceinline__ void step_blocks(const Batch<kSmall, kCopy>& B, const Step& S, uint32_t t, uint64_t block0, uint64_t n) {
     using State = typename std::conditional<kSmall, uint8_t, float>::type;
-    if (S.skip && *S.skip != 0) return;
-    // the tensor of this tile (uniform)
-    uint32_t t = 0;
-    for (uint32_t hi = B.count - 1; t < hi;) {
-        const uint32_t mid = (t + hi) / 2;
-        if (blockIdx.x < B.tiles[mid]) hi = mid;
-        else t = mid + 1;
-    }
-    const uint64_t n = B.n[t], tile = blockIdx.x - (t ? B.tiles[t - 1] : 0);
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
-    const uint64_t block0 = tile * (kTile / kBlock) + wave * kBlocks;
+    const uint32_t lane = lane_id();
     P* p = (P*)B.param[t];
     const G* g = (const G*)B.grad[t];
     State *m = (State*)B.m[t], *v = (State*)B.v[t];
-    Four<P> qp[kBlocks];
-    Four<G> qg[kBlocks];
-    Four<State> qm[kBlocks], qv[kBlocks];
-    float ms[kBlocks], vs[kBlocks];
+    Four<P> qp[BLOCKS];
+    Four<G> qg[BLOCKS];
+    Four<State> qm[BLOCKS], qv[BLOCKS];
+    float ms[BLOCKS], vs[BLOCKS];
 #pragma unroll
-    for (uint32_t b = 0; b < kBlocks; ++b) {
+    for (uint32_t b = 0; b < BLOCKS; ++b) {
         const uint64_t i = (block0 + b) * kBlock + lane * 4;
-        load4(p, i, n, qp[b]);
-        load4(g, i, n, qg[b]);
-        load4(m, i, n, qm[b]);
-        load4(v, i, n, qv[b]);
+        qp[b].template load<kWhole>(p, i, n);
+        qg[b].template load<kWhole>(g, i, n);
+        qm[b].template load<kWhole>(m, i, n);
+        qv[b].template load<kWhole>(v, i, n);
         if constexpr (kSmall) {
-            const bool have = (block0 + b) * kBlock < n;
-            ms[b] = have ? B.m_scale[t][block0 + b] : 0.0f;
-            vs[b] = have ? B.v_scale[t][block0 + b] : 0.0f;
+            ms[b] = B.m_scale[t][block0 + b];
+            vs[b] = B.v_scale[t][block0 + b];
         }
     }
     Factors f = S.f;
@@ -172,84 +208,149 @@ __global__ __launch_bounds__(256) void adamw_kernel(Batch B, Step S, int32_t cop
     key += B.number[t] * 0x9E3779B9u;
     const float gs = S.grad_scale ? *S.grad_scale : 1.0f;
 #pragma unroll
-    for (uint32_t b = 0; b < kBlocks; ++b) {
+    for (uint32_t b = 0; b < BLOCKS; ++b) {
         const uint64_t i = (block0 + b) * kBlock + lane * 4;
-        if ((block0 + b) * kBlock >= n) break;
         float nm[4], nv[4], root[4], np[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float gk = to_f32(qg[b].v[k]);
+            float gk = qg[b].get(k);
             if (S.grad_scale) gk = gk * gs;
-            float om, ov;
+            float om = qm[b].get(k), ov = qv[b].get(k);
             if constexpr (kSmall) {
-                om = from_code(qm[b].v[k]) * ms[b];
-                ov = from_code(qv[b].v[k]) * vs[b];
+                om = om * ms[b];
+                ov = ov * vs[b];
                 ov = ov * ov;
-            } else {
-                om = qm[b].v[k];
-                ov = qv[b].v[k];
             }
             nm[k] = om * S.b1 + gk * S.a1;
             nv[k] = ov * S.b2 + gk * gk * S.a2;
             root[k] = sqrtf(nv[k]);
-            np[k] = to_f32(qp[b].v[k]) * f.decay - nm[k] * f.rate / (root[k] * f.root + S.eps);
-            qp[b].v[k] = from_f32<P>(np[k]);
+            np[k] = qp[b].get(k) * f.decay - nm[k] * f.rate / (root[k] * f.root + S.eps);
         }
-        store4(p, i, n, qp[b]);
-        if (B.copy[t]) {
-            if (copy_type == CBH_TYPE_F32) store_copy<float>(B.copy[t], i, n, np);
-            else if (copy_type == CBH_TYPE_F16) store_copy<_Float16>(B.copy[t], i, n, np);
-            else store_copy<bf16_t>(B.copy[t], i, n, np);
+        qp[b].set(np);
+        qp[b].template store<kWhole>(p, i, n);
+        if constexpr (kCopy) {
+            auto copy = [&](auto type) {
+                Four<decltype(type)> q;
+                q.set(np);
+                q.template store<kWhole>((decltype(type)*)B.copy[t], i, n);
+            };
+            if (B.copy_type == CBH_TYPE_F32) copy(float{});
+            else if (B.copy_type == CBH_TYPE_F16) copy(_Float16{});
+            else copy(bf16_t{});
         }
         if constexpr (kSmall) {
             float lm = 0.0f, lv = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (i + k < n) {
+                if (kWhole || i + k < n) {
                     lm = fmaxf(lm, finite_abs(nm[k]));
                     lv = fmaxf(lv, finite_abs(root[k]));
                 }
             const float sm = block_scale(wave_reduce(lm, MaxF())), sv = block_scale(wave_reduce(lv, MaxF()));
-            const float im = sm > 0.0f ? 1.0f / sm : 0.0f, iv = sv > 0.0f ? 1.0f / sv : 0.0f;
+            const float im = inverse(sm), iv = inverse(sv);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t r = mix((uint32_t)(i + k) + key);
-                qm[b].v[k] = (uint8_t)to_code(nm[k], im, r & 0xFFFF, false);
-                qv[b].v[k] = (uint8_t)to_code(root[k], iv, r >> 16, true);
+                nm[k] = copysignf(round_code(nm[k], im, r & 0xFFFF, false), nm[k]);
+                nv[k] = round_code(root[k], iv, r >> 16, true);
             }
             if (lane == 0) {
                 B.m_scale[t][block0 + b] = sm;
                 B.v_scale[t][block0 + b] = sv;
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                qm[b].v[k] = nm[k];
-                qv[b].v[k] = nv[k];
-            }
         }
-        store4(m, i, n, qm[b]);
-        store4(v, i, n, qv[b]);
+        qm[b].set(nm);
+        qv[b].set(nv);
+        qm[b].template store<kWhole>(m, i, n);
+        qv[b].template store<kWhole>(v, i, n);
+    }
+}
+
+template <class P, class G, bool kSmall, bool kCopy>
+__global__ __launch_bounds__(256) void adamw_kernel(Batch<kSmall, kCopy> B, Step S) {
+    if (S.skip && *S.skip != 0) return;
+    // the tensor of this tile (uniform)
+    uint32_t t = 0;
+    for (uint32_t hi = B.count - 1; t < hi;) {
+        const uint32_t mid = (t + hi) / 2;
+        if (blockIdx.x < B.tiles[mid]) hi = mid;
+        else t = mid + 1;
+    }
+    const uint64_t n = B.n[t], tile = blockIdx.x - (t ? B.tiles[t - 1] : 0);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint64_t block0 = tile * (kTile / kBlock) + wave * kBlocks;
+    if ((block0 + kBlocks) * kBlock <= n) {
+        step_blocks<P, G, kSmall, kCopy, true, kBlocks>(B, S, t, block0, n);
+    } else {   // the end of a tensor
+#pragma unroll 1
+        for (uint32_t b = 0; b < kBlocks && (block0 + b) * kBlock < n; ++b)
+            step_blocks<P, G, kSmall, kCopy, false, 1>(B, S, t, block0 + b, n);
     }
 }
 
 // ---- host -----------------------------------------------------------------------------------
-using Launch = void (*)(const Batch&, const Step&, int32_t, unsigned, hipStream_t);
-template <class P, class G, bool kSmall>
-void launch(const Batch& B, const Step& S, int32_t copy_type, unsigned grid, hipStream_t st) {
-    adamw_kernel<P, G, kSmall><<<grid, 256, 0, st>>>(B, S, copy_type);
+struct Run {   // tensors of one launch's types: collected until a launch is full
+    const cbh_adamw_tensor* tensors;
+    uint32_t count;
+    const cbh_adamw_tensor& first;
+    const Step& S;
+    hipStream_t st;
+    std::vector<char>& done;
+};
+template <class P, class G, bool kSmall, bool kCopy>
+hipError_t launch_all(const Run& R) {
+    Batch<kSmall, kCopy> B;
+    B.count = 0;
+    B.copy_type = R.first.copy_type;
+    auto flush = [&] {
+        if (!B.count) return hipSuccess;
+        adamw_kernel<P, G, kSmall, kCopy><<<B.tiles[B.count - 1], 256, 0, R.st>>>(B, R.S);
+        B.count = 0;
+        return hipGetLastError();
+    };
+    for (uint32_t j = (uint32_t)(&R.first - R.tensors); j < R.count; ++j) {
+        const cbh_adamw_tensor& t = R.tensors[j];
+        if (R.done[j] || t.n == 0 || t.param_type != R.first.param_type || t.grad_type != R.first.grad_type || !t.copy != !kCopy ||
+            (kCopy && t.copy_type != R.first.copy_type))
+            continue;
+        R.done[j] = 1;
+        // (a launch holds fewer than 2^32 threads; a longer tensor takes several)
+        constexpr uint64_t kMost = 1ull << 22;
+        const uint64_t all = (t.n + kTile - 1) / kTile;
+        for (uint64_t at = 0; at < all; at += kMost) {
+            const uint64_t tiles = std::min(kMost, all - at), off = at * kTile;
+            if (B.count == B.N || (B.count && B.tiles[B.count - 1] + tiles > kMost)) {
+                const hipError_t e = flush();
+                if (e != hipSuccess) return e;
+            }
+            const uint32_t c = B.count++;
+            const size_t s = kSmall ? 1 : 4;
+            B.param[c] = (char*)t.param + off * sizeof(P);
+            B.grad[c] = (const char*)t.grad + off * sizeof(G);
+            B.m[c] = (char*)t.exp_avg + off * s;
+            B.v[c] = (char*)t.exp_avg_sq + off * s;
+            if constexpr (kSmall) {
+                B.m_scale[c] = t.exp_avg_scale + off / kBlock;
+                B.v_scale[c] = t.exp_avg_sq_scale + off / kBlock;
+            }
+            if constexpr (kCopy) B.copy[c] = (char*)t.copy + off * type_bytes(t.copy_type);
+            B.n[c] = std::min<uint64_t>(t.n - off, tiles * kTile);
+            B.tiles[c] = (c ? B.tiles[c - 1] : 0) + (uint32_t)tiles;
+            B.number[c] = t.number;   // (a value's place counts modulo 2^32, which divides off)
+        }
+    }
+    return flush();
 }
 template <class P, class G>
-Launch pick(int32_t state) {
-    return state == CBH_STATE_F8 ? launch<P, G, true> : launch<P, G, false>;
+hipError_t launch_all(const Run& R, int32_t state) {
+    if (state == CBH_STATE_F8) return R.first.copy ? launch_all<P, G, true, true>(R) : launch_all<P, G, true, false>(R);
+    return R.first.copy ? launch_all<P, G, false, true>(R) : launch_all<P, G, false, false>(R);
 }
 template <class P>
-Launch pick(int32_t grad, int32_t state) {
-    return grad == CBH_TYPE_F32 ? pick<P, float>(state) : grad == CBH_TYPE_F16 ? pick<P, _Float16>(state) : pick<P, bf16_t>(state);
-}
-Launch pick(int32_t param, int32_t grad, int32_t state) {
-    return param == CBH_TYPE_F32 ? pick<float>(grad, state)
-                                 : param == CBH_TYPE_F16 ? pick<_Float16>(grad, state) : pick<bf16_t>(grad, state);
+hipError_t launch_all(const Run& R, int32_t state) {
+    return R.first.grad_type == CBH_TYPE_F32   ? launch_all<P, float>(R, state)
+           : R.first.grad_type == CBH_TYPE_F16 ? launch_all<P, _Float16>(R, state)
+                                               : launch_all<P, bf16_t>(R, state);
 }
 
 bool is_type(int32_t t) { return t == CBH_TYPE_F32 || t == CBH_TYPE_F16 || t == CBH_TYPE_BF16; }
@@ -320,44 +421,11 @@ extern "C" int cbh_adamw_step(const cbh_adamw_tensor* tensors, uint32_t count, c
         std::vector<char> done(count, 0);
         for (uint32_t i = 0; i < count; ++i) {
             if (done[i] || tensors[i].n == 0) continue;
-            const cbh_adamw_tensor& a = tensors[i];
-            const int32_t copy_type = a.copy ? a.copy_type : CBH_TYPE_F32;
-            const Launch run = pick(a.param_type, a.grad_type, A.state);
-            Batch B;
-            B.count = 0;
-            auto flush = [&] {
-                if (!B.count) return hipSuccess;
-                run(B, S, copy_type, (unsigned)B.tiles[B.count - 1], (hipStream_t)stream);
-                B.count = 0;
-                return hipGetLastError();
-            };
-            for (uint32_t j = i; j < count; ++j) {
-                const cbh_adamw_tensor& t = tensors[j];
-                if (done[j] || t.n == 0 || t.param_type != a.param_type || t.grad_type != a.grad_type ||
-                    (t.copy ? t.copy_type : copy_type) != copy_type)
-                    continue;
-                done[j] = 1;
-                // (a launch holds fewer than 2^32 threads; a longer tensor takes several)
-                constexpr uint64_t kMost = 1ull << 22;
-                const uint64_t all = (t.n + kTile - 1) / kTile;
-                for (uint64_t at = 0; at < all; at += kMost) {
-                    const uint64_t tiles = std::min(kMost, all - at), off = at * kTile;
-                    if (B.count == kBatch || (B.count && B.tiles[B.count - 1] + tiles > kMost)) CLS_TRY(flush());
-                    const uint32_t c = B.count++;
-                    B.param[c] = (char*)t.param + off * type_bytes(t.param_type);
-                    B.grad[c] = (const char*)t.grad + off * type_bytes(t.grad_type);
-                    const size_t s = A.state == CBH_STATE_F8 ? 1 : 4;
-                    B.m[c] = (char*)t.exp_avg + off * s;
-                    B.v[c] = (char*)t.exp_avg_sq + off * s;
-                    B.m_scale[c] = t.exp_avg_scale ? t.exp_avg_scale + off / kBlock : nullptr;
-                    B.v_scale[c] = t.exp_avg_sq_scale ? t.exp_avg_sq_scale + off / kBlock : nullptr;
-                    B.copy[c] = t.copy ? (char*)t.copy + off * type_bytes(t.copy_type) : nullptr;
-                    B.n[c] = std::min<uint64_t>(t.n - off, tiles * kTile);
-                    B.tiles[c] = (c ? B.tiles[c - 1] : 0) + tiles;
-                    B.number[c] = t.number;   // (a value's place counts modulo 2^32, which divides off)
-                }
-            }
-            CLS_TRY(flush());
+            const Run R{tensors, count, tensors[i], S, (hipStream_t)stream, done};
+            const int32_t type = tensors[i].param_type;
+            CLS_TRY(type == CBH_TYPE_F32   ? launch_all<float>(R, A.state)
+                    : type == CBH_TYPE_F16 ? launch_all<_Float16>(R, A.state)
+                                           : launch_all<bf16_t>(R, A.state));
         }
         return CBH_OK;
     } catch (const std::exception& e) {

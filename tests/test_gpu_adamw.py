@@ -104,6 +104,10 @@ def check(new, ts, kind, small, copy=None, number=0, **kw):
         e = expected(t, small, number=number + i, **kw)
         for name in e:
             want = O.round_to(e[name], kind) if name == "p" else e[name]
+            if want.dtype == np.uint8:   # (0x7F and 0xFF are both NaN)
+                got, want = (np.where(c & 0x7F == 0x7F, 0x7F, c) for c in (u[name], want))
+                assert np.array_equal(got, want), (i, len(t["p"]), name)
+                continue
             assert np.array_equal(u[name], want, equal_nan=u[name].dtype.kind == "f"), (i, len(t["p"]), name)
         if copy:
             assert np.array_equal(u["c"], O.round_to(e["p"], copy), equal_nan=True), (i, "copy")
@@ -168,7 +172,7 @@ def test_nan_infinity_and_the_ends_of_f32(small):
     check(new, [t], "f32", small, step=2)
     if small:
         u = new[0]
-        assert (u["m"][:3] & 0x7F == 0x7F).all() and (u["v"][:3] == 0x7F).all()
+        assert (u["m"][:3] & 0x7F == 0x7F).all() and (u["v"][:3] & 0x7F == 0x7F).all()
         assert (u["m"][8:256] & 0x7F != 0x7F).all() and np.isfinite(u["ms"]).all() and np.isfinite(u["vs"]).all()
 
 
