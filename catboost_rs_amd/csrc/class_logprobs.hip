@@ -75,14 +75,18 @@ struct PartStat {   // of a part of a row, between launches
     double s, t;
     float m, none;
 };
+// Those of a workgroup's threads together, in a fixed order; every thread gets them.  One barrier; tmp: one a wave.
 template <int THREADS>
-__device__ __forceinline__ void block_stat(RunningStat& r, float c, float* tmp_f, double* tmp_d) {
-    const float m = block_reduce<THREADS>(r.m, MaxF(), tmp_f);
-    r.raise(m, c);
-    double v[2] = {r.s, r.t};
-    block_sums<THREADS>(v, tmp_d);
-    r.s = v[0];
-    r.t = v[1];
+__device__ __forceinline__ void block_stat(RunningStat& r, float c, PartStat* tmp) {
+    r.raise(wave_reduce(r.m, MaxF()), c);
+    r.s = wave_reduce(r.s, Add());
+    r.t = wave_reduce(r.t, Add());
+    if (THREADS == 64) return;
+    if (lane_id() == 0) tmp[threadIdx.x / 64] = PartStat{r.s, r.t, r.m, 0.0f};
+    __syncthreads();
+    r = RunningStat();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) r.join(tmp[w].m, tmp[w].s, tmp[w].t, c);
 }
 
 struct Asked {   // what is asked of every row, and where it goes
@@ -144,52 +148,65 @@ __device__ __forceinline__ void write_stats(const Asked& A, uint64_t row, const 
         A.stats[row * 3 + 2] = (float)e;
     }
 }
+// The log probabilities of a row's entries from, from + step, ...; the first of them by a score that was read before.
+template <class T>
+__device__ __forceinline__ uint32_t given_class(const Asked& A, uint64_t row, uint32_t i) {
+    return A.logprob && i < A.n_given ? (uint32_t)A.given[row * A.n_given + i] : ~0u;
+}
+template <class T>
+__device__ __forceinline__ float given_score(const Asked& A, const Rows<T>& X, uint64_t row, uint32_t j) {
+    if (j >= X.classes) return 0.0f;
+    const float x = to_f32(X.data[(int64_t)row * X.rs + (int64_t)j * X.cs]);
+    return A.allowed && !is_allowed(A.allowed + (int64_t)row * A.allowed_stride, j) ? -INFINITY : x;
+}
 template <class T>
 __device__ __forceinline__ void write_given(const Asked& A, const Rows<T>& X, uint64_t row, const RowStat& q, uint32_t from,
-                                            uint32_t step) {
+                                            uint32_t step, uint32_t j, float x) {
     if (!A.logprob) return;
-    const uint32_t* words = A.allowed ? A.allowed + (int64_t)row * A.allowed_stride : nullptr;
     for (uint32_t i = from; i < A.n_given; i += step) {
-        const uint32_t j = (uint32_t)A.given[row * A.n_given + i];
-        float lp = 0.0f;
-        if (j < X.classes) {
-            float x = to_f32(X.data[(int64_t)row * X.rs + (int64_t)j * X.cs]);
-            if (words && !is_allowed(words, j)) x = -INFINITY;
-            lp = log_prob(x, q, A.it);
+        if (i != from) {
+            j = given_class<T>(A, row, i);
+            x = given_score(A, X, row, j);
         }
-        A.logprob[row * A.n_given + i] = lp;
+        A.logprob[row * A.n_given + i] = j < X.classes ? log_prob(x, q, A.it) : 0.0f;
     }
 }
-// The `got` keys of best, the largest first.
+// The k largest of the `got` keys of best (0: none), the largest first.
 template <int THREADS>
 __device__ __forceinline__ void write_top(const Asked& A, uint64_t row, const u64* best, uint32_t got, const RowStat& q) {
     for (uint32_t i = threadIdx.x; i < got; i += THREADS) {
         const u64 key = best[i];
         uint32_t rank = 0;
         for (uint32_t j = 0; j < got; ++j) rank += best[j] > key;
+        if (key == 0 || rank >= A.k) continue;
         const float x = key_score((uint32_t)(key >> 32));
         A.top_logprob[row * A.k + rank] = log_prob(x, q, A.it);
         A.top_index[row * A.k + rank] = x == -INFINITY ? -1 : (int32_t)~(uint32_t)key;
     }
 }
 
-// A workgroup takes a row, or one of the `parts` segments of a row (few rows of many classes), whose sums and
-// k largest keys go to the workspace for join_kernel.  How the largest are found:
-//   kNone    k = 0
-//   kGroups  a bound from the maxima of every 32 classes, kept in LDS; the groups that reach it are read again
-//   kWhole   digits of the keys of all classes, read again for every digit (a k that is large beside the row)
-enum Select { kNone, kGroups, kWhole };
+// Keys of a segment that are kept beside its k largest: as many as reach the bound are mostly, and need no selection.
+constexpr uint32_t kSpare = 64;
+
+// A workgroup takes a row, or one of the `parts` segments of a row (few rows of many classes).  Sums and k largest keys
+// go to the workspace for finish_kernel, but for whole rows without the latter.  (With the epilogue in this kernel too, whose addresses and
+// f64 values do not fit beside the selection's, it took 165 registers and 4096 x 8192 bf16, k 64: 108 us.)  How the largest are found:
+//   kNone     k = 0
+//   kGroups   a bound from the maxima of every 32 classes, kept in LDS; the groups that reach it are read again
+//   kVectors  the same of every 4 or 8 classes, a vector
+//   kWhole    digits of the keys of all classes, read again for every digit (a k that is large beside the row)
+enum Select { kNone, kGroups, kVectors, kWhole };
 template <class T, bool kUnit, bool kMask, int THREADS, Select kSel, int CAP>
 __global__ __launch_bounds__(THREADS) void logprobs_kernel(Rows<T> X, Asked A, uint32_t parts, uint32_t seg,
                                                            PartStat* __restrict__ part_stat, u64* __restrict__ part_keys) {
-    constexpr int V = Pack<T>::V, U = kPacks<T>, W = THREADS / 64, KMAX = kSel == kWhole ? (int)kMaxTop : CAP / 2;
+    constexpr int V = Pack<T>::V, U = kPacks<T>, W = THREADS / 64, KMAX = kSel == kWhole ? (int)kMaxTop : CAP / 2 + (int)kSpare;
     extern __shared__ uint32_t groups[];
-    __shared__ u64 cand[kSel == kGroups ? W : 1][kSel == kGroups ? CAP : 1];
+    constexpr bool kBound = kSel == kGroups || kSel == kVectors;
+    __shared__ u64 cand[kBound ? W : 1][kBound ? CAP : 1];
     __shared__ u64 best[kSel == kNone ? 1 : KMAX];
     __shared__ CountLds lds;
     __shared__ uint32_t counts[W], nbest;
-    __shared__ float tmp_f[W];
-    __shared__ double tmp_d[W * 2];
+    __shared__ PartStat tmp[W];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = lane_id();
 
     for (uint64_t job = blockIdx.x; job < X.rows * parts; job += gridDim.x) {
@@ -201,8 +218,15 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(Rows<T> X, Asked A, u
             const float x = to_f32(x0[kUnit ? (int64_t)i : (int64_t)i * X.cs]);
             return kMask && !is_allowed(words, i) ? -INFINITY : x;
         };
+        auto vector_key = [&](uint32_t i) {   // the largest key of the classes from i on
+            uint32_t key = 0;
+            for (uint32_t j = i; j < min(i + V, n); ++j) key = max(key, order_key(score(j)));
+            return key;
+        };
         const uint32_t n_segs = (n + kSeg - 1) / kSeg;
         RunningStat run;
+        uint32_t own = ~0u;
+        if constexpr (kSel == kNone) own = parts == 1 ? given_class<T>(A, row, threadIdx.x) : ~0u;
         for (uint32_t s = wave; s < n_segs; s += W) {
             float x[U][V], vm[U], gm = -INFINITY;
             load_allowed<T, kUnit, kMask>(x0, X.cs, words, s * kSeg, n, x);
@@ -217,35 +241,55 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(Rows<T> X, Asked A, u
             if constexpr (kSel == kGroups) {
                 const uint32_t g = s * 64 + group_of<V>(lane);
                 uint32_t key = order_key(group_max<V>(vm, lane, MaxF()));
-                if (__any(run.s != run.s)) {   // since a NaN, which is the largest of its group, or +inf
+                // since a NaN, which is the largest of its group, or +inf (the tile is read again: kept until here, its scores
+                // took the kernel from 103 to 165 registers)
+                if (__any(run.s != run.s)) {
                     uint32_t keys[U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        keys[u] = 0;
-#pragma unroll
-                        for (int v = 0; v < V; ++v) keys[u] = max(keys[u], order_key(x[u][v]));
-                    }
+                    for (int u = 0; u < U; ++u) keys[u] = vector_key(s * kSeg + (u * 64 + lane) * V);
                     key = group_max<V>(keys, lane, MaxU());
                 }
                 groups[g] = g * kGroup < n ? key : 0;
+            } else if constexpr (kSel == kVectors) {
+                const bool nan = __any(run.s != run.s);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t i = s * kSeg + (u * 64 + lane) * V;
+                    groups[(s * U + u) * 64 + lane] = i >= n ? 0 : nan ? vector_key(i) : order_key(vm[u]);
+                }
             }
         }
         if (kSel != kNone && threadIdx.x == 0) nbest = 0;
-        __syncthreads();
-        block_stat<THREADS>(run, A.c, tmp_f, tmp_d);
-        const RowStat q = row_stat(run);
-        if (parts == 1) {
+        if (kSel != kNone && THREADS == 64) __syncthreads();
+        if (kSel == kNone && parts == 1) {
+            const float own_score = given_score(A, X, row, own);
+            block_stat<THREADS>(run, A.c, tmp);
+            const RowStat q = row_stat(run);
             if (threadIdx.x == 0) write_stats(A, row, run, q);
-            write_given(A, X, row, q, threadIdx.x, THREADS);
-        } else if (threadIdx.x == 0) {
-            part_stat[job] = PartStat{run.s, run.t, run.m, 0.0f};
+            write_given(A, X, row, q, threadIdx.x, THREADS, own, own_score);
+        } else {
+            block_stat<THREADS>(run, A.c, tmp);
+            if (threadIdx.x == 0) part_stat[job] = PartStat{run.s, run.t, run.m, 0.0f};
         }
-        if constexpr (kSel == kGroups) {
-            const uint32_t bound =
-                (uint32_t)kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, n_segs * 64, A.k, &lds);
+        if constexpr (kBound) {
+            const uint32_t n_groups = n_segs * (kSel == kGroups ? 64 : 64 * U);
+            const uint32_t bound = (uint32_t)kth_of<THREADS>([&](uint32_t i) { return (u64)groups[i]; }, n_groups, A.k, &lds);
             Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
             C.set_bound((u64)bound << 32);
             for (uint32_t s = wave; s < n_segs; s += W) {
+                if constexpr (kSel == kVectors) {
+                    for (int u = 0; u < U; ++u) {
+                        const bool hit = groups[(s * U + u) * 64 + lane] >= bound;
+                        if (!__any(hit)) continue;
+                        const uint32_t i = s * kSeg + (u * 64 + lane) * V;
+                        for (int v = 0; v < V; ++v) {
+                            const bool have = hit && i + v < n;
+                            const float x = have ? score(i + v) : -INFINITY;
+                            if (__any(have && !(x < C.fbound))) C.offer(x, first + i + v, have, A.k);
+                        }
+                    }
+                    continue;
+                }
                 u64 hit = __ballot(groups[s * 64 + lane] >= bound);
                 while (hit) {   // two groups at a time, a class a lane
                     const uint32_t a = (uint32_t)__builtin_ctzll(hit);
@@ -264,7 +308,7 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(Rows<T> X, Asked A, u
 #pragma unroll
             for (int w = 0; w < W; ++w) total += counts[w];
             u64 kth = 1;
-            if (total > A.k) kth = kth_of<THREADS>(cand_at, W * CAP, A.k, &lds);
+            if (total > A.k + kSpare) kth = kth_of<THREADS>(cand_at, W * CAP, A.k, &lds);
             for (uint32_t i = threadIdx.x; i < W * CAP; i += THREADS) {
                 const u64 key = cand_at(i);
                 if (key >= kth) best[atomicAdd(&nbest, 1u)] = key;
@@ -281,45 +325,55 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(Rows<T> X, Asked A, u
         if constexpr (kSel != kNone) {
             __syncthreads();
             const uint32_t got = nbest;
-            if (parts == 1) write_top<THREADS>(A, row, best, got, q);
-            else
-                for (uint32_t i = threadIdx.x; i < A.k; i += THREADS) part_keys[job * A.k + i] = i < got ? best[i] : 0;
+            const uint32_t slots = A.k + kSpare;
+            for (uint32_t i = threadIdx.x; i < slots; i += THREADS) part_keys[job * slots + i] = i < got ? best[i] : 0;
         }
         __syncthreads();
     }
 }
 
-// The segments of a row together.
+// What is written of a row, from its sums and largest keys, or from those of its segments.
 template <class T, int THREADS>
-__global__ __launch_bounds__(THREADS) void join_kernel(Rows<T> X, Asked A, uint32_t parts, const PartStat* __restrict__ part_stat,
-                                                       const u64* __restrict__ part_keys) {
-    __shared__ u64 best[kMaxTop];
+__global__ __launch_bounds__(THREADS) void finish_kernel(Rows<T> X, Asked A, uint32_t parts, const PartStat* __restrict__ part_stat,
+                                                         const u64* __restrict__ part_keys) {
+    __shared__ u64 best[kMaxTop + kSpare];
     __shared__ CountLds lds;
     __shared__ uint32_t nbest;
-    __shared__ float tmp_f[THREADS / 64];
-    __shared__ double tmp_d[THREADS / 64 * 2];
+    __shared__ PartStat tmp[THREADS / 64];
+    const uint32_t slots = A.k + kSpare;
     for (uint64_t row = blockIdx.x; row < X.rows; row += gridDim.x) {
-        const u64* keys = part_keys + row * parts * A.k;
+        const u64* keys = part_keys + row * parts * slots;
+        uint32_t got = A.k;
         if (threadIdx.x == 0) nbest = 0;
         RunningStat run;
-        for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
-            const PartStat ps = part_stat[row * parts + p];
-            run.join(ps.m, ps.s, ps.t, A.c);
+        const uint32_t own = given_class<T>(A, row, threadIdx.x);
+        const float own_score = given_score(A, X, row, own);
+        if (parts == 1) {
+            const PartStat ps = part_stat[row];
+            run.m = ps.m, run.s = ps.s, run.t = ps.t;
+            got = slots;
+            if (A.k)
+                for (uint32_t i = threadIdx.x; i < slots; i += THREADS) best[i] = keys[i];
+            __syncthreads();
+        } else {
+            for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
+                const PartStat ps = part_stat[row * parts + p];
+                run.join(ps.m, ps.s, ps.t, A.c);
+            }
+            block_stat<THREADS>(run, A.c, tmp);
+            if (A.k) {
+                const u64 kth = kth_of<THREADS>([&](uint32_t i) { return keys[i]; }, parts * slots, A.k, &lds);
+                for (uint32_t i = threadIdx.x; i < parts * slots; i += THREADS) {
+                    const u64 key = keys[i];
+                    if (key != 0 && key >= kth) best[atomicAdd(&nbest, 1u)] = key;
+                }
+                __syncthreads();
+            }
         }
-        __syncthreads();
-        block_stat<THREADS>(run, A.c, tmp_f, tmp_d);
         const RowStat q = row_stat(run);
         if (threadIdx.x == 0) write_stats(A, row, run, q);
-        write_given(A, X, row, q, threadIdx.x, THREADS);
-        if (A.k) {
-            const u64 kth = kth_of<THREADS>([&](uint32_t i) { return keys[i]; }, parts * A.k, A.k, &lds);
-            for (uint32_t i = threadIdx.x; i < parts * A.k; i += THREADS) {
-                const u64 key = keys[i];
-                if (key != 0 && key >= kth) best[atomicAdd(&nbest, 1u)] = key;
-            }
-            __syncthreads();
-            write_top<THREADS>(A, row, best, nbest, q);
-        }
+        write_given(A, X, row, q, threadIdx.x, THREADS, own, own_score);
+        if (A.k) write_top<THREADS>(A, row, best, got, q);
         __syncthreads();
     }
 }
@@ -330,7 +384,7 @@ __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
     const uint32_t n = X.classes;
     for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
         const T* x0 = X.data + (int64_t)row * X.rs;
-        const uint32_t bits = A.allowed ? A.allowed[(int64_t)row * A.allowed_stride] : ~0u;
+        const uint32_t bits = A.allowed ? A.allowed[(int64_t)row * A.allowed_stride] : ~0u, own = given_class<T>(A, row, 0);
         float x[NMAX];
         RunningStat run;
 #pragma unroll
@@ -343,7 +397,7 @@ __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
         for (int i = 0; i < NMAX; ++i) run.add_one(x[i], A.c);
         const RowStat q = row_stat(run);
         write_stats(A, row, run, q);
-        write_given(A, X, row, q, 0, 1);
+        write_given(A, X, row, q, 0, 1, own, given_score(A, X, row, own));
         if constexpr (kTop) {
             uint32_t key[NMAX], rank[NMAX];
 #pragma unroll
@@ -369,6 +423,176 @@ __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
     }
 }
 
+// ---- short rows -------------------------------------------------------------------------------
+// Over the G lanes of a group; every lane gets it.
+template <int G, class V, class Op>
+__device__ __forceinline__ V group_reduce(V v, Op op) {
+    if constexpr (G >= 2) v = op(v, dpp_move<0xB1, 0xf>(v, v));     // lanes 1 0 3 2
+    if constexpr (G >= 4) v = op(v, dpp_move<0x4E, 0xf>(v, v));     // lanes 2 3 0 1
+    if constexpr (G >= 8) v = op(v, dpp_move<0x141, 0xf>(v, v));    // mirrored within 8
+    if constexpr (G >= 16) v = op(v, dpp_move<0x140, 0xf>(v, v));   // mirrored within 16
+    if constexpr (G >= 32) v = op(v, __shfl_xor(v, 16));
+    if constexpr (G >= 64) v = op(v, __shfl_xor(v, 32));
+    return v;
+}
+// A lane's scores of a row of at most G R V classes: vector u of lane l holds the classes from (u G + l) V on (kVec), or one
+// class, (u G + l).
+template <class T, bool kVec>
+constexpr int kWide = kVec ? Pack<T>::V : 1;
+template <class T, int G, int R, bool kVec>
+__device__ __forceinline__ void load_short(const T* row, int64_t cs, uint32_t l, uint32_t n, const uint32_t* words,
+                                           float (&x)[R][kWide<T, kVec>]) {
+    constexpr int V = kWide<T, kVec>;
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const uint32_t i = (u * G + l) * V;
+        if constexpr (kVec) load_pack<T, true>(row, 1, i, n, -INFINITY, x[u]);
+        else x[u][0] = i < n ? to_f32(row[(int64_t)i * cs]) : -INFINITY;
+    }
+    if (words) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const uint32_t i = (u * G + l) * V, bits = i < n ? words[i >> 5] >> (i & 31) : 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[u][v] = bits >> v & 1 ? x[u][v] : -INFINITY;
+        }
+    }
+}
+
+// The largest bound that k of a wave's keys reach, the highest bits first, from the one in which they differ on (0: no key; at least k
+// are not 0); it may end below the k-th largest where exactly k are at the bound or above.
+template <int N>
+__device__ __forceinline__ uint32_t wave_kth(const uint32_t (&key)[N], uint32_t k) {
+    uint32_t hi = key[0], lo = key[0] - 1;   // (0 is no key: the largest here)
+#pragma unroll
+    for (int r = 1; r < N; ++r) {
+        hi = max(hi, key[r]);
+        lo = min(lo, key[r] - 1);
+    }
+    hi = wave_reduce(hi, MaxU());
+    lo = ~wave_reduce(~lo, MaxU()) + 1;
+    const int bits = hi > lo ? 32 - __builtin_clz(hi ^ lo) : 0;
+    uint32_t bound = bits == 32 ? 0 : hi >> bits << bits;
+    for (int b = bits - 1; b >= 0; --b) {
+        const uint32_t t = bound | 1u << b;
+        uint32_t c = 0;
+#pragma unroll
+        for (int r = 0; r < N; ++r) c += (uint32_t)__popcll(__ballot(key[r] >= t));
+        if (c >= k) bound = t;
+        if (c == k) break;
+    }
+    return bound;
+}
+
+// Rows of up to 2048 classes in the registers of G lanes, 64 for the largest classes.  Those: the k-th largest of the vectors'
+// maxima, where there are at least 4 k, is a bound that k classes reach, else that of all classes; those that reach it are
+// listed in LDS and take the places that the count of larger ones gives.
+constexpr uint32_t kShort = 2048;
+template <class T, int G, int R, bool kVec, int CAP>
+__global__ __launch_bounds__(256) void logprobs_short_kernel(Rows<T> X, Asked A) {
+    constexpr int V = kWide<T, kVec>;
+    __shared__ u64 cand[4][CAP ? CAP : 1];
+    const uint32_t l = threadIdx.x % G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), n = X.classes;
+    for (uint64_t first = (uint64_t)blockIdx.x * (256 / G); first < X.rows; first += (uint64_t)gridDim.x * (256 / G)) {
+        const uint64_t mine = first + threadIdx.x / G, row = min(mine, X.rows - 1);
+        const bool there = mine < X.rows;   // (the same in a wave where G = 64)
+        const uint32_t* words = A.allowed ? A.allowed + (int64_t)row * A.allowed_stride : nullptr;
+        float x[R][V], lm = -INFINITY, se = 0.0f, sy = 0.0f;
+        load_short<T, G, R, kVec>(X.data + (int64_t)row * X.rs, X.cs, l, n, words, x);
+        const uint32_t own = given_class<T>(A, row, l);
+        const float own_score = given_score(A, X, row, own);
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+#pragma unroll
+            for (int v = 0; v < V; ++v) lm = fmaxf(lm, x[u][v]);
+        RunningStat run;
+        run.m = fmaxf(kLowest, group_reduce<G>(lm, MaxF()));
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float e, ey;
+                run.weigh(x[u][v], A.c, e, ey);
+                se += e;
+                sy += ey;
+            }
+        run.s = group_reduce<G>((double)se, Add());
+        run.t = group_reduce<G>((double)sy, Add());
+        const RowStat q = row_stat(run);
+        if (there && l == 0) write_stats(A, row, run, q);
+        if (there) write_given(A, X, row, q, l, G, own, own_score);
+        if constexpr (CAP > 0) {
+            static_assert(G == 64, "a row a wave");
+            if (!there) continue;
+            uint32_t key[R * V], most[R];
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                most[u] = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    key[u * V + v] = (u * G + l) * V + v < n ? order_key(x[u][v]) : 0;
+                    most[u] = max(most[u], key[u * V + v]);
+                }
+            }
+            Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
+            C.set_bound((u64)(A.k * 4 <= n / V ? wave_kth(most, A.k) : wave_kth(key, A.k)) << 32);
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const uint32_t i = (u * G + l) * V + v;
+                    if (__any(i < n && !(x[u][v] < C.fbound))) C.offer(x[u][v], i, i < n, A.k);
+                }
+            wave_fence();
+            for (uint32_t i = l; i < C.count; i += 64) {
+                const u64 key = cand[wave][i];
+                uint32_t rank = 0;
+                for (uint32_t j = 0; j < C.count; ++j) rank += cand[wave][j] > key;
+                if (rank >= A.k) continue;
+                const float y = key_score((uint32_t)(key >> 32));
+                A.top_logprob[row * A.k + rank] = log_prob(y, q, A.it);
+                A.top_index[row * A.k + rank] = y == -INFINITY ? -1 : (int32_t)~(uint32_t)key;
+            }
+            wave_fence();
+        }
+    }
+}
+template <class T, int G, int R, bool kVec>
+void launch_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
+    const unsigned grid = row_grid((X.rows + 256 / G - 1) / (256 / G));
+    if constexpr (G == 64) {
+        if (A.k) {
+            if (A.k <= 128) logprobs_short_kernel<T, G, R, kVec, 256><<<grid, 256, 0, st>>>(X, A);
+            else logprobs_short_kernel<T, G, R, kVec, 2048><<<grid, 256, 0, st>>>(X, A);
+            return;
+        }
+    }
+    logprobs_short_kernel<T, G, R, kVec, 0><<<grid, 256, 0, st>>>(X, A);
+}
+template <class T>
+int run_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
+    constexpr uint32_t V = Pack<T>::V;
+    const uint32_t n = X.classes;
+    // by vectors where they fill the lanes: half of them, or a part of the wave's for the sums alone
+    if (X.cs == 1 && (n > 32 * V || !A.k)) {
+        if (n <= 8 * V) launch_short<T, 8, 1, true>(X, A, st);
+        else if (n <= 16 * V) launch_short<T, 16, 1, true>(X, A, st);
+        else if (n <= 32 * V) launch_short<T, 32, 1, true>(X, A, st);
+        else if (n <= 64 * V) launch_short<T, 64, 1, true>(X, A, st);
+        else if (n <= 128 * V) launch_short<T, 64, 2, true>(X, A, st);
+        else if (n <= 256 * V) launch_short<T, 64, 4, true>(X, A, st);
+        else launch_short<T, 64, 32 / V, true>(X, A, st);
+    } else {
+        if (n <= 64) launch_short<T, 64, 1, false>(X, A, st);
+        else if (n <= 128) launch_short<T, 64, 2, false>(X, A, st);
+        else if (n <= 256) launch_short<T, 64, 4, false>(X, A, st);
+        else if (n <= 512) launch_short<T, 64, 8, false>(X, A, st);
+        else launch_short<T, 64, 32, false>(X, A, st);
+    }
+    CLS_TRY(hipGetLastError());
+    return CBH_OK;
+}
+
 // Segments of a row: one, unless the rows alone leave CUs idle and a row is long.  They start at a multiple of 32
 // classes, a word of the allowed ones.
 constexpr uint32_t kMinSeg = 16384, kMaxGroupSegs = 64;
@@ -383,31 +607,41 @@ Plan plan_parts(uint64_t rows, uint32_t classes) {
     return Plan{(classes + seg - 1) / seg, seg};
 }
 
+// Rows enough to fill the chip are taken by workgroups of one wave, whose barriers cost nothing; long rows whose largest are
+// asked for are not (4096 x 8192 bf16, k 5: 34 against 43 us; 4096 x 65536: 178 against 136).
+constexpr uint64_t kManyRows = 2048;
+constexpr uint32_t kWaveRow = 16384;
 template <class T, bool kUnit, bool kMask>
 int launch_rows(const Rows<T>& X, const Asked& A, const Plan& P, void* workspace, hipStream_t st) {
     const uint32_t n = X.classes, k = A.k, seg = P.seg;
-    PartStat* ps = P.parts > 1 ? (PartStat*)workspace : nullptr;
-    u64* pk = P.parts > 1 ? (u64*)(ps + X.rows * P.parts) : nullptr;
+    PartStat* ps = (PartStat*)workspace;
+    u64* pk = (u64*)(ps + X.rows * P.parts);   // (neither is touched for whole rows without a k, which have no workspace)
     const unsigned grid = row_grid(X.rows * P.parts);
     const uint32_t shortest = n - seg * (P.parts - 1);
-#define RUN(TH, SEL, CAP, LDS) logprobs_kernel<T, kUnit, kMask, TH, SEL, CAP><<<grid, TH, LDS, st>>>(X, A, P.parts, seg, ps, pk)
-    // by groups where k is at most a quarter of the shortest segment's
+    const bool many = X.rows * P.parts >= kManyRows && (k == 0 || seg <= kWaveRow);
+#define RUN(SEL, CAP, LDS)                                                                                              \
+    (many ? logprobs_kernel<T, kUnit, kMask, 64, SEL, CAP><<<grid, 64, LDS, st>>>(X, A, P.parts, seg, ps, pk) \
+          : logprobs_kernel<T, kUnit, kMask, 256, SEL, CAP><<<grid, 256, LDS, st>>>(X, A, P.parts, seg, ps, pk))
+    // by groups, or vectors, where k is at most a quarter of the shortest segment's
     const size_t lds = sizeof(uint32_t) * 64 * ((seg + kSeg - 1) / kSeg);
-    if (n <= 2048) {
-        if (k == 0) RUN(64, kNone, 2, 0);
-        else RUN(64, kWhole, 2, 0);
-    } else if (k == 0) {
-        RUN(256, kNone, 2, 0);
+    constexpr uint32_t V = Pack<T>::V;
+    const size_t lds_v = sizeof(uint32_t) * (kSeg / V) * ((seg + kSeg - 1) / kSeg);
+    if (k == 0) {
+        RUN(kNone, 2, 0);
     } else if (k * 4 <= shortest / kGroup) {
-        if (k <= 128) RUN(256, kGroups, 256, lds);
-        else RUN(256, kGroups, 2048, lds);
+        if (k <= 128) RUN(kGroups, 256, lds);
+        else RUN(kGroups, 2048, lds);
+    } else if (k * 4 <= shortest / V && lds_v <= 65536) {
+        if (k <= 128) RUN(kVectors, 256, lds_v);
+        else RUN(kVectors, 2048, lds_v);
     } else {
-        RUN(256, kWhole, 2, 0);
+        RUN(kWhole, 2, 0);
     }
 #undef RUN
     CLS_TRY(hipGetLastError());
-    if (P.parts > 1) {
-        join_kernel<T, 256><<<row_grid(X.rows), 256, 0, st>>>(X, A, P.parts, ps, pk);
+    if (P.parts > 1 || k) {
+        if (P.parts == 1 && k <= 256) finish_kernel<T, 64><<<row_grid(X.rows), 64, 0, st>>>(X, A, 1, ps, pk);
+        else finish_kernel<T, 256><<<row_grid(X.rows), 256, 0, st>>>(X, A, P.parts, ps, pk);
         CLS_TRY(hipGetLastError());
     }
     return CBH_OK;
@@ -428,6 +662,7 @@ int run_logprobs(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int6
         CLS_TRY(hipGetLastError());
         return CBH_OK;
     }
+    if (n <= kShort) return run_short(X, A, st);
     const Plan P = plan_parts(rows, n);
     if (cs == 1) return A.allowed ? launch_rows<T, true, true>(X, A, P, workspace, st) : launch_rows<T, true, false>(X, A, P, workspace, st);
     return A.allowed ? launch_rows<T, false, true>(X, A, P, workspace, st) : launch_rows<T, false, false>(X, A, P, workspace, st);
@@ -464,7 +699,7 @@ __device__ __forceinline__ RowFactors row_factors(const Upstream& P, uint64_t ro
     f.m = none ? 0.0f : s[0];
     f.log_z = (double)s[1];
     f.far = (double)s[2];
-    const double r = none ? 0.0 : -P.it * exp(-f.log_z);
+    const double r = none ? 0.0 : -P.it * exp_f64(-f.log_z);
     f.a = none ? 0.0f : clamp_finite(r * (f.G + f.h * f.far));
     f.b = none ? 0.0f : clamp_finite(r * f.h * kLn2);
     return f;
@@ -539,6 +774,56 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P
     }
 }
 
+// Rows of up to 2048 classes in the registers of G lanes.  Lists of more than kShortGiven entries go the other ways: the owner of a
+// class goes through the whole list for it.
+constexpr uint32_t kShortGiven = 8;
+template <class T, int G, int R>
+__global__ __launch_bounds__(256) void logprob_grad_short_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs) {
+    constexpr int V = Pack<T>::V;
+    const uint32_t l = threadIdx.x % G, n = X.classes;
+    for (uint64_t first = (uint64_t)blockIdx.x * (256 / G); first < X.rows; first += (uint64_t)gridDim.x * (256 / G)) {
+        const uint64_t mine = first + threadIdx.x / G, row = min(mine, X.rows - 1);
+        const uint32_t* words = P.allowed ? P.allowed + (int64_t)row * P.allowed_stride : nullptr;
+        const int32_t* given = P.given + row * P.n_given;
+        const float* g = P.logprob_grad + row * P.n_given;
+        const T* x0 = X.data + (int64_t)row * X.rs;
+        float x[R][V];
+        load_short<T, G, R, true>(x0, 1, l, n, nullptr, x);
+        double sum = 0.0;
+        bool some = false;
+        for (uint32_t i = 0; i < P.n_given; ++i)
+            if ((uint32_t)given[i] < n) {
+                sum += (double)g[i];
+                some |= g[i] != 0.0f;
+            }
+        const RowFactors f = row_factors(P, row, sum, some);
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const uint32_t i = (u * G + l) * V, bits = words && i < n ? words[i >> 5] >> (i & 31) : ~0u;
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[u][v] = f.zero || !(bits >> v & 1) ? 0.0f : grad_of(x[u][v], f, P.c);
+        }
+        if (!f.zero)
+            for (uint32_t i = 0; i < P.n_given; ++i) {
+                const uint32_t j = (uint32_t)given[i];
+                if (j >= n || j / V % G != l || (words && !is_allowed(words, j))) continue;
+                double own = 0.0;
+                for (uint32_t e = 0; e < P.n_given; ++e) own += (uint32_t)given[e] == j ? (double)g[e] : 0.0;
+                const float y = grad_of_given(to_f32(x0[j]), own, f, P.it);
+#pragma unroll
+                for (int u = 0; u < R; ++u)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[u][v] = (u * G + l) * V + v == j ? y : x[u][v];
+            }
+        if (mine >= X.rows) continue;
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const uint32_t i = (u * G + l) * V;
+            if (i < n) store_pack<T, true>(grad + (int64_t)row * grs, 1, i, n, x[u]);
+        }
+    }
+}
+
 // Few classes, and rows next to each other: a thread takes `seg` classes of a row.
 template <class T, bool kMask>
 __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs,
@@ -582,7 +867,20 @@ int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t 
              int64_t grs, int64_t gcs, hipStream_t st) {
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
     T* g = (T*)grad;
-    if (n <= 32 || (rs == 1 && grs == 1 && cs != 1)) {
+    constexpr uint32_t V = Pack<T>::V;
+    if (cs == 1 && gcs == 1 && n <= kShort && P.n_given <= kShortGiven) {
+#define RUN(G, R) logprob_grad_short_kernel<T, G, R><<<row_grid((rows + 256 / G - 1) / (256 / G)), 256, 0, st>>>(X, P, g, grs)
+        if (n <= 2 * V) RUN(2, 1);
+        else if (n <= 4 * V) RUN(4, 1);
+        else if (n <= 8 * V) RUN(8, 1);
+        else if (n <= 16 * V) RUN(16, 1);
+        else if (n <= 32 * V) RUN(32, 1);
+        else if (n <= 64 * V) RUN(64, 1);
+        else if (n <= 128 * V) RUN(64, 2);
+        else if (n <= 256 * V) RUN(64, 4);
+        else RUN(64, (int)(32 / V));
+#undef RUN
+    } else if (n <= 32 || (rs == 1 && grs == 1 && cs != 1)) {
         const uint32_t seg = 32, segs = (n + seg - 1) / seg;
         const unsigned grid = row_grid((rows + 255) / 256 * segs);
         if (P.allowed) logprob_grad_few_kernel<T, true><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, segs, seg);
@@ -618,9 +916,9 @@ int check_lists(const void* given, uint32_t n_given, uint64_t rows, uint32_t cla
 }  // namespace
 
 extern "C" uint64_t cbh_class_logprobs_workspace(uint64_t rows, uint32_t classes, uint32_t k) {
-    if (classes <= 32) return 0;
+    if (classes <= kShort) return 0;
     const Plan P = plan_parts(rows, classes);
-    return P.parts == 1 ? 0 : rows * P.parts * (8 * (uint64_t)k + sizeof(PartStat));
+    return P.parts == 1 && k == 0 ? 0 : rows * P.parts * (8 * (uint64_t)(k ? k + kSpare : 0) + sizeof(PartStat));
 }
 
 extern "C" int cbh_class_logprobs(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,

@@ -21,7 +21,8 @@ pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1, 1, 1), (3, 2, 2, 1), (700, 10, 3, 3), (70, 32, 1, 32), (9, 33, 2, 5), (5, 64, 64, 64), (4, 1000, 1, 5),
           (3, 2048, 7, 256), (2, 2049, 1, 300), (2, 5000, 3, 1024), (5, 50021, 4, 20), (2, 8193, 1, 0), (1, 70001, 1, 64),
-          (3, 140003, 2, 257), (600, 4099, 1, 9), (1, 40000, 1024, 0), (300, 20, 40, 0)]
+          (3, 140003, 2, 257), (600, 4099, 1, 9), (1, 40000, 1024, 0), (300, 20, 40, 0),
+          (333, 70, 1, 14), (65, 129, 8, 0), (70, 256, 9, 64), (31, 257, 2, 65), (1001, 40, 1, 0), (9, 700, 1, 0), (6, 2048, 1, 64)]
 
 
 def words(allowed):
