@@ -215,7 +215,8 @@ def class_logprobs(scores, given=None, *, temperature=1.0, k=0, allowed=None):
     [rows] or [rows][m], or None; an index outside the classes is no entry and has 0.  ``allowed`` as in
     :func:`sample_classes`.  Gives ``logprob`` f32 of given's shape, ``entropy`` [rows] f32 in nats, ``stats`` [rows][3]
     f32 (what :func:`logprob_gradients` takes), ``top_logprob`` [rows][k] f32, largest first, and ``top_index``
-    [rows][k] i32 (-1 where fewer classes have a probability); 0 <= k <= min(classes, 1024)."""
+    [rows][k] i32 (-1 where fewer classes have a probability); 0 <= k <= min(classes, 1024).  ``logprob`` is None without
+    ``given``, the top ones are without ``k``."""
     torch = _state.get("torch") or _bind()
     t, n, m, rs, cs = _scores(torch, scores)
     given, count = (None, 0) if given is None else _given(torch, given, n, scores)
@@ -224,15 +225,16 @@ def class_logprobs(scores, given=None, *, temperature=1.0, k=0, allowed=None):
     k = k if 0 <= k <= 1024 else 1 << 30   # (refused below, before anything of that size is allocated)
     with _on(scores):
         dev, f32 = scores.device, torch.float32
-        logprob = torch.empty((n, 0) if given is None else given.shape, dtype=f32, device=dev)
+        logprob = None if given is None else torch.empty(given.shape, dtype=f32, device=dev)
         entropy, stats = torch.empty(n, dtype=f32, device=dev), torch.empty((n, 3), dtype=f32, device=dev)
-        shape = (n, k if k <= 1024 else 0)
-        top_logprob, top_index = torch.empty(shape, dtype=f32, device=dev), torch.empty(shape, dtype=torch.int32, device=dev)
+        top_logprob = top_index = None
+        if 0 < k <= 1024:
+            top_logprob, top_index = torch.empty((n, k), dtype=f32, device=dev), torch.empty((n, k), dtype=torch.int32, device=dev)
         size = _state["logprobs_ws"](n, m, k) if k <= 1024 else 0
         ws = _workspace(torch, size, scores)
         _state["check"](_state["logprobs"](scores.data_ptr(), t, n, m, rs, cs, _addr(given), count, float(temperature),
-                                           _addr(allowed), astride, k, logprob.data_ptr(), entropy.data_ptr(),
-                                           stats.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), _addr(ws),
+                                           _addr(allowed), astride, k, _addr(logprob), entropy.data_ptr(),
+                                           stats.data_ptr(), _addr(top_logprob), _addr(top_index), _addr(ws),
                                            size, _stream(scores)))
     return ClassLogprobs(logprob, entropy, stats, top_logprob, top_index)
 

@@ -187,6 +187,7 @@ __device__ __forceinline__ void write_top(const Asked& A, uint64_t row, const u6
 
 // Keys of a segment that are kept beside its k largest: as many as reach the bound are mostly, and need no selection.
 constexpr uint32_t kSpare = 64;
+constexpr uint32_t kRanked = 384;   // keys of a row that are ranked among one another without a selection
 
 // A workgroup takes a row, or one of the `parts` segments of a row (few rows of many classes).  Sums and k largest keys
 // go to the workspace for finish_kernel, but for whole rows without the latter.  (With the epilogue in this kernel too, whose addresses and
@@ -348,28 +349,38 @@ __global__ __launch_bounds__(THREADS) void finish_kernel(Rows<T> X, Asked A, uin
         RunningStat run;
         const uint32_t own = given_class<T>(A, row, threadIdx.x);
         const float own_score = given_score(A, X, row, own);
-        if (parts == 1) {
-            const PartStat ps = part_stat[row];
-            run.m = ps.m, run.s = ps.s, run.t = ps.t;
-            got = slots;
-            if (A.k)
-                for (uint32_t i = threadIdx.x; i < slots; i += THREADS) best[i] = keys[i];
-            __syncthreads();
-        } else {
-            for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
-                const PartStat ps = part_stat[row * parts + p];
-                run.join(ps.m, ps.s, ps.t, A.c);
+        for (uint32_t p = threadIdx.x; p < parts; p += THREADS) {
+            const PartStat ps = part_stat[row * parts + p];
+            run.join(ps.m, ps.s, ps.t, A.c);
+        }
+        __syncthreads();
+        if (A.k) {   // (their order does not matter: a key's place is the count of larger ones)
+            for (uint32_t i = threadIdx.x; i < parts * slots; i += THREADS) {
+                const u64 key = keys[i];
+                if (key == 0) continue;
+                const uint32_t at = atomicAdd(&nbest, 1u);
+                if (at < kMaxTop + kSpare) best[at] = key;
             }
-            block_stat<THREADS>(run, A.c, tmp);
-            if (A.k) {
-                const u64 kth = kth_of<THREADS>([&](uint32_t i) { return keys[i]; }, parts * slots, A.k, &lds);
-                for (uint32_t i = threadIdx.x; i < parts * slots; i += THREADS) {
-                    const u64 key = keys[i];
+            __syncthreads();
+            got = nbest;
+            if (got > A.k && got > kRanked) {
+                const bool here = got <= kMaxTop + kSpare;
+                const uint32_t n = here ? got : parts * slots;
+                auto key_at = [&](uint32_t i) { return here ? best[i] : keys[i]; };
+                const u64 kth = kth_of<THREADS>(key_at, n, A.k, &lds);
+                // (in place: a round's keys are read before any of it is written, and none lands behind what was read)
+                if (threadIdx.x == 0) nbest = 0;
+                for (uint32_t i0 = 0; i0 < n; i0 += THREADS) {
+                    const uint32_t i = i0 + threadIdx.x;
+                    const u64 key = i < n ? key_at(i) : 0;
+                    __syncthreads();
                     if (key != 0 && key >= kth) best[atomicAdd(&nbest, 1u)] = key;
+                    __syncthreads();
                 }
-                __syncthreads();
+                got = A.k;
             }
         }
+        block_stat<THREADS>(run, A.c, tmp);
         const RowStat q = row_stat(run);
         if (threadIdx.x == 0) write_stats(A, row, run, q);
         write_given(A, X, row, q, threadIdx.x, THREADS, own, own_score);
@@ -413,12 +424,17 @@ __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
                     rank[i] += ahead;
                     rank[j] += !ahead;
                 }
+            for (uint32_t r = 0; r < A.k; ++r) {
+                float y = 0.0f;
+                int32_t at = -1;
 #pragma unroll
-            for (int i = 0; i < NMAX; ++i)
-                if ((uint32_t)i < n && rank[i] < A.k) {
-                    A.top_logprob[row * A.k + rank[i]] = log_prob(key_score(key[i]), q, A.it);
-                    A.top_index[row * A.k + rank[i]] = x[i] == -INFINITY ? -1 : i;
+                for (int i = 0; i < NMAX; ++i) {
+                    y = rank[i] == r ? x[i] : y;
+                    at = rank[i] == r ? i : at;
                 }
+                A.top_logprob[row * A.k + r] = log_prob(y, q, A.it);
+                A.top_index[row * A.k + r] = y == -INFINITY ? -1 : at;
+            }
         }
     }
 }
@@ -655,7 +671,9 @@ int run_logprobs(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int6
         const unsigned grid = row_grid((rows + 255) / 256);
 #define FEW(N) (A.k ? logprobs_few_kernel<T, N, true><<<grid, 256, 0, st>>>(X, A) \
                     : logprobs_few_kernel<T, N, false><<<grid, 256, 0, st>>>(X, A))
-        if (n <= 8) FEW(8);
+        if (n <= 4) FEW(4);
+        else if (n <= 8) FEW(8);
+        else if (n <= 12) FEW(12);
         else if (n <= 16) FEW(16);
         else FEW(32);
 #undef FEW
@@ -824,20 +842,24 @@ __global__ __launch_bounds__(256) void logprob_grad_short_kernel(Rows<T> X, Upst
     }
 }
 
-// Few classes, and rows next to each other: a thread takes `seg` classes of a row.
-template <class T, bool kMask>
+// Few classes, and rows next to each other: a thread takes up to NMAX classes of a row, in registers.  The
+// f64 of a row's factors and entries is a thread's, not a group of lanes': 1M x 10 f32 by rows takes 42 us by groups.
+template <class T, int NMAX>
 __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs,
-                                                               int64_t gcs, uint32_t segs, uint32_t seg) {
+                                                               int64_t gcs, uint32_t segs) {
     const uint64_t blocks = (X.rows + 255) / 256;
     for (uint64_t job = blockIdx.x; job < blocks * segs; job += gridDim.x) {
         const uint64_t row = job % blocks * 256 + threadIdx.x;
         if (row >= X.rows) continue;
-        const uint32_t first = (uint32_t)(job / blocks) * seg, end = min(X.classes, first + seg);
-        const T* x0 = X.data + (int64_t)row * X.rs;
-        T* g0 = grad + (int64_t)row * grs;
-        const uint32_t* words = kMask ? P.allowed + (int64_t)row * P.allowed_stride : nullptr;
+        const uint32_t first = (uint32_t)(job / blocks) * NMAX, n = min(X.classes - first, (uint32_t)NMAX);
+        const T* x0 = X.data + (int64_t)row * X.rs + (int64_t)first * X.cs;
+        T* g0 = grad + (int64_t)row * grs + (int64_t)first * gcs;
+        const uint32_t bits = P.allowed ? P.allowed[(int64_t)row * P.allowed_stride + first / 32] >> first % 32 : ~0u;
         const int32_t* given = P.given + row * P.n_given;
         const float* g = P.logprob_grad + row * P.n_given;
+        float x[NMAX];
+#pragma unroll
+        for (int j = 0; j < NMAX; ++j) x[j] = (uint32_t)j < n ? to_f32(x0[(int64_t)j * X.cs]) : -INFINITY;
         double G = 0.0;
         bool some = false;
         for (uint32_t i = 0; i < P.n_given; ++i)
@@ -846,19 +868,26 @@ __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstre
                 some |= g[i] != 0.0f;
             }
         const RowFactors f = row_factors(P, row, G, some);
-        for (uint32_t j = first; j < end; ++j) {
-            float v = 0.0f;
-            if (!f.zero && !(kMask && !is_allowed(words, j))) v = grad_of(to_f32(x0[(int64_t)j * X.cs]), f, P.c);
-            g0[(int64_t)j * gcs] = from_f32<T>(v);
-        }
-        if (f.zero) continue;
+        float y[NMAX];
+#pragma unroll
+        for (int j = 0; j < NMAX; ++j) y[j] = f.zero || !(bits >> j & 1) ? 0.0f : grad_of(x[j], f, P.c);
+        uint32_t done = f.zero ? ~0u : ~bits;
         for (uint32_t i = 0; i < P.n_given; ++i) {
-            const uint32_t j = (uint32_t)given[i];
-            if (j < first || j >= end || (kMask && !is_allowed(words, j))) continue;
+            const uint32_t j = (uint32_t)given[i] - first;
+            if ((uint32_t)given[i] >= X.classes || j >= n || (done >> j & 1)) continue;
+            done |= 1u << j;
             double sum = 0.0;
-            for (uint32_t e = 0; e < P.n_given; ++e) sum += (uint32_t)given[e] == j ? (double)g[e] : 0.0;
-            g0[(int64_t)j * gcs] = from_f32<T>(grad_of_given(to_f32(x0[(int64_t)j * X.cs]), sum, f, P.it));
+            for (uint32_t e = i; e < P.n_given; ++e) sum += (uint32_t)given[e] - first == j ? (double)g[e] : 0.0;
+            float at = 0.0f;
+#pragma unroll
+            for (int q = 0; q < NMAX; ++q) at = (uint32_t)q == j ? x[q] : at;
+            at = grad_of_given(at, sum, f, P.it);
+#pragma unroll
+            for (int q = 0; q < NMAX; ++q) y[q] = (uint32_t)q == j ? at : y[q];
         }
+#pragma unroll
+        for (int j = 0; j < NMAX; ++j)
+            if ((uint32_t)j < n) g0[(int64_t)j * gcs] = from_f32<T>(y[j]);
     }
 }
 
@@ -868,11 +897,16 @@ int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t 
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
     T* g = (T*)grad;
     constexpr uint32_t V = Pack<T>::V;
-    if (cs == 1 && gcs == 1 && n <= kShort && P.n_given <= kShortGiven) {
+    if (n <= 32 || (rs == 1 && grs == 1 && cs != 1)) {
+        const unsigned grid = row_grid((rows + 255) / 256 * ((n + 31) / 32));
+        if (n <= 4) logprob_grad_few_kernel<T, 4><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
+        else if (n <= 8) logprob_grad_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
+        else if (n <= 12) logprob_grad_few_kernel<T, 12><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
+        else if (n <= 16) logprob_grad_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
+        else logprob_grad_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, (n + 31) / 32);
+    } else if (cs == 1 && gcs == 1 && n <= kShort && P.n_given <= kShortGiven) {
 #define RUN(G, R) logprob_grad_short_kernel<T, G, R><<<row_grid((rows + 256 / G - 1) / (256 / G)), 256, 0, st>>>(X, P, g, grs)
-        if (n <= 2 * V) RUN(2, 1);
-        else if (n <= 4 * V) RUN(4, 1);
-        else if (n <= 8 * V) RUN(8, 1);
+        if (n <= 8 * V) RUN(8, 1);
         else if (n <= 16 * V) RUN(16, 1);
         else if (n <= 32 * V) RUN(32, 1);
         else if (n <= 64 * V) RUN(64, 1);
@@ -880,11 +914,6 @@ int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t 
         else if (n <= 256 * V) RUN(64, 4);
         else RUN(64, (int)(32 / V));
 #undef RUN
-    } else if (n <= 32 || (rs == 1 && grs == 1 && cs != 1)) {
-        const uint32_t seg = 32, segs = (n + seg - 1) / seg;
-        const unsigned grid = row_grid((rows + 255) / 256 * segs);
-        if (P.allowed) logprob_grad_few_kernel<T, true><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, segs, seg);
-        else logprob_grad_few_kernel<T, false><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, segs, seg);
     } else {
         const uint32_t segs = (n + kGradSeg - 1) / kGradSeg;
         const unsigned grid = row_grid((rows * segs + 3) / 4);
