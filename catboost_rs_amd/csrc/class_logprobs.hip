@@ -389,27 +389,66 @@ __global__ __launch_bounds__(THREADS) void finish_kernel(Rows<T> X, Asked A, uin
     }
 }
 
-// Few classes: a row a thread, its scores in registers; a score's place is the count of those ahead.
-template <class T, int NMAX, bool kTop>
+// A row of at most NMAX classes in a thread's registers; kWhole: whole vectors of classes next to each other.
+template <class T, int NMAX, bool kWhole>
+__device__ __forceinline__ void load_few(const T* row, int64_t cs, uint32_t n, float (&x)[NMAX]) {
+    constexpr int V = kWhole && Pack<T>::V <= NMAX ? Pack<T>::V : 1;
+#pragma unroll
+    for (int j = 0; j < NMAX; j += V) {
+        if constexpr (V > 1) {
+            Pack<T> p;
+            if ((uint32_t)j < n) p.w = ((const Loose<T>*)(row + j))->w;
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[j + v] = (uint32_t)j < n ? p.get(v) : -INFINITY;
+        } else {
+            x[j] = (uint32_t)j < n ? to_f32(row[(int64_t)j * cs]) : -INFINITY;
+        }
+    }
+}
+
+// Few classes: a row a thread, its scores in registers.  Up to 32: a score's place is the count of those ahead; up to 64, for which
+// there are too many pairs (rows next to each other): the largest one after another.
+template <class T, int NMAX, bool kWhole, bool kTop>
 __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
     const uint32_t n = X.classes;
     for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
         const T* x0 = X.data + (int64_t)row * X.rs;
-        const uint32_t bits = A.allowed ? A.allowed[(int64_t)row * A.allowed_stride] : ~0u, own = given_class<T>(A, row, 0);
+        const uint32_t own = given_class<T>(A, row, 0);
         float x[NMAX];
         RunningStat run;
+        load_few<T, NMAX, kWhole>(x0, X.cs, n, x);
+        if (A.allowed) {
+            const uint32_t* words = A.allowed + (int64_t)row * A.allowed_stride;
+            const uint32_t low = words[0], high = NMAX > 32 && n > 32 ? words[1] : 0;
 #pragma unroll
-        for (int i = 0; i < NMAX; ++i) {
-            x[i] = (uint32_t)i < n ? to_f32(x0[(int64_t)i * X.cs]) : -INFINITY;
-            if (!(bits >> i & 1)) x[i] = -INFINITY;
-            run.m = fmaxf(run.m, x[i]);
+            for (int i = 0; i < NMAX; ++i) x[i] = (i < 32 ? low : high) >> (i & 31) & 1 ? x[i] : -INFINITY;
         }
+#pragma unroll
+        for (int i = 0; i < NMAX; ++i) run.m = fmaxf(run.m, x[i]);
 #pragma unroll
         for (int i = 0; i < NMAX; ++i) run.add_one(x[i], A.c);
         const RowStat q = row_stat(run);
         write_stats(A, row, run, q);
         write_given(A, X, row, q, 0, 1, own, given_score(A, X, row, own));
-        if constexpr (kTop) {
+        if constexpr (kTop && NMAX > 32) {
+            uint32_t key[NMAX];
+#pragma unroll
+            for (int i = 0; i < NMAX; ++i) key[i] = (uint32_t)i < n ? order_key(x[i]) : 0;
+            for (uint32_t r = 0; r < A.k; ++r) {
+                uint32_t most = 0;
+                int32_t at = 0;
+#pragma unroll
+                for (int i = 0; i < NMAX; ++i) {
+                    at = key[i] > most ? i : at;
+                    most = max(key[i], most);
+                }
+#pragma unroll
+                for (int i = 0; i < NMAX; ++i) key[i] = i == at ? 0 : key[i];
+                const float y = key_score(most);
+                A.top_logprob[row * A.k + r] = log_prob(y, q, A.it);
+                A.top_index[row * A.k + r] = y == -INFINITY ? -1 : at;
+            }
+        } else if constexpr (kTop) {
             uint32_t key[NMAX], rank[NMAX];
 #pragma unroll
             for (int i = 0; i < NMAX; ++i) {
@@ -550,20 +589,45 @@ __global__ __launch_bounds__(256) void logprobs_short_kernel(Rows<T> X, Asked A)
                     most[u] = max(most[u], key[u * V + v]);
                 }
             }
-            Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
-            C.set_bound((u64)(A.k * 4 <= n / V ? wave_kth(most, A.k) : wave_kth(key, A.k)) << 32);
+            uint32_t bound;
+            if (A.k <= 8 && n >= 32 * V) {   // (the lanes' maxima, a NaN left out: k lanes reach the smallest of the k largest)
+                uint32_t larger = 0;
+#pragma unroll 16
+                for (int j = 0; j < 64; ++j) larger += read_lane(lm, j) > lm;
+                bound = order_key(-wave_reduce(larger < A.k ? -lm : -INFINITY, MaxF()));
+            } else {
+                bound = A.k * 4 <= n / V ? wave_kth(most, A.k) : wave_kth(key, A.k);
+            }
+            bound = max(bound, 1u);   // (0 is no key)
+            uint32_t count = 0;
 #pragma unroll
-            for (int u = 0; u < R; ++u)
+            for (int r = 0; r < R * V; ++r) count += (uint32_t)__popcll(__ballot(key[r] >= bound));
+            if (count <= (uint32_t)CAP) {
+                count = 0;
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const uint32_t i = (u * G + l) * V + v;
-                    if (__any(i < n && !(x[u][v] < C.fbound))) C.offer(x[u][v], i, i < n, A.k);
+                for (int r = 0; r < R * V; ++r) {
+                    const u64 b = __ballot(key[r] >= bound);
+                    const uint32_t i = (r / V * G + l) * V + r % V;
+                    if (key[r] >= bound) cand[wave][count + (uint32_t)__popcll(b & ((1ull << l) - 1))] = (u64)key[r] << 32 | (uint32_t)~i;
+                    count += (uint32_t)__popcll(b);
                 }
+            } else {   // many equal ones: class by class, and only the k largest kept as the list fills
+                Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
+                C.set_bound((u64)(bound - 1) << 32 | 0xFFFFFFFFu);
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+                    const uint32_t i = i0 + l;
+                    float y = -INFINITY;
+                    if (i < n && !(words && !is_allowed(words, i))) y = to_f32(X.data[(int64_t)row * X.rs + (int64_t)i * X.cs]);
+                    C.offer(y, i, i < n, A.k);
+                }
+                count = C.count;
+            }
             wave_fence();
-            for (uint32_t i = l; i < C.count; i += 64) {
+            for (uint32_t i = l; i < count; i += 64) {
                 const u64 key = cand[wave][i];
                 uint32_t rank = 0;
-                for (uint32_t j = 0; j < C.count; ++j) rank += cand[wave][j] > key;
+                for (uint32_t j = 0; j < count; ++j) rank += cand[wave][j] > key;
                 if (rank >= A.k) continue;
                 const float y = key_score((uint32_t)(key >> 32));
                 A.top_logprob[row * A.k + rank] = log_prob(y, q, A.it);
@@ -591,7 +655,8 @@ int run_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
     const uint32_t n = X.classes;
     // by vectors where they fill the lanes: half of them, or a part of the wave's for the sums alone
     if (X.cs == 1 && (n > 32 * V || !A.k)) {
-        if (n <= 8 * V) launch_short<T, 8, 1, true>(X, A, st);
+        if (n <= 4 * V) launch_short<T, 4, 1, true>(X, A, st);
+        else if (n <= 8 * V) launch_short<T, 8, 1, true>(X, A, st);
         else if (n <= 16 * V) launch_short<T, 16, 1, true>(X, A, st);
         else if (n <= 32 * V) launch_short<T, 32, 1, true>(X, A, st);
         else if (n <= 64 * V) launch_short<T, 64, 1, true>(X, A, st);
@@ -667,16 +732,20 @@ template <class T>
 int run_logprobs(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t cs, const Asked& A, void* workspace,
                  hipStream_t st) {
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
-    if (n <= 32) {
+    // (by rows and without a k, from 17 classes on a group of lanes reads them better)
+    if (n <= 64 && (n <= 32 || (rs == 1 && cs != 1)) && !(cs == 1 && n > 16 && !A.k)) {
         const unsigned grid = row_grid((rows + 255) / 256);
-#define FEW(N) (A.k ? logprobs_few_kernel<T, N, true><<<grid, 256, 0, st>>>(X, A) \
-                    : logprobs_few_kernel<T, N, false><<<grid, 256, 0, st>>>(X, A))
+#define FEW_(N, UNIT) (A.k ? logprobs_few_kernel<T, N, UNIT, true><<<grid, 256, 0, st>>>(X, A) \
+                           : logprobs_few_kernel<T, N, UNIT, false><<<grid, 256, 0, st>>>(X, A))
+#define FEW(N) (cs == 1 && n % Pack<T>::V == 0 ? FEW_(N, true) : FEW_(N, false))
         if (n <= 4) FEW(4);
         else if (n <= 8) FEW(8);
         else if (n <= 12) FEW(12);
         else if (n <= 16) FEW(16);
-        else FEW(32);
+        else if (n <= 32) FEW(32);
+        else FEW_(64, false);
 #undef FEW
+#undef FEW_
         CLS_TRY(hipGetLastError());
         return CBH_OK;
     }
@@ -844,7 +913,7 @@ __global__ __launch_bounds__(256) void logprob_grad_short_kernel(Rows<T> X, Upst
 
 // Few classes, and rows next to each other: a thread takes up to NMAX classes of a row, in registers.  The
 // f64 of a row's factors and entries is a thread's, not a group of lanes': 1M x 10 f32 by rows takes 42 us by groups.
-template <class T, int NMAX>
+template <class T, int NMAX, bool kWhole>
 __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs,
                                                                int64_t gcs, uint32_t segs) {
     const uint64_t blocks = (X.rows + 255) / 256;
@@ -858,8 +927,7 @@ __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstre
         const int32_t* given = P.given + row * P.n_given;
         const float* g = P.logprob_grad + row * P.n_given;
         float x[NMAX];
-#pragma unroll
-        for (int j = 0; j < NMAX; ++j) x[j] = (uint32_t)j < n ? to_f32(x0[(int64_t)j * X.cs]) : -INFINITY;
+        load_few<T, NMAX, kWhole>(x0, X.cs, n, x);
         double G = 0.0;
         bool some = false;
         for (uint32_t i = 0; i < P.n_given; ++i)
@@ -885,9 +953,18 @@ __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstre
 #pragma unroll
             for (int q = 0; q < NMAX; ++q) y[q] = (uint32_t)q == j ? at : y[q];
         }
+        constexpr int V = kWhole && Pack<T>::V <= NMAX ? Pack<T>::V : 1;
 #pragma unroll
-        for (int j = 0; j < NMAX; ++j)
-            if ((uint32_t)j < n) g0[(int64_t)j * gcs] = from_f32<T>(y[j]);
+        for (int j = 0; j < NMAX; j += V) {
+            if constexpr (V > 1) {
+                float part[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) part[v] = y[j + v];
+                if ((uint32_t)j < n) store_pack<T, true>(g0, 1, j, n, part);
+            } else {
+                if ((uint32_t)j < n) g0[(int64_t)j * gcs] = from_f32<T>(y[j]);
+            }
+        }
     }
 }
 
@@ -897,16 +974,20 @@ int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t 
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
     T* g = (T*)grad;
     constexpr uint32_t V = Pack<T>::V;
-    if (n <= 32 || (rs == 1 && grs == 1 && cs != 1)) {
+    const bool unit = cs == 1 && gcs == 1, lanes = unit && n <= kShort && P.n_given <= kShortGiven;
+    if (!(lanes && n > 16) && (n <= 32 || (rs == 1 && grs == 1 && cs != 1))) {
         const unsigned grid = row_grid((rows + 255) / 256 * ((n + 31) / 32));
-        if (n <= 4) logprob_grad_few_kernel<T, 4><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
-        else if (n <= 8) logprob_grad_few_kernel<T, 8><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
-        else if (n <= 12) logprob_grad_few_kernel<T, 12><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
-        else if (n <= 16) logprob_grad_few_kernel<T, 16><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, 1);
-        else logprob_grad_few_kernel<T, 32><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, (n + 31) / 32);
-    } else if (cs == 1 && gcs == 1 && n <= kShort && P.n_given <= kShortGiven) {
+#define RUN(N) (unit && n % V == 0 ? logprob_grad_few_kernel<T, N, true><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, (n + 31) / 32) \
+                     : logprob_grad_few_kernel<T, N, false><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, (n + 31) / 32))
+        if (n <= 4) RUN(4);
+        else if (n <= 8) RUN(8);
+        else if (n <= 16) RUN(16);
+        else RUN(32);
+#undef RUN
+    } else if (lanes) {
 #define RUN(G, R) logprob_grad_short_kernel<T, G, R><<<row_grid((rows + 256 / G - 1) / (256 / G)), 256, 0, st>>>(X, P, g, grs)
-        if (n <= 8 * V) RUN(8, 1);
+        if (n <= 4 * V) RUN(4, 1);
+        else if (n <= 8 * V) RUN(8, 1);
         else if (n <= 16 * V) RUN(16, 1);
         else if (n <= 32 * V) RUN(32, 1);
         else if (n <= 64 * V) RUN(64, 1);
@@ -917,7 +998,6 @@ int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t 
     } else {
         const uint32_t segs = (n + kGradSeg - 1) / kGradSeg;
         const unsigned grid = row_grid((rows * segs + 3) / 4);
-        const bool unit = cs == 1 && gcs == 1;
 #define RUN(UNIT, MASK) logprob_grad_kernel<T, UNIT, MASK><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, segs)
         if (unit) P.allowed ? RUN(true, true) : RUN(true, false);
         else P.allowed ? RUN(false, true) : RUN(false, false);

@@ -22,7 +22,8 @@ pytestmark = pytest.mark.gpu
 SHAPES = [(1, 1, 1, 1), (3, 2, 2, 1), (700, 10, 3, 3), (70, 32, 1, 32), (9, 33, 2, 5), (5, 64, 64, 64), (4, 1000, 1, 5),
           (3, 2048, 7, 256), (2, 2049, 1, 300), (2, 5000, 3, 1024), (5, 50021, 4, 20), (2, 8193, 1, 0), (1, 70001, 1, 64),
           (3, 140003, 2, 257), (600, 4099, 1, 9), (1, 40000, 1024, 0), (300, 20, 40, 0),
-          (333, 70, 1, 14), (65, 129, 8, 0), (70, 256, 9, 64), (31, 257, 2, 65), (1001, 40, 1, 0), (9, 700, 1, 0), (6, 2048, 1, 64)]
+          (333, 70, 1, 14), (65, 129, 8, 0), (70, 256, 9, 64), (31, 257, 2, 65), (1001, 40, 1, 0), (9, 700, 1, 0), (6, 2048, 1, 64),
+          (300, 40, 3, 40), (259, 64, 2, 7), (70, 17, 1, 0), (70, 33, 9, 0)]
 
 
 def words(allowed):
@@ -148,6 +149,20 @@ def test_shapes(rows, n, m, k, kind):
             up = g.standard_normal((rows, m))
             check_grad(x, given, up, None, t, kind, order, allowed, tag)
             check_grad(x, given, up, g.standard_normal(rows), t, kind, order, allowed, tag)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("order", ["rows", "classes", "padded"])
+def test_every_number_of_few_classes(order, kind):
+    g = np.random.default_rng(11)
+    for n in range(1, 72):
+        rows = 67
+        x, given = O.scores(g, rows, n, "normal"), given_of(g, rows, n, 2)
+        for name, allowed in masks(g, rows, n)[::2]:
+            for k in (0, min(n, 3), n):
+                check(x, given, 1.2, k, kind, order, allowed, (n, k, name))
+            up = g.standard_normal((rows, 2))
+            check_grad(x, given, up, None if n % 2 else g.standard_normal(rows), 1.2, kind, order, allowed, (n, name))
 
 
 @pytest.mark.parametrize("values", ["ties", "equal", "rising", "masked", "sharp"])
