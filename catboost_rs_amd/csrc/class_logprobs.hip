@@ -413,16 +413,14 @@ __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
     const uint32_t n = X.classes;
     for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
         const T* x0 = X.data + (int64_t)row * X.rs;
+        const uint32_t* words = A.allowed + (int64_t)row * A.allowed_stride;
+        const uint32_t low = A.allowed ? words[0] : ~0u, high = NMAX > 32 && A.allowed && n > 32 ? words[1] : ~0u;
         const uint32_t own = given_class<T>(A, row, 0);
         float x[NMAX];
         RunningStat run;
         load_few<T, NMAX, kWhole>(x0, X.cs, n, x);
-        if (A.allowed) {
-            const uint32_t* words = A.allowed + (int64_t)row * A.allowed_stride;
-            const uint32_t low = words[0], high = NMAX > 32 && n > 32 ? words[1] : 0;
 #pragma unroll
-            for (int i = 0; i < NMAX; ++i) x[i] = (i < 32 ? low : high) >> (i & 31) & 1 ? x[i] : -INFINITY;
-        }
+        for (int i = 0; i < NMAX; ++i) x[i] = (i < 32 ? low : high) >> (i & 31) & 1 ? x[i] : -INFINITY;
 #pragma unroll
         for (int i = 0; i < NMAX; ++i) run.m = fmaxf(run.m, x[i]);
 #pragma unroll
@@ -579,41 +577,41 @@ __global__ __launch_bounds__(256) void logprobs_short_kernel(Rows<T> X, Asked A)
         if constexpr (CAP > 0) {
             static_assert(G == 64, "a row a wave");
             if (!there) continue;
-            uint32_t key[R * V], most[R];
-#pragma unroll
-            for (int u = 0; u < R; ++u) {
-                most[u] = 0;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    key[u * V + v] = (u * G + l) * V + v < n ? order_key(x[u][v]) : 0;
-                    most[u] = max(most[u], key[u * V + v]);
-                }
-            }
-            uint32_t bound;
-            if (A.k <= 8 && n >= 32 * V) {   // (the lanes' maxima, a NaN left out: k lanes reach the smallest of the k largest)
+            float bound;   // k classes reach it (NaN: all do)
+            if (kVec && A.k <= 8 && n >= 32 * V) {   // of the lanes' maxima, a NaN left out: the smallest of the k largest
                 uint32_t larger = 0;
 #pragma unroll 16
                 for (int j = 0; j < 64; ++j) larger += read_lane(lm, j) > lm;
-                bound = order_key(-wave_reduce(larger < A.k ? -lm : -INFINITY, MaxF()));
+                bound = -wave_reduce(larger < A.k ? -lm : -INFINITY, MaxF());
             } else {
-                bound = A.k * 4 <= n / V ? wave_kth(most, A.k) : wave_kth(key, A.k);
+                uint32_t key[R * V], most[R];
+#pragma unroll
+                for (int u = 0; u < R; ++u) {
+                    most[u] = 0;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        key[u * V + v] = (u * G + l) * V + v < n ? order_key(x[u][v]) : 0;
+                        most[u] = max(most[u], key[u * V + v]);
+                    }
+                }
+                bound = key_score(A.k * 4 <= n / V ? wave_kth(most, A.k) : wave_kth(key, A.k));
             }
-            bound = max(bound, 1u);   // (0 is no key)
             uint32_t count = 0;
 #pragma unroll
-            for (int r = 0; r < R * V; ++r) count += (uint32_t)__popcll(__ballot(key[r] >= bound));
-            if (count <= (uint32_t)CAP) {
-                count = 0;
+            for (int u = 0; u < R; ++u)
 #pragma unroll
-                for (int r = 0; r < R * V; ++r) {
-                    const u64 b = __ballot(key[r] >= bound);
-                    const uint32_t i = (r / V * G + l) * V + r % V;
-                    if (key[r] >= bound) cand[wave][count + (uint32_t)__popcll(b & ((1ull << l) - 1))] = (u64)key[r] << 32 | (uint32_t)~i;
+                for (int v = 0; v < V; ++v) {
+                    const uint32_t i = (u * G + l) * V + v;
+                    const bool in = i < n && !(x[u][v] < bound);
+                    const u64 b = __ballot(in);
+                    if (b == 0) continue;
+                    const uint32_t at = count + (uint32_t)__popcll(b & ((1ull << l) - 1));
+                    if (in && at < (uint32_t)CAP) cand[wave][at] = rank_key(x[u][v], i);
                     count += (uint32_t)__popcll(b);
                 }
-            } else {   // many equal ones: class by class, and only the k largest kept as the list fills
+            if (count > (uint32_t)CAP) {   // many equal ones: class by class, and only the k largest kept as the list fills
                 Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
-                C.set_bound((u64)(bound - 1) << 32 | 0xFFFFFFFFu);
+                wave_fence();
 #pragma unroll 1
                 for (uint32_t i0 = 0; i0 < n; i0 += 64) {
                     const uint32_t i = i0 + l;
@@ -643,7 +641,7 @@ void launch_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
     if constexpr (G == 64) {
         if (A.k) {
             if (A.k <= 128) logprobs_short_kernel<T, G, R, kVec, 256><<<grid, 256, 0, st>>>(X, A);
-            else logprobs_short_kernel<T, G, R, kVec, 2048><<<grid, 256, 0, st>>>(X, A);
+            else logprobs_short_kernel<T, G, R, kVec, 1152><<<grid, 256, 0, st>>>(X, A);
             return;
         }
     }
