@@ -11,31 +11,108 @@ namespace {
 using namespace cbh::cls;
 
 // ---- rows -----------------------------------------------------------------------------------
-// A thread takes a vector of a row of the output.
+struct Lookup {
+    const int32_t* index;   // [rows][list]
+    uint64_t rows;
+    uint32_t entries, dim, list;
+    float scale;
+};
+// Four indices of a row's list, from i on; `entries` where it ends.
+__device__ __forceinline__ void load_indices(const Lookup& L, const int32_t* ix, uint32_t i, uint32_t (&e)[4]) {
+    typedef int32_t Quad __attribute__((ext_vector_type(4), aligned(4)));
+    if (i + 4 <= L.list) {
+        const Quad q = *(const Quad*)(ix + i);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) e[u] = (uint32_t)q[u];
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) e[u] = i + u < L.list ? (uint32_t)ix[i + u] : L.entries;
+    }
+}
+// A group of `lanes` lanes takes a row of the output, a vector a lane, four rows of the table on their way at a time.
 template <class T, bool kUnit>
-__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint32_t entries, uint32_t dim, int64_t rs,
-                                                     int64_t cs, const int32_t* __restrict__ index, uint64_t rows, uint32_t list,
-                                                     float scale, T* __restrict__ out, uint32_t vecs) {
+__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, int64_t rs, int64_t cs, Lookup L,
+                                                     T* __restrict__ out, uint32_t lanes) {
     constexpr int V = Pack<T>::V;
-    const uint64_t jobs = rows * vecs;
-    for (uint64_t job = (uint64_t)blockIdx.x * 256 + threadIdx.x; job < jobs; job += (uint64_t)gridDim.x * 256) {
-        const uint64_t row = job / vecs;
-        const uint32_t c = (uint32_t)(job % vecs) * V;
-        const int32_t* ix = index + row * list;
+    const uint32_t tiles = (L.dim + lanes * V - 1) / (lanes * V), per = 256 / lanes;
+    const uint64_t jobs = (L.rows + per - 1) / per * tiles;
+    for (uint64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const uint64_t row = job / tiles * per + threadIdx.x / lanes;
+        const uint32_t c = ((uint32_t)(job % tiles) * lanes + threadIdx.x % lanes) * V;
+        if (row >= L.rows || c >= L.dim) continue;
+        const int32_t* ix = L.index + row * L.list;
         float acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        for (uint32_t i = 0; i < list; ++i) {
-            const uint32_t e = (uint32_t)ix[i];
-            if (e >= entries) continue;
-            float x[V];
-            load_pack<T, kUnit>(table + (int64_t)e * rs, cs, c, dim, 0.0f, x);
+        for (uint32_t i = 0; i < L.list; i += 4) {
+            uint32_t e[4];
+            load_indices(L, ix, i, e);
+            Pack<T> p[4];
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] += x[v];
+            for (int u = 0; u < 4; ++u) {
+                const T* at = table + (int64_t)e[u] * rs;
+                if (e[u] >= L.entries) {
+                    p[u].w = Words{};
+                } else if (kUnit && c + V <= L.dim) {
+                    p[u].w = ((const Loose<T>*)(at + c))->w;
+                } else {
+                    float x[V];
+                    load_pack<T, kUnit>(at, cs, c, L.dim, 0.0f, x);
+                    p[u].set(x);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] += p[u].get(v);
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] *= scale;
-        store_pack<T, true>(out + row * dim, 1, c, dim, acc);
+        for (int v = 0; v < V; ++v) acc[v] *= L.scale;
+        store_pack<T, true>(out + row * L.dim, 1, c, L.dim, acc);
+    }
+}
+// Long lists over few entries: a workgroup holds `lanes` vectors of every entry in LDS and takes a part of the rows.
+constexpr uint32_t kLdsThreads = 1024, kLdsBytes = 163840;   // (one workgroup a CU)
+template <class T>
+__global__ __launch_bounds__(kLdsThreads) void lookup_lds_kernel(const T* __restrict__ table, int64_t rs, Lookup L, T* __restrict__ out,
+                                                                 uint32_t lanes, uint32_t tiles, uint64_t part) {
+    constexpr int V = Pack<T>::V;
+    extern __shared__ Words held[];   // [entries + 1][lanes]; the last is 0, for what is no entry
+    const uint32_t c0 = blockIdx.x % tiles * lanes * V, lane = threadIdx.x % lanes, c = c0 + lane * V;
+    const int shift = 31 - __builtin_clz(lanes);
+    if (threadIdx.x < lanes) held[L.entries * lanes + threadIdx.x] = Words{};
+    for (uint32_t i = threadIdx.x; i < L.entries * lanes; i += kLdsThreads) {
+        float x[V];
+        Pack<T> p;
+        load_pack<T, true>(table + (int64_t)(i / lanes) * rs, 1, c0 + i % lanes * V, L.dim, 0.0f, x);
+        p.set(x);
+        held[i] = p.w;
+    }
+    __syncthreads();
+    const uint64_t from = blockIdx.x / tiles * part, to = min(L.rows, from + part);
+    if (c >= L.dim) return;
+    for (uint64_t row = from + threadIdx.x / lanes; row < to; row += kLdsThreads / lanes) {
+        const int32_t* ix = L.index + row * L.list;
+        float acc[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        uint32_t next[4];
+        load_indices(L, ix, 0, next);
+        for (uint32_t i = 0; i < L.list; i += 4) {
+            uint32_t e[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) e[u] = next[u];
+            load_indices(L, ix, i + 4 < L.list ? i + 4 : i, next);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const Pack<T> p{held[(min(e[u], L.entries) << shift) + lane]};
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] += p.get(v);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] *= L.scale;
+        store_pack<T, true>(out + row * L.dim, 1, c, L.dim, acc);
     }
 }
 
@@ -556,12 +633,28 @@ int check_scale(double scale) {
 }
 
 template <class T>
-int run_lookup(const void* table, uint32_t entries, uint32_t dim, int64_t rs, int64_t cs, const int32_t* index, uint64_t rows,
-               uint32_t list, double scale, void* out, hipStream_t st) {
-    const uint32_t vecs = (dim + Pack<T>::V - 1) / Pack<T>::V;
-    const unsigned grid = row_grid((rows * vecs + 255) / 256);
-    if (cs == 1) lookup_kernel<T, true><<<grid, 256, 0, st>>>((const T*)table, entries, dim, rs, cs, index, rows, list, (float)scale, (T*)out, vecs);
-    else lookup_kernel<T, false><<<grid, 256, 0, st>>>((const T*)table, entries, dim, rs, cs, index, rows, list, (float)scale, (T*)out, vecs);
+int run_lookup(const void* table, int64_t rs, int64_t cs, const Lookup& L, void* out, hipStream_t st) {
+    constexpr uint32_t V = Pack<T>::V;
+    uint32_t lanes = 1;
+    while (lanes < 64 && lanes * V < L.dim) lanes *= 2;
+    // in LDS: lists long enough that an entry is read often
+    uint32_t held = lanes;
+    while (held > 1 && (L.entries + 1ull) * held * 16 > kLdsBytes) held /= 2;
+    if (cs == 1 && L.list >= 8 && L.rows * L.list >= 256ull * L.entries && (L.entries + 1ull) * held * 16 <= kLdsBytes) {
+        const uint32_t tiles = (L.dim + held * V - 1) / (held * V);
+        const uint64_t least = kLdsThreads / held;   // rows of one round
+        const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>((256 + tiles - 1) / tiles, (L.rows + 2 * least - 1) / (2 * least)));
+        const uint64_t part = (L.rows + parts - 1) / parts;
+        const size_t lds = (L.entries + 1) * (size_t)held * 16;
+        if (lds > 65536) CLS_TRY(hipFuncSetAttribute((const void*)lookup_lds_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes));
+        lookup_lds_kernel<T><<<(unsigned)((L.rows + part - 1) / part * tiles), kLdsThreads, lds, st>>>((const T*)table, rs, L, (T*)out, held, tiles, part);
+        CLS_TRY(hipGetLastError());
+        return CBH_OK;
+    }
+    const uint32_t tiles = (L.dim + lanes * V - 1) / (lanes * V), per = 256 / lanes;
+    const unsigned grid = row_grid((L.rows + per - 1) / per * tiles);
+    if (cs == 1) lookup_kernel<T, true><<<grid, 256, 0, st>>>((const T*)table, rs, cs, L, (T*)out, lanes);
+    else lookup_kernel<T, false><<<grid, 256, 0, st>>>((const T*)table, rs, cs, L, (T*)out, lanes);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
@@ -578,7 +671,8 @@ extern "C" int cbh_lookup_rows(const void* table, int32_t type, uint32_t entries
         if (rc == CBH_OK) rc = check_scale(scale);
         if (rc != CBH_OK || rows == 0) return rc;
         hipStream_t st = (hipStream_t)stream;
-#define RUN(T) run_lookup<T>(table, entries, dim, row_stride, column_stride, index, rows, list, scale, out, st)
+        const Lookup L{index, rows, entries, dim, list, (float)scale};
+#define RUN(T) run_lookup<T>(table, row_stride, column_stride, L, out, st)
         switch (type) {
             case CBH_TYPE_F32: return RUN(float);
             case CBH_TYPE_F16: return RUN(_Float16);
