@@ -124,11 +124,16 @@ struct Sort {
     uint32_t n, entries, list;
     uint32_t blocks, digits;   // of a pass by digits; digits a power of two
     int shift, bits;
-    uint8_t* mark;             // [entries]: cleared here, set where an entry's sum is taken
+    uint32_t segs, seg_blocks; // parts of the places that are sorted by themselves, and a part's blocks
+    uint8_t* mark;             // [segs][entries]: cleared here, set where an entry's sum is taken
 };
+constexpr uint32_t kNoEntry = ~0u;   // (in the sorted list)
+__device__ __forceinline__ u64 sorted_key(const Sort& S, uint32_t seg, uint32_t entry, uint32_t place) {
+    return (u64)(entry < S.entries ? seg * S.entries + entry : kNoEntry) << 32 | place / S.list;
+}
 __device__ __forceinline__ uint32_t place_entry(const Sort& S, uint32_t i) { return min((uint32_t)S.index[i], S.entries); }
 __device__ __forceinline__ void clear_marks(const Sort& S, uint32_t block, uint32_t blocks) {
-    for (uint64_t v = (uint64_t)block * 256 + threadIdx.x; v < S.entries; v += (uint64_t)blocks * 256) S.mark[v] = 0;
+    for (uint64_t v = (uint64_t)block * 256 + threadIdx.x; v < (uint64_t)S.segs * S.entries; v += (uint64_t)blocks * 256) S.mark[v] = 0;
 }
 
 // Few places: a workgroup takes 64 of them and counts, over all places, those ahead of each; a wave a quarter of them.
@@ -163,7 +168,7 @@ __global__ __launch_bounds__(256) void rank_kernel(Sort S, u64* __restrict__ out
     ahead[wave][lane] = count;
     __syncthreads();
     if (wave == 0 && at < S.n)
-        out[ahead[0][lane] + ahead[1][lane] + ahead[2][lane] + ahead[3][lane]] = (u64)mine << 32 | at / S.list;
+        out[ahead[0][lane] + ahead[1][lane] + ahead[2][lane] + ahead[3][lane]] = sorted_key(S, 0, mine, at);
 }
 
 // Many places: radix sort of (entry, place), least significant digits first, of up to 11 bits.  A workgroup ranks
@@ -193,13 +198,14 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const u64* __restrict__
     __syncthreads();
     for (uint32_t d = threadIdx.x; d < S.digits; d += 256) counts[(uint64_t)blockIdx.x * S.digits + d] = count[d];
 }
-// For every digit the running sum over the blocks, in place, and its total.  A workgroup takes 64 digits, its waves
-// a part of the blocks each.
+// For every part and digit the running sum over the blocks, in place, and its total.  A workgroup takes 64 digits, its
+// waves some of the blocks each.
 constexpr uint32_t kScanWaves = 16;
 __global__ __launch_bounds__(1024) void sort_scan_kernel(Sort S, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
     __shared__ uint32_t part[kScanWaves][64];
     const uint32_t wave = threadIdx.x / 64, lane = lane_id(), d = blockIdx.x * 64 + lane;
-    const uint32_t each = (S.blocks + kScanWaves - 1) / kScanWaves, b0 = min(S.blocks, wave * each), b1 = min(S.blocks, b0 + each);
+    const uint32_t first = blockIdx.y * S.seg_blocks, end = min(S.blocks, first + S.seg_blocks);
+    const uint32_t each = (S.seg_blocks + kScanWaves - 1) / kScanWaves, b0 = min(end, first + wave * each), b1 = min(end, b0 + each);
     uint32_t sum = 0;
     if (d < S.digits) {
 #pragma unroll 8
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(1024) void sort_scan_kernel(Sort S, uint32_t* __res
             at += c[j];
         }
     }
-    if (wave == kScanWaves - 1) totals[d] = at;
+    if (wave == kScanWaves - 1) totals[blockIdx.y * S.digits + d] = at;
 }
 // Keys to their places: the digits below, then the blocks before, then the waves before, then the rounds before, then the lanes
 // before.  Without `totals` the counts are as they were counted, and few blocks': each adds them up for itself.
@@ -230,6 +236,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
     __shared__ uint32_t at[4][1 << kMaxDigitBits];
     __shared__ uint32_t sums[4];
     const uint32_t wave = threadIdx.x / 64, lane = lane_id(), from = (blockIdx.x * 4 + wave) * ROUNDS * 64;
+    const uint32_t seg = blockIdx.x / S.seg_blocks;
     u64 key[ROUNDS];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
@@ -251,7 +258,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
         total[j] = before[j] = 0;
         if (j >= run || d >= S.digits) continue;
         if (totals) {
-            total[j] = totals[d];
+            total[j] = totals[seg * S.digits + d];
             before[j] = counts[(uint64_t)blockIdx.x * S.digits + d];
         } else {
 #pragma unroll 8
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
     const uint32_t upto = wave_scan(mine, Add(), 0u);
     if (lane == 63) sums[wave] = upto;
     __syncthreads();
-    uint32_t base = upto - mine;
+    uint32_t base = seg * S.seg_blocks * ROUNDS * 256 + upto - mine;   // (a part keeps its places)
     for (uint32_t w = 0; w < wave; ++w) base += sums[w];
 #pragma unroll
     for (uint32_t j = 0; j < kRun; ++j) {
@@ -293,7 +300,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
         }
         if (have) {
             const uint32_t place = at[wave][d] + (uint32_t)__popcll(same & ((1ull << lane) - 1));
-            out[place] = kLast ? key[r] >> 32 << 32 | (uint32_t)key[r] / S.list : key[r];
+            out[place] = kLast ? sorted_key(S, seg, (uint32_t)(key[r] >> 32), (uint32_t)key[r]) : key[r];
         }
         wave_fence();
         if (have && (same >> lane) == 1) at[wave][d] += (uint32_t)__popcll(same);   // (the last of the equal ones)
@@ -304,10 +311,11 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
 // ---- sums -----------------------------------------------------------------------------------
 constexpr uint32_t kSumThreads = 512;
 struct Table {
-    const u64* sorted;   // (entry, row)
-    uint32_t n, entries, dim;
+    const u64* sorted;   // (entry, row); kNoEntry, or more than the entries: none
+    uint32_t n, entries, dim;  // (entries: of all parts of the places)
     uint32_t lanes, places;    // of a group: lanes that hold a row's vectors, and places that it adds up
     uint32_t chunk, chunks;    // places of a workgroup
+    bool by_chiplet;           // an eighth of the chunks, one after another, to each of the chip's eight dies
     float scale;
     float* part;         // [chunks][2][dim]: of the first run, where it began before; of the last, where it goes on
     uint8_t* mark;
@@ -349,10 +357,13 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
     __shared__ uint32_t flags[kSumThreads], head[kSumThreads], tail[kSumThreads];
     const uint32_t width = B.lanes * V, tiles = (B.dim + width - 1) / width, per = kSumThreads / B.lanes;
     const uint32_t group = threadIdx.x / B.lanes, in = threadIdx.x % B.lanes;
-    for (uint64_t job = blockIdx.x; job < (uint64_t)B.chunks * tiles; job += gridDim.x) {
-        const uint32_t chunk = (uint32_t)(job / tiles), c0 = (uint32_t)(job % tiles) * width, c = c0 + in * V;
+    const uint32_t eighth = (B.chunks + 7) / 8;
+    for (uint64_t job = blockIdx.x; job < (uint64_t)eighth * 8 * tiles; job += gridDim.x) {
+        const uint32_t chunk = B.by_chiplet ? (uint32_t)(job % 8) * eighth + (uint32_t)(job / 8 / tiles) : (uint32_t)(job / tiles);
+        if (chunk >= B.chunks) continue;
+        const uint32_t c0 = (uint32_t)((B.by_chiplet ? job / 8 : job) % tiles) * width, c = c0 + in * V;
         const uint32_t from = min(B.n, chunk * B.chunk + group * B.places), to = min(B.n, from + B.places);
-        uint32_t cur = B.entries, flag = 0;
+        uint32_t cur = kNoEntry, flag = 0;
         bool before = false;
         float acc[V];
 #pragma unroll
@@ -383,7 +394,7 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
 #pragma unroll
                 for (int u = 0; u < kFly; ++u) {
                     const u64 key = B.sorted[min(i0 + u, to - 1)];
-                    e[u] = i0 + u < to ? (uint32_t)(key >> 32) : B.entries;
+                    e[u] = i0 + u < to ? (uint32_t)(key >> 32) : kNoEntry;
                     const T* row = grad + (int64_t)(uint32_t)key * rs;
                     if (e[u] >= B.entries) {
                         p[u].w = Words{};
@@ -509,11 +520,29 @@ __global__ __launch_bounds__(256) void table_join_kernel(Table B, uint32_t join_
     }
 }
 
+// The parts' sums together.
+template <class O>
+__global__ __launch_bounds__(256) void table_parts_kernel(const float* __restrict__ sums, const uint8_t* __restrict__ mark, uint32_t segs,
+                                                          uint32_t entries, uint32_t dim, float scale, O* __restrict__ out) {
+    const uint64_t all = (uint64_t)entries * dim;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t e = (uint32_t)(i / dim);
+        float sum = 0.0f;
+        for (uint32_t s = 0; s < segs; ++s)
+            if (mark[(uint64_t)s * entries + e]) sum += sums[s * all + i];
+        out[i] = from_f32<O>(sum * scale);
+    }
+}
+
 // ---- host -----------------------------------------------------------------------------------
+// Long lists read a row's gradient many times.  Where all rows pass a die's 4 MB of second-level cache and the entries are few, the places are
+// sorted and added up in eight parts, one a die, whose rows are fewer; the parts' sums are added then.
+constexpr uint32_t kParts = 8;
 struct Layout {
     uint32_t n, passes, bits, rounds, blocks;
     uint32_t lanes, places, chunk, chunks;
-    uint64_t keys, counts, totals, mark, part, bytes;   // offsets; keys: two arrays
+    uint32_t segs, seg_blocks;
+    uint64_t keys, counts, totals, mark, part, sums, bytes;   // offsets; keys: two arrays
 };
 Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint32_t vec) {
     Layout L{};
@@ -524,6 +553,10 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     L.bits = L.passes ? (bits + L.passes - 1) / L.passes : 0;
     L.rounds = L.n <= 1u << 19 ? 4 : 16;
     L.blocks = (L.n + L.rounds * 256 - 1) / (L.rounds * 256);
+    const uint64_t cells = (uint64_t)entries * dim;
+    const bool parted = L.passes && list >= 8 && rows * dim * (16 / vec) > 4u << 20 && (uint64_t)entries * kParts * 16 <= L.n && cells <= 1u << 20;
+    L.segs = parted ? kParts : 1;
+    L.seg_blocks = std::max(1u, (L.blocks + L.segs - 1) / L.segs);
     L.lanes = 1;
     while (L.lanes < 64 && L.lanes * vec < dim) L.lanes *= 2;
     L.places = L.n <= 1u << 17 ? 16 : 32;
@@ -537,8 +570,9 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     };
     L.keys = take((L.passes > 1 ? 16 : 8) * (uint64_t)L.n);
     L.counts = take(L.passes ? 4ull * L.blocks << L.bits : 0);
-    L.totals = take(L.passes ? 4ull << L.bits : 0);
-    L.mark = take(L.n ? entries : 0);
+    L.totals = take(L.passes ? (4ull << L.bits) * L.segs : 0);
+    L.mark = take(L.n ? (uint64_t)entries * L.segs : 0);
+    L.sums = take(L.segs > 1 ? 4 * cells * L.segs : 0);
     L.part = take(8ull * L.chunks * dim);
     L.bytes = at;
     return L;
@@ -548,14 +582,21 @@ template <class T, class O>
 int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, void* out, hipStream_t st) {
     const uint32_t tiles = (B.dim + B.lanes * Pack<T>::V - 1) / (B.lanes * Pack<T>::V);
     if (B.n) {
-        const unsigned grid = row_grid((uint64_t)B.chunks * tiles);
+        const unsigned grid = row_grid((uint64_t)(B.chunks + 7) / 8 * 8 * tiles);
         if (cs == 1) table_sum_kernel<T, O, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, (O*)out);
         else table_sum_kernel<T, O, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, (O*)out);
         CLS_TRY(hipGetLastError());
     }
     const uint32_t join = B.chunks > 1 ? std::min<uint32_t>(B.chunks - 1, 1u << 14) : 0;
-    const uint32_t zero = std::min<uint32_t>((B.entries + kZeroRows - 1) / kZeroRows, 1u << 14);
-    table_join_kernel<O><<<join + zero, 256, 0, st>>>(B, join, (O*)out);
+    const uint32_t zero = B.by_chiplet ? 0 : std::min<uint32_t>((B.entries + kZeroRows - 1) / kZeroRows, 1u << 14);
+    table_join_kernel<O><<<std::max(1u, join + zero), 256, 0, st>>>(B, join, (O*)out);
+    CLS_TRY(hipGetLastError());
+    return CBH_OK;
+}
+template <class O>
+int launch_parts(const Layout& L, char* ws, uint32_t entries, uint32_t dim, float scale, void* out, hipStream_t st) {
+    const unsigned grid = (unsigned)std::min<uint64_t>(((uint64_t)entries * dim + 255) / 256, 4096);
+    table_parts_kernel<O><<<grid, 256, 0, st>>>((const float*)(ws + L.sums), (const uint8_t*)(ws + L.mark), L.segs, entries, dim, scale, (O*)out);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
@@ -576,7 +617,7 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
     u64* b = a + L.n;
     const u64* in = nullptr;
     uint32_t* counts = (uint32_t*)(ws + L.counts);
-    uint32_t* totals = L.blocks <= kOwnScan ? nullptr : (uint32_t*)(ws + L.totals);
+    uint32_t* totals = L.blocks <= kOwnScan && L.segs == 1 ? nullptr : (uint32_t*)(ws + L.totals);
     for (uint32_t p = 0; p < L.passes; ++p) {
         S.shift = (int)(p * L.bits);
         const bool first = p == 0, last = p + 1 == L.passes;
@@ -584,7 +625,7 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
         else sort_count_kernel<false, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts);
         CLS_TRY(hipGetLastError());
         if (totals) {
-            sort_scan_kernel<<<(S.digits + 63) / 64, 64 * kScanWaves, 0, st>>>(S, counts, totals);
+            sort_scan_kernel<<<dim3((S.digits + 63) / 64, S.segs), 64 * kScanWaves, 0, st>>>(S, counts, totals);
             CLS_TRY(hipGetLastError());
         }
 #define SCATTER(F, L_) sort_scatter_kernel<F, L_, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts, totals, a)
@@ -599,7 +640,7 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
     return CBH_OK;
 }
 int sort_places(const int32_t* index, uint32_t entries, uint32_t list, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
-    const Sort S{index, L.n, entries, list, L.blocks, 1u << L.bits, 0, (int)L.bits, (uint8_t*)(ws + L.mark)};
+    const Sort S{index, L.n, entries, list, L.blocks, 1u << L.bits, 0, (int)L.bits, L.segs, L.seg_blocks, (uint8_t*)(ws + L.mark)};
     *sorted = (u64*)(ws + L.keys);
     if (L.passes) return L.rounds == 4 ? sort_by_digits<4>(S, L, ws, sorted, st) : sort_by_digits<16>(S, L, ws, sorted, st);
     const uint32_t clear = std::min<uint32_t>((entries + 4095) / 4096, 1024);
@@ -710,12 +751,21 @@ extern "C" int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t row
             rc = sort_places(index, entries, list, L, ws, &sorted, st);
             if (rc != CBH_OK) return rc;
         }
-        const Table B{sorted,  L.n,          entries,                dim,                    L.lanes, L.places, L.chunk,
-                      L.chunks, (float)scale, (float*)(ws + L.part), (uint8_t*)(ws + L.mark)};
+        const bool parted = L.segs > 1;
+        const Table B{sorted,  L.n,      L.segs * entries, dim,    L.lanes,        L.places, L.chunk,
+                      L.chunks, parted, parted ? 1.0f : (float)scale, (float*)(ws + L.part), (uint8_t*)(ws + L.mark)};
+        void* sums = parted ? (void*)(ws + L.sums) : table_grad;
+        const int32_t sum_type = parted ? CBH_TYPE_F32 : grad_type;
         switch (type) {
-            case CBH_TYPE_F32: return launch_sums<float>(grad, row_stride, column_stride, B, table_grad, grad_type, st);
-            case CBH_TYPE_F16: return launch_sums<_Float16>(grad, row_stride, column_stride, B, table_grad, grad_type, st);
-            default: return launch_sums<bf16_t>(grad, row_stride, column_stride, B, table_grad, grad_type, st);
+            case CBH_TYPE_F32: rc = launch_sums<float>(grad, row_stride, column_stride, B, sums, sum_type, st); break;
+            case CBH_TYPE_F16: rc = launch_sums<_Float16>(grad, row_stride, column_stride, B, sums, sum_type, st); break;
+            default: rc = launch_sums<bf16_t>(grad, row_stride, column_stride, B, sums, sum_type, st);
+        }
+        if (rc != CBH_OK || !parted) return rc;
+        switch (grad_type) {
+            case CBH_TYPE_F32: return launch_parts<float>(L, ws, entries, dim, (float)scale, table_grad, st);
+            case CBH_TYPE_F16: return launch_parts<_Float16>(L, ws, entries, dim, (float)scale, table_grad, st);
+            default: return launch_parts<bf16_t>(L, ws, entries, dim, (float)scale, table_grad, st);
         }
     } catch (const std::exception& e) {
         return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
