@@ -179,16 +179,23 @@ __device__ __forceinline__ u64 sort_key(const u64* in, const Sort& S, uint32_t i
     return kFirst ? (u64)place_entry(S, i) << 32 | i : in[i];
 }
 __device__ __forceinline__ uint32_t digit_of(u64 key, const Sort& S) { return (uint32_t)(key >> 32 >> S.shift) & (S.digits - 1); }
+// The block of the places that this workgroup takes (S.blocks and more: none): a part's blocks on one die, so that its stores
+// to scattered places meet in that die's cache.
+__device__ __forceinline__ uint32_t sort_block(const Sort& S) {
+    return S.segs == 1 ? blockIdx.x : blockIdx.x % S.segs * S.seg_blocks + blockIdx.x / S.segs;
+}
 // Keys of every digit in every block: counts [block][digit].
 template <bool kFirst, int ROUNDS>
 __global__ __launch_bounds__(256) void sort_count_kernel(const u64* __restrict__ in, Sort S, uint32_t* __restrict__ counts) {
     __shared__ uint32_t count[1 << kMaxDigitBits];
     if (kFirst) clear_marks(S, blockIdx.x, gridDim.x);
+    const uint32_t block = sort_block(S);
+    if (block >= S.blocks) return;
     for (uint32_t d = threadIdx.x; d < S.digits; d += 256) count[d] = 0;
     uint32_t digit[ROUNDS];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        const uint32_t i = (blockIdx.x * ROUNDS + r) * 256 + threadIdx.x;
+        const uint32_t i = (block * ROUNDS + r) * 256 + threadIdx.x;
         digit[r] = i < S.n ? digit_of(sort_key<kFirst>(in, S, i), S) : ~0u;
     }
     __syncthreads();
@@ -196,7 +203,7 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const u64* __restrict__
     for (int r = 0; r < ROUNDS; ++r)
         if (digit[r] != ~0u) atomicAdd(&count[digit[r]], 1u);
     __syncthreads();
-    for (uint32_t d = threadIdx.x; d < S.digits; d += 256) counts[(uint64_t)blockIdx.x * S.digits + d] = count[d];
+    for (uint32_t d = threadIdx.x; d < S.digits; d += 256) counts[(uint64_t)block * S.digits + d] = count[d];
 }
 // For every part and digit the running sum over the blocks, in place, and its total.  A workgroup takes 64 digits, its
 // waves some of the blocks each.
@@ -235,8 +242,9 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
                                                            const uint32_t* __restrict__ totals, u64* __restrict__ out) {
     __shared__ uint32_t at[4][1 << kMaxDigitBits];
     __shared__ uint32_t sums[4];
-    const uint32_t wave = threadIdx.x / 64, lane = lane_id(), from = (blockIdx.x * 4 + wave) * ROUNDS * 64;
-    const uint32_t seg = blockIdx.x / S.seg_blocks;
+    const uint32_t block = sort_block(S), seg = block / S.seg_blocks;
+    if (block >= S.blocks) return;
+    const uint32_t wave = threadIdx.x / 64, lane = lane_id(), from = (block * 4 + wave) * ROUNDS * 64;
     u64 key[ROUNDS];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
@@ -259,13 +267,13 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const u64* __restrict
         if (j >= run || d >= S.digits) continue;
         if (totals) {
             total[j] = totals[seg * S.digits + d];
-            before[j] = counts[(uint64_t)blockIdx.x * S.digits + d];
+            before[j] = counts[(uint64_t)block * S.digits + d];
         } else {
 #pragma unroll 8
             for (uint32_t b = 0; b < S.blocks; ++b) {
                 const uint32_t c = counts[(uint64_t)b * S.digits + d];
                 total[j] += c;
-                before[j] += b < blockIdx.x ? c : 0;
+                before[j] += b < block ? c : 0;
             }
         }
         mine += total[j];
@@ -345,20 +353,74 @@ __device__ __forceinline__ void store_values(O* row, uint32_t c, uint32_t dim, c
     }
 }
 
+// Few places in one workgroup: each thread counts those ahead of its own, among them the ones of the waves before with the same entry.
+constexpr uint32_t kAllMost = kSumThreads;
+__device__ __forceinline__ void sort_all(const Sort& S, uint32_t* entry, u64* list) {
+    const uint32_t n4 = (S.n + 3) / 4 * 4, t = threadIdx.x, wave0 = t / 64 * 64, wave1 = min(wave0 + 64, n4);
+    const uint32_t mine = t < S.n ? place_entry(S, t) : ~0u;
+    entry[t] = mine;
+    __syncthreads();
+    typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+    const Quad* q = (const Quad*)entry;
+    uint32_t ahead = 0;
+    if (wave0 < n4) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < wave0 / 4; ++i) {
+            const Quad e = q[i];
+            ahead += (e[0] <= mine) + (e[1] <= mine) + (e[2] <= mine) + (e[3] <= mine);
+        }
+        for (uint32_t i = wave0; i < wave1; ++i) ahead += entry[i] < mine || (entry[i] == mine && i < t);
+#pragma unroll 4
+        for (uint32_t i = wave1 / 4; i < n4 / 4; ++i) {
+            const Quad e = q[i];
+            ahead += (e[0] < mine) + (e[1] < mine) + (e[2] < mine) + (e[3] < mine);
+        }
+        if (t < S.n) list[ahead] = sorted_key(S, 0, mine, t);
+    }
+    __syncthreads();
+}
+// The entries that do not occur among few places: `blocks` workgroups, 512 entries at a time.
+template <class O>
+__device__ __forceinline__ void zero_rest(const Sort& S, uint32_t dim, uint32_t block, uint32_t blocks, uint32_t* occurs, O* out) {
+    constexpr uint32_t V = 16 / sizeof(O);
+    const uint32_t vecs = (dim + V - 1) / V, mine = threadIdx.x < S.n ? place_entry(S, threadIdx.x) : ~0u;
+    for (uint64_t row0 = (uint64_t)block * kSumThreads; row0 < S.entries; row0 += (uint64_t)blocks * kSumThreads) {
+        __syncthreads();
+        occurs[threadIdx.x] = 0;
+        __syncthreads();
+        if (mine < S.entries && mine >= row0 && mine - row0 < kSumThreads) occurs[mine - row0] = 1;
+        __syncthreads();
+        const uint32_t rows = (uint32_t)min((uint64_t)kSumThreads, S.entries - row0);
+        float z[V] = {};
+        for (uint64_t j = threadIdx.x; j < (uint64_t)rows * vecs; j += kSumThreads) {
+            const uint32_t r = (uint32_t)(j / vecs);
+            if (!occurs[r]) store_pack<O, true>(out + (row0 + r) * dim, 1, (uint32_t)(j % vecs) * V, dim, z);
+        }
+    }
+}
+
 // A group of lanes takes `places` of the list, eight rows on their way at a time, and writes the runs that lie within them.
 // What of a run lies in several groups goes to LDS and is added up there, in the groups' order, a column a thread; what lies in several
 // workgroups, by join_kernel.
 enum { kHead = 1, kHeadEnds = 2, kTail = 4, kGoesOn = 8 };
-template <class T, class O, bool kUnit>
+// kAll: all places are one chunk, which the workgroup sorts by itself; behind the workgroups of the columns come those of the entries that do not
+// occur.
+template <class T, class O, bool kUnit, bool kAll>
 __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restrict__ grad, int64_t rs, int64_t cs, Table B,
-                                                                O* __restrict__ out) {
+                                                                Sort S, O* __restrict__ out) {
     constexpr int V = Pack<T>::V, kFly = 8;
     __shared__ float slot[2][kSumThreads * V];   // [head, tail][group][column]
     __shared__ uint32_t flags[kSumThreads], head[kSumThreads], tail[kSumThreads];
     const uint32_t width = B.lanes * V, tiles = (B.dim + width - 1) / width, per = kSumThreads / B.lanes;
     const uint32_t group = threadIdx.x / B.lanes, in = threadIdx.x % B.lanes;
+    __shared__ u64 list[kAll ? kAllMost : 1];
+    if constexpr (kAll) {
+        if (blockIdx.x >= tiles) return zero_rest<O>(S, B.dim, blockIdx.x - tiles, gridDim.x - tiles, (uint32_t*)list, out);
+        sort_all(S, (uint32_t*)slot, list);
+        B.sorted = list;
+    }
     const uint32_t eighth = (B.chunks + 7) / 8;
-    for (uint64_t job = blockIdx.x; job < (uint64_t)eighth * 8 * tiles; job += gridDim.x) {
+    for (uint64_t job = blockIdx.x; job < (kAll ? (uint64_t)tiles : (uint64_t)eighth * 8 * tiles); job += kAll ? tiles : gridDim.x) {
         const uint32_t chunk = B.by_chiplet ? (uint32_t)(job % 8) * eighth + (uint32_t)(job / 8 / tiles) : (uint32_t)(job / tiles);
         if (chunk >= B.chunks) continue;
         const uint32_t c0 = (uint32_t)((B.by_chiplet ? job / 8 : job) % tiles) * width, c = c0 + in * V;
@@ -381,7 +443,7 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[v] = acc[v] * B.scale;
                 store_values<O, V>(out + (uint64_t)cur * B.dim, c, B.dim, y);
-                if (c == 0) B.mark[cur] = 1;
+                if (!kAll && c == 0) B.mark[cur] = 1;
             }
         };
         if (from < to) {
@@ -443,7 +505,7 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
                     if (f & kHeadEnds) {
                         if (began) out[(uint64_t)head[a] * B.dim + c0 + q] = from_f32<O>(sum * B.scale);
                         else B.part[(uint64_t)chunk * 2 * B.dim + c0 + q] = sum;
-                        if (c0 + q == 0) B.mark[head[a]] = 1;
+                        if (!kAll && c0 + q == 0) B.mark[head[a]] = 1;
                     }
                 }
                 if (f & kTail) {
@@ -559,9 +621,14 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     L.seg_blocks = std::max(1u, (L.blocks + L.segs - 1) / L.segs);
     L.lanes = 1;
     while (L.lanes < 64 && L.lanes * vec < dim) L.lanes *= 2;
+    // workgroups that fill the chip about once (1024 of 512 threads): several rounds wait for the last one's few
+    const uint64_t tiles = (dim + L.lanes * vec - 1) / (L.lanes * vec), per = kSumThreads / L.lanes;
     L.places = L.n <= 1u << 17 ? 16 : 32;
+    while (L.places < 128 && (uint64_t)L.n * tiles > 1024 * per * L.places) L.places *= 2;
+    if (L.n <= kAllMost) L.places = (uint32_t)std::max<uint64_t>(1, (L.n + per - 1) / per);   // one chunk
     L.chunk = L.places * (kSumThreads / L.lanes);
     L.chunks = (L.n + L.chunk - 1) / L.chunk;
+    if (L.n <= kAllMost) return L;   // (no workspace)
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t p = at;
@@ -579,12 +646,19 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
 }
 
 template <class T, class O>
-int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, void* out, hipStream_t st) {
+int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const Sort& S, void* out, hipStream_t st) {
     const uint32_t tiles = (B.dim + B.lanes * Pack<T>::V - 1) / (B.lanes * Pack<T>::V);
+    if (S.n && S.n <= kAllMost) {
+        const unsigned grid = tiles + std::min<uint32_t>((S.entries + kSumThreads - 1) / kSumThreads, 1u << 14);
+        if (cs == 1) table_sum_kernel<T, O, true, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
+        else table_sum_kernel<T, O, false, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
+        CLS_TRY(hipGetLastError());
+        return CBH_OK;
+    }
     if (B.n) {
         const unsigned grid = row_grid((uint64_t)(B.chunks + 7) / 8 * 8 * tiles);
-        if (cs == 1) table_sum_kernel<T, O, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, (O*)out);
-        else table_sum_kernel<T, O, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, (O*)out);
+        if (cs == 1) table_sum_kernel<T, O, true, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
+        else table_sum_kernel<T, O, false, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         CLS_TRY(hipGetLastError());
     }
     const uint32_t join = B.chunks > 1 ? std::min<uint32_t>(B.chunks - 1, 1u << 14) : 0;
@@ -601,11 +675,11 @@ int launch_parts(const Layout& L, char* ws, uint32_t entries, uint32_t dim, floa
     return CBH_OK;
 }
 template <class T>
-int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, void* out, int32_t type, hipStream_t st) {
+int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const Sort& S, void* out, int32_t type, hipStream_t st) {
     switch (type) {
-        case CBH_TYPE_F32: return launch_sums<T, float>(grad, rs, cs, B, out, st);
-        case CBH_TYPE_F16: return launch_sums<T, _Float16>(grad, rs, cs, B, out, st);
-        default: return launch_sums<T, bf16_t>(grad, rs, cs, B, out, st);
+        case CBH_TYPE_F32: return launch_sums<T, float>(grad, rs, cs, B, S, out, st);
+        case CBH_TYPE_F16: return launch_sums<T, _Float16>(grad, rs, cs, B, S, out, st);
+        default: return launch_sums<T, bf16_t>(grad, rs, cs, B, S, out, st);
     }
 }
 
@@ -616,19 +690,20 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
     u64* a = (u64*)(ws + L.keys);
     u64* b = a + L.n;
     const u64* in = nullptr;
+    const unsigned grid = L.segs * L.seg_blocks;   // (one part: the blocks)
     uint32_t* counts = (uint32_t*)(ws + L.counts);
     uint32_t* totals = L.blocks <= kOwnScan && L.segs == 1 ? nullptr : (uint32_t*)(ws + L.totals);
     for (uint32_t p = 0; p < L.passes; ++p) {
         S.shift = (int)(p * L.bits);
         const bool first = p == 0, last = p + 1 == L.passes;
-        if (first) sort_count_kernel<true, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts);
-        else sort_count_kernel<false, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts);
+        if (first) sort_count_kernel<true, ROUNDS><<<grid, 256, 0, st>>>(in, S, counts);
+        else sort_count_kernel<false, ROUNDS><<<grid, 256, 0, st>>>(in, S, counts);
         CLS_TRY(hipGetLastError());
         if (totals) {
             sort_scan_kernel<<<dim3((S.digits + 63) / 64, S.segs), 64 * kScanWaves, 0, st>>>(S, counts, totals);
             CLS_TRY(hipGetLastError());
         }
-#define SCATTER(F, L_) sort_scatter_kernel<F, L_, ROUNDS><<<L.blocks, 256, 0, st>>>(in, S, counts, totals, a)
+#define SCATTER(F, L_) sort_scatter_kernel<F, L_, ROUNDS><<<grid, 256, 0, st>>>(in, S, counts, totals, a)
         if (first) last ? SCATTER(true, true) : SCATTER(true, false);
         else last ? SCATTER(false, true) : SCATTER(false, false);
 #undef SCATTER
@@ -639,11 +714,10 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
     }
     return CBH_OK;
 }
-int sort_places(const int32_t* index, uint32_t entries, uint32_t list, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
-    const Sort S{index, L.n, entries, list, L.blocks, 1u << L.bits, 0, (int)L.bits, L.segs, L.seg_blocks, (uint8_t*)(ws + L.mark)};
+int sort_places(const Sort& S, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
     *sorted = (u64*)(ws + L.keys);
     if (L.passes) return L.rounds == 4 ? sort_by_digits<4>(S, L, ws, sorted, st) : sort_by_digits<16>(S, L, ws, sorted, st);
-    const uint32_t clear = std::min<uint32_t>((entries + 4095) / 4096, 1024);
+    const uint32_t clear = std::min<uint32_t>((S.entries + 4095) / 4096, 1024);
     rank_kernel<<<(L.n + 63) / 64 + clear, 256, 0, st>>>(S, *sorted);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
@@ -747,8 +821,9 @@ extern "C" int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t row
         hipStream_t st = (hipStream_t)stream;
         char* ws = (char*)workspace;
         u64* sorted = nullptr;
-        if (L.n) {
-            rc = sort_places(index, entries, list, L, ws, &sorted, st);
+        const Sort S{index, L.n, entries, list, L.blocks, 1u << L.bits, 0, (int)L.bits, L.segs, L.seg_blocks, (uint8_t*)(ws + L.mark)};
+        if (L.n > kAllMost) {
+            rc = sort_places(S, L, ws, &sorted, st);
             if (rc != CBH_OK) return rc;
         }
         const bool parted = L.segs > 1;
@@ -757,9 +832,9 @@ extern "C" int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t row
         void* sums = parted ? (void*)(ws + L.sums) : table_grad;
         const int32_t sum_type = parted ? CBH_TYPE_F32 : grad_type;
         switch (type) {
-            case CBH_TYPE_F32: rc = launch_sums<float>(grad, row_stride, column_stride, B, sums, sum_type, st); break;
-            case CBH_TYPE_F16: rc = launch_sums<_Float16>(grad, row_stride, column_stride, B, sums, sum_type, st); break;
-            default: rc = launch_sums<bf16_t>(grad, row_stride, column_stride, B, sums, sum_type, st);
+            case CBH_TYPE_F32: rc = launch_sums<float>(grad, row_stride, column_stride, B, S, sums, sum_type, st); break;
+            case CBH_TYPE_F16: rc = launch_sums<_Float16>(grad, row_stride, column_stride, B, S, sums, sum_type, st); break;
+            default: rc = launch_sums<bf16_t>(grad, row_stride, column_stride, B, S, sums, sum_type, st);
         }
         if (rc != CBH_OK || !parted) return rc;
         switch (grad_type) {

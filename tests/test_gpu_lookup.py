@@ -22,6 +22,7 @@ SHAPES = [(1, 1, 1, 1), (3, 1, 5, 4), (70, 1, 10, 33), (1000, 1, 50, 8), (5, 7, 
           (2, 1, 7, 4099), (16384, 1, 40, 16), (16385, 1, 70000, 16), (70001, 5, 131, 6),
           (8192, 1, 600, 9), (8193, 1, 600, 9), (32769, 1, 5000, 2), (131073, 1, 3000, 8), (200000, 3, 70000, 1), (9000, 1, 5000000, 2),
           (2500, 41, 300, 70), (700, 33, 5, 3), (5000, 100, 1500, 19), (1500, 9, 40, 200),
+          (512, 1, 70000, 300), (513, 1, 900, 30), (100, 5, 1500, 9), (255, 2, 3, 700),
           (16500, 33, 700, 70), (150001, 8, 60, 16), (21000, 13, 2100, 100)]
 
 

@@ -66,9 +66,10 @@ def test_table_arguments_are_checked(lib, f):
 
 def test_table_workspace_is_checked(lib):
     assert lookup(lib, table=None) == -5 and table(lib, grad=None) == -5 and table(lib, out_type=5) == -4
-    need = lib.cbh_lookup_gradients_workspace(3, 2, 10, 4)
-    assert need > 0
-    assert table(lib, size=need - 1) == -1 and table(lib, ws=None) == -1 and table(lib, ws=P + 8) == -1
+    need = lib.cbh_lookup_gradients_workspace(3000, 2, 10, 4)
+    assert need > 0 and lib.cbh_lookup_gradients_workspace(256, 2, 10, 4) == 0
+    assert table(lib, rows=3000, size=need - 1) == -1
+    assert table(lib, rows=3000, ws=None) == -1 and table(lib, rows=3000, ws=P + 8) == -1
     # what the entry refuses needs none
     assert lib.cbh_lookup_gradients_workspace(1 << 31, 1, 10, 4) == 0
 
