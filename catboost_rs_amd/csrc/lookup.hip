@@ -133,25 +133,29 @@ __device__ __forceinline__ u64 sorted_key(const Sort& S, uint32_t seg, uint32_t 
 }
 __device__ __forceinline__ uint32_t place_entry(const Sort& S, uint32_t i) { return min((uint32_t)S.index[i], S.entries); }
 __device__ __forceinline__ void clear_marks(const Sort& S, uint32_t block, uint32_t blocks) {
-    for (uint64_t v = (uint64_t)block * 256 + threadIdx.x; v < (uint64_t)S.segs * S.entries; v += (uint64_t)blocks * 256) S.mark[v] = 0;
+    for (uint64_t v = (uint64_t)block * blockDim.x + threadIdx.x; v < (uint64_t)S.segs * S.entries; v += (uint64_t)blocks * blockDim.x) S.mark[v] = 0;
 }
 
-// Few places: a workgroup takes 64 of them and counts, over all places, those ahead of each; a wave a quarter of them.
-constexpr uint32_t kRankMost = 8192;
-__global__ __launch_bounds__(256) void rank_kernel(Sort S, u64* __restrict__ out) {
+// Few places: a workgroup takes 64 of them and counts, over all places, those ahead of each; a wave a sixteenth of them.
+constexpr uint32_t kRankMost = 8192, kRankWaves = 16;
+__global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(Sort S, u64* __restrict__ out) {
     __shared__ uint32_t entry[kRankMost];
-    __shared__ uint32_t ahead[4][64];
+    __shared__ uint32_t ahead[kRankWaves][64];
     const uint32_t blocks = (S.n + 63) / 64;
     if (blockIdx.x >= blocks) return clear_marks(S, blockIdx.x - blocks, gridDim.x - blocks);
-    const uint32_t n4 = (S.n + 15) / 16 * 16;   // (four quarters of whole vectors; what lies behind the places is behind all)
-    for (uint32_t i = threadIdx.x; i < n4; i += 256) entry[i] = i < S.n ? place_entry(S, i) : ~0u;
+    const uint32_t n64 = (S.n + 63) / 64 * 64;   // (sixteenths of whole vectors; what lies behind the places is behind all)
+#pragma unroll
+    for (uint32_t r = 0; r < kRankMost / 64 / kRankWaves; ++r) {
+        const uint32_t i = r * 64 * kRankWaves + threadIdx.x;
+        if (i < n64) entry[i] = i < S.n ? place_entry(S, i) : ~0u;
+    }
     __syncthreads();
     const uint32_t wave = threadIdx.x / 64, lane = lane_id(), at = blockIdx.x * 64 + lane;
     const uint32_t mine = at < S.n ? entry[at] : ~0u;
-    const uint32_t from = wave * (n4 / 4), to = from + n4 / 4;
+    const uint32_t from = wave * (n64 / kRankWaves), to = from + n64 / kRankWaves;
     // places before this workgroup's go ahead of an equal one, those behind it do not
     uint32_t count = 0;
-    const uint32_t own0 = min(max(blockIdx.x * 64, from), to), own1 = min(max(min(blockIdx.x * 64 + 64, n4), from), to);
+    const uint32_t own0 = min(max(blockIdx.x * 64, from), to), own1 = min(max(min(blockIdx.x * 64 + 64, n64), from), to);
     typedef uint32_t Quad __attribute__((ext_vector_type(4)));
     const Quad* q = (const Quad*)entry;
 #pragma unroll 4
@@ -167,8 +171,12 @@ __global__ __launch_bounds__(256) void rank_kernel(Sort S, u64* __restrict__ out
     }
     ahead[wave][lane] = count;
     __syncthreads();
-    if (wave == 0 && at < S.n)
-        out[ahead[0][lane] + ahead[1][lane] + ahead[2][lane] + ahead[3][lane]] = sorted_key(S, 0, mine, at);
+    if (wave == 0 && at < S.n) {
+        uint32_t place = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kRankWaves; ++w) place += ahead[w][lane];
+        out[place] = sorted_key(S, 0, mine, at);
+    }
 }
 
 // Many places: radix sort of (entry, place), least significant digits first, of up to 11 bits.  A workgroup ranks
@@ -379,43 +387,51 @@ __device__ __forceinline__ void sort_all(const Sort& S, uint32_t* entry, u64* li
     }
     __syncthreads();
 }
-// The entries that do not occur among few places: `blocks` workgroups, 512 entries at a time.
+// Entries that a workgroup clears at a time: about 64 KB of them, for enough workgroups.
+template <class O>
+__host__ __device__ inline uint32_t zero_rows(uint32_t dim, uint32_t most) {
+    const uint32_t rows = 65536 / (uint32_t)sizeof(O) / dim;
+    return rows < 8 ? 8 : rows < most ? rows : most;
+}
+// The entries that do not occur among few places: `blocks` workgroups.
 template <class O>
 __device__ __forceinline__ void zero_rest(const Sort& S, uint32_t dim, uint32_t block, uint32_t blocks, uint32_t* occurs, O* out) {
     constexpr uint32_t V = 16 / sizeof(O);
     const uint32_t vecs = (dim + V - 1) / V, mine = threadIdx.x < S.n ? place_entry(S, threadIdx.x) : ~0u;
-    for (uint64_t row0 = (uint64_t)block * kSumThreads; row0 < S.entries; row0 += (uint64_t)blocks * kSumThreads) {
+    const uint32_t most = zero_rows<O>(dim, kSumThreads);
+    for (uint64_t row0 = (uint64_t)block * most; row0 < S.entries; row0 += (uint64_t)blocks * most) {
         __syncthreads();
         occurs[threadIdx.x] = 0;
         __syncthreads();
-        if (mine < S.entries && mine >= row0 && mine - row0 < kSumThreads) occurs[mine - row0] = 1;
+        if (mine < S.entries && mine >= row0 && mine - row0 < most) occurs[mine - row0] = 1;
         __syncthreads();
-        const uint32_t rows = (uint32_t)min((uint64_t)kSumThreads, S.entries - row0);
+        const uint32_t rows = (uint32_t)min((uint64_t)most, S.entries - row0);
         float z[V] = {};
-        for (uint64_t j = threadIdx.x; j < (uint64_t)rows * vecs; j += kSumThreads) {
-            const uint32_t r = (uint32_t)(j / vecs);
-            if (!occurs[r]) store_pack<O, true>(out + (row0 + r) * dim, 1, (uint32_t)(j % vecs) * V, dim, z);
+        for (uint32_t j = threadIdx.x; j < rows * vecs; j += kSumThreads) {
+            const uint32_t r = j / vecs;
+            if (!occurs[r]) store_pack<O, true>(out + (row0 + r) * dim, 1, j % vecs * V, dim, z);
         }
     }
 }
 
 // A group of lanes takes `places` of the list, eight rows on their way at a time, and writes the runs that lie within them.
-// What of a run lies in several groups goes to LDS and is added up there, in the groups' order, a column a thread; what lies in several
-// workgroups, by join_kernel.
-enum { kHead = 1, kHeadEnds = 2, kTail = 4, kGoesOn = 8 };
+// What of a run lies in several groups goes to LDS and is added up, in the groups' order, by the group in which it begins; what lies
+// in several workgroups, by join_kernel.
+enum { kHead = 1, kHeadEnds = 2, kTail = 4 };   // the first run began before; and ends here; the last begins here and goes on
 // kAll: all places are one chunk, which the workgroup sorts by itself; behind the workgroups of the columns come those of the entries that do not
 // occur.
 template <class T, class O, bool kUnit, bool kAll>
 __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restrict__ grad, int64_t rs, int64_t cs, Table B,
                                                                 Sort S, O* __restrict__ out) {
     constexpr int V = Pack<T>::V, kFly = 8;
-    __shared__ float slot[2][kSumThreads * V];   // [head, tail][group][column]
-    __shared__ uint32_t flags[kSumThreads], head[kSumThreads], tail[kSumThreads];
+    __shared__ float slot[kSumThreads * V];   // heads [group][column]
+    __shared__ uint32_t flags[kSumThreads];
     const uint32_t width = B.lanes * V, tiles = (B.dim + width - 1) / width, per = kSumThreads / B.lanes;
     const uint32_t group = threadIdx.x / B.lanes, in = threadIdx.x % B.lanes;
     __shared__ u64 list[kAll ? kAllMost : 1];
     if constexpr (kAll) {
         if (blockIdx.x >= tiles) return zero_rest<O>(S, B.dim, blockIdx.x - tiles, gridDim.x - tiles, (uint32_t*)list, out);
+        static_assert(kAllMost <= kSumThreads * V, "entries in the heads' place");
         sort_all(S, (uint32_t*)slot, list);
         B.sorted = list;
     }
@@ -430,13 +446,13 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
         float acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        auto keep = [&](uint32_t which) {
+        auto keep = [&] {
 #pragma unroll
-            for (int v = 0; v < V; ++v) slot[which][threadIdx.x * V + v] = acc[v];
+            for (int v = 0; v < V; ++v) slot[threadIdx.x * V + v] = acc[v];
         };
         auto finish = [&] {   // the run of cur ends within the group
             if (before) {
-                keep(0);
+                keep();
                 flag |= kHead | kHeadEnds;
             } else if (cur < B.entries && c < B.dim) {
                 float y[V];
@@ -449,7 +465,6 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
         if (from < to) {
             cur = entry_at(B, from);
             before = from > 0 && cur < B.entries && entry_at(B, from - 1) == cur;
-            if (in == 0) head[group] = cur;
             for (uint32_t i0 = from; i0 < to; i0 += kFly) {
                 uint32_t e[kFly];
                 Pack<T> p[kFly];
@@ -485,61 +500,63 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
             if (!after) {
                 finish();
             } else {
-                keep(before ? 0 : 1);
-                flag |= before ? kHead | kGoesOn : kTail | kGoesOn;
+                if (before) keep();
+                flag |= before ? kHead : kTail;   // (a tail stays in acc)
             }
         }
-        if (in == 0) {
-            flags[group] = flag;
-            tail[group] = cur;
-        }
+        if (in == 0) flags[group] = flag;
         __syncthreads();
-        for (uint32_t q = threadIdx.x; q < width; q += kSumThreads) {
-            if (c0 + q >= B.dim) break;
-            float sum = 0.0f;
-            bool began = false, on = false;   // the run began in this workgroup; goes on from the last group
-            for (uint32_t a = 0; a < per; ++a) {
-                const uint32_t f = flags[a];
-                if (f & kHead) {
-                    sum += slot[0][a * width + q];
-                    if (f & kHeadEnds) {
-                        if (began) out[(uint64_t)head[a] * B.dim + c0 + q] = from_f32<O>(sum * B.scale);
-                        else B.part[(uint64_t)chunk * 2 * B.dim + c0 + q] = sum;
-                        if (!kAll && c0 + q == 0) B.mark[head[a]] = 1;
-                    }
-                }
-                if (f & kTail) {
-                    sum = slot[1][a * width + q];
-                    began = true;
-                }
-                on = f & kGoesOn;
+        // a run's parts, by the group in which it begins, or by the first where it began before the chunk
+        const bool tails = flag & kTail, heads = group == 0 && (flag & kHead);
+        if ((tails || heads) && c < B.dim) {
+            if (tails && heads) {   // (a head that ends here, before the tail)
+                float y[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = slot[threadIdx.x * V + v];
+                store_values<float, V>(B.part + (uint64_t)chunk * 2 * B.dim, c, B.dim, y);
+            } else if (heads) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] = slot[threadIdx.x * V + v];
             }
-            if (on) {   // (past this workgroup: a run that goes on from a group has its next part in the one behind)
-                B.part[((uint64_t)chunk * 2 + began) * B.dim + c0 + q] = sum;
-                if (c0 + q == 0) B.mark[tail[per - 1]] = 1;
+            uint32_t last = tails ? 0u : flag, a = group + 1;
+            while (!(last & kHeadEnds) && a < per && (flags[a] & kHead)) {
+                last = flags[a];
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] += slot[(a * B.lanes + in) * V + v];
+                ++a;
             }
+            if (!(last & kHeadEnds) || !tails) {   // past this workgroup, or from before it
+                float* p = B.part + ((uint64_t)chunk * 2 + tails) * B.dim;
+                store_values<float, V>(p, c, B.dim, acc);
+            } else {
+                float y[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v] = acc[v] * B.scale;
+                store_values<O, V>(out + (uint64_t)cur * B.dim, c, B.dim, y);
+            }
+            if (!kAll && c == 0 && tails) B.mark[cur] = 1;
         }
         __syncthreads();
     }
 }
 
 // Runs of several workgroups, by that of the chunk in which they begin; and the entries that do not occur.
-constexpr uint32_t kZeroRows = 256;
 template <class O>
 __global__ __launch_bounds__(256) void table_join_kernel(Table B, uint32_t join_blocks, O* __restrict__ out) {
-    __shared__ uint32_t list[kZeroRows], count;
+    __shared__ uint32_t list[256], count;
     __shared__ float sum[4][64];
     const uint32_t wave = threadIdx.x / 64, lane = lane_id();
     if (blockIdx.x >= join_blocks) {
         constexpr uint32_t V = 16 / sizeof(O);
         const uint32_t vecs = (B.dim + V - 1) / V;
-        for (uint64_t row0 = (uint64_t)(blockIdx.x - join_blocks) * kZeroRows; row0 < B.entries;
-             row0 += (uint64_t)(gridDim.x - join_blocks) * kZeroRows) {
+        const uint32_t most = zero_rows<O>(B.dim, 256);
+        for (uint64_t row0 = (uint64_t)(blockIdx.x - join_blocks) * most; row0 < B.entries;
+             row0 += (uint64_t)(gridDim.x - join_blocks) * most) {
             __syncthreads();
             if (threadIdx.x == 0) count = 0;
             __syncthreads();
             const uint64_t row = row0 + threadIdx.x;
-            if (row < B.entries && (!B.n || !B.mark[row])) list[atomicAdd(&count, 1u)] = threadIdx.x;   // (their order does not matter)
+            if (threadIdx.x < most && row < B.entries && (!B.n || !B.mark[row])) list[atomicAdd(&count, 1u)] = threadIdx.x;   // (their order does not matter)
             __syncthreads();
             float z[V] = {};
             for (uint32_t j = threadIdx.x; j < count * vecs; j += 256)
@@ -623,7 +640,7 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     while (L.lanes < 64 && L.lanes * vec < dim) L.lanes *= 2;
     // workgroups that fill the chip about once (1024 of 512 threads): several rounds wait for the last one's few
     const uint64_t tiles = (dim + L.lanes * vec - 1) / (L.lanes * vec), per = kSumThreads / L.lanes;
-    L.places = L.n <= 1u << 17 ? 16 : 32;
+    L.places = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(8, (L.n <= 1u << 17 ? 256 : 512) / per));
     while (L.places < 128 && (uint64_t)L.n * tiles > 1024 * per * L.places) L.places *= 2;
     if (L.n <= kAllMost) L.places = (uint32_t)std::max<uint64_t>(1, (L.n + per - 1) / per);   // one chunk
     L.chunk = L.places * (kSumThreads / L.lanes);
@@ -645,11 +662,16 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     return L;
 }
 
+template <class O>
+uint32_t zero_blocks(uint32_t entries, uint32_t dim, uint32_t most) {
+    const uint32_t rows = zero_rows<O>(dim, most);
+    return std::min<uint32_t>((entries + rows - 1) / rows, 1u << 14);
+}
 template <class T, class O>
 int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const Sort& S, void* out, hipStream_t st) {
     const uint32_t tiles = (B.dim + B.lanes * Pack<T>::V - 1) / (B.lanes * Pack<T>::V);
     if (S.n && S.n <= kAllMost) {
-        const unsigned grid = tiles + std::min<uint32_t>((S.entries + kSumThreads - 1) / kSumThreads, 1u << 14);
+        const unsigned grid = tiles + zero_blocks<O>(S.entries, B.dim, kSumThreads);
         if (cs == 1) table_sum_kernel<T, O, true, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         else table_sum_kernel<T, O, false, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         CLS_TRY(hipGetLastError());
@@ -662,7 +684,7 @@ int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const 
         CLS_TRY(hipGetLastError());
     }
     const uint32_t join = B.chunks > 1 ? std::min<uint32_t>(B.chunks - 1, 1u << 14) : 0;
-    const uint32_t zero = B.by_chiplet ? 0 : std::min<uint32_t>((B.entries + kZeroRows - 1) / kZeroRows, 1u << 14);
+    const uint32_t zero = B.by_chiplet ? 0 : zero_blocks<O>(B.entries, B.dim, 256);
     table_join_kernel<O><<<std::max(1u, join + zero), 256, 0, st>>>(B, join, (O*)out);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
@@ -717,8 +739,8 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
 int sort_places(const Sort& S, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
     *sorted = (u64*)(ws + L.keys);
     if (L.passes) return L.rounds == 4 ? sort_by_digits<4>(S, L, ws, sorted, st) : sort_by_digits<16>(S, L, ws, sorted, st);
-    const uint32_t clear = std::min<uint32_t>((S.entries + 4095) / 4096, 1024);
-    rank_kernel<<<(L.n + 63) / 64 + clear, 256, 0, st>>>(S, *sorted);
+    const uint32_t clear = std::min<uint32_t>((S.entries + 16383) / 16384, 1024);
+    rank_kernel<<<(L.n + 63) / 64 + clear, 64 * kRankWaves, 0, st>>>(S, *sorted);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
