@@ -6,8 +6,9 @@
    (``apply_oblivious``): raw scores [classes][rows].
 2. ``top_classes`` keeps the teacher's k largest scores of every row and its log-sum-exp: what a
    student needs, in a fraction of the memory of the scores.
-3. A linear student in torch is trained on ``distill_gradients`` alone; it never sees a label.
-4. ``sample_classes`` draws an answer of the student for every row, within a nucleus.
+3. A linear student in torch is trained on ``distill_gradients`` alone, by ``AdamW`` steps; it never sees a label.
+4. ``sample_classes`` draws an answer of the student for every row, within a nucleus; ``class_logprobs`` says how
+   probable the labels are to it.
 
 torch is imported first: one HIP runtime serves the process.
 """
@@ -52,11 +53,12 @@ def main(rows=20_000, features=12, classes=10, k=3, temperature=2.0, steps=60):
 
     inputs = torch.from_numpy(x).cuda()
     weight = torch.zeros(classes, features, device="cuda")
+    optimizer = cb.AdamW([weight], lr=0.05, weight_decay=0.0)
     losses = []
     for _ in range(steps):
         scores = (weight @ inputs).t()                                  # class-major, as the teacher's
         loss, grad = cb.distill_gradients(scores, values, index, top_lse=lse, temperature=temperature)
-        weight -= (2.0 / rows) * (grad.t() @ inputs.t())
+        optimizer.step([grad.t() @ inputs.t() / rows])
         losses.append(loss.mean())
     losses = torch.stack(losses).tolist()
 
@@ -65,8 +67,10 @@ def main(rows=20_000, features=12, classes=10, k=3, temperature=2.0, steps=60):
     drawn, logprob = cb.sample_classes(scores, uniform, top_p=0.9)
     best, _ = cb.sample_classes(scores, uniform, temperature=0.0)
     agree = (best == index[:, 0]).float().mean().item()
+    labels = cb.class_logprobs(scores, torch.from_numpy(y.astype(np.int32)).cuda())
     print(f"distillation loss {losses[0]:.4f} -> {losses[-1]:.4f}; the student's first class is the teacher's on "
-          f"{agree:.1%} of the rows; mean log probability of a drawn class {logprob.mean().item():.3f}")
+          f"{agree:.1%} of the rows; mean log probability of a drawn class {logprob.mean().item():.3f}, of the label "
+          f"{labels.logprob.mean().item():.3f}")
     return losses, agree, drawn
 
 

@@ -304,6 +304,25 @@ def check_refusals():
     assert opt.steps == 0
 
 
+def check_example():
+    """The additive student runs, and its gradient is that of its loss (a plain one in 64 bits, by autograd)."""
+    from examples import additive_student as A
+    losses, held = A.main(rows=2000, steps=3)
+    assert len(losses) == 3 and all(np.isfinite(losses)) and bool(torch.isfinite(held).all())
+    x, y = A.table(500, 5, 7)
+    index, entries = A.binned(x, 9)
+    held = torch.randn(entries, 7, generator=torch.Generator(device=DEVICE).manual_seed(9), device=DEVICE)
+    index, label = torch.from_numpy(index).cuda(), torch.from_numpy(y.astype(np.int32)).cuda()
+    loss, grad = A.loss_and_gradient(held, index, label)
+    leaf = held.double().requires_grad_()
+    logp = torch.log_softmax(leaf[index.long()].sum(1), 1)
+    plain = -(logp.gather(1, label.long()[:, None]).mean() - 0.01 * (logp.exp() * logp).sum(1).mean())
+    plain.backward()
+    # scores are sums of five f32 values of up to 4; a gradient is a sum of up to 500 of them, each a p to 40 roundings, over 500 rows
+    assert abs(loss.item() - plain.item()) < 1e-5
+    assert (grad - leaf.grad).abs().max().item() < 500 / 500 * 60 * 2.0 ** -23
+
+
 if __name__ == "__main__":
     for name, f in list(globals().items()):
         if name.startswith("check_"):
