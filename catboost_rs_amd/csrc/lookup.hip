@@ -10,6 +10,26 @@
 namespace {
 using namespace cbh::cls;
 
+// A vector of a row, from column c on.  kWhole: all rows are whole vectors of columns next to each other.  Else its values are loaded
+// one by one where it does not lie whole in its row, without a branch between them (behind the end the last column again): guarded, each
+// was waited for.
+template <class T, bool kWhole>
+__device__ __forceinline__ Pack<T> load_columns(const T* row, int64_t cs, uint32_t c, uint32_t dim) {
+    constexpr int V = Pack<T>::V;
+    Pack<T> p;
+    if (kWhole || (cs == 1 && c + V <= dim)) {
+        p.w = ((const Loose<T>*)(row + c))->w;
+    } else {
+        float x[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = to_f32(row[(int64_t)min(c + v, dim - 1) * cs]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = c + v < dim ? x[v] : 0.0f;
+        p.set(x);
+    }
+    return p;
+}
+
 // ---- rows -----------------------------------------------------------------------------------
 struct Lookup {
     const int32_t* index;   // [rows][list]
@@ -30,7 +50,7 @@ __device__ __forceinline__ void load_indices(const Lookup& L, const int32_t* ix,
     }
 }
 // A group of `lanes` lanes takes a row of the output, a vector a lane, four rows of the table on their way at a time.
-template <class T, bool kUnit>
+template <class T, bool kWhole>
 __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, int64_t rs, int64_t cs, Lookup L,
                                                      T* __restrict__ out, uint32_t lanes) {
     constexpr int V = Pack<T>::V;
@@ -44,22 +64,19 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table
         float acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        uint32_t next[4];
+        load_indices(L, ix, 0, next);
         for (uint32_t i = 0; i < L.list; i += 4) {
             uint32_t e[4];
-            load_indices(L, ix, i, e);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) e[u] = next[u];
+            if (i + 4 < L.list) load_indices(L, ix, i + 4, next);
             Pack<T> p[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const T* at = table + (int64_t)e[u] * rs;
-                if (e[u] >= L.entries) {
-                    p[u].w = Words{};
-                } else if (kUnit && c + V <= L.dim) {
-                    p[u].w = ((const Loose<T>*)(at + c))->w;
-                } else {
-                    float x[V];
-                    load_pack<T, kUnit>(at, cs, c, L.dim, 0.0f, x);
-                    p[u].set(x);
-                }
+                // (without a branch: what is no entry reads the first and drops it)
+                p[u] = load_columns<T, kWhole>(table + (int64_t)(e[u] < L.entries ? e[u] : 0) * rs, cs, c, L.dim);
+                if (e[u] >= L.entries) p[u].w = Words{};
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
@@ -82,11 +99,8 @@ __global__ __launch_bounds__(kLdsThreads) void lookup_lds_kernel(const T* __rest
     const int shift = 31 - __builtin_clz(lanes);
     if (threadIdx.x < lanes) held[L.entries * lanes + threadIdx.x] = Words{};
     for (uint32_t i = threadIdx.x; i < L.entries * lanes; i += kLdsThreads) {
-        float x[V];
-        Pack<T> p;
-        load_pack<T, true>(table + (int64_t)(i / lanes) * rs, 1, c0 + i % lanes * V, L.dim, 0.0f, x);
-        p.set(x);
-        held[i] = p.w;
+        const uint32_t at = c0 + i % lanes * V;
+        held[i] = at < L.dim ? load_columns<T, false>(table + (int64_t)(i / lanes) * rs, 1, at, L.dim).w : Words{};
     }
     __syncthreads();
     const uint64_t from = blockIdx.x / tiles * part, to = min(L.rows, from + part);
@@ -138,11 +152,21 @@ __device__ __forceinline__ void clear_marks(const Sort& S, uint32_t block, uint3
 
 // Few places: a workgroup takes 64 of them and counts, over all places, those ahead of each; a wave a sixteenth of them.
 constexpr uint32_t kRankMost = 8192, kRankWaves = 16;
-__global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(Sort S, u64* __restrict__ out) {
+template <class O>
+__global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(Sort S, u64* __restrict__ out, O* __restrict__ grad, uint64_t cells) {
     __shared__ uint32_t entry[kRankMost];
     __shared__ uint32_t ahead[kRankWaves][64];
     const uint32_t blocks = (S.n + 63) / 64;
-    if (blockIdx.x >= blocks) return clear_marks(S, blockIdx.x - blocks, gridDim.x - blocks);
+    if (blockIdx.x >= blocks) {   // the whole gradient is cleared: few of its entries occur, and are written over
+        constexpr uint32_t V = 16 / sizeof(O);
+        typedef uint32_t Unaligned __attribute__((ext_vector_type(4), aligned(2)));
+        for (uint64_t i = ((uint64_t)(blockIdx.x - blocks) * blockDim.x + threadIdx.x) * V; i < cells; i += (uint64_t)(gridDim.x - blocks) * blockDim.x * V) {
+            if (i + V <= cells) __builtin_nontemporal_store(Words{}, (Unaligned*)(grad + i));
+            else
+                for (uint64_t j = i; j < cells; ++j) grad[j] = from_f32<O>(0.0f);
+        }
+        return;
+    }
     const uint32_t n64 = (S.n + 63) / 64 * 64;   // (sixteenths of whole vectors; what lies behind the places is behind all)
 #pragma unroll
     for (uint32_t r = 0; r < kRankMost / 64 / kRankWaves; ++r) {
@@ -334,7 +358,7 @@ struct Table {
     bool by_chiplet;           // an eighth of the chunks, one after another, to each of the chip's eight dies
     float scale;
     float* part;         // [chunks][2][dim]: of the first run, where it began before; of the last, where it goes on
-    uint8_t* mark;
+    uint8_t* mark;       // null: what does not occur is 0 already
 };
 __device__ __forceinline__ uint32_t entry_at(const Table& B, uint32_t i) { return (uint32_t)(B.sorted[i] >> 32); }
 
@@ -420,7 +444,7 @@ __device__ __forceinline__ void zero_rest(const Sort& S, uint32_t dim, uint32_t 
 enum { kHead = 1, kHeadEnds = 2, kTail = 4 };   // the first run began before; and ends here; the last begins here and goes on
 // kAll: all places are one chunk, which the workgroup sorts by itself; behind the workgroups of the columns come those of the entries that do not
 // occur.
-template <class T, class O, bool kUnit, bool kAll>
+template <class T, class O, bool kWhole, bool kAll>
 __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restrict__ grad, int64_t rs, int64_t cs, Table B,
                                                                 Sort S, O* __restrict__ out) {
     constexpr int V = Pack<T>::V, kFly = 8;
@@ -440,6 +464,7 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
         const uint32_t chunk = B.by_chiplet ? (uint32_t)(job % 8) * eighth + (uint32_t)(job / 8 / tiles) : (uint32_t)(job / tiles);
         if (chunk >= B.chunks) continue;
         const uint32_t c0 = (uint32_t)((B.by_chiplet ? job / 8 : job) % tiles) * width, c = c0 + in * V;
+        const uint32_t column = c < B.dim ? c : 0;   // (a lane behind the row reads its beginning)
         const uint32_t from = min(B.n, chunk * B.chunk + group * B.places), to = min(B.n, from + B.places);
         uint32_t cur = kNoEntry, flag = 0;
         bool before = false;
@@ -459,7 +484,7 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[v] = acc[v] * B.scale;
                 store_values<O, V>(out + (uint64_t)cur * B.dim, c, B.dim, y);
-                if (!kAll && c == 0) B.mark[cur] = 1;
+                if (!kAll && c == 0 && B.mark) B.mark[cur] = 1;
             }
         };
         if (from < to) {
@@ -472,16 +497,8 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
                 for (int u = 0; u < kFly; ++u) {
                     const u64 key = B.sorted[min(i0 + u, to - 1)];
                     e[u] = i0 + u < to ? (uint32_t)(key >> 32) : kNoEntry;
-                    const T* row = grad + (int64_t)(uint32_t)key * rs;
-                    if (e[u] >= B.entries) {
-                        p[u].w = Words{};
-                    } else if (kUnit && c + V <= B.dim) {
-                        p[u].w = ((const Loose<T>*)(row + c))->w;
-                    } else {
-                        float x[V];
-                        load_pack<T, kUnit>(row, cs, c, B.dim, 0.0f, x);
-                        p[u].set(x);
-                    }
+                    p[u] = load_columns<T, kWhole>(grad + (int64_t)(uint32_t)key * rs, cs, column, B.dim);   // (without a branch)
+                    if (e[u] >= B.entries) p[u].w = Words{};
                 }
 #pragma unroll
                 for (int u = 0; u < kFly; ++u) {
@@ -534,7 +551,7 @@ __global__ __launch_bounds__(kSumThreads) void table_sum_kernel(const T* __restr
                 for (int v = 0; v < V; ++v) y[v] = acc[v] * B.scale;
                 store_values<O, V>(out + (uint64_t)cur * B.dim, c, B.dim, y);
             }
-            if (!kAll && c == 0 && tails) B.mark[cur] = 1;
+            if (!kAll && c == 0 && tails && B.mark) B.mark[cur] = 1;
         }
         __syncthreads();
     }
@@ -638,6 +655,8 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     L.seg_blocks = std::max(1u, (L.blocks + L.segs - 1) / L.segs);
     L.lanes = 1;
     while (L.lanes < 64 && L.lanes * vec < dim) L.lanes *= 2;
+    // few places in one chunk: fewer lanes a group, so that eight places are a group's, one after another
+    while (L.n <= kAllMost && L.lanes > 8 && kSumThreads / L.lanes * 8 < L.n) L.lanes /= 2;
     // workgroups that fill the chip about once (1024 of 512 threads): several rounds wait for the last one's few
     const uint64_t tiles = (dim + L.lanes * vec - 1) / (L.lanes * vec), per = kSumThreads / L.lanes;
     L.places = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(8, (L.n <= 1u << 17 ? 256 : 512) / per));
@@ -655,7 +674,7 @@ Layout layout(uint64_t rows, uint32_t list, uint32_t entries, uint32_t dim, uint
     L.keys = take((L.passes > 1 ? 16 : 8) * (uint64_t)L.n);
     L.counts = take(L.passes ? 4ull * L.blocks << L.bits : 0);
     L.totals = take(L.passes ? (4ull << L.bits) * L.segs : 0);
-    L.mark = take(L.n ? (uint64_t)entries * L.segs : 0);
+    L.mark = take(L.passes ? (uint64_t)entries * L.segs : 0);
     L.sums = take(L.segs > 1 ? 4 * cells * L.segs : 0);
     L.part = take(8ull * L.chunks * dim);
     L.bytes = at;
@@ -670,22 +689,24 @@ uint32_t zero_blocks(uint32_t entries, uint32_t dim, uint32_t most) {
 template <class T, class O>
 int launch_sums(const void* grad, int64_t rs, int64_t cs, const Table& B, const Sort& S, void* out, hipStream_t st) {
     const uint32_t tiles = (B.dim + B.lanes * Pack<T>::V - 1) / (B.lanes * Pack<T>::V);
+    const bool whole = cs == 1 && B.dim % Pack<T>::V == 0;
     if (S.n && S.n <= kAllMost) {
         const unsigned grid = tiles + zero_blocks<O>(S.entries, B.dim, kSumThreads);
-        if (cs == 1) table_sum_kernel<T, O, true, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
+        if (whole) table_sum_kernel<T, O, true, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         else table_sum_kernel<T, O, false, true><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         CLS_TRY(hipGetLastError());
         return CBH_OK;
     }
     if (B.n) {
         const unsigned grid = row_grid((uint64_t)(B.chunks + 7) / 8 * 8 * tiles);
-        if (cs == 1) table_sum_kernel<T, O, true, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
+        if (whole) table_sum_kernel<T, O, true, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         else table_sum_kernel<T, O, false, false><<<grid, kSumThreads, 0, st>>>((const T*)grad, rs, cs, B, S, (O*)out);
         CLS_TRY(hipGetLastError());
     }
     const uint32_t join = B.chunks > 1 ? std::min<uint32_t>(B.chunks - 1, 1u << 14) : 0;
-    const uint32_t zero = B.by_chiplet ? 0 : zero_blocks<O>(B.entries, B.dim, 256);
-    table_join_kernel<O><<<std::max(1u, join + zero), 256, 0, st>>>(B, join, (O*)out);
+    const uint32_t zero = B.by_chiplet || (B.n && !B.mark) ? 0 : zero_blocks<O>(B.entries, B.dim, 256);
+    if (join + zero == 0) return CBH_OK;
+    table_join_kernel<O><<<join + zero, 256, 0, st>>>(B, join, (O*)out);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
@@ -736,11 +757,12 @@ int sort_by_digits(Sort S, const Layout& L, char* ws, u64** sorted, hipStream_t 
     }
     return CBH_OK;
 }
-int sort_places(const Sort& S, const Layout& L, char* ws, u64** sorted, hipStream_t st) {
-    *sorted = (u64*)(ws + L.keys);
-    if (L.passes) return L.rounds == 4 ? sort_by_digits<4>(S, L, ws, sorted, st) : sort_by_digits<16>(S, L, ws, sorted, st);
-    const uint32_t clear = std::min<uint32_t>((S.entries + 16383) / 16384, 1024);
-    rank_kernel<<<(L.n + 63) / 64 + clear, 64 * kRankWaves, 0, st>>>(S, *sorted);
+// Few places: sorted by one launch, which clears the gradient too.
+template <class O>
+int rank_places(const Sort& S, u64* sorted, void* out, uint32_t dim, hipStream_t st) {
+    const uint64_t cells = (uint64_t)S.entries * dim, each = 64 * kRankWaves * (16 / sizeof(O)) * 4;
+    const unsigned clear = (unsigned)std::min<uint64_t>((cells + each - 1) / each, 2048);
+    rank_kernel<O><<<(S.n + 63) / 64 + clear, 64 * kRankWaves, 0, st>>>(S, sorted, (O*)out, cells);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
 }
@@ -790,7 +812,7 @@ int run_lookup(const void* table, int64_t rs, int64_t cs, const Lookup& L, void*
     }
     const uint32_t tiles = (L.dim + lanes * V - 1) / (lanes * V), per = 256 / lanes;
     const unsigned grid = row_grid((L.rows + per - 1) / per * tiles);
-    if (cs == 1) lookup_kernel<T, true><<<grid, 256, 0, st>>>((const T*)table, rs, cs, L, (T*)out, lanes);
+    if (cs == 1 && L.dim % V == 0) lookup_kernel<T, true><<<grid, 256, 0, st>>>((const T*)table, rs, cs, L, (T*)out, lanes);
     else lookup_kernel<T, false><<<grid, 256, 0, st>>>((const T*)table, rs, cs, L, (T*)out, lanes);
     CLS_TRY(hipGetLastError());
     return CBH_OK;
@@ -845,12 +867,15 @@ extern "C" int cbh_lookup_gradients(const void* grad, int32_t type, uint64_t row
         u64* sorted = nullptr;
         const Sort S{index, L.n, entries, list, L.blocks, 1u << L.bits, 0, (int)L.bits, L.segs, L.seg_blocks, (uint8_t*)(ws + L.mark)};
         if (L.n > kAllMost) {
-            rc = sort_places(S, L, ws, &sorted, st);
+            sorted = (u64*)(ws + L.keys);
+            if (L.passes) rc = L.rounds == 4 ? sort_by_digits<4>(S, L, ws, &sorted, st) : sort_by_digits<16>(S, L, ws, &sorted, st);
+            else if (grad_type == CBH_TYPE_F32) rc = rank_places<float>(S, sorted, table_grad, dim, st);
+            else rc = rank_places<_Float16>(S, sorted, table_grad, dim, st);   // (0 is the same in both 16-bit types)
             if (rc != CBH_OK) return rc;
         }
         const bool parted = L.segs > 1;
         const Table B{sorted,  L.n,      L.segs * entries, dim,    L.lanes,        L.places, L.chunk,
-                      L.chunks, parted, parted ? 1.0f : (float)scale, (float*)(ws + L.part), (uint8_t*)(ws + L.mark)};
+                      L.chunks, parted, parted ? 1.0f : (float)scale, (float*)(ws + L.part), L.passes ? (uint8_t*)(ws + L.mark) : nullptr};
         void* sums = parted ? (void*)(ws + L.sums) : table_grad;
         const int32_t sum_type = parted ? CBH_TYPE_F32 : grad_type;
         switch (type) {
