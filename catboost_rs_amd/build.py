@@ -21,7 +21,8 @@ OUT = os.path.join(HERE, "libcbhip.so")
 OBJ_DIR = os.path.join(HERE, "_build")
 
 SOURCES = ["session.hip", "entry.hip", "apply.hip", "borders.hip", "categorical.hip", "class_top.hip",
-           "class_distill.hip", "class_sample.hip", "class_logprobs.hip", "lookup.hip", "adamw.hip", "driver.cpp"]
+           "class_distill.hip", "class_sample.hip", "class_logprobs.hip", "class_logprobs_short.hip", "class_logprob_grad.hip",
+           "lookup.hip", "adamw.hip", "driver.cpp"]
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 

@@ -6,184 +6,10 @@
 //   grad_j = (sum of g_i of j's entries - p_j (G + h (d_j + E))) / t,  p_j = e^d_j / Z,  G = sum of all g_i
 // log Z and E are both at least 0: the entropy is no difference, and log p_j + entropy = d_j + E holds for
 // a row of nearly equal scores too, where either is a small difference of large numbers.
-#include "class_scores.hpp"
+#include "class_logprobs.hpp"
 
 namespace {
 using namespace cbh::cls;
-
-constexpr uint32_t kMaxTop = 1024, kMaxGiven = 1024;
-constexpr double kLn2 = 0.6931471805599453;
-constexpr float kFar = -200.0f;   // 2^y is 0 in f32 from -150 down: a y of less, -inf too, has no part in the sums
-
-// The running sums of a softmax with those of its entropy: s = sum 2^y, t = sum 2^y y, y = (x - m) c.
-struct RunningStat : Running {
-    double t = 0.0;
-    __device__ __forceinline__ void raise(float to, float c) {
-        if (to > m) {
-            const float y = fmaxf((m - to) * c, -1e30f);   // (finite: 0 times it is 0)
-            const double f = (double)exp2_fast(y);
-            t = f * (t + (double)y * s);
-            s *= f;
-            m = to;
-        }
-    }
-    __device__ __forceinline__ void weigh(float x, float c, float& e, float& ey) const {
-        const float y = (x - m) * c;
-        e = exp2_fast(y);   // (NaN stays)
-        ey = e * fmaxf(y, kFar);
-    }
-    // (sums of a tile side by side, then together, then in f64)
-    template <int U, int V>
-    __device__ __forceinline__ void add(const float (&x)[U][V], float c) {
-        float e[V], ey[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) weigh(x[0][v], c, e[v], ey[v]);
-#pragma unroll
-        for (int u = 1; u < U; ++u)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float a, b;
-                weigh(x[u][v], c, a, b);
-                e[v] += a;
-                ey[v] += b;
-            }
-#pragma unroll
-        for (int o = V / 2; o > 0; o /= 2)
-#pragma unroll
-            for (int v = 0; v < o; ++v) {
-                e[v] += e[v + o];
-                ey[v] += ey[v + o];
-            }
-        s += (double)e[0];
-        t += (double)ey[0];
-    }
-    __device__ __forceinline__ void add_one(float x, float c) {
-        float e, ey;
-        weigh(x, c, e, ey);
-        s += (double)e;
-        t += (double)ey;
-    }
-    __device__ __forceinline__ void join(float m2, double s2, double t2, float c) {
-        raise(m2, c);
-        const float y = fmaxf((m2 - m) * c, -1e30f);
-        const double f = (double)exp2_fast(y);
-        s += s2 * f;
-        t += f * (t2 + (double)y * s2);
-    }
-};
-struct PartStat {   // of a part of a row, between launches
-    double s, t;
-    float m, none;
-};
-// Those of a workgroup's threads together, in a fixed order; every thread gets them.  One barrier; tmp: one a wave.
-template <int THREADS>
-__device__ __forceinline__ void block_stat(RunningStat& r, float c, PartStat* tmp) {
-    r.raise(wave_reduce(r.m, MaxF()), c);
-    r.s = wave_reduce(r.s, Add());
-    r.t = wave_reduce(r.t, Add());
-    if (THREADS == 64) return;
-    if (lane_id() == 0) tmp[threadIdx.x / 64] = PartStat{r.s, r.t, r.m, 0.0f};
-    __syncthreads();
-    r = RunningStat();
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) r.join(tmp[w].m, tmp[w].s, tmp[w].t, c);
-}
-
-struct Asked {   // what is asked of every row, and where it goes
-    const int32_t* given;
-    const uint32_t* allowed;   // nullable
-    int64_t allowed_stride;
-    uint32_t n_given, k;
-    float c;      // log2(e) / t
-    double it;    // 1 / t
-    float *logprob, *entropy, *stats, *top_logprob;
-    int32_t* top_index;
-};
-__device__ __forceinline__ bool is_allowed(const uint32_t* words, uint32_t j) { return words[j >> 5] >> (j & 31) & 1; }
-
-// A tile's scores, -inf where a class is not allowed; `words` are those from the tile's row segment on.
-template <class T, bool kUnit, bool kMask>
-__device__ __forceinline__ void load_allowed(const T* row, int64_t cs, const uint32_t* words, uint32_t base, uint32_t n,
-                                             float (&x)[kPacks<T>][Pack<T>::V]) {
-    constexpr int V = Pack<T>::V, U = kPacks<T>;
-    const uint32_t lane = lane_id();
-    uint32_t bits[U];
-    if constexpr (kMask) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t i = base + (u * 64 + lane) * V;
-            bits[u] = i < n ? words[i >> 5] >> (i & 31) : 0;
-        }
-    }
-    load_tile<T, kUnit>(row, cs, base, n, -INFINITY, x);
-    if constexpr (kMask) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[u][v] = bits[u] >> v & 1 ? x[u][v] : -INFINITY;
-    }
-}
-
-// What is written of a row from its sums: the statistics by one thread, given classes by all.
-struct RowStat {
-    double m, log_z;   // (f64: logprob is rounded once)
-    bool none;         // a row of -inf alone
-};
-__device__ __forceinline__ RowStat row_stat(const RunningStat& r) {
-    RowStat q;
-    q.none = r.s == 0.0;
-    q.m = (double)r.m;
-    q.log_z = q.none ? 0.0 : log(r.s);
-    return q;
-}
-__device__ __forceinline__ float log_prob(float x, const RowStat& q, double it) {
-    return x == -INFINITY && q.log_z == q.log_z ? x : (float)(((double)x - q.m) * it - q.log_z);
-}
-__device__ __forceinline__ void write_stats(const Asked& A, uint64_t row, const RunningStat& r, const RowStat& q) {
-    const double e = q.none ? 0.0 : -r.t / r.s * kLn2, nan = r.s - r.s;   // (nan: 0 of a finite sum)
-    if (A.entropy) A.entropy[row] = (float)(q.log_z + e);
-    if (A.stats) {
-        A.stats[row * 3] = q.none ? -INFINITY : (float)(q.m + nan);
-        A.stats[row * 3 + 1] = q.none ? -INFINITY : (float)q.log_z;
-        A.stats[row * 3 + 2] = (float)e;
-    }
-}
-// The log probabilities of a row's entries from, from + step, ...; the first of them by a score that was read before.
-template <class T>
-__device__ __forceinline__ uint32_t given_class(const Asked& A, uint64_t row, uint32_t i) {
-    return A.logprob && i < A.n_given ? (uint32_t)A.given[row * A.n_given + i] : ~0u;
-}
-template <class T>
-__device__ __forceinline__ float given_score(const Asked& A, const Rows<T>& X, uint64_t row, uint32_t j) {
-    if (j >= X.classes) return 0.0f;
-    const float x = to_f32(X.data[(int64_t)row * X.rs + (int64_t)j * X.cs]);
-    return A.allowed && !is_allowed(A.allowed + (int64_t)row * A.allowed_stride, j) ? -INFINITY : x;
-}
-template <class T>
-__device__ __forceinline__ void write_given(const Asked& A, const Rows<T>& X, uint64_t row, const RowStat& q, uint32_t from,
-                                            uint32_t step, uint32_t j, float x) {
-    if (!A.logprob) return;
-    for (uint32_t i = from; i < A.n_given; i += step) {
-        if (i != from) {
-            j = given_class<T>(A, row, i);
-            x = given_score(A, X, row, j);
-        }
-        A.logprob[row * A.n_given + i] = j < X.classes ? log_prob(x, q, A.it) : 0.0f;
-    }
-}
-// The k largest of the `got` keys of best (0: none), the largest first.
-template <int THREADS>
-__device__ __forceinline__ void write_top(const Asked& A, uint64_t row, const u64* best, uint32_t got, const RowStat& q) {
-    for (uint32_t i = threadIdx.x; i < got; i += THREADS) {
-        const u64 key = best[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < got; ++j) rank += best[j] > key;
-        if (key == 0 || rank >= A.k) continue;
-        const float x = key_score((uint32_t)(key >> 32));
-        A.top_logprob[row * A.k + rank] = log_prob(x, q, A.it);
-        A.top_index[row * A.k + rank] = x == -INFINITY ? -1 : (int32_t)~(uint32_t)key;
-    }
-}
 
 // Keys of a segment that are kept beside its k largest: as many as reach the bound are mostly, and need no selection.
 constexpr uint32_t kSpare = 64;
@@ -389,289 +215,6 @@ __global__ __launch_bounds__(THREADS) void finish_kernel(Rows<T> X, Asked A, uin
     }
 }
 
-// A row of at most NMAX classes in a thread's registers; kWhole: whole vectors of classes next to each other.
-template <class T, int NMAX, bool kWhole>
-__device__ __forceinline__ void load_few(const T* row, int64_t cs, uint32_t n, float (&x)[NMAX]) {
-    constexpr int V = kWhole && Pack<T>::V <= NMAX ? Pack<T>::V : 1;
-#pragma unroll
-    for (int j = 0; j < NMAX; j += V) {
-        if constexpr (V > 1) {
-            Pack<T> p;
-            if ((uint32_t)j < n) p.w = ((const Loose<T>*)(row + j))->w;
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[j + v] = (uint32_t)j < n ? p.get(v) : -INFINITY;
-        } else {
-            x[j] = (uint32_t)j < n ? to_f32(row[(int64_t)j * cs]) : -INFINITY;
-        }
-    }
-}
-
-// Few classes: a row a thread, its scores in registers.  Up to 32: a score's place is the count of those ahead; up to 64, for which
-// there are too many pairs (rows next to each other): the largest one after another.
-template <class T, int NMAX, bool kWhole, bool kTop>
-__global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
-    const uint32_t n = X.classes;
-    for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
-        const T* x0 = X.data + (int64_t)row * X.rs;
-        const uint32_t* words = A.allowed + (int64_t)row * A.allowed_stride;
-        const uint32_t low = A.allowed ? words[0] : ~0u, high = NMAX > 32 && A.allowed && n > 32 ? words[1] : ~0u;
-        const uint32_t own = given_class<T>(A, row, 0);
-        float x[NMAX];
-        RunningStat run;
-        load_few<T, NMAX, kWhole>(x0, X.cs, n, x);
-#pragma unroll
-        for (int i = 0; i < NMAX; ++i) x[i] = (i < 32 ? low : high) >> (i & 31) & 1 ? x[i] : -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NMAX; ++i) run.m = fmaxf(run.m, x[i]);
-#pragma unroll
-        for (int i = 0; i < NMAX; ++i) run.add_one(x[i], A.c);
-        const RowStat q = row_stat(run);
-        write_stats(A, row, run, q);
-        write_given(A, X, row, q, 0, 1, own, given_score(A, X, row, own));
-        if constexpr (kTop && NMAX > 32) {
-            uint32_t key[NMAX];
-#pragma unroll
-            for (int i = 0; i < NMAX; ++i) key[i] = (uint32_t)i < n ? order_key(x[i]) : 0;
-            for (uint32_t r = 0; r < A.k; ++r) {
-                uint32_t most = 0;
-                int32_t at = 0;
-#pragma unroll
-                for (int i = 0; i < NMAX; ++i) {
-                    at = key[i] > most ? i : at;
-                    most = max(key[i], most);
-                }
-#pragma unroll
-                for (int i = 0; i < NMAX; ++i) key[i] = i == at ? 0 : key[i];
-                const float y = key_score(most);
-                A.top_logprob[row * A.k + r] = log_prob(y, q, A.it);
-                A.top_index[row * A.k + r] = y == -INFINITY ? -1 : at;
-            }
-        } else if constexpr (kTop) {
-            uint32_t key[NMAX], rank[NMAX];
-#pragma unroll
-            for (int i = 0; i < NMAX; ++i) {
-                key[i] = (uint32_t)i < n ? order_key(x[i]) : 0;
-                rank[i] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < NMAX; ++i)
-#pragma unroll
-                for (int j = 0; j < i; ++j) {
-                    const bool ahead = key[j] >= key[i];
-                    rank[i] += ahead;
-                    rank[j] += !ahead;
-                }
-            for (uint32_t r = 0; r < A.k; ++r) {
-                float y = 0.0f;
-                int32_t at = -1;
-#pragma unroll
-                for (int i = 0; i < NMAX; ++i) {
-                    y = rank[i] == r ? x[i] : y;
-                    at = rank[i] == r ? i : at;
-                }
-                A.top_logprob[row * A.k + r] = log_prob(y, q, A.it);
-                A.top_index[row * A.k + r] = y == -INFINITY ? -1 : at;
-            }
-        }
-    }
-}
-
-// ---- short rows -------------------------------------------------------------------------------
-// Over the G lanes of a group; every lane gets it.
-template <int G, class V, class Op>
-__device__ __forceinline__ V group_reduce(V v, Op op) {
-    if constexpr (G >= 2) v = op(v, dpp_move<0xB1, 0xf>(v, v));     // lanes 1 0 3 2
-    if constexpr (G >= 4) v = op(v, dpp_move<0x4E, 0xf>(v, v));     // lanes 2 3 0 1
-    if constexpr (G >= 8) v = op(v, dpp_move<0x141, 0xf>(v, v));    // mirrored within 8
-    if constexpr (G >= 16) v = op(v, dpp_move<0x140, 0xf>(v, v));   // mirrored within 16
-    if constexpr (G >= 32) v = op(v, __shfl_xor(v, 16));
-    if constexpr (G >= 64) v = op(v, __shfl_xor(v, 32));
-    return v;
-}
-// A lane's scores of a row of at most G R V classes: vector u of lane l holds the classes from (u G + l) V on (kVec), or one
-// class, (u G + l).
-template <class T, bool kVec>
-constexpr int kWide = kVec ? Pack<T>::V : 1;
-template <class T, int G, int R, bool kVec>
-__device__ __forceinline__ void load_short(const T* row, int64_t cs, uint32_t l, uint32_t n, const uint32_t* words,
-                                           float (&x)[R][kWide<T, kVec>]) {
-    constexpr int V = kWide<T, kVec>;
-#pragma unroll
-    for (int u = 0; u < R; ++u) {
-        const uint32_t i = (u * G + l) * V;
-        if constexpr (kVec) load_pack<T, true>(row, 1, i, n, -INFINITY, x[u]);
-        else x[u][0] = i < n ? to_f32(row[(int64_t)i * cs]) : -INFINITY;
-    }
-    if (words) {
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            const uint32_t i = (u * G + l) * V, bits = i < n ? words[i >> 5] >> (i & 31) : 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[u][v] = bits >> v & 1 ? x[u][v] : -INFINITY;
-        }
-    }
-}
-
-// The largest bound that k of a wave's keys reach, the highest bits first, from the one in which they differ on (0: no key; at least k
-// are not 0); it may end below the k-th largest where exactly k are at the bound or above.
-template <int N>
-__device__ __forceinline__ uint32_t wave_kth(const uint32_t (&key)[N], uint32_t k) {
-    uint32_t hi = key[0], lo = key[0] - 1;   // (0 is no key: the largest here)
-#pragma unroll
-    for (int r = 1; r < N; ++r) {
-        hi = max(hi, key[r]);
-        lo = min(lo, key[r] - 1);
-    }
-    hi = wave_reduce(hi, MaxU());
-    lo = ~wave_reduce(~lo, MaxU()) + 1;
-    const int bits = hi > lo ? 32 - __builtin_clz(hi ^ lo) : 0;
-    uint32_t bound = bits == 32 ? 0 : hi >> bits << bits;
-    for (int b = bits - 1; b >= 0; --b) {
-        const uint32_t t = bound | 1u << b;
-        uint32_t c = 0;
-#pragma unroll
-        for (int r = 0; r < N; ++r) c += (uint32_t)__popcll(__ballot(key[r] >= t));
-        if (c >= k) bound = t;
-        if (c == k) break;
-    }
-    return bound;
-}
-
-// Rows of up to 2048 classes in the registers of G lanes, 64 for the largest classes.  Those: the k-th largest of the vectors'
-// maxima, where there are at least 4 k, is a bound that k classes reach, else that of all classes; those that reach it are
-// listed in LDS and take the places that the count of larger ones gives.
-constexpr uint32_t kShort = 2048;
-template <class T, int G, int R, bool kVec, int CAP>
-__global__ __launch_bounds__(256) void logprobs_short_kernel(Rows<T> X, Asked A) {
-    constexpr int V = kWide<T, kVec>;
-    __shared__ u64 cand[4][CAP ? CAP : 1];
-    const uint32_t l = threadIdx.x % G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), n = X.classes;
-    for (uint64_t first = (uint64_t)blockIdx.x * (256 / G); first < X.rows; first += (uint64_t)gridDim.x * (256 / G)) {
-        const uint64_t mine = first + threadIdx.x / G, row = min(mine, X.rows - 1);
-        const bool there = mine < X.rows;   // (the same in a wave where G = 64)
-        const uint32_t* words = A.allowed ? A.allowed + (int64_t)row * A.allowed_stride : nullptr;
-        float x[R][V], lm = -INFINITY, se = 0.0f, sy = 0.0f;
-        load_short<T, G, R, kVec>(X.data + (int64_t)row * X.rs, X.cs, l, n, words, x);
-        const uint32_t own = given_class<T>(A, row, l);
-        const float own_score = given_score(A, X, row, own);
-#pragma unroll
-        for (int u = 0; u < R; ++u)
-#pragma unroll
-            for (int v = 0; v < V; ++v) lm = fmaxf(lm, x[u][v]);
-        RunningStat run;
-        run.m = fmaxf(kLowest, group_reduce<G>(lm, MaxF()));
-#pragma unroll
-        for (int u = 0; u < R; ++u)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float e, ey;
-                run.weigh(x[u][v], A.c, e, ey);
-                se += e;
-                sy += ey;
-            }
-        run.s = group_reduce<G>((double)se, Add());
-        run.t = group_reduce<G>((double)sy, Add());
-        const RowStat q = row_stat(run);
-        if (there && l == 0) write_stats(A, row, run, q);
-        if (there) write_given(A, X, row, q, l, G, own, own_score);
-        if constexpr (CAP > 0) {
-            static_assert(G == 64, "a row a wave");
-            if (!there) continue;
-            float bound;   // k classes reach it (NaN: all do)
-            if (kVec && A.k <= 8 && n >= 32 * V) {   // of the lanes' maxima, a NaN left out: the smallest of the k largest
-                uint32_t larger = 0;
-#pragma unroll 16
-                for (int j = 0; j < 64; ++j) larger += read_lane(lm, j) > lm;
-                bound = -wave_reduce(larger < A.k ? -lm : -INFINITY, MaxF());
-            } else {
-                uint32_t key[R * V], most[R];
-#pragma unroll
-                for (int u = 0; u < R; ++u) {
-                    most[u] = 0;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        key[u * V + v] = (u * G + l) * V + v < n ? order_key(x[u][v]) : 0;
-                        most[u] = max(most[u], key[u * V + v]);
-                    }
-                }
-                bound = key_score(A.k * 4 <= n / V ? wave_kth(most, A.k) : wave_kth(key, A.k));
-            }
-            uint32_t count = 0;
-#pragma unroll
-            for (int u = 0; u < R; ++u)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const uint32_t i = (u * G + l) * V + v;
-                    const bool in = i < n && !(x[u][v] < bound);
-                    const u64 b = __ballot(in);
-                    if (b == 0) continue;
-                    const uint32_t at = count + (uint32_t)__popcll(b & ((1ull << l) - 1));
-                    if (in && at < (uint32_t)CAP) cand[wave][at] = rank_key(x[u][v], i);
-                    count += (uint32_t)__popcll(b);
-                }
-            if (count > (uint32_t)CAP) {   // many equal ones: class by class, and only the k largest kept as the list fills
-                Candidates<CAP> C{cand[wave], 0, 0, key_score(0)};
-                wave_fence();
-#pragma unroll 1
-                for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-                    const uint32_t i = i0 + l;
-                    float y = -INFINITY;
-                    if (i < n && !(words && !is_allowed(words, i))) y = to_f32(X.data[(int64_t)row * X.rs + (int64_t)i * X.cs]);
-                    C.offer(y, i, i < n, A.k);
-                }
-                count = C.count;
-            }
-            wave_fence();
-            for (uint32_t i = l; i < count; i += 64) {
-                const u64 key = cand[wave][i];
-                uint32_t rank = 0;
-                for (uint32_t j = 0; j < count; ++j) rank += cand[wave][j] > key;
-                if (rank >= A.k) continue;
-                const float y = key_score((uint32_t)(key >> 32));
-                A.top_logprob[row * A.k + rank] = log_prob(y, q, A.it);
-                A.top_index[row * A.k + rank] = y == -INFINITY ? -1 : (int32_t)~(uint32_t)key;
-            }
-            wave_fence();
-        }
-    }
-}
-template <class T, int G, int R, bool kVec>
-void launch_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
-    const unsigned grid = row_grid((X.rows + 256 / G - 1) / (256 / G));
-    if constexpr (G == 64) {
-        if (A.k) {
-            if (A.k <= 128) logprobs_short_kernel<T, G, R, kVec, 256><<<grid, 256, 0, st>>>(X, A);
-            else logprobs_short_kernel<T, G, R, kVec, 1152><<<grid, 256, 0, st>>>(X, A);
-            return;
-        }
-    }
-    logprobs_short_kernel<T, G, R, kVec, 0><<<grid, 256, 0, st>>>(X, A);
-}
-template <class T>
-int run_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
-    constexpr uint32_t V = Pack<T>::V;
-    const uint32_t n = X.classes;
-    // by vectors where they fill the lanes: half of them, or a part of the wave's for the sums alone
-    if (X.cs == 1 && (n > 32 * V || !A.k)) {
-        if (n <= 4 * V) launch_short<T, 4, 1, true>(X, A, st);
-        else if (n <= 8 * V) launch_short<T, 8, 1, true>(X, A, st);
-        else if (n <= 16 * V) launch_short<T, 16, 1, true>(X, A, st);
-        else if (n <= 32 * V) launch_short<T, 32, 1, true>(X, A, st);
-        else if (n <= 64 * V) launch_short<T, 64, 1, true>(X, A, st);
-        else if (n <= 128 * V) launch_short<T, 64, 2, true>(X, A, st);
-        else if (n <= 256 * V) launch_short<T, 64, 4, true>(X, A, st);
-        else launch_short<T, 64, 32 / V, true>(X, A, st);
-    } else {
-        if (n <= 64) launch_short<T, 64, 1, false>(X, A, st);
-        else if (n <= 128) launch_short<T, 64, 2, false>(X, A, st);
-        else if (n <= 256) launch_short<T, 64, 4, false>(X, A, st);
-        else if (n <= 512) launch_short<T, 64, 8, false>(X, A, st);
-        else launch_short<T, 64, 32, false>(X, A, st);
-    }
-    CLS_TRY(hipGetLastError());
-    return CBH_OK;
-}
-
 // Segments of a row: one, unless the rows alone leave CUs idle and a row is long.  They start at a multiple of 32
 // classes, a word of the allowed ones.
 constexpr uint32_t kMinSeg = 16384, kMaxGroupSegs = 64;
@@ -730,294 +273,10 @@ template <class T>
 int run_logprobs(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t cs, const Asked& A, void* workspace,
                  hipStream_t st) {
     const Rows<T> X{(const T*)scores, rows, n, rs, cs};
-    // (by rows and without a k, from 17 classes on a group of lanes reads them better)
-    if (n <= 64 && (n <= 32 || (rs == 1 && cs != 1)) && !(cs == 1 && n > 16 && !A.k)) {
-        const unsigned grid = row_grid((rows + 255) / 256);
-#define FEW_(N, UNIT) (A.k ? logprobs_few_kernel<T, N, UNIT, true><<<grid, 256, 0, st>>>(X, A) \
-                           : logprobs_few_kernel<T, N, UNIT, false><<<grid, 256, 0, st>>>(X, A))
-#define FEW(N) (cs == 1 && n % Pack<T>::V == 0 ? FEW_(N, true) : FEW_(N, false))
-        if (n <= 4) FEW(4);
-        else if (n <= 8) FEW(8);
-        else if (n <= 12) FEW(12);
-        else if (n <= 16) FEW(16);
-        else if (n <= 32) FEW(32);
-        else FEW_(64, false);
-#undef FEW
-#undef FEW_
-        CLS_TRY(hipGetLastError());
-        return CBH_OK;
-    }
-    if (n <= kShort) return run_short(X, A, st);
+    if (n <= kShort) return run_short_rows(X, A, st);
     const Plan P = plan_parts(rows, n);
     if (cs == 1) return A.allowed ? launch_rows<T, true, true>(X, A, P, workspace, st) : launch_rows<T, true, false>(X, A, P, workspace, st);
     return A.allowed ? launch_rows<T, false, true>(X, A, P, workspace, st) : launch_rows<T, false, false>(X, A, P, workspace, st);
-}
-
-// ---- gradient -------------------------------------------------------------------------------
-struct Upstream {
-    const int32_t* given;
-    const float* logprob_grad;
-    const float* entropy_grad;   // nullable
-    const float* stats;
-    const uint32_t* allowed;     // nullable
-    int64_t allowed_stride;
-    uint32_t n_given;
-    float c;
-    double it;
-};
-// The factors of a row: grad_j = 2^y (a + b y), y = (x_j - m) c, beside the entries' own.
-struct RowFactors {
-    float m, a, b;
-    double log_z, far, G, h;
-    bool zero;   // all derivatives are 0
-};
-__device__ __forceinline__ float clamp_finite(double v) {   // (2^y = 0 times it is 0)
-    return v != v ? (float)v : (float)fmin(fmax(v, -3.4e38), 3.4e38);
-}
-__device__ __forceinline__ RowFactors row_factors(const Upstream& P, uint64_t row, double G, bool any) {
-    RowFactors f;
-    const float* s = P.stats + row * 3;
-    f.h = P.entropy_grad ? (double)P.entropy_grad[row] : 0.0;
-    f.zero = !any && f.h == 0.0;
-    f.G = G;
-    const bool none = s[1] == -INFINITY;   // a row of -inf alone: no class has a probability
-    f.m = none ? 0.0f : s[0];
-    f.log_z = (double)s[1];
-    f.far = (double)s[2];
-    const double r = none ? 0.0 : -P.it * exp_f64(-f.log_z);
-    f.a = none ? 0.0f : clamp_finite(r * (f.G + f.h * f.far));
-    f.b = none ? 0.0f : clamp_finite(r * f.h * kLn2);
-    return f;
-}
-__device__ __forceinline__ float grad_of(float x, const RowFactors& f, float c) {
-    const float y = (x - f.m) * c;
-    return exp2_fast(y) * (f.a + f.b * fmaxf(y, kFar));
-}
-// That of a class with entries whose derivatives add up to g.
-__device__ __forceinline__ float grad_of_given(float x, double g, const RowFactors& f, double it) {
-    const double d = ((double)x - (double)f.m) * it, p = f.log_z == -INFINITY ? 0.0 : exp_f64(d - f.log_z);
-    return (float)(it * (g - (p == 0.0 ? 0.0 : p * (f.G + f.h * (d + f.far)))));
-}
-
-// A wave takes a segment of a row; classes with entries are written over.
-constexpr uint32_t kGradSeg = 4 * kSeg;
-template <class T, bool kUnit, bool kMask>
-__global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs,
-                                                           int64_t gcs, uint32_t segs) {
-    constexpr int V = Pack<T>::V, U = kPacks<T>;
-    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    for (uint64_t job = (uint64_t)blockIdx.x * 4 + wave; job < X.rows * segs; job += (uint64_t)gridDim.x * 4) {
-        const uint64_t row = job / segs;
-        const uint32_t first = (uint32_t)(job % segs) * kGradSeg, n = min(X.classes - first, kGradSeg);
-        const T* x0 = X.data + (int64_t)row * X.rs + (int64_t)first * X.cs;
-        T* g0 = grad + (int64_t)row * grs + (int64_t)first * gcs;
-        const uint32_t* words = kMask ? P.allowed + (int64_t)row * P.allowed_stride + first / 32 : nullptr;
-        const int32_t* given = P.given + row * P.n_given;
-        const float* g = P.logprob_grad + row * P.n_given;
-        double G = 0.0;
-        bool some = false;
-        for (uint32_t i = lane; i < P.n_given; i += 64)
-            if ((uint32_t)given[i] < X.classes) {
-                G += (double)g[i];
-                some |= g[i] != 0.0f;
-            }
-        G = wave_reduce(G, Add());
-        const RowFactors f = row_factors(P, row, G, __any(some));
-        for (uint32_t base = 0; base < n; base += kSeg) {
-            float x[U][V];
-            uint32_t bits[U];
-            if (!f.zero) load_tile<T, kUnit>(x0, X.cs, base, n, -INFINITY, x);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t i = base + (u * 64 + lane) * V;
-                if constexpr (kMask) bits[u] = i < n ? words[i >> 5] >> (i & 31) : 0;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    x[u][v] = f.zero ? 0.0f : grad_of(x[u][v], f, P.c);
-                    if constexpr (kMask) x[u][v] = bits[u] >> v & 1 ? x[u][v] : 0.0f;
-                }
-                if (i < n) store_pack<T, kUnit>(g0, gcs, i, n, x[u]);
-            }
-        }
-        if (f.zero) continue;
-        __threadfence_block();   // (the stores above are done)
-        for (uint32_t i = lane; i < P.n_given; i += 64) {
-            const uint32_t j = (uint32_t)given[i];
-            if (j >= X.classes || j < first || j - first >= n) continue;
-            if (kMask && !is_allowed(words, j - first)) continue;
-            double sum = 0.0;
-            bool again = false;   // (the first of a class's entries writes)
-            for (uint32_t e = 0; e < P.n_given; ++e)
-                if ((uint32_t)given[e] == j) {
-                    sum += (double)g[e];
-                    again |= e < i;
-                }
-            if (again) continue;
-            const float x = to_f32(x0[kUnit ? (int64_t)(j - first) : (int64_t)(j - first) * X.cs]);
-            g0[kUnit ? (int64_t)(j - first) : (int64_t)(j - first) * gcs] = from_f32<T>(grad_of_given(x, sum, f, P.it));
-        }
-    }
-}
-
-// Rows of up to 2048 classes in the registers of G lanes.  Lists of more than kShortGiven entries go the other ways: the owner of a
-// class goes through the whole list for it.
-constexpr uint32_t kShortGiven = 8;
-template <class T, int G, int R>
-__global__ __launch_bounds__(256) void logprob_grad_short_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs) {
-    constexpr int V = Pack<T>::V;
-    const uint32_t l = threadIdx.x % G, n = X.classes;
-    for (uint64_t first = (uint64_t)blockIdx.x * (256 / G); first < X.rows; first += (uint64_t)gridDim.x * (256 / G)) {
-        const uint64_t mine = first + threadIdx.x / G, row = min(mine, X.rows - 1);
-        const uint32_t* words = P.allowed ? P.allowed + (int64_t)row * P.allowed_stride : nullptr;
-        const int32_t* given = P.given + row * P.n_given;
-        const float* g = P.logprob_grad + row * P.n_given;
-        const T* x0 = X.data + (int64_t)row * X.rs;
-        float x[R][V];
-        load_short<T, G, R, true>(x0, 1, l, n, nullptr, x);
-        double sum = 0.0;
-        bool some = false;
-        for (uint32_t i = 0; i < P.n_given; ++i)
-            if ((uint32_t)given[i] < n) {
-                sum += (double)g[i];
-                some |= g[i] != 0.0f;
-            }
-        const RowFactors f = row_factors(P, row, sum, some);
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            const uint32_t i = (u * G + l) * V, bits = words && i < n ? words[i >> 5] >> (i & 31) : ~0u;
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[u][v] = f.zero || !(bits >> v & 1) ? 0.0f : grad_of(x[u][v], f, P.c);
-        }
-        if (!f.zero)
-            for (uint32_t i = 0; i < P.n_given; ++i) {
-                const uint32_t j = (uint32_t)given[i];
-                if (j >= n || j / V % G != l || (words && !is_allowed(words, j))) continue;
-                double own = 0.0;
-                for (uint32_t e = 0; e < P.n_given; ++e) own += (uint32_t)given[e] == j ? (double)g[e] : 0.0;
-                const float y = grad_of_given(to_f32(x0[j]), own, f, P.it);
-#pragma unroll
-                for (int u = 0; u < R; ++u)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) x[u][v] = (u * G + l) * V + v == j ? y : x[u][v];
-            }
-        if (mine >= X.rows) continue;
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            const uint32_t i = (u * G + l) * V;
-            if (i < n) store_pack<T, true>(grad + (int64_t)row * grs, 1, i, n, x[u]);
-        }
-    }
-}
-
-// Few classes, and rows next to each other: a thread takes up to NMAX classes of a row, in registers.  The
-// f64 of a row's factors and entries is a thread's, not a group of lanes': 1M x 10 f32 by rows takes 42 us by groups.
-template <class T, int NMAX, bool kWhole>
-__global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs,
-                                                               int64_t gcs, uint32_t segs) {
-    const uint64_t blocks = (X.rows + 255) / 256;
-    for (uint64_t job = blockIdx.x; job < blocks * segs; job += gridDim.x) {
-        const uint64_t row = job % blocks * 256 + threadIdx.x;
-        if (row >= X.rows) continue;
-        const uint32_t first = (uint32_t)(job / blocks) * NMAX, n = min(X.classes - first, (uint32_t)NMAX);
-        const T* x0 = X.data + (int64_t)row * X.rs + (int64_t)first * X.cs;
-        T* g0 = grad + (int64_t)row * grs + (int64_t)first * gcs;
-        const uint32_t bits = P.allowed ? P.allowed[(int64_t)row * P.allowed_stride + first / 32] >> first % 32 : ~0u;
-        const int32_t* given = P.given + row * P.n_given;
-        const float* g = P.logprob_grad + row * P.n_given;
-        float x[NMAX];
-        load_few<T, NMAX, kWhole>(x0, X.cs, n, x);
-        double G = 0.0;
-        bool some = false;
-        for (uint32_t i = 0; i < P.n_given; ++i)
-            if ((uint32_t)given[i] < X.classes) {
-                G += (double)g[i];
-                some |= g[i] != 0.0f;
-            }
-        const RowFactors f = row_factors(P, row, G, some);
-        float y[NMAX];
-#pragma unroll
-        for (int j = 0; j < NMAX; ++j) y[j] = f.zero || !(bits >> j & 1) ? 0.0f : grad_of(x[j], f, P.c);
-        uint32_t done = f.zero ? ~0u : ~bits;
-        for (uint32_t i = 0; i < P.n_given; ++i) {
-            const uint32_t j = (uint32_t)given[i] - first;
-            if ((uint32_t)given[i] >= X.classes || j >= n || (done >> j & 1)) continue;
-            done |= 1u << j;
-            double sum = 0.0;
-            for (uint32_t e = i; e < P.n_given; ++e) sum += (uint32_t)given[e] - first == j ? (double)g[e] : 0.0;
-            float at = 0.0f;
-#pragma unroll
-            for (int q = 0; q < NMAX; ++q) at = (uint32_t)q == j ? x[q] : at;
-            at = grad_of_given(at, sum, f, P.it);
-#pragma unroll
-            for (int q = 0; q < NMAX; ++q) y[q] = (uint32_t)q == j ? at : y[q];
-        }
-        constexpr int V = kWhole && Pack<T>::V <= NMAX ? Pack<T>::V : 1;
-#pragma unroll
-        for (int j = 0; j < NMAX; j += V) {
-            if constexpr (V > 1) {
-                float part[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) part[v] = y[j + v];
-                if ((uint32_t)j < n) store_pack<T, true>(g0, 1, j, n, part);
-            } else {
-                if ((uint32_t)j < n) g0[(int64_t)j * gcs] = from_f32<T>(y[j]);
-            }
-        }
-    }
-}
-
-template <class T>
-int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t cs, const Upstream& P, void* grad,
-             int64_t grs, int64_t gcs, hipStream_t st) {
-    const Rows<T> X{(const T*)scores, rows, n, rs, cs};
-    T* g = (T*)grad;
-    constexpr uint32_t V = Pack<T>::V;
-    const bool unit = cs == 1 && gcs == 1, lanes = unit && n <= kShort && P.n_given <= kShortGiven;
-    if (!(lanes && n > 16) && (n <= 32 || (rs == 1 && grs == 1 && cs != 1))) {
-        const unsigned grid = row_grid((rows + 255) / 256 * ((n + 31) / 32));
-#define RUN(N) (unit && n % V == 0 ? logprob_grad_few_kernel<T, N, true><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, (n + 31) / 32) \
-                     : logprob_grad_few_kernel<T, N, false><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, (n + 31) / 32))
-        if (n <= 4) RUN(4);
-        else if (n <= 8) RUN(8);
-        else if (n <= 16) RUN(16);
-        else RUN(32);
-#undef RUN
-    } else if (lanes) {
-#define RUN(G, R) logprob_grad_short_kernel<T, G, R><<<row_grid((rows + 256 / G - 1) / (256 / G)), 256, 0, st>>>(X, P, g, grs)
-        if (n <= 4 * V) RUN(4, 1);
-        else if (n <= 8 * V) RUN(8, 1);
-        else if (n <= 16 * V) RUN(16, 1);
-        else if (n <= 32 * V) RUN(32, 1);
-        else if (n <= 64 * V) RUN(64, 1);
-        else if (n <= 128 * V) RUN(64, 2);
-        else if (n <= 256 * V) RUN(64, 4);
-        else RUN(64, (int)(32 / V));
-#undef RUN
-    } else {
-        const uint32_t segs = (n + kGradSeg - 1) / kGradSeg;
-        const unsigned grid = row_grid((rows * segs + 3) / 4);
-#define RUN(UNIT, MASK) logprob_grad_kernel<T, UNIT, MASK><<<grid, 256, 0, st>>>(X, P, g, grs, gcs, segs)
-        if (unit) P.allowed ? RUN(true, true) : RUN(true, false);
-        else P.allowed ? RUN(false, true) : RUN(false, false);
-#undef RUN
-    }
-    CLS_TRY(hipGetLastError());
-    return CBH_OK;
-}
-
-// What both ask of the given and allowed classes.
-int check_lists(const void* given, uint32_t n_given, uint64_t rows, uint32_t classes, const uint32_t* allowed,
-                int64_t allowed_stride) {
-    if (n_given > kMaxGiven) return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "at most 1024 given classes a row");
-    if (rows && n_given && !given) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "given is null");
-    if (allowed) {
-        if ((uintptr_t)allowed % 4) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "allowed is not aligned to 4");
-        if (allowed_stride != 0 && allowed_stride < (int64_t)((classes + 31) / 32))
-            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "allowed_stride is 0 or at least ceil(classes / 32)");
-        if ((double)allowed_stride * (double)rows > 1.0e18)
-            return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, "strides pass the address range");
-    }
-    return CBH_OK;
 }
 
 }  // namespace
@@ -1056,37 +315,6 @@ extern "C" int cbh_class_logprobs(const void* scores, int32_t type, uint64_t row
             case CBH_TYPE_F16: return run_logprobs<_Float16>(scores, rows, classes, row_stride, class_stride, A, workspace, st);
             default: return run_logprobs<bf16_t>(scores, rows, classes, row_stride, class_stride, A, workspace, st);
         }
-    } catch (const std::exception& e) {
-        return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
-    }
-}
-
-extern "C" int cbh_logprob_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes,
-                                     int64_t row_stride, int64_t class_stride, const int32_t* given, uint32_t n_given,
-                                     const float* logprob_grad, const float* entropy_grad, const float* stats,
-                                     double temperature, const uint32_t* allowed, int64_t allowed_stride, void* grad,
-                                     int64_t grad_row_stride, int64_t grad_class_stride, void* stream) {
-    try {
-        int rc = check_scores(scores, type, rows, classes, row_stride, class_stride);
-        if (rc != CBH_OK) return rc;
-        rc = check_lists(given, n_given, rows, classes, allowed, allowed_stride);
-        if (rc != CBH_OK) return rc;
-        if (!good_temperature(temperature)) return cbh_internal_fail(CBH_ERR_OUT_OF_RANGE, kBadTemperature);
-        if (rows == 0) return CBH_OK;
-        if (n_given && !logprob_grad) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "logprob_grad is null");
-        if (!stats || !grad) return cbh_internal_fail(CBH_ERR_INVALID_ARG, "stats or grad is null");
-        rc = check_scores(grad, type, rows, classes, grad_row_stride, grad_class_stride);
-        if (rc != CBH_OK) return rc;
-        const Upstream P{given, logprob_grad, entropy_grad, stats, allowed, allowed_stride, n_given,
-                         (float)(1.4426950408889634 / temperature), 1.0 / temperature};
-        hipStream_t st = (hipStream_t)stream;
-#define RUN(T) run_grad<T>(scores, rows, classes, row_stride, class_stride, P, grad, grad_row_stride, grad_class_stride, st)
-        switch (type) {
-            case CBH_TYPE_F32: return RUN(float);
-            case CBH_TYPE_F16: return RUN(_Float16);
-            default: return RUN(bf16_t);
-        }
-#undef RUN
     } catch (const std::exception& e) {
         return cbh_internal_fail(CBH_ERR_DEVICE, e.what());
     }
