@@ -9,12 +9,15 @@ using namespace cbh::cls;
 // there are too many pairs (rows next to each other): the largest one after another.
 template <class T, int NMAX, bool kWhole, bool kTop>
 __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
+    constexpr bool kEach = NMAX <= 8;   // (so few classes: the log probability of each, once)
     const uint32_t n = X.classes;
     for (uint64_t row = (uint64_t)blockIdx.x * 256 + threadIdx.x; row < X.rows; row += (uint64_t)gridDim.x * 256) {
         const T* x0 = X.data + (int64_t)row * X.rs;
         const uint32_t* words = A.allowed + (int64_t)row * A.allowed_stride;
         const uint32_t low = A.allowed ? words[0] : ~0u, high = NMAX > 32 && A.allowed && n > 32 ? words[1] : ~0u;
-        const uint32_t own = given_class<T>(A, row, 0);
+        uint32_t own = ~0u;
+        if constexpr (!kEach) own = given_class<T>(A, row, 0);
+        const float own_score = given_score(A, X, row, own);
         float x[NMAX];
         RunningStat run;
         load_few<T, NMAX, kWhole>(x0, X.cs, n, x);
@@ -26,7 +29,26 @@ __global__ __launch_bounds__(256) void logprobs_few_kernel(Rows<T> X, Asked A) {
         for (int i = 0; i < NMAX; ++i) run.add_one(x[i], A.c);
         const RowStat q = row_stat(run);
         write_stats(A, row, run, q);
-        write_given(A, X, row, q, 0, 1, own, given_score(A, X, row, own));
+        if constexpr (!kEach) {
+            write_given(A, X, row, q, 0, 1, own, own_score);
+        } else if (A.logprob) {   // four indices on their way at a time
+            float lp[NMAX];
+#pragma unroll
+            for (int i = 0; i < NMAX; ++i) lp[i] = log_prob(x[i], q, A.it);
+            for (uint32_t i0 = 0; i0 < A.n_given; i0 += 4) {
+                uint32_t j[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) j[u] = given_class<T>(A, row, i0 + u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (i0 + u >= A.n_given) break;
+                    float y = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NMAX; ++i) y = j[u] == (uint32_t)i ? lp[i] : y;
+                    A.logprob[row * A.n_given + i0 + u] = j[u] >= n ? 0.0f : y;
+                }
+            }
+        }
         if constexpr (kTop && NMAX > 32) {
             uint32_t key[NMAX];
 #pragma unroll
