@@ -81,11 +81,11 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P
         for (uint32_t base = 0; base < n; base += kSeg) {
             float x[U][V];
             uint32_t bits[U];
+            if constexpr (kMask) tile_bits<T>(words, base, n, bits);
             if (!f.zero) load_tile<T, kUnit>(x0, X.cs, base, n, -INFINITY, x);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t i = base + (u * 64 + lane) * V;
-                if constexpr (kMask) bits[u] = i < n ? words[i >> 5] >> (i & 31) : 0;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     x[u][v] = f.zero ? 0.0f : grad_of(x[u][v], f, P.c);

@@ -181,11 +181,16 @@ __global__ __launch_bounds__(THREADS) void finish_kernel(Rows<T> X, Asked A, uin
         }
         __syncthreads();
         if (A.k) {   // (their order does not matter: a key's place is the count of larger ones)
-            for (uint32_t i = threadIdx.x; i < parts * slots; i += THREADS) {
-                const u64 key = keys[i];
-                if (key == 0) continue;
-                const uint32_t at = atomicAdd(&nbest, 1u);
-                if (at < kMaxTop + kSpare) best[at] = key;
+            for (uint32_t i0 = threadIdx.x; i0 < parts * slots; i0 += 4 * THREADS) {
+                u64 key[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) key[u] = i0 + u * THREADS < parts * slots ? keys[i0 + u * THREADS] : 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (key[u] == 0) continue;
+                    const uint32_t at = atomicAdd(&nbest, 1u);
+                    if (at < kMaxTop + kSpare) best[at] = key[u];
+                }
             }
             __syncthreads();
             got = nbest;
@@ -252,9 +257,11 @@ int launch_rows(const Rows<T>& X, const Asked& A, const Plan& P, void* workspace
         RUN(kNone, 2, 0);
     } else if (k * 4 <= shortest / kGroup) {
         if (k <= 128) RUN(kGroups, 256, lds);
+        else if (k <= 256) RUN(kGroups, 512, lds);
         else RUN(kGroups, 2048, lds);
     } else if (k * 4 <= shortest / V && lds_v <= 65536) {
         if (k <= 128) RUN(kVectors, 256, lds_v);
+        else if (k <= 256) RUN(kVectors, 512, lds_v);
         else RUN(kVectors, 2048, lds_v);
     } else {
         RUN(kWhole, 2, 0);

@@ -23,7 +23,7 @@ SHAPES = [(1, 1, 1, 1), (3, 2, 2, 1), (700, 10, 3, 3), (70, 32, 1, 32), (9, 33, 
           (3, 2048, 7, 256), (2, 2049, 1, 300), (2, 5000, 3, 1024), (5, 50021, 4, 20), (2, 8193, 1, 0), (1, 70001, 1, 64),
           (3, 140003, 2, 257), (600, 4099, 1, 9), (1, 40000, 1024, 0), (300, 20, 40, 0),
           (333, 70, 1, 14), (65, 129, 8, 0), (70, 256, 9, 64), (31, 257, 2, 65), (1001, 40, 1, 0), (9, 700, 1, 0), (6, 2048, 1, 64),
-          (300, 40, 3, 40), (259, 64, 2, 7), (70, 17, 1, 0), (70, 33, 9, 0)]
+          (2, 40000, 1, 200), (2, 9000, 1, 256), (2100, 2500, 1, 130), (300, 40, 3, 40), (259, 64, 2, 7), (70, 17, 1, 0), (70, 33, 9, 0)]
 
 
 def words(allowed):
