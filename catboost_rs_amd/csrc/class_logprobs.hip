@@ -1,11 +1,14 @@
-// Log probabilities of given classes, entropy and the most probable classes, in one pass over the
-// scores; and the gradient of a function of them, in another.
+// Log probabilities of given classes, entropy and the most probable classes, in one pass over the scores.
 //
 // With d_j = (x_j - m) / t over the allowed classes, m the largest score:
 //   Z = sum e^d_j,  E = -sum e^d_j d_j / Z,  logprob of c = d_c - log Z,  entropy = log Z + E
-//   grad_j = (sum of g_i of j's entries - p_j (G + h (d_j + E))) / t,  p_j = e^d_j / Z,  G = sum of all g_i
-// log Z and E are both at least 0: the entropy is no difference, and log p_j + entropy = d_j + E holds for
-// a row of nearly equal scores too, where either is a small difference of large numbers.
+// log Z and E are both at least 0: the entropy is no difference of large numbers, and log p_j + entropy = d_j + E holds
+// for a row of nearly equal scores too.  The sums run along with the running maximum: when it rises from m to m',
+// sum e^d d becomes e^((m - m') / t) (sum e^d d + (m - m') / t sum e^d).
+//
+// What has to be read is the scores.  Without a k: 4096 x 65536 bf16 99 us, 537 MB at 5.4 TB/s, a copy's rate.  With one, bound by the
+// row's end, a selection of dependent steps in LDS that four workgroups a CU hide in part: 4096 x 65536 bf16, k 5:
+// 128 us; 777 x 50021 f32 with allowed classes, four entries and k 20: 60 us, 155 MB at 2.6 TB/s, on 777 workgroups.
 #include "class_logprobs.hpp"
 
 namespace {

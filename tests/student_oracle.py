@@ -35,7 +35,10 @@ def logprobs(x, given, t, k, allowed=None):
         lp = np.where(ok, np.take_along_axis(d, np.where(ok, given, 0), 1) - base[:, None], 0.0)
         x = masked(x, allowed)
         key = np.where(np.isnan(x), np.inf, x)
-        order = np.lexsort((np.broadcast_to(np.arange(n), x.shape), -key, ~np.isnan(x)), axis=1)[:, :k]
+        if np.isnan(x).any():
+            order = np.lexsort((np.broadcast_to(np.arange(n), x.shape), -key, ~np.isnan(x)), axis=1)[:, :k]
+        else:
+            order = np.argsort(-key, axis=1, kind="stable")[:, :k]
         top = np.take_along_axis(d, order, 1) - base[:, None]
         top = np.where(np.isnan(log_z)[:, None], np.nan, top)
         lp = np.where(np.isnan(log_z)[:, None] & ok, np.nan, lp)

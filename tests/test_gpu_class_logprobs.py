@@ -141,7 +141,7 @@ def masks(g, rows, n):
 @pytest.mark.parametrize("rows,n,m,k", SHAPES)
 def test_shapes(rows, n, m, k, kind):
     g = np.random.default_rng(rows * n + k)
-    for order, t in (("rows", 1.0), ("padded", 1.5)) + ((("classes", 0.7), ("reversed", 2.0)) if n <= 9000 else ()):
+    for order, t in (("rows", 1.0), ("padded", 1.5)) + ((("classes", 0.7), ("reversed", 2.0)) if n <= 9000 and rows * n < 2_000_000 else ()):
         x, given = O.scores(g, rows, n, "normal"), given_of(g, rows, n, m)
         for name, allowed in masks(g, rows, n):
             tag = (order, t, name)
