@@ -116,7 +116,7 @@ class AdamW:
         return given
 
     def _scalar(self, torch, x, dtype, what):
-        if x.numel() != 1 or x.dtype != dtype or x.device != self.params[0].device:
+        if not isinstance(x, torch.Tensor) or x.numel() != 1 or x.dtype != dtype or x.device != self.params[0].device:
             raise ValueError(f"{what} must be a {dtype} tensor of one value beside the weights")
         return x.data_ptr()
 

@@ -87,11 +87,11 @@ def check(x, given, t, k, kind, order, allowed=None, tag=""):
     close(st[:, 2], est[:, 2], e + np.abs(np.nan_to_num(est[:, 2])) * 2.0 ** -24, (tag, "far"))
 
 
-def run_grad(x, given, g, h, st, t, kind, order, allowed=None):
+def run_grad(x, given, g, h, st, t, kind, order, allowed=None, to=None):
     rows, n = x.shape
     L = cb.load()
     with Buffers() as b:
-        block, at, grs, gcs = laid(np.zeros_like(x), kind, order)
+        block, at, grs, gcs = laid(np.zeros_like(x), kind, to or order)
         out = b.put(np.full(block.shape, 77, block.dtype))
         gp, up, sp = b.put(given.astype(np.int32)), b.put(g.astype(np.float32)), b.put(st.astype(np.float32))
         hp = None if h is None else b.put(h.astype(np.float32))
@@ -208,6 +208,20 @@ def test_rows_without_a_derivative_are_not_read():
         for order in ("rows", "classes"):
             check_grad(x, given, up, None, 1.0, "f32", order, None, (rows, n, order))
             check_grad(x, given, up, np.where(np.arange(rows) == 3, 0.5, 0.0), 1.0, "f32", order, None, (rows, n, order))
+
+
+@pytest.mark.parametrize("rows,n", [(70, 10), (70, 40), (9, 700), (5, 5003)])
+def test_a_gradient_laid_otherwise_than_the_scores(rows, n):
+    g = np.random.default_rng(12)
+    x, given = O.scores(g, rows, n, "normal"), given_of(g, rows, n, 2)
+    up, h = g.standard_normal((rows, 2)), g.standard_normal(rows)
+    _, *st = S.row_stats(x, 1.0)
+    st = np.stack(st, 1)
+    want = run_grad(x, given, up, h, st, 1.0, "f32", "rows")
+    for order, to in (("rows", "classes"), ("classes", "rows"), ("padded", "reversed"), ("reversed", "padded"), ("classes", "padded")):
+        got = run_grad(x, given, up, h, st, 1.0, "f32", order, to=to)
+        # (the ways differ in where a class with entries is rounded, not in what it is)
+        assert np.allclose(got, want, rtol=2.0 ** -19, atol=2.0 ** -21), (order, to)
 
 
 @pytest.mark.parametrize("t", [1e-38, 1e-20, 1e-3, 1e3, 1e20, 1e36])

@@ -199,6 +199,61 @@ def check_graph_replays():
             assert opts[0].steps.item() == 5
 
 
+def check_graphs_of_tables():
+    """Every way of the sort, and the tables held in LDS beyond what a launch has without asking, captured and replayed."""
+    g = torch.Generator(device=DEVICE).manual_seed(11)
+    for rows, many, entries, dim in ((300, 1, 50, 9), (900, 3, 5000, 30), (30000, 1, 300, 16), (20000, 2, 90000, 8), (8000, 40, 1280, 64),
+                                     (33000, 40, 1280, 64)):
+        table, up = torch.randn(entries, dim, generator=g, device=DEVICE), torch.randn(rows, dim, generator=g, device=DEVICE)
+        index = torch.randint(-1, entries, (rows, many), generator=g, device=DEVICE).int()
+
+        def step():
+            return cb.lookup_rows(table, index, 0.5), cb.lookup_gradients(up, index, entries)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        with torch.cuda.graph(other):
+            out2 = step()
+        for seed in range(3):
+            for x in (table, up):
+                x.copy_(torch.randn(x.shape, generator=g, device=DEVICE))
+            index.copy_(torch.randint(-1, entries, (rows, many), generator=g, device=DEVICE))
+            graph.replay()
+            other.replay()
+            torch.cuda.synchronize()
+            for a, b, c in zip(out, out2, step()):
+                assert torch.equal(a, c) and torch.equal(b, c), (rows, many, entries, seed)
+
+
+def check_weights_that_move():
+    """A weight whose memory is replaced between steps is found again; one that changes its type or shape is refused."""
+    p = torch.nn.Parameter(torch.ones(300, device=DEVICE))
+    opt = cb.AdamW([p], lr=0.5, weight_decay=0.0)
+    grad = torch.ones(300, device=DEVICE)
+    opt.step([grad])
+    old = p.data
+    p.data = p.data.clone()
+    before = old.clone()
+    opt.step([grad])
+    assert torch.equal(old, before) and not torch.equal(p.data, before)
+    for bad in (p.data.half(), p.data[:200].clone(), p.data.cpu()):
+        keep, p.data = p.data, bad
+        try:
+            opt.step([torch.ones_like(bad, device=DEVICE)] if bad.numel() != 300 else [grad])
+        except ValueError:
+            p.data = keep
+            continue
+        raise AssertionError(bad.dtype)
+    opt.step([grad])
+    assert opt.steps == 3
+
+
 def check_no_rows():
     x, i = torch.empty(0, 7, device=DEVICE), torch.empty(0, 2, device=DEVICE, dtype=torch.int32)
     got = cb.class_logprobs(x, i, k=3)
@@ -299,6 +354,11 @@ def check_refusals():
     refuses(ValueError, opt.step, [table.double()])
     refuses(ValueError, opt.step, [table], grad_scale=table)
     refuses(ValueError, opt.step, [table], skip=torch.zeros(1, device=DEVICE))
+    refuses(ValueError, opt.step, [table], grad_scale=0.5)
+    refuses(ValueError, opt.step, [table], skip=1)
+    refuses(ValueError, opt.step, [table.cpu()])
+    refuses(ValueError, opt.step, [[1.0]])
+    refuses(TypeError, opt.step, table[0, 0])
     refuses(cb.CbhError, opt.step, [table], lr=float("nan"))
     refuses(cb.CbhError, cb.AdamW([table, table]).step, [table, table])
     assert opt.steps == 0
