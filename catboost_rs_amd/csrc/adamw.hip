@@ -409,6 +409,12 @@ extern "C" int cbh_adamw_step(const cbh_adamw_tensor* tensors, uint32_t count, c
         std::sort(written.begin(), written.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
         for (size_t i = 1; i < written.size(); ++i)
             if (written[i].from < written[i - 1].to) return invalid("tensors that are written overlap");
+        for (uint32_t i = 0; i < count; ++i) {
+            if (tensors[i].n == 0) continue;
+            const uintptr_t from = (uintptr_t)tensors[i].grad, to = from + tensors[i].n * type_bytes(tensors[i].grad_type);
+            const auto next = std::lower_bound(written.begin(), written.end(), to, [](const Span& a, uintptr_t at) { return a.from < at; });
+            if (next != written.begin() && next[-1].to > from) return invalid("a gradient overlaps a tensor that is written");
+        }
 
         Step S{};
         S.lr = A.lr, S.beta1 = A.beta1, S.beta2 = A.beta2, S.weight_decay = A.weight_decay;

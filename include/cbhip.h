@@ -649,7 +649,7 @@ typedef struct {
     uint32_t seed;
     int32_t state;                /* CBH_STATE_* */
 } cbh_adamw_settings;
-/* tensors: HOST array [count].  Parameters, states and copies may not overlap one another (refused). */
+/* tensors: HOST array [count].  Parameters, states and copies may overlap neither one another nor a gradient (refused). */
 int cbh_adamw_step(const cbh_adamw_tensor* tensors, uint32_t count, const cbh_adamw_settings* settings, void* stream);
 
 /* Version / build information. */

@@ -112,6 +112,14 @@ def test_adamw_refuses_the_same_memory_twice(lib):
     assert adamw(lib, state=1, tensor=dict(exp_avg_scale=6 * P)) == -5
 
 
+def test_adamw_refuses_a_gradient_that_it_would_write_over(lib):
+    far = {k: 100 * P + i * P for i, k in enumerate(("param", "exp_avg", "exp_avg_sq"))}
+    for grad in (P, P + 60, P - 60, 3 * P, 4 * P + 4, 100 * P + 32):
+        assert adamw(lib, tensor=[dict(grad=grad), far]) == -5
+    assert adamw(lib, tensor=dict(copy=7 * P, grad=7 * P)) == -5
+    assert adamw(lib, state=1, tensor=dict(grad=6 * P)) == -5
+
+
 def test_no_work_is_no_error(lib):
     s = scores(rows=0, data=None)
     assert lib.cbh_class_logprobs(*s, None, 1, 1.0, None, 0, 3, None, None, None, None, None, None, 0, None) == 0
