@@ -55,7 +55,7 @@ class AdamW:
         self._look_at_weights(torch)
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
         self.state, self.steps, self.seed = state, steps, int(seed) & 0xFFFFFFFF
-        small = state == "f8"
+        small = self._small = state == "f8"
         kind = torch.float8_e4m3fn if small else torch.float32
         self.exp_avg = self._states(torch, exp_avg, kind, None, "exp_avg")
         self.exp_avg_sq = self._states(torch, exp_avg_sq, kind, None, "exp_avg_sq")
@@ -153,9 +153,11 @@ class AdamW:
         addresses = list(map(torch.Tensor.data_ptr, params))
         if addresses != self._addresses:   # (weights that moved; the memory of the old ones is kept until then, so that it is nobody else's)
             self._look_at_weights(torch)
+        elif not all(map(torch.Tensor.is_contiguous, params)):
+            raise ValueError("params must be contiguous")
         records["grad"] = list(map(torch.Tensor.data_ptr, grads))
         s = _Settings(beta1=self.beta1, beta2=self.beta2, eps=self.eps, weight_decay=self.weight_decay, seed=self.seed,
-                      state=1 if self.state == "f8" else 0)
+                      state=1 if self._small else 0)
         lr = self.lr if lr is None else lr
         if isinstance(lr, torch.Tensor):
             s.lr_device = self._scalar(torch, lr, torch.float32, "lr")
@@ -166,11 +168,16 @@ class AdamW:
         if skip is not None:
             s.skip = self._scalar(torch, skip, torch.int32, "skip")
         with _on(params[0]):
+            counted = None
             if isinstance(self.steps, torch.Tensor):
-                self.steps.add_(1 if skip is None else (skip.view(self.steps.shape) == 0))
-                s.step_device = self.steps.data_ptr()
+                s.step_device = self._scalar(torch, self.steps, torch.int64, "steps")
+                counted = 1 if skip is None else (skip.view(self.steps.shape) == 0)
+                self.steps.add_(counted)
             else:
                 s.step = self.steps + 1
-            _state["check"](_state["adamw"](records.ctypes.data, len(params), C.byref(s), _stream(params[0])))
-        if not isinstance(self.steps, torch.Tensor):
+            code = _state["adamw"](records.ctypes.data, len(params), C.byref(s), _stream(params[0]))
+            if code and counted is not None:   # (a step that was refused is not counted)
+                self.steps.sub_(1 if skip is None else counted.to(torch.int64))
+            _state["check"](code)
+        if counted is None:
             self.steps += 1

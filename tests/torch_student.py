@@ -266,6 +266,28 @@ def check_no_rows():
     cb.AdamW([]).step([])
 
 
+def check_steps_that_are_refused():
+    """Nothing of a step that is refused is done: neither weights nor a counter on the GPU."""
+    p, grad = torch.ones(20, 20, device=DEVICE), torch.ones(20, 20, device=DEVICE)
+    for skip in (None, torch.zeros(1, dtype=torch.int32, device=DEVICE), torch.ones(1, dtype=torch.int32, device=DEVICE)):
+        opt = cb.AdamW([p], steps=torch.full((1,), 4, dtype=torch.int64, device=DEVICE))
+        tries = [(cb.CbhError, lambda: opt.step([grad], lr=float("nan"), skip=skip))]
+        good = opt.steps
+        for steps in (good.cpu(), good.int(), good.repeat(2)):
+            tries.append((ValueError, lambda steps=steps: (setattr(opt, "steps", steps), opt.step([grad], skip=skip))))
+        whole = p.data
+        tries.append((ValueError, lambda: (setattr(opt, "steps", good), setattr(p, "data", whole.t()), opt.step([grad], skip=skip))))
+        for error, f in tries:
+            try:
+                f()
+            except error:
+                pass
+            else:
+                raise AssertionError("a step was not refused")
+        p.data = whole
+        assert good.item() == 4 and bool((p == 1).all()) and bool((opt.exp_avg[0] == 0).all())
+
+
 def check_far_rows():
     """Offsets past 32 bits: the last rows of matrices of more than 2^32 elements."""
     rows, n = 70001, 65536
@@ -357,6 +379,7 @@ def check_refusals():
     refuses(ValueError, opt.step, [table], grad_scale=0.5)
     refuses(ValueError, opt.step, [table], skip=1)
     refuses(ValueError, opt.step, [table.cpu()])
+    refuses(cb.CbhError, opt.step, [table])   # (the weight as its own gradient)
     refuses(ValueError, opt.step, [[1.0]])
     refuses(TypeError, opt.step, table[0, 0])
     refuses(cb.CbhError, opt.step, [table], lr=float("nan"))
