@@ -5,7 +5,7 @@
 //
 // Every value is read and written once: 60M values with 8-bit states and bf16 gradients 165 us, 840 MB at 5.1 TB/s, a copy's rate; what
 // it computes (a correctly rounded root and division, the hash, the codes: about 100 instructions a value) hides behind that.  150 tensors
-// of 4M values: two launches of 8 us, and 58 us of a call from Python, most of it the looking at 150 gradients.  8-bit states are m and sqrt(v) as e4m3 codes over a power of two that a
+// of 4M values: two launches of 8 us, and 63 us of a call from Python, most of it the looking at 150 gradients and weights.  8-bit states are m and sqrt(v) as e4m3 codes over a power of two that a
 // block of 256 values shares: a wave takes a block, four values a lane.  sqrt(v), not v: the codes reach from 448 down to 2^-9, 18
 // binades, which are 36 of v.
 #include <vector>
