@@ -20,15 +20,16 @@ struct Upstream {
     float c;
     double it;
 };
-// The factors of a row: grad_j = 2^y (a + b y), y = (x_j - m) c, beside the entries' own.
+// The factors of a row: grad_j = 2^y (a + b y), y = (x_j - m) c, beside the entries' own.  Up to kWidest a and b are f32: their sum is
+// finite then, and 0 times it is 0.  Beyond (derivatives over a small temperature: 1 / t reaches 1e38) what a class has may still be
+// a number of f32, or 0: the row is `wide`, and each of its classes f64.
+constexpr double kWidest = 1e30;
 struct RowFactors {
     float m, a, b;
     double log_z, far, G, h;
     bool zero;   // all derivatives are 0
+    bool wide;
 };
-__device__ __forceinline__ float clamp_finite(double v) {   // (2^y = 0 times it is 0)
-    return v != v ? (float)v : (float)fmin(fmax(v, -3.4e38), 3.4e38);
-}
 __device__ __forceinline__ RowFactors row_factors(const Upstream& P, uint64_t row, double G, bool any) {
     RowFactors f;
     const float* s = P.stats + row * 3;
@@ -40,8 +41,10 @@ __device__ __forceinline__ RowFactors row_factors(const Upstream& P, uint64_t ro
     f.log_z = (double)s[1];
     f.far = (double)s[2];
     const double r = none ? 0.0 : -P.it * exp_f64(-f.log_z);
-    f.a = none ? 0.0f : clamp_finite(r * (f.G + f.h * f.far));
-    f.b = none ? 0.0f : clamp_finite(r * f.h * kLn2);
+    const double a = none ? 0.0 : r * (f.G + f.h * f.far), b = none ? 0.0 : r * f.h * kLn2;
+    f.a = (float)a;
+    f.b = (float)b;
+    f.wide = !f.zero && (fabs(a) > kWidest || fabs(b) > kWidest);
     return f;
 }
 __device__ __forceinline__ float grad_of(float x, const RowFactors& f, float c) {
@@ -54,7 +57,7 @@ __device__ __forceinline__ float grad_of_given(float x, double g, const RowFacto
     return (float)(it * (g - (p == 0.0 ? 0.0 : p * (f.G + f.h * (d + f.far)))));
 }
 
-// A wave takes a segment of a row; classes with entries are written over.
+// A wave takes a segment of a row; classes with entries, or all of a wide row, are written over.
 constexpr uint32_t kGradSeg = 4 * kSeg;
 template <class T, bool kUnit, bool kMask>
 __global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P, T* __restrict__ grad, int64_t grs,
@@ -88,7 +91,7 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P
                 const uint32_t i = base + (u * 64 + lane) * V;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    x[u][v] = f.zero ? 0.0f : grad_of(x[u][v], f, P.c);
+                    x[u][v] = f.zero || f.wide ? 0.0f : grad_of(x[u][v], f, P.c);
                     if constexpr (kMask) x[u][v] = bits[u] >> v & 1 ? x[u][v] : 0.0f;
                 }
                 if (i < n) store_pack<T, kUnit>(g0, gcs, i, n, x[u]);
@@ -96,8 +99,8 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P
         }
         if (f.zero) continue;
         __threadfence_block();   // (the stores above are done)
-        for (uint32_t i = lane; i < P.n_given; i += 64) {
-            const uint32_t j = (uint32_t)given[i];
+        for (uint32_t i = lane; i < (f.wide ? n : P.n_given); i += 64) {
+            const uint32_t j = f.wide ? first + i : (uint32_t)given[i];
             if (j >= X.classes || j < first || j - first >= n) continue;
             if (kMask && !is_allowed(words, j - first)) continue;
             double sum = 0.0;
@@ -107,7 +110,7 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(Rows<T> X, Upstream P
                     sum += (double)g[e];
                     again |= e < i;
                 }
-            if (again) continue;
+            if (again && !f.wide) continue;
             const float x = to_f32(x0[kUnit ? (int64_t)(j - first) : (int64_t)(j - first) * X.cs]);
             g0[kUnit ? (int64_t)(j - first) : (int64_t)(j - first) * gcs] = from_f32<T>(grad_of_given(x, sum, f, P.it));
         }
@@ -141,11 +144,11 @@ __global__ __launch_bounds__(256) void logprob_grad_short_kernel(Rows<T> X, Upst
         for (int u = 0; u < R; ++u) {
             const uint32_t i = (u * G + l) * V, bits = words && i < n ? words[i >> 5] >> (i & 31) : ~0u;
 #pragma unroll
-            for (int v = 0; v < V; ++v) x[u][v] = f.zero || !(bits >> v & 1) ? 0.0f : grad_of(x[u][v], f, P.c);
+            for (int v = 0; v < V; ++v) x[u][v] = f.zero || f.wide || !(bits >> v & 1) ? 0.0f : grad_of(x[u][v], f, P.c);
         }
         if (!f.zero)
-            for (uint32_t i = 0; i < P.n_given; ++i) {
-                const uint32_t j = (uint32_t)given[i];
+            for (uint32_t i = 0; i < (f.wide ? n : P.n_given); ++i) {
+                const uint32_t j = f.wide ? i : (uint32_t)given[i];
                 if (j >= n || j / V % G != l || (words && !is_allowed(words, j))) continue;
                 double own = 0.0;
                 for (uint32_t e = 0; e < P.n_given; ++e) own += (uint32_t)given[e] == j ? (double)g[e] : 0.0;
@@ -201,19 +204,20 @@ __global__ __launch_bounds__(256) void logprob_grad_few_kernel(Rows<T> X, Upstre
         const RowFactors f = row_factors(P, row, G, some);
         float y[NMAX];
 #pragma unroll
-        for (int j = 0; j < NMAX; ++j) y[j] = f.zero || !(bits >> j & 1) ? 0.0f : grad_of(x[j], f, P.c);
+        for (int j = 0; j < NMAX; ++j) y[j] = f.zero || f.wide || !(bits >> j & 1) ? 0.0f : grad_of(x[j], f, P.c);
         if constexpr (kSums) {
+            if (f.wide) listed = ~0u;
 #pragma unroll
             for (int j = 0; j < NMAX; ++j)
                 if (!f.zero && (listed & bits) >> j & 1) y[j] = grad_of_given(x[j], own[j], f, P.it);
         } else {
             uint32_t done = f.zero ? ~0u : ~bits;
-            for (uint32_t i = 0; i < P.n_given; ++i) {
-                const uint32_t j = (uint32_t)given[i] - first;
-                if ((uint32_t)given[i] >= X.classes || j >= n || (done >> j & 1)) continue;
+            for (uint32_t i = 0; i < (f.wide ? n : P.n_given); ++i) {
+                const uint32_t c = f.wide ? first + i : (uint32_t)given[i], j = c - first;
+                if (c >= X.classes || j >= n || (done >> j & 1)) continue;
                 done |= 1u << j;
                 double sum = 0.0;
-                for (uint32_t e = i; e < P.n_given; ++e) sum += (uint32_t)given[e] - first == j ? (double)g[e] : 0.0;
+                for (uint32_t e = f.wide ? 0 : i; e < P.n_given; ++e) sum += (uint32_t)given[e] - first == j ? (double)g[e] : 0.0;
                 float at = 0.0f;
 #pragma unroll
                 for (int q = 0; q < NMAX; ++q) at = (uint32_t)q == j ? x[q] : at;
