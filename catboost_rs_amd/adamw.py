@@ -39,6 +39,9 @@ class AdamW:
 
     ``steps`` is a number, or an i64 tensor of one value on the GPU: then every step adds 1 to it on the stream (not
     where ``skip`` holds a step back), and a step may be captured into a graph.
+
+    A step counts as an in-place change of what it writes (the tensors' version counters): the backward pass of a graph that
+    was recorded with the weights as they were raises, as after torch's own updates.
     """
 
     def __init__(self, params, *, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state="f32", exp_avg=None,
@@ -99,6 +102,7 @@ class AdamW:
                 raise ValueError(f"params must be float32, float16 or bfloat16, not {p.dtype}")
             if not p.is_contiguous():
                 raise ValueError("params must be contiguous")
+        self._counters = None
         self._addresses = [p.data_ptr() for p in self.params]
         self._weights = [p.untyped_storage() for p in self.params]
         self._records["param"] = self._addresses
@@ -114,6 +118,14 @@ class AdamW:
             if not isinstance(x, torch.Tensor) or x.shape != s or x.dtype != dtype or x.device != p.device or not x.is_contiguous():
                 raise ValueError(f"{what} must be contiguous {dtype} tensors of shape {[list(s) for s in shapes]}")
         return given
+
+    def _written(self, grads):
+        """What a step with these gradients (None: all of them) writes, a tensor for every version counter: views share their
+        base's."""
+        lists = [x for x in (self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.copies)
+                 if x is not None]
+        all_ = [t for x in lists for i, t in enumerate(x) if t is not None and (grads is None or grads[i] is not None)]
+        return list({id(b): b for b in (t if t._base is None else t._base for t in all_)}.values())
 
     def _scalar(self, torch, x, dtype, what):
         if not isinstance(x, torch.Tensor) or x.numel() != 1 or x.dtype != dtype or x.device != self.params[0].device:
@@ -133,11 +145,12 @@ class AdamW:
             raise ValueError("grads must be a tensor or None for every weight")
         if not params:
             return
-        dev, records = params[0].device, self._records
+        dev, records, some = params[0].device, self._records, None
         # (attribute by attribute over all tensors: a loop over them would cost more than the step of small ones)
         try:
             shapes, records["n"] = list(map(_SHAPE, grads)), self._sizes
         except AttributeError:   # (a weight without a gradient: nothing of it is touched)
+            some = grads
             records["n"] = np.where([g is None for g in grads], 0, self._sizes)
             grads = [p if g is None else g for g, p in zip(grads, params)]
             shapes = [getattr(g, "shape", None) for g in grads]
@@ -179,5 +192,8 @@ class AdamW:
             if code and counted is not None:   # (a step that was refused is not counted)
                 self.steps.sub_(1 if skip is None else counted.to(torch.int64))
             _state["check"](code)
+        if some is None and self._counters is None:
+            self._counters = self._written(None)
+        torch.autograd.graph.increment_version(self._counters if some is None else self._written(some))
         if counted is None:
             self.steps += 1
