@@ -38,7 +38,8 @@ class AdamW:
     weights beside f32 ones.
 
     ``steps`` is a number, or an i64 tensor of one value on the GPU: then every step adds 1 to it on the stream (not
-    where ``skip`` holds a step back), and a step may be captured into a graph.
+    where ``skip`` holds a step back), and a step may be captured into a graph.  With a number a capture is refused: the
+    graph's replays would all be the same step.
 
     A step counts as an in-place change of what it writes (the tensors' version counters): the backward pass of a graph that
     was recorded with the weights as they were raises, as after torch's own updates.
@@ -187,6 +188,8 @@ class AdamW:
                 counted = 1 if skip is None else (skip.view(self.steps.shape) == 0)
                 self.steps.add_(counted)
             else:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a step that is captured into a graph needs its number on the GPU: give AdamW steps as an int64 tensor")
                 s.step = self.steps + 1
             code = _state["adamw"](records.ctypes.data, len(params), C.byref(s), _stream(params[0]))
             if code and counted is not None:   # (a step that was refused is not counted)

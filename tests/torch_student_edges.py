@@ -67,6 +67,25 @@ def check_inference_tensors():
     assert opt.steps == 2 and bool((p < 0.5).all())
 
 
+def check_a_captured_step_counts_on_the_device():
+    """A number of steps would be a constant of the graph: refused, and nothing is changed."""
+    p, grad = torch.ones(30, device=DEVICE), torch.ones(30, device=DEVICE)
+    opt = cb.AdamW([p])
+    opt.step([grad])
+    before = p.clone()
+    graph = torch.cuda.CUDAGraph()
+
+    def capture():
+        with torch.cuda.graph(graph):
+            opt.step([grad])
+
+    refuses(RuntimeError, capture)
+    torch.cuda.synchronize()
+    assert opt.steps == 1 and torch.equal(p, before)
+    opt.step([grad])
+    assert opt.steps == 2 and not torch.equal(p, before)
+
+
 if __name__ == "__main__":
     for name, f in list(globals().items()):
         if name.startswith("check_"):
