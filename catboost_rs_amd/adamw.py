@@ -35,7 +35,8 @@ class AdamW:
     ``exp_avg_sq_scale`` f32 of every 256 values; rounded by random bits of ``seed`` and the step).  States of an
     earlier run are given by those names, as lists of tensors, and kept, not copied; with ``steps``, the number of steps
     that they are after.  ``copies``: a list of tensors (or None) that get the new weights rounded to their type: 16-bit
-    weights beside f32 ones.
+    weights beside f32 ones.  The handle's tuples of weights, states and copies stay; the memory of their tensors may be written
+    and may move between steps.  A step with a weight that changed its shape or type is refused.
 
     ``steps`` is a number, or an i64 tensor of one value on the GPU: then every step adds 1 to it on the stream (not
     where ``skip`` holds a step back), and a step may be captured into a graph.  With a number a capture is refused: the
@@ -48,52 +49,47 @@ class AdamW:
     def __init__(self, params, *, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state="f32", exp_avg=None,
                  exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None, copies=None, steps=0, seed=0):
         torch = _state.get("torch") or _bind()
-        self.params = list(params)
+        self._params = tuple(params)
         if state not in ("f32", "f8"):
             raise ValueError("state must be 'f32' or 'f8'")
         for p in self.params:
             if not isinstance(p, torch.Tensor):
                 raise ValueError("params must be torch tensors")
         self._shapes, self._types = [p.shape for p in self.params], [p.dtype for p in self.params]
-        self._records = np.zeros(len(self.params), np.dtype(_Tensor))
-        self._look_at_weights(torch)
+        self._check_weights()
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
         self.state, self.steps, self.seed = state, steps, int(seed) & 0xFFFFFFFF
         small = self._small = state == "f8"
-        kind = torch.float8_e4m3fn if small else torch.float32
-        self.exp_avg = self._states(torch, exp_avg, kind, None, "exp_avg")
-        self.exp_avg_sq = self._states(torch, exp_avg_sq, kind, None, "exp_avg_sq")
-        blocks = [((p.numel() + BLOCK - 1) // BLOCK,) for p in self.params]
-        self.exp_avg_scale = self._states(torch, exp_avg_scale, torch.float32, blocks, "exp_avg_scale") if small else None
-        self.exp_avg_sq_scale = self._states(torch, exp_avg_sq_scale, torch.float32, blocks, "exp_avg_sq_scale") if small else None
         if not small and (exp_avg_scale is not None or exp_avg_sq_scale is not None):
             raise ValueError("states in f32 have no scales")
-        self.copies = [None] * len(self.params) if copies is None else list(copies)
-        if len(self.copies) != len(self.params):
-            raise ValueError("copies must be a tensor or None for every weight")
-        for c, p in zip(self.copies, self.params):
-            if c is not None and (not isinstance(c, torch.Tensor) or c.dtype not in _TYPE or c.shape != p.shape
-                                  or c.device != p.device or not c.is_contiguous()):
-                raise ValueError("a copy must be a contiguous float32, float16 or bfloat16 tensor of its weight's shape and device")
+        kind = torch.float8_e4m3fn if small else torch.float32
+        blocks = [((p.numel() + BLOCK - 1) // BLOCK,) for p in self.params]
+        # what every list of states holds: types and shapes
+        self._kinds = {"exp_avg": (kind, self._shapes), "exp_avg_sq": (kind, self._shapes)}
+        if small:
+            self._kinds.update(exp_avg_scale=(torch.float32, blocks), exp_avg_sq_scale=(torch.float32, blocks))
+        self._states = {}
+        given = dict(exp_avg=exp_avg, exp_avg_sq=exp_avg_sq, exp_avg_scale=exp_avg_scale, exp_avg_sq_scale=exp_avg_sq_scale)
+        for name, x in given.items():
+            if name in self._kinds and x is None:
+                kind, shapes = self._kinds[name]
+                x = [torch.zeros(s, dtype=torch.float32, device=p.device).to(kind) for s, p in zip(shapes, self.params)]
+            self._states[name] = None if x is None else tuple(x)
+        self._copies = (None,) * len(self.params) if copies is None else tuple(copies)
         if isinstance(steps, torch.Tensor):
             if steps.dtype != torch.int64 or steps.numel() != 1 or (self.params and steps.device != self.params[0].device):
                 raise ValueError("steps must be a number, or an int64 tensor of one value beside the weights")
         elif steps < 0:
             raise ValueError("steps must not be negative")
-        # what of the library's records of the tensors does not change from step to step; the states' memory stays alive and in
-        # place with its storage
-        self._fixed = [x for x in (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale) if x is not None]
-        self._fixed = [t.untyped_storage() for x in self._fixed + [self.copies] for t in x if t is not None]
-        for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
-            if getattr(self, name) is not None:
-                self._records[name] = [t.data_ptr() for t in getattr(self, name)]
-        self._records["copy"] = [0 if c is None else c.data_ptr() for c in self.copies]
-        self._records["copy_type"] = [0 if c is None else _TYPE[c.dtype] for c in self.copies]
+        # what of the library's records of the tensors does not change from step to step
+        self._records = np.zeros(len(self.params), np.dtype(_Tensor))
         self._records["param_type"] = [_TYPE[t] for t in self._types]
         self._records["number"] = range(len(self.params))
         self._sizes = np.array([p.numel() for p in self.params], np.uint64)
+        self._grad_types = None
+        self._look(torch)
 
-    def _look_at_weights(self, torch):
+    def _check_weights(self):
         for p, shape, dtype in zip(self.params, self._shapes, self._types):
             if p.shape != shape or p.dtype != dtype:
                 raise ValueError("a weight is not what it was: its shape or type changed")
@@ -103,28 +99,46 @@ class AdamW:
                 raise ValueError(f"params must be float32, float16 or bfloat16, not {p.dtype}")
             if not p.is_contiguous():
                 raise ValueError("params must be contiguous")
-        self._counters = None
-        self._addresses = [p.data_ptr() for p in self.params]
-        self._weights = [p.untyped_storage() for p in self.params]
-        self._records["param"] = self._addresses
 
-    def _states(self, torch, given, dtype, shapes, what):
-        shapes = [p.shape for p in self.params] if shapes is None else shapes
-        if given is None:
-            return [torch.zeros(s, dtype=torch.float32, device=p.device).to(dtype) for s, p in zip(shapes, self.params)]
-        given = list(given)
-        if len(given) != len(self.params):
-            raise ValueError(f"{what} must be a tensor for every weight")
-        for x, s, p in zip(given, shapes, self.params):
-            if not isinstance(x, torch.Tensor) or x.shape != s or x.dtype != dtype or x.device != p.device or not x.is_contiguous():
-                raise ValueError(f"{what} must be contiguous {dtype} tensors of shape {[list(s) for s in shapes]}")
-        return given
+    # what a step writes: tuples, whose tensors may be written and moved
+    params = property(lambda self: self._params)
+    exp_avg = property(lambda self: self._states["exp_avg"])
+    exp_avg_sq = property(lambda self: self._states["exp_avg_sq"])
+    exp_avg_scale = property(lambda self: self._states["exp_avg_scale"])
+    exp_avg_sq_scale = property(lambda self: self._states["exp_avg_sq_scale"])
+    copies = property(lambda self: self._copies)
+
+    def _look(self, torch):
+        """Checks weights, states and copies and takes their addresses: at first, and where one of them moved."""
+        self._check_weights()
+        for what, (dtype, shapes) in self._kinds.items():
+            x = self._states[what]
+            if len(x) != len(self.params):
+                raise ValueError(f"{what} must be a tensor for every weight")
+            for t, s, p in zip(x, shapes, self.params):
+                if not isinstance(t, torch.Tensor) or t.shape != s or t.dtype != dtype or t.device != p.device or not t.is_contiguous():
+                    raise ValueError(f"{what} must be contiguous {dtype} tensors of shape {[list(s) for s in shapes]}")
+        if len(self.copies) != len(self.params):
+            raise ValueError("copies must be a tensor or None for every weight")
+        for c, p in zip(self.copies, self.params):
+            if c is not None and (not isinstance(c, torch.Tensor) or c.dtype not in _TYPE or c.shape != p.shape
+                                  or c.device != p.device or not c.is_contiguous()):
+                raise ValueError("a copy must be a contiguous float32, float16 or bfloat16 tensor of its weight's shape and device")
+        self._records["param"] = [p.data_ptr() for p in self.params]
+        for name in self._kinds:
+            self._records[name] = [t.data_ptr() for t in self._states[name]]
+        self._records["copy"] = [0 if c is None else c.data_ptr() for c in self.copies]
+        self._records["copy_type"] = [0 if c is None else _TYPE[c.dtype] for c in self.copies]
+        lists = [self.params] + [self._states[name] for name in self._kinds]
+        self._held = [t for x in lists for t in x] + [c for c in self.copies if c is not None]
+        self._addresses = [t.data_ptr() for t in self._held]
+        self._memory = [t.untyped_storage() for t in self._held]   # (kept: what moves leaves its memory to nobody else before it is seen)
+        self._counters = None
 
     def _written(self, grads):
         """What a step with these gradients (None: all of them) writes, a tensor for every version counter: views share their
         base's."""
-        lists = [x for x in (self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.copies)
-                 if x is not None]
+        lists = [self.params, self.copies] + [self._states[name] for name in self._kinds]
         all_ = [t for x in lists for i, t in enumerate(x) if t is not None and (grads is None or grads[i] is not None)]
         return list({id(b): b for b in (t if t._base is None else t._base for t in all_)}.values())
 
@@ -157,18 +171,20 @@ class AdamW:
             shapes = [getattr(g, "shape", None) for g in grads]
         try:
             same = shapes == self._shapes and set(map(torch.Tensor.get_device, grads)) == {dev.index}
-            records["grad_type"] = list(map(_TYPE.__getitem__, map(_DTYPE, grads)))
+            types = list(map(_DTYPE, grads))
+            if types != self._grad_types:
+                records["grad_type"] = [_TYPE[t] for t in types]
+                self._grad_types = types
         except (KeyError, TypeError, AttributeError):
             same = False
         if not same:
             raise ValueError("a gradient must be a float32, float16 or bfloat16 tensor of its weight's shape and device")
         if not all(map(torch.Tensor.is_contiguous, grads)):
             grads = [g.contiguous() for g in grads]
-        addresses = list(map(torch.Tensor.data_ptr, params))
-        if addresses != self._addresses:   # (weights that moved; the memory of the old ones is kept until then, so that it is nobody else's)
-            self._look_at_weights(torch)
-        elif not all(map(torch.Tensor.is_contiguous, params)):
-            raise ValueError("params must be contiguous")
+        # (weights, states or copies that moved, weights of another shape or type in the same place)
+        if (list(map(torch.Tensor.data_ptr, self._held)) != self._addresses or list(map(_SHAPE, params)) != self._shapes
+                or list(map(_DTYPE, params)) != self._types or not all(map(torch.Tensor.is_contiguous, params))):
+            self._look(torch)
         records["grad"] = list(map(torch.Tensor.data_ptr, grads))
         s = _Settings(beta1=self.beta1, beta2=self.beta2, eps=self.eps, weight_decay=self.weight_decay, seed=self.seed,
                       state=1 if self._small else 0)

@@ -86,6 +86,79 @@ def check_a_captured_step_counts_on_the_device():
     assert opt.steps == 2 and not torch.equal(p, before)
 
 
+def check_weights_that_change_in_place():
+    """A weight that becomes a shorter or another type's view of its own memory is refused, and nothing is written."""
+    whole = torch.ones(300, device=DEVICE)
+    p = torch.nn.Parameter(whole)
+    opt = cb.AdamW([p], lr=0.5)
+    grad = torch.ones(300, device=DEVICE)
+    at = p.data_ptr()
+    for bad in (whole[:200], whole.view(torch.float16)[:300], whole.view(torch.bfloat16)[:300], whole.view(30, 10)):
+        p.data = bad
+        assert p.data_ptr() == at
+        for g in (grad, torch.ones(bad.shape, device=DEVICE)):
+            refuses(ValueError, lambda: opt.step([g]))
+    p.data = whole
+    assert bool((whole == 1).all()) and opt.steps == 0
+    opt.step([grad])
+    assert opt.steps == 1 and bool((whole < 1).all())
+
+
+def check_states_and_copies_that_move():
+    """What a state's or a copy's memory became is what the next step goes on with."""
+    for state in ("f32", "f8"):
+        g = torch.Generator(device=DEVICE).manual_seed(3)
+        first = torch.randn(700, generator=g, device=DEVICE)
+        a, b = first.clone(), first.clone()
+        copy = torch.zeros(700, device=DEVICE, dtype=torch.bfloat16)
+        one, two = cb.AdamW([a], state=state, lr=0.1), cb.AdamW([b], state=state, lr=0.1, copies=[copy])
+        names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if state == "f8" else [])
+        bits = torch.uint8 if state == "f8" else torch.int32
+
+        def step():
+            grad = torch.randn(700, generator=g, device=DEVICE)
+            one.step([grad])
+            two.step([grad])
+            assert torch.equal(a, b) and torch.equal(two.copies[0], b.bfloat16())
+            for name in names:
+                x, y = getattr(one, name)[0], getattr(two, name)[0]
+                kind = torch.int32 if x.dtype == torch.float32 else bits
+                assert torch.equal(x.view(kind), y.view(kind)), (state, name)
+
+        step()
+        for name in names:
+            # other memory
+            old = getattr(two, name)[0].data
+            before = old.clone()
+            getattr(two, name)[0].data = old.clone()
+            step()
+            assert torch.equal(old.view(torch.uint8), before.view(torch.uint8)), (state, name)
+            refuses(AttributeError, lambda: getattr(two, name).append(old))   # (the tuples stay)
+            refuses(AttributeError, lambda: setattr(two, name, [old]))
+            # memory given up for a while
+            x = getattr(two, name)[0]
+            saved, storage = x.clone(), x.untyped_storage()
+            size = storage.size()
+            storage.resize_(0)
+            refuses(cb.CbhError, lambda: two.step([first]))
+            other = torch.full((4000,), 7.0, device=DEVICE)   # (perhaps where it was)
+            refuses(cb.CbhError, lambda: two.step([first]))
+            assert bool((other == 7).all())
+            storage.resize_(size)
+            x.copy_(saved)
+            step()
+            # what does not fit is refused, and put right again
+            good = x.data
+            for bad in (good[:-1].clone(), good.to(torch.float64), torch.cat([good, good])[::2]):
+                x.data = bad
+                refuses(ValueError, lambda: two.step([first]))
+            x.data = good
+            step()
+        two.copies[0].data = torch.zeros(700, device=DEVICE, dtype=torch.bfloat16)
+        step()
+        assert one.steps == two.steps
+
+
 if __name__ == "__main__":
     for name, f in list(globals().items()):
         if name.startswith("check_"):
