@@ -259,7 +259,8 @@ int run_grad(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_t 
 #undef RUN
     } else if (lanes) {
 #define RUN(G, R) logprob_grad_short_kernel<T, G, R><<<row_grid((rows + 256 / G - 1) / (256 / G)), 256, 0, st>>>(X, P, g, grs)
-        if (n <= 4 * V) RUN(4, 1);
+        constexpr uint32_t least = 32 / V;   // (lanes: from 17 classes on)
+        if (n <= least * V) RUN((int)least, 1);
         else if (n <= 8 * V) RUN(8, 1);
         else if (n <= 16 * V) RUN(16, 1);
         else if (n <= 32 * V) RUN(32, 1);

@@ -249,9 +249,8 @@ int launch_rows(const Rows<T>& X, const Asked& A, const Plan& P, void* workspace
     const unsigned grid = row_grid(X.rows * P.parts);
     const uint32_t shortest = n - seg * (P.parts - 1);
     const bool many = X.rows * P.parts >= kManyRows && (k == 0 || seg <= kWaveRow);
-#define RUN(SEL, CAP, LDS)                                                                                              \
-    (many ? logprobs_kernel<T, kUnit, kMask, 64, SEL, CAP><<<grid, 64, LDS, st>>>(X, A, P.parts, seg, ps, pk) \
-          : logprobs_kernel<T, kUnit, kMask, 256, SEL, CAP><<<grid, 256, LDS, st>>>(X, A, P.parts, seg, ps, pk))
+#define RUN_BY(THREADS, SEL, CAP, LDS) logprobs_kernel<T, kUnit, kMask, THREADS, SEL, CAP><<<grid, THREADS, LDS, st>>>(X, A, P.parts, seg, ps, pk)
+#define RUN(SEL, CAP, LDS) (many ? RUN_BY(64, SEL, CAP, LDS) : RUN_BY(256, SEL, CAP, LDS))
     // by groups, or vectors, where k is at most a quarter of the shortest segment's
     const size_t lds = sizeof(uint32_t) * 64 * ((seg + kSeg - 1) / kSeg);
     constexpr uint32_t V = Pack<T>::V;
@@ -259,9 +258,10 @@ int launch_rows(const Rows<T>& X, const Asked& A, const Plan& P, void* workspace
     if (k == 0) {
         RUN(kNone, 2, 0);
     } else if (k * 4 <= shortest / kGroup) {
+        // (a k of more than 128 is a quarter of the groups of rows beyond kWaveRow only)
         if (k <= 128) RUN(kGroups, 256, lds);
-        else if (k <= 256) RUN(kGroups, 512, lds);
-        else RUN(kGroups, 2048, lds);
+        else if (k <= 256) RUN_BY(256, kGroups, 512, lds);
+        else RUN_BY(256, kGroups, 2048, lds);
     } else if (k * 4 <= shortest / V && lds_v <= 65536) {
         if (k <= 128) RUN(kVectors, 256, lds_v);
         else if (k <= 256) RUN(kVectors, 512, lds_v);
@@ -270,6 +270,7 @@ int launch_rows(const Rows<T>& X, const Asked& A, const Plan& P, void* workspace
         RUN(kWhole, 2, 0);
     }
 #undef RUN
+#undef RUN_BY
     CLS_TRY(hipGetLastError());
     if (P.parts > 1 || k) {
         if (P.parts == 1 && k <= 256) finish_kernel<T, 64><<<row_grid(X.rows), 64, 0, st>>>(X, A, 1, ps, pk);

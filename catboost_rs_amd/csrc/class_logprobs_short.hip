@@ -241,7 +241,8 @@ int run_short(const Rows<T>& X, const Asked& A, hipStream_t st) {
     const uint32_t n = X.classes;
     // by vectors where they fill the lanes: half of them, or a part of the wave's for the sums alone
     if (X.cs == 1 && (n > 32 * V || !A.k)) {
-        if (n <= 4 * V) launch_short<T, 4, 1, true>(X, A, st);
+        constexpr uint32_t least = 32 / V;   // (lanes: from 17 classes on)
+        if (n <= least * V) launch_short<T, (int)least, 1, true>(X, A, st);
         else if (n <= 8 * V) launch_short<T, 8, 1, true>(X, A, st);
         else if (n <= 16 * V) launch_short<T, 16, 1, true>(X, A, st);
         else if (n <= 32 * V) launch_short<T, 32, 1, true>(X, A, st);
