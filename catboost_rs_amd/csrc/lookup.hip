@@ -802,10 +802,19 @@ int run_lookup(const void* table, int64_t rs, int64_t cs, const Lookup& L, void*
     constexpr uint32_t V = Pack<T>::V;
     uint32_t lanes = 1;
     while (lanes < 64 && lanes * V < L.dim) lanes *= 2;
-    // in LDS: lists long enough that an entry is read often
+    // In LDS: lists long enough that an entry is read often, and 64 bytes of every entry in it, or its whole row.  Of less, each list is
+    // read by many workgroups, and rows are written in pieces of lines that lanes do not share.  By LDS and from the caches, us: 400000
+    // lists of 8 f32, 2500 entries of 64 columns (64 bytes held) 34 and 37, 4000 of 64 (32 bytes) 134 and 37, 9000 of 64 (16 bytes) 254
+    // and 40; 200000 lists of 40, 1280 of 64, 62 and 89.  Less of a row pays where the caches' way is slow: rows that are no whole vectors
+    // are read value by value (400000 lists of 8 over 9000 entries, 16 bytes: bf16 of 30 columns 64 and 108, of 255 723 and 484; f32 of 5
+    // columns 14 and 33, of 13 38 and 35; 100000 lists of 40, 5200 entries of 255 bf16, 195 and 389), and a large table is not in the
+    // second level (60000 lists of 40, 9000 entries of 1000 f32, 702 and 849, of 256 287 and 316; in it, 5200 of 256, 284 and 183).
     uint32_t held = lanes;
     while (held > 1 && (L.entries + 1ull) * held * 16 > kLdsBytes) held /= 2;
-    if (cs == 1 && L.list >= 8 && L.rows * L.list >= 256ull * L.entries && (L.entries + 1ull) * held * 16 <= kLdsBytes) {
+    const bool lists_long = L.list >= 32;
+    const uint32_t share = L.dim % V == 0 ? 1 : V == 4 ? 2 : lists_long ? 64 : 8;   // of a row's vectors, one that is enough
+    const bool pays = held >= 4 || lanes <= held * share || (lists_long && (uint64_t)L.entries * L.dim * sizeof(T) > 8u << 20);
+    if (cs == 1 && L.list >= 8 && L.rows * L.list >= 256ull * L.entries && pays && (L.entries + 1ull) * held * 16 <= kLdsBytes) {
         const uint32_t tiles = (L.dim + held * V - 1) / (held * V);
         const uint64_t least = kLdsThreads / held;   // rows of one round
         const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>((256 + tiles - 1) / tiles, (L.rows + 2 * least - 1) / (2 * least)));
