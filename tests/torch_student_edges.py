@@ -159,6 +159,34 @@ def check_states_and_copies_that_move():
         assert one.steps == two.steps
 
 
+def check_weights_of_16_bits():
+    """Steps of 16-bit weights through the handle, bit for bit the plain implementation's, and far larger than a rounding."""
+    import numpy as np
+
+    from tests import class_scores_oracle as O
+    from tests import student_oracle as S
+    from tests.test_gpu_adamw import expected
+
+    for dtype, kind in ((torch.bfloat16, "bf16"), (torch.float16, "f16")):
+        for small in (False, True):
+            g = torch.Generator(device=DEVICE).manual_seed(7)
+            params = [torch.randn(shape, generator=g, device=DEVICE).to(dtype) for shape in ((300, 3), (1,), (257,))]
+            opt = cb.AdamW(params, lr=0.25, state="f8" if small else "f32", seed=11)
+            held = [dict(p=p.float().cpu().numpy().reshape(-1), m=np.zeros(p.numel(), np.uint8 if small else np.float32)) for p in params]
+            for t in held:
+                t["v"] = t["m"].copy()
+                t["ms"] = t["vs"] = np.zeros(-(-len(t["p"]) // S.BLOCK), np.float32)
+            for n in range(1, 6):
+                grads = [torch.randn(p.shape, generator=g, device=DEVICE).to(dtype) for p in params]
+                before = [p.clone() for p in params]
+                opt.step(grads)
+                for i, (t, q, p) in enumerate(zip(held, grads, params)):
+                    e = expected(dict(t, g=q.float().cpu().numpy().reshape(-1)), small, seed=11, number=i, step=n, lr=0.25)
+                    held[i] = dict(t, **dict(e, p=O.round_to(e["p"], kind)))
+                    assert np.array_equal(p.float().cpu().numpy().reshape(-1), held[i]["p"]), (kind, small, n, i)
+                assert (params[0] != before[0]).float().mean().item() > 0.9, (kind, small, n)
+
+
 if __name__ == "__main__":
     for name, f in list(globals().items()):
         if name.startswith("check_"):
