@@ -293,7 +293,7 @@ int run_logprobs(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int6
 }  // namespace
 
 extern "C" uint64_t cbh_class_logprobs_workspace(uint64_t rows, uint32_t classes, uint32_t k) {
-    if (classes <= kShort) return 0;
+    if (classes <= kShort || classes > kMaxClasses) return 0;   // (more is refused)
     const Plan P = plan_parts(rows, classes);
     return P.parts == 1 && k == 0 ? 0 : rows * P.parts * (8 * (uint64_t)(k ? k + kSpare : 0) + sizeof(PartStat));
 }

@@ -1495,7 +1495,7 @@ int run_sample(const void* scores, uint64_t rows, uint32_t n, int64_t rs, int64_
 }  // namespace
 
 extern "C" uint64_t cbh_sample_classes_workspace(uint64_t rows, uint32_t classes) {
-    if (rows == 0 || classes <= kMidClasses) return 0;
+    if (rows == 0 || classes <= kMidClasses || classes > kMaxClasses) return 0;   // (more is refused)
     // a last chunk of fewer rows has more parts a row, and at most as many in all as a full one may have
     size_t most = 0, bytes = 0;
     (void)plan(std::min(rows, kChunkRows), classes, nullptr, &most);
