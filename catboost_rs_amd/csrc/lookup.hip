@@ -807,12 +807,13 @@ int run_lookup(const void* table, int64_t rs, int64_t cs, const Lookup& L, void*
     // lists of 8 f32, 2500 entries of 64 columns (64 bytes held) 34 and 37, 4000 of 64 (32 bytes) 134 and 37, 9000 of 64 (16 bytes) 254
     // and 40; 200000 lists of 40, 1280 of 64, 62 and 89.  Less of a row pays where the caches' way is slow: rows that are no whole vectors
     // are read value by value (400000 lists of 8 over 9000 entries, 16 bytes: bf16 of 30 columns 64 and 108, of 255 723 and 484; f32 of 5
-    // columns 14 and 33, of 13 38 and 35; 100000 lists of 40, 5200 entries of 255 bf16, 195 and 389), and a large table is not in the
+    // columns 14 and 33, of 13 38 and 35; 100000 lists of 40, 5200 entries of 255 bf16, 195 and 389, f32, 32 bytes of 4000 entries of 70, 106 and 137), and a large table is not in the
     // second level (60000 lists of 40, 9000 entries of 1000 f32, 702 and 849, of 256 287 and 316; in it, 5200 of 256, 284 and 183).
     uint32_t held = lanes;
     while (held > 1 && (L.entries + 1ull) * held * 16 > kLdsBytes) held /= 2;
     const bool lists_long = L.list >= 32;
-    const uint32_t share = L.dim % V == 0 ? 1 : V == 4 ? 2 : lists_long ? 64 : 8;   // of a row's vectors, one that is enough
+    // of a row's vectors, one that is enough
+    const uint32_t share = L.dim % V == 0 ? 1 : lists_long && (V == 8 || held >= 2) ? 64 : V == 8 ? 8 : 2;
     const bool pays = held >= 4 || lanes <= held * share || (lists_long && (uint64_t)L.entries * L.dim * sizeof(T) > 8u << 20);
     if (cs == 1 && L.list >= 8 && L.rows * L.list >= 256ull * L.entries && pays && (L.entries + 1ull) * held * 16 <= kLdsBytes) {
         const uint32_t tiles = (L.dim + held * V - 1) / (held * V);

@@ -22,7 +22,7 @@ def way(rows, many, entries, dim, kind):
     held = lanes
     while held > 1 and (entries + 1) * held * 16 > 163840:
         held //= 2
-    share = 1 if dim % vec == 0 else 2 if vec == 4 else 64 if many >= 32 else 8
+    share = 1 if dim % vec == 0 else 64 if many >= 32 and (vec == 8 or held >= 2) else 8 if vec == 8 else 2
     fits = many >= 8 and rows * many >= 256 * entries and (entries + 1) * held * 16 <= 163840
     large = many >= 32 and entries * dim * (16 // vec) > 8 << 20
     return (held if fits and (held >= 4 or lanes <= held * share or large) else 0), lanes
