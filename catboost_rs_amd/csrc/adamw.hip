@@ -3,11 +3,12 @@
 //   g = grad gs;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - m lr / (1 - b1^s) / (sqrt(v) / sqrt(1 - b2^s) + eps)
 //
-// Every value is read and written once: 60M values with 8-bit states and bf16 gradients 165 us, 840 MB at 5.1 TB/s, a copy's rate; what
-// it computes (a correctly rounded root and division, the hash, the codes: about 100 instructions a value) hides behind that.  150 tensors
-// of 4M values: two launches of 8 us, and 63 us of a call from Python, most of it the looking at 150 gradients and weights.  8-bit states are m and sqrt(v) as e4m3 codes over a power of two that a
-// block of 256 values shares: a wave takes a block, four values a lane.  sqrt(v), not v: the codes reach from 448 down to 2^-9, 18
-// binades, which are 36 of v.
+// Every value is read and written once: 60M f32 values with 8-bit states and bf16 gradients 165 us, 840 MB at 5.1 TB/s, a copy's rate; what
+// it computes (a correctly rounded root and division, the hash, the codes: about 100 instructions a value) hides behind that.  It does not
+// where weights have 16 bits too: 152 us, 600 MB at 4.0 TB/s.  150 tensors of 4M values: launches of 14 us (the 76 largest) and 8 us, and
+// 90 us of a call from Python, which looks at 150 gradients, weights and their states.  8-bit states are m and sqrt(v) as e4m3 codes
+// over a power of two that a block of 256 values shares: a wave takes a block, four values a lane.  sqrt(v), not v: the codes reach from
+// 448 down to 2^-9, 18 binades, which are 36 of v.
 #include <vector>
 
 #include "class_scores.hpp"
@@ -65,6 +66,7 @@ __host__ __device__ inline Factors factors(double lr, double weight_decay, doubl
     return Factors{(float)(1.0 - lr * weight_decay), (float)(lr / (1.0 - power(beta1, s))),
                    (float)(1.0 / sqrt(1.0 - power(beta2, s)))};
 }
+// (the factors: the halves of Knuth's multiplier for 64 bits, 6364136223846793005)
 __host__ __device__ inline uint32_t mix(uint32_t x) {
     x = (x ^ x >> 16) * 0x5851F42Du;
     x = (x ^ x >> 15) * 0x4C957F2Du;

@@ -6,7 +6,7 @@
 // for a row of nearly equal scores too.  The sums run along with the running maximum: when it rises from m to m',
 // sum e^d d becomes e^((m - m') / t) (sum e^d d + (m - m') / t sum e^d).
 //
-// What has to be read is the scores.  Without a k: 4096 x 65536 bf16 99 us, 537 MB at 5.4 TB/s, a copy's rate.  With one, bound by the
+// What has to be read is the scores.  Without a k: 4096 x 65536 bf16 99 us, 537 MB at 5.4 TB/s, the memory's rate.  With one, bound by the
 // row's end, a selection of dependent steps in LDS that four workgroups a CU hide in part: 4096 x 65536 bf16, k 5:
 // 128 us; 777 x 50021 f32 with allowed classes, four entries and k 20: 50 us, 155 MB at 3.1 TB/s, on 777 workgroups.
 #include "class_logprobs.hpp"

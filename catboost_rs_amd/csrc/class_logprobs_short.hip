@@ -1,9 +1,10 @@
 // Log probabilities of short rows: up to 64 classes by a thread a row, up to 2048 in the registers of a
 // wave's lanes or of some of them.  A row is read once, its maximum is known before its exponentials.
 //
-// 1M x 10 f32 class-major, one entry, k 3: 30 us, 88 MB at 2.9 TB/s; bound by f64 (the logarithm, the sums), the comparisons of all pairs
-// and stores of 12 bytes a row.  20000 x 1000 f32 without a k 19 us, k 5 42; 35431 x 70 bf16 13 and 34: the call itself
-// costs 13.  With a k bound by vector instructions: the descent over the keys' bits, and the ranking.
+// 1M x 10 f32 class-major, one entry, k 3: 30 us, 88 MB at 2.9 TB/s.  Without a k 16 us, near the memory's rate: what a k adds is the
+// comparisons of all pairs, a choice among all classes and an f64 log probability for each place, and stores of 4 bytes, 4 k apart.
+// 20000 x 1000 f32 without a k 19 us, k 5 42; 35431 x 70 bf16 13, k 5 30: the call itself costs 13.  With a k bound by vector
+// instructions: the descent over the keys' bits, and the ranking.
 #include "class_logprobs.hpp"
 
 namespace {

@@ -7,10 +7,12 @@
 // is joined in the chunks' order.
 //
 // Rows: 200000 lists of 40 over 1280 entries of 64 f32 57 us; 84 MB cross the memory, but 2.05 GB the LDS that holds the
-// table, at 36 TB/s (from the caches 103 us at 20 TB/s).  32 rows of 256 bf16: a call's 8.5 us.
-// Gradient: 262144 places of 50021 entries, 256 columns, bf16 to f32 87 us: sort 31, sums 43 (185 MB at 4.3 TB/s), join
-// and zeros 12.  65536 lists of 40 over 1280 entries of 64 f32 110 us: sort 46 (2.6M keys, scattered stores), sums 58 (671 MB
-// of rows at 11.6 TB/s from the second-level caches), join and parts 13.  Up to 512 places one launch, up to 8192 three.
+// table, at 36 TB/s (from the caches 78 us).  The LDS is at work for 40% of that, half of it on bank conflicts, the vector units for
+// 48%: neither is full, the rest waits for lists and sums.  32 rows of 256 bf16: a call's 8.5 us.
+// Gradient: 262144 places of 50021 entries, 256 columns, bf16 to f32 87 us: sort 32, sums 43 (185 MB at 4.3 TB/s), join and zeros 12.
+// 65536 lists of 40 over 1280 entries of 64 f32 110 us: sort 46 (2.6M keys, scattered stores), sums 58 (671 MB of rows at 11.6 TB/s from
+// the second-level caches), join and parts 13 (the parts under the profiler, where a kernel takes longer than among others).  Up
+// to 512 places one launch, up to 8192 three.
 #include "class_scores.hpp"
 
 namespace {
@@ -805,10 +807,12 @@ int run_lookup(const void* table, int64_t rs, int64_t cs, const Lookup& L, void*
     // In LDS: lists long enough that an entry is read often, and 64 bytes of every entry in it, or its whole row.  Of less, each list is
     // read by many workgroups, and rows are written in pieces of lines that lanes do not share.  By LDS and from the caches, us: 400000
     // lists of 8 f32, 2500 entries of 64 columns (64 bytes held) 34 and 37, 4000 of 64 (32 bytes) 134 and 37, 9000 of 64 (16 bytes) 254
-    // and 40; 200000 lists of 40, 1280 of 64, 62 and 89.  Less of a row pays where the caches' way is slow: rows that are no whole vectors
-    // are read value by value (400000 lists of 8 over 9000 entries, 16 bytes: bf16 of 30 columns 64 and 108, of 255 723 and 484; f32 of 5
-    // columns 14 and 33, of 13 38 and 35; 100000 lists of 40, 5200 entries of 255 bf16, 195 and 389, f32, 32 bytes of 4000 entries of 70, 106 and 137), and a large table is not in the
-    // second level (60000 lists of 40, 9000 entries of 1000 f32, 702 and 849, of 256 287 and 316; in it, 5200 of 256, 284 and 183).
+    // and 40; 200000 lists of 40, 1280 of 64, 58 and 78.
+    // Less of a row pays where the caches' way is slow.  Rows that are no whole vectors are read value by value: 400000 lists of 8 over
+    // 9000 entries, 16 bytes of 30 bf16 64 and 108, of 255 723 and 484, of 5 f32 14 and 33, of 13 38 and 35; 100000 lists of 40 over 5200
+    // entries of 255 bf16 195 and 389; over 4000 of 70 f32 (32 bytes) 106 and 137, 5200 of 255 (16 bytes) 300 and 357, 9000 of 30 100
+    // and 53.  And a large table is not in the second level: 60000 lists of 40 over 9000 entries of 1000 f32 702 and 849, 100000 over
+    // 9000 of 256 287 and 316; in it, 5200 of 256, 284 and 183.
     uint32_t held = lanes;
     while (held > 1 && (L.entries + 1ull) * held * 16 > kLdsBytes) held /= 2;
     const bool lists_long = L.list >= 32;

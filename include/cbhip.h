@@ -583,7 +583,7 @@ int cbh_class_logprobs(const void* scores, int32_t type, uint64_t rows, uint32_t
  * gave for these scores, temperature and allowed classes.  With p_j = exp(d_j - log Z), G = sum g of the entries:
  *   grad_j = (sum of g_i of the entries i with class j - p_j (G + h (d_j + E))) / t, 0 where j is not allowed
  * rounded once to the scores' type.  Entries of one class add up.  A row whose g (of entries) and h are all 0 gives 0
- * whatever its scores hold, and is not read; a row of -inf alone gives its entries' g / t alone where they are
+ * whatever its scores hold; a row of -inf alone gives its entries' g / t alone where they are
  * allowed; NaN or +inf in a row makes its gradient NaN where allowed.  `grad` has strides of its own and may not overlap
  * an input. */
 int cbh_logprob_gradients(const void* scores, int32_t type, uint64_t rows, uint32_t classes, int64_t row_stride,
