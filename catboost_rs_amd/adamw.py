@@ -28,7 +28,7 @@ class _Settings(C.Structure):
 class AdamW:
     """Weights ``params`` (torch tensors f32, f16 or bf16 on one GPU, contiguous) with the states that AdamW keeps of
     them; :meth:`step` takes their gradients and updates weights and states in place (``cbh_adamw_step``: the formulas are
-    there).
+    there).  One rate and one weight decay for all of them: what takes others is a handle of its own.
 
     ``state``: ``"f32"`` (``exp_avg`` and ``exp_avg_sq``, f32 of the weights' shapes) or ``"f8"`` (float8_e4m3fn codes
     of the first moment and of the square root of the second, with the scales ``exp_avg_scale`` and

@@ -243,7 +243,8 @@ def logprob_gradients(scores, given, logprob_grad, stats, *, entropy_grad=None, 
     """Gradient by the scores, in their type and layout, of a function of what :func:`class_logprobs` gave for
     them (``cbh_logprob_gradients``): ``logprob_grad`` f32 of given's shape and ``entropy_grad`` [rows] f32 are its
     derivatives by the log probabilities and the entropy, ``stats`` what the forward call returned;
-    ``temperature`` and ``allowed`` are those of that call.  A row of zeros in both gives 0 whatever its scores
+    ``temperature`` and ``allowed`` are those of that call.  For the entropy's derivative alone, ``given`` and
+    ``logprob_grad`` may be [rows][0].  A row of zeros in both gives 0 whatever its scores
     hold."""
     torch = _state.get("torch") or _bind()
     t, n, m, rs, cs = _scores(torch, scores)

@@ -1,4 +1,4 @@
-"""AdamW over torch tensors where a program does the unusual (in a process of its own: torch is imported first there)."""
+"""AdamW and log probabilities over torch tensors where a program does the unusual (in a process of its own: torch is imported first there)."""
 import os
 import subprocess
 import sys

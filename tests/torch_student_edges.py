@@ -1,4 +1,4 @@
-"""AdamW over torch tensors where a program does the unusual: run by tests/test_gpu_student_edges.py in a process of its
+"""AdamW and log probabilities over torch tensors where a program does the unusual: run by tests/test_gpu_student_edges.py in a process of its
 own, or by hand (python tests/torch_student_edges.py, on a GPU)."""
 import os
 import sys
@@ -185,6 +185,27 @@ def check_weights_of_16_bits():
                     held[i] = dict(t, **dict(e, p=O.round_to(e["p"], kind)))
                     assert np.array_equal(p.float().cpu().numpy().reshape(-1), held[i]["p"]), (kind, small, n, i)
                 assert (params[0] != before[0]).float().mean().item() > 0.9, (kind, small, n)
+
+
+def check_lists_of_no_classes():
+    """Nothing given: the entropy's derivative alone, as with entries that are none; and a step without any gradient."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for rows, n in ((300, 7), (300, 30), (40, 900), (5, 5000)):
+            g = torch.Generator(device=DEVICE).manual_seed(n)
+            x = torch.randn(rows, n, generator=g, device=DEVICE).to(dtype)
+            none, no = torch.empty(rows, 0, dtype=torch.int32, device=DEVICE), torch.full((rows, 1), -1, dtype=torch.int32, device=DEVICE)
+            up, h = torch.empty(rows, 0, device=DEVICE), torch.randn(rows, generator=g, device=DEVICE)
+            for y in (x, x.t().contiguous().t()):
+                got = cb.class_logprobs(y, none, k=2)
+                assert got.logprob.shape == (rows, 0) and torch.equal(got.stats, cb.class_logprobs(y, no, k=2).stats)
+                a = cb.logprob_gradients(y, none, up, got.stats, entropy_grad=h)
+                b = cb.logprob_gradients(y, no, torch.ones(rows, 1, device=DEVICE), got.stats, entropy_grad=h)
+                assert torch.equal(a, b) and bool((a != 0).any())
+                assert bool((cb.logprob_gradients(y, none, up, got.stats) == 0).all())
+    p = torch.ones(30, device=DEVICE)
+    opt = cb.AdamW([p])
+    opt.step([None])
+    assert opt.steps == 1 and bool((p == 1).all()) and p._version == 0
 
 
 if __name__ == "__main__":
